@@ -59,6 +59,22 @@ class AttnPagedArgs(ctypes.Structure):
     ]
 
 
+class AttnSparseArgs(ctypes.Structure):
+    _fields_ = [
+        ("p", AttnPagedArgs), ("pool_pages", c_int64), ("rope_positions", c_int64), ("row_seq", c_void_p), ("seqs", c_int32),
+        ("summaries", c_void_p), ("selected", c_void_p), ("top", c_int32), ("sink", c_int32), ("recent", c_int32),
+    ]
+
+
+class KvReadArgs(ctypes.Structure):
+    _fields_ = [
+        ("pages", c_void_p), ("page_table", c_void_p), ("page_size", c_int32), ("max_pages", c_int32), ("q8", c_int32),
+        ("pool_pages", c_int64), ("summaries", c_void_p), ("positions", c_void_p), ("row_seq", c_void_p),
+        ("rows", c_int32), ("seqs", c_int32), ("hkv", c_int32), ("dh", c_int32), ("f16", c_int32),
+        ("k_out", c_void_p), ("v_out", c_void_p), ("k_max", c_void_p), ("k_min", c_void_p),
+    ]
+
+
 class ModelDims(ctypes.Structure):
     _fields_ = [
         ("vocab", c_int64), ("d_model", c_int64), ("layers", c_int64), ("ctx", c_int64),
@@ -144,6 +160,13 @@ SIGNATURES = {
     "hero_read_probe": (c_int, [c_void_p, c_int64, c_int32, c_void_p, c_void_p]),
     "hero_q8_0_gemv_prefetch": (c_int, [c_void_p, c_int64, c_int64, c_void_p]),
     "hero_attn_decode_paged": (c_int, [POINTER(AttnPagedArgs), c_void_p]),
+    "hero_kv_summary_bytes": (c_int64, [c_int64, c_int32, c_int32]),
+    "hero_kv_append_paged": (c_int, [POINTER(AttnSparseArgs), c_void_p]),
+    "hero_kv_read_paged": (c_int, [POINTER(KvReadArgs), c_void_p]),
+    "hero_attn_select_work_bytes": (c_int64, [c_int64, c_int32, c_int64]),
+    "hero_attn_select_pages": (c_int, [POINTER(AttnSparseArgs), c_void_p]),
+    "hero_attn_sparse_work_bytes": (c_int64, [c_int64, c_int32, c_int32, c_int32, c_int32, c_int32]),
+    "hero_attn_sparse_paged": (c_int, [POINTER(AttnSparseArgs), c_void_p]),
     "hero_model_open": (c_int, [c_char_p, POINTER(c_void_p)]),
     "hero_model_open_image": (c_int, [c_void_p, c_size_t, POINTER(c_void_p)]),
     "hero_model_close": (None, [c_void_p]),

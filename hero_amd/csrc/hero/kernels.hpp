@@ -243,6 +243,69 @@ void attn_paged_plan(int64_t max_ctx, int window, int B, int Hkv, int* split, in
 int64_t attn_paged_work_floats(int B, int Hq, int nsplit, int Dh);
 void launch_attn_paged(const AttnPagedArgs& p, hipStream_t s);
 
+// kvcache.hip, sparse.hip: the long-context use of the paged cache -- rows of
+// many sequences appended with their page summaries, rows read back, the pages
+// each row attends to selected by a score over the summaries, and the
+// attention over the selected pages.
+struct PagedRows {            // which rows of which sequences, and the cache they live in
+    uint16_t* pages;          // pool as in AttnPagedArgs
+    const int32_t* page_table;// [seqs][max_pages]; entries outside [0, pool_pages) hold nothing
+    int64_t pool_pages;
+    int page_size, max_pages, q8;
+    uint8_t* summaries;       // [pool_pages] of kv_summary_page_bytes
+    const int32_t* positions; // [rows]; < 0 or past the table: the row is left out
+    const int32_t* row_seq;   // [rows]; null: row r is sequence r
+    int rows, seqs, Hkv, Dh;
+};
+// A page's summary: [Hkv][2][Dh] int8 -- round(max_t k[t][c] / d), then
+// round(-min_t k[t][c] / d), d = (largest magnitude of both) / 127 -- and per
+// K/V head the fp32 value of d rounded to 11 significant bits, to 16 bytes.
+__host__ __device__ inline int64_t kv_summary_page_bytes(int64_t Hkv, int64_t Dh) { return Hkv * 2 * Dh + (Hkv * 4 + 15) / 16 * 16; }
+struct KvAppendArgs {
+    PagedRows c;
+    const float* proj;        // as in AttnDecodeArgs
+    int64_t proj_stride, k_off, v_off;
+    const float* q_gamma;
+    const float* k_gamma;
+    float eps;
+    const float* rope_cs;     // [rope_positions][Dh/2][2]
+    int64_t rope_positions;
+    float* q_rot;             // [rows][Hq][Dh]
+    int Hq;
+};
+void launch_kv_append(const KvAppendArgs& a, hipStream_t s);
+struct KvReadArgs {
+    PagedRows c;
+    int f16;                  // outputs as fp16 instead of fp32
+    void* out[4];             // k, v and the page's per-channel max and min, [rows][Hkv*Dh]; each may be null
+};
+void launch_kv_read(const KvReadArgs& a, hipStream_t s);
+struct SelectArgs {
+    PagedRows c;
+    const float* q_rot;
+    int Hq;
+    int top, sink, recent;
+    int32_t* selected;        // [rows][Hkv][top]
+    uint64_t* keys;           // scores as ordered keys, [rows][Hkv][max_pages]
+};
+inline int64_t attn_select_work_bytes(int64_t rows, int64_t Hkv, int64_t max_pages) { return rows * Hkv * max_pages * 8; }
+void launch_attn_select(const SelectArgs& a, hipStream_t s);
+struct SparseAttnArgs {
+    PagedRows c;
+    const float* q_rot;
+    const float* proj;        // the gates: [q | gate] pairs at 0
+    int64_t proj_stride;
+    float score_scale;
+    int Hq;
+    int top;
+    const int32_t* selected;  // [rows][Hkv][top]
+    float* out_f32;           // [rows][Hq*Dh]; may be null
+    void* act_out;            // Q8_0 activations [rows][Hq*Dh]; may be null
+    float* work;
+};
+int64_t attn_sparse_work_bytes(int64_t rows, int64_t Hq, int64_t Hkv, int64_t Dh, int64_t page_size, int64_t top);
+void launch_attn_sparse(const SparseAttnArgs& a, hipStream_t s);
+
 // gemma.hip: the Gemma 4 text model's own kernels (one row: a decode step)
 // x[D] = the embedding row of *id times embed_scale, act = its Q8_0 row, and
 // tok[PL] = the per-layer table's row of *id times token_scale

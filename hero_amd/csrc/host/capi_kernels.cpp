@@ -568,4 +568,178 @@ int hero_attn_decode_paged(const hero_attn_paged_args* p, void* stream) {
     });
 }
 
+// ---- long contexts over the paged cache
+namespace {
+constexpr int64_t kMaxRowHeads = int64_t(1) << 23;  // (row, query head) pairs: grids stay below 2^32 lanes
+
+void check_paged_rows(const PagedRows& c, const int32_t* row_seq) {
+    require(c.Dh == 128 || (c.Dh == 256 && c.q8 == 0), "heads of 128 channels, or of 256 in fp16 pages");
+    require(c.q8 == 0 || c.q8 == 1, "q8 must be 0 or 1");
+    require(c.page_size >= 16 && c.page_size <= 256 && c.page_size % 16 == 0, "page_size must be a multiple of 16, 16 .. 256");
+    require(c.max_pages > 0 && int64_t(c.page_size) * c.max_pages <= (int64_t(1) << 24), "bad page geometry");
+    require(c.pool_pages > 0 && c.pool_pages <= (int64_t(1) << 31), "pool_pages out of range");
+    require(c.rows > 0 && c.seqs > 0 && c.Hkv > 0 && c.Hkv <= 1024 && c.rows <= kMaxRowHeads / c.Hkv, "bad row, sequence or head count");
+    require(row_seq || c.rows <= c.seqs, "without row_seq every row needs a sequence of its own");
+    require(c.positions && c.page_table, "null pointer");
+    require(aligned(c.positions, 4) && aligned(c.page_table, 4) && aligned(row_seq, 4), "positions, page_table and row_seq must be 4-byte aligned");
+}
+
+PagedRows sparse_rows(const hero_attn_sparse_args* p) {
+    require(p != nullptr, "null args");
+    const hero_attn_decode_args& a = p->p.a;
+    PagedRows c{};
+    c.pages = p->p.pages;
+    c.page_table = p->p.page_table;
+    c.pool_pages = p->pool_pages;
+    c.page_size = p->p.page_size;
+    c.max_pages = p->p.max_pages;
+    c.q8 = p->p.q8;
+    c.summaries = static_cast<uint8_t*>(p->summaries);
+    c.positions = a.positions;
+    c.row_seq = p->row_seq;
+    c.rows = a.b;
+    c.seqs = p->seqs;
+    c.Hkv = a.hkv;
+    c.Dh = a.dh;
+    check_paged_rows(c, p->row_seq);
+    require(a.hq > 0 && a.hq % a.hkv == 0 && a.hq / a.hkv <= kAttnMaxGroup, "1 to 8 query heads per KV head");
+    require(a.b <= kMaxRowHeads / a.hq, "too many rows");
+    require(a.window == 0, "window must be 0 (full attention)");
+    require(a.q_rot && aligned(a.q_rot, 16), "q_rot: 16-byte aligned device memory");
+    return c;
+}
+
+void check_selection(const hero_attn_sparse_args& p) {
+    require(p.top >= 1 && p.top <= 4096, "top must be in 1 .. 4096");
+    require(p.selected && aligned(p.selected, 4), "selected: device memory, 4-byte aligned");
+}
+}  // namespace
+
+int64_t hero_kv_summary_bytes(int64_t pool_pages, int32_t hkv, int32_t head_dim) {
+    if (pool_pages <= 0 || pool_pages > (int64_t(1) << 31) || hkv <= 0 || hkv > 1024 || (head_dim != 128 && head_dim != 256)) return -1;
+    return pool_pages * kv_summary_page_bytes(hkv, head_dim);
+}
+
+int hero_kv_append_paged(const hero_attn_sparse_args* p, void* stream) {
+    return guard([&] {
+        KvAppendArgs g{};
+        g.c = sparse_rows(p);
+        const hero_attn_decode_args& a = p->p.a;
+        require(a.proj && a.q_gamma && a.k_gamma && a.rope_cs && g.c.pages && g.c.summaries, "null pointer");
+        require(aligned(g.c.pages, 16) && aligned(g.c.summaries, 16), "pages and summaries must be 16-byte aligned");
+        require(aligned(a.proj, 4) && aligned(a.q_gamma, 4) && aligned(a.k_gamma, 4) && aligned(a.rope_cs, 8), "misaligned pointer");
+        require(p->rope_positions > 0, "rope_positions must be positive");
+        const int64_t qw = 2 * int64_t(a.hq) * a.dh, kw = int64_t(a.hkv) * a.dh;
+        require(a.k_off >= 0 && a.v_off >= 0 && a.proj_stride >= qw && a.k_off + kw <= a.proj_stride && a.v_off + kw <= a.proj_stride,
+                "q, k or v slices outside the projection row");
+        g.proj = a.proj;
+        g.proj_stride = a.proj_stride;
+        g.k_off = a.k_off;
+        g.v_off = a.v_off;
+        g.q_gamma = a.q_gamma;
+        g.k_gamma = a.k_gamma;
+        g.eps = a.eps;
+        g.rope_cs = a.rope_cs;
+        g.rope_positions = p->rope_positions;
+        g.q_rot = a.q_rot;
+        g.Hq = a.hq;
+        launch_kv_append(g, as_stream(stream));
+        check_launch("hero_kv_append_paged");
+    });
+}
+
+int hero_kv_read_paged(const hero_kv_read_args* p, void* stream) {
+    return guard([&] {
+        require(p != nullptr, "null args");
+        KvReadArgs g{};
+        g.c.pages = const_cast<uint16_t*>(p->pages);
+        g.c.page_table = p->page_table;
+        g.c.pool_pages = p->pool_pages;
+        g.c.page_size = p->page_size;
+        g.c.max_pages = p->max_pages;
+        g.c.q8 = p->q8;
+        g.c.summaries = static_cast<uint8_t*>(const_cast<void*>(p->summaries));
+        g.c.positions = p->positions;
+        g.c.row_seq = p->row_seq;
+        g.c.rows = p->rows;
+        g.c.seqs = p->seqs;
+        g.c.Hkv = p->hkv;
+        g.c.Dh = p->dh;
+        check_paged_rows(g.c, p->row_seq);
+        require(p->f16 == 0 || p->f16 == 1, "f16 must be 0 or 1");
+        require(p->k_out || p->v_out || p->k_max || p->k_min, "no output");
+        require(p->pages || !(p->k_out || p->v_out), "null pages");
+        require(p->summaries || !(p->k_max || p->k_min), "the bounds need summaries");
+        require(aligned(p->pages, 16) && aligned(p->summaries, 16), "pages and summaries must be 16-byte aligned");
+        require(aligned(p->k_out, 16) && aligned(p->v_out, 16) && aligned(p->k_max, 16) && aligned(p->k_min, 16), "outputs must be 16-byte aligned");
+        g.f16 = p->f16;
+        g.out[0] = p->k_out;
+        g.out[1] = p->v_out;
+        g.out[2] = p->k_max;
+        g.out[3] = p->k_min;
+        launch_kv_read(g, as_stream(stream));
+        check_launch("hero_kv_read_paged");
+    });
+}
+
+int64_t hero_attn_select_work_bytes(int64_t rows, int32_t hkv, int64_t max_pages) {
+    if (rows <= 0 || hkv <= 0 || rows > kMaxRowHeads / hkv || max_pages <= 0 || max_pages > (int64_t(1) << 20)) return -1;
+    return attn_select_work_bytes(rows, hkv, max_pages);
+}
+
+int hero_attn_select_pages(const hero_attn_sparse_args* p, void* stream) {
+    return guard([&] {
+        SelectArgs g{};
+        g.c = sparse_rows(p);
+        check_selection(*p);
+        require(p->sink >= 0 && p->recent >= 1 && int64_t(p->sink) + p->recent <= p->top, "sink >= 0, recent >= 1 and sink + recent <= top");
+        require(g.c.summaries && aligned(g.c.summaries, 16), "summaries: 16-byte aligned device memory");
+        require(p->p.work && aligned(p->p.work, 16), "work: 16-byte aligned device memory");
+        require(p->p.work_bytes >= attn_select_work_bytes(g.c.rows, g.c.Hkv, g.c.max_pages), "work_bytes below hero_attn_select_work_bytes");
+        g.q_rot = p->p.a.q_rot;
+        g.Hq = p->p.a.hq;
+        g.top = p->top;
+        g.sink = p->sink;
+        g.recent = p->recent;
+        g.selected = p->selected;
+        g.keys = reinterpret_cast<uint64_t*>(p->p.work);
+        launch_attn_select(g, as_stream(stream));
+        check_launch("hero_attn_select_pages");
+    });
+}
+
+int64_t hero_attn_sparse_work_bytes(int64_t rows, int32_t hq, int32_t hkv, int32_t head_dim, int32_t page_size, int32_t top) {
+    if (rows <= 0 || hkv <= 0 || hq <= 0 || hq % hkv || hq / hkv > kAttnMaxGroup || rows > kMaxRowHeads / hq || (head_dim != 128 && head_dim != 256) ||
+        page_size < 16 || page_size > 256 || page_size % 16 || top < 1 || top > 4096)
+        return -1;
+    return attn_sparse_work_bytes(rows, hq, hkv, head_dim, page_size, top);
+}
+
+int hero_attn_sparse_paged(const hero_attn_sparse_args* p, void* stream) {
+    return guard([&] {
+        SparseAttnArgs g{};
+        g.c = sparse_rows(p);
+        check_selection(*p);
+        const hero_attn_decode_args& a = p->p.a;
+        require(a.proj && aligned(a.proj, 4) && g.c.pages && aligned(g.c.pages, 16), "proj and pages: device memory, pages 16-byte aligned");
+        require(a.proj_stride >= 2 * int64_t(a.hq) * a.dh, "gates outside the projection row");
+        require(a.out_f32 || a.act_out, "no output");
+        require(aligned(a.out_f32, 16) && aligned(a.act_out, 16), "outputs must be 16-byte aligned");
+        const int64_t need = attn_sparse_work_bytes(g.c.rows, a.hq, a.hkv, a.dh, g.c.page_size, p->top);
+        require(need == 0 || (p->p.work && aligned(p->p.work, 16) && p->p.work_bytes >= need), "work: 16-byte aligned, hero_attn_sparse_work_bytes");
+        g.q_rot = a.q_rot;
+        g.proj = a.proj;
+        g.proj_stride = a.proj_stride;
+        g.score_scale = a.score_scale;
+        g.Hq = a.hq;
+        g.top = p->top;
+        g.selected = p->selected;
+        g.out_f32 = a.out_f32;
+        g.act_out = a.act_out;
+        g.work = p->p.work;
+        launch_attn_sparse(g, as_stream(stream));
+        check_launch("hero_attn_sparse_paged");
+    });
+}
+
 }  // extern "C"

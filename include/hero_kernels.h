@@ -348,6 +348,101 @@ int hero_read_probe(const void* p, int64_t bytes, int32_t workgroups, uint32_t* 
 int hero_q8_0_gemv_prefetch(const void* packed, int64_t n, int64_t k, void* stream);
 int hero_attn_decode_paged(const hero_attn_paged_args* args, void* stream);
 
+/* ---- long contexts over the paged cache --------------------------------------
+ * No counterpart in the reference. A serving loop appends rows (decoded tokens
+ * of many sequences, prompt chunks, or both in one call) to the paged cache,
+ * selects for each row the pages worth attending to by a cheap score, and runs
+ * the gated attention over those pages alone. The pool is the one
+ * hero_attn_decode_paged reads and writes (fp16 or Q8_0 pages); rows appended
+ * here equal the ones appended there bit for bit.
+ *
+ * Rows: row r (of p.a.b) is the token at p.a.positions[r] of sequence
+ * row_seq[r] (row_seq NULL: of sequence r). Sequence s owns row s of
+ * p.page_table [seqs][max_pages]; entries outside [0, pool_pages) hold nothing:
+ * no key is stored to or read from them. A row whose position is negative or
+ * past the table, or whose sequence is not in [0, seqs), is left out: its
+ * outputs stay as they were (its list of selected pages is filled with -1). A
+ * key that is not at or before a row's position has no influence on the row,
+ * whatever the pool holds there. Pages of 16 to 256 positions, a multiple of
+ * 16; heads of 128 channels (fp16 and Q8_0) or 256 (fp16), at most 8 query
+ * heads per K/V head, at most 2^23 (row, query head) pairs a call. Full
+ * attention only: p.a.window must be 0. All calls of a stream may share one
+ * workspace; calls that may overlap need one each. */
+typedef struct hero_attn_sparse_args {
+    hero_attn_paged_args p;      /* p.a.k_cache, v_cache, scores, max_ctx unused */
+    int64_t pool_pages;          /* pages in the pool (and in summaries) */
+    int64_t rope_positions;      /* rows of p.a.rope_cs; append leaves out rows past them */
+    const int32_t* row_seq;      /* [p.a.b] or NULL */
+    int32_t seqs;                /* sequences of p.page_table; >= p.a.b if row_seq is NULL */
+    void* summaries;             /* hero_kv_summary_bytes(pool_pages, hkv, dh) */
+    int32_t* selected;           /* [p.a.b][hkv][top] logical pages, -1: none */
+    int32_t top, sink, recent;   /* pages per (row, K/V head); of them always the first and the last */
+} hero_attn_sparse_args;
+
+/* Bytes of the page summaries of a pool: per page and K/V head the largest and
+ * the negated smallest value of each channel over the stored keys as int8
+ * [2][dh], and their common step (fp32, 11 significant bits), see
+ * hero_kv_append_paged. */
+int64_t hero_kv_summary_bytes(int64_t pool_pages, int32_t hkv, int32_t head_dim);
+
+/* The K/V half of the paged attention for any rows: q and k RMSNorm + RoPE
+ * (nm/src/components.hpp:176-181, nm/src/attention.hpp:76-91; q to p.a.q_rot),
+ * k and v to their page slots as fp16 (round to nearest even) or Q8_0
+ * (nm/src/quant_i8.hpp:70-80), and the summary of every page a row fell into,
+ * over the page's slots up to the row's. Uses p.a.proj, proj_stride, k_off,
+ * v_off, q_gamma, k_gamma, eps, rope_cs, positions, q_rot, b, hq, hkv, dh, the
+ * page fields and everything above but selected, top, sink and recent. The rows
+ * of one sequence stand together, positions ascending by one; a page belongs
+ * to one sequence of the call. */
+int hero_kv_append_paged(const hero_attn_sparse_args* args, void* stream);
+
+/* Rows of the cache back as fp32 (exact) or fp16 (rounded once; exact for fp16
+ * pages): row r's k and v of all heads to k_out and v_out [rows][hkv*dh], and
+ * the bounds that its page's summary stands for to k_max and k_min. Each output
+ * may be NULL; summaries is needed for the bounds only. Outputs 16-byte
+ * aligned. A row in a page that holds nothing is left out. */
+typedef struct hero_kv_read_args {
+    const uint16_t* pages;
+    const int32_t* page_table;   /* [seqs][max_pages] */
+    int32_t page_size, max_pages, q8;
+    int64_t pool_pages;
+    const void* summaries;
+    const int32_t* positions;    /* [rows] */
+    const int32_t* row_seq;      /* [rows], or NULL: row r is sequence r */
+    int32_t rows, seqs, hkv, dh;
+    int32_t f16;                 /* 0: fp32 outputs, 1: fp16 */
+    void *k_out, *v_out, *k_max, *k_min;
+} hero_kv_read_args;
+int hero_kv_read_paged(const hero_kv_read_args* args, void* stream);
+
+/* The pages each row attends to, per K/V head: selected[r][g] = `top` logical
+ * pages in ascending order (fewer, then -1, where the row sees fewer). Always
+ * the first `sink` and the last `recent` pages the row sees (recent >= 1,
+ * sink + recent <= top <= 4096), then the best by score, ties to the lowest
+ * page: score = max over the group's query heads of
+ *   step_q * step_page * sum_c max(q8_c max8_c, q8_c min8_c),
+ * q8 = the head of p.a.q_rot as round(q / (amax / 127)), step_q = amax / 127 at
+ * 11 bits, max8, min8 and step_page the page's summary. The integer sum and
+ * both steps make the score exact in 64 bits, so the lists do not depend on an
+ * order of summation. With non-finite queries or keys the choice among pages is
+ * unspecified. Uses p.a.q_rot, positions, b, hq, hkv, dh, page_table, page_size,
+ * max_pages, work (hero_attn_select_work_bytes, 16-byte aligned). */
+int64_t hero_attn_select_work_bytes(int64_t rows, int32_t hkv, int64_t max_pages);
+int hero_attn_select_pages(const hero_attn_sparse_args* args, void* stream);
+
+/* Gated GQA attention (the attention body of nm/src/qwen35.hpp:387-393) of each
+ * row over the positions of its selected pages, up to its own position:
+ * softmax(score_scale * q . k), the weighted sum of the values, sigmoid(gate).
+ * `selected` may hold pages in any order; entries outside the row's pages count
+ * as none, a page that is listed twice counts twice, and a row with no page
+ * gets zeros. Outputs: out_f32 and / or act_out (Q8_0 activations), at least
+ * one. Uses p.a.q_rot, proj (the gates), proj_stride, positions, score_scale, b,
+ * hq, hkv, dh, the page fields and work (hero_attn_sparse_work_bytes, 16-byte
+ * aligned). Results agree with the sequential reference over the stored keys
+ * and values to fp32 rounding. */
+int64_t hero_attn_sparse_work_bytes(int64_t rows, int32_t hq, int32_t hkv, int32_t head_dim, int32_t page_size, int32_t top);
+int hero_attn_sparse_paged(const hero_attn_sparse_args* args, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
