@@ -26,7 +26,10 @@ namespace {
 constexpr int kApRows = 64;  // rows per pass of the K/V part
 constexpr int kApQ = 32;     // (row, query head) items per workgroup of the q part
 
+// x rounded to fp32 by whatever formed it, then to fp16 (the compiler may not
+// round a product to fp16 at once)
 __device__ __forceinline__ uint16_t f16_bits(float x) {
+    asm("" : "+v"(x));
     const _Float16 h = _Float16(x);
     uint16_t b;
     __builtin_memcpy(&b, &h, 2);

@@ -547,6 +547,29 @@ def test_attend_of_small_and_large_queries(lib, q8, scale):
     check_attend(c, 8, q, proj, [0], [250], sel, got, act)
 
 
+@pytest.mark.parametrize("q8", [False, True])
+def test_attend_weights_keep_both_their_terms(lib, q8):
+    """Nearly equal weights of 32 keys over many rows: the bound is then 7e-6 of
+    the mean value, half of what one weight kept to fp16 only would be off by."""
+    rng = np.random.default_rng(77)
+    c = Cache(rng, 64, 1, 8, 128, 32, q8)
+    q, proj = (rng.standard_normal((64, 32, 128)) * 0.02).astype(np.float32), np.full((64, 8192), 20, np.float32)
+    sel = np.zeros((64, 8, 1), np.int32)
+    got, act = run_attend(lib, c, 32, q, proj, range(64), [31] * 64, sel, row_seq=False)
+    check_attend(c, 32, q, proj, range(64), [31] * 64, sel, got, act)
+
+
+def test_attend_of_subnormal_values(lib):
+    """Cached values below fp16's normal range are not flushed."""
+    rng = np.random.default_rng(78)
+    c = Cache(rng, 1, 2, 2, 128, 64)
+    c.kv[:, 1] = (rng.integers(-1023, 1024, c.kv[:, 1].shape) * 2.0 ** -24).astype(np.float16)
+    q, proj = rng.standard_normal((1, 8, 128)).astype(np.float32), rng.standard_normal((1, 2048)).astype(np.float32)
+    sel = np.array([[[0, 1]] * 2], np.int32)
+    got, act = run_attend(lib, c, 8, q, proj, [0], [100], sel)
+    check_attend(c, 8, q, proj, [0], [100], sel, got, act)
+
+
 def test_attend_of_values_of_every_size(lib):
     """Cached values from fp16's smallest to its largest, keys among them."""
     rng = np.random.default_rng(14)
