@@ -25,6 +25,19 @@ namespace hero {
 namespace {
 
 // ---- selection ----------------------------------------------------------------------
+// Scores are int8 matrix products of 16 pages x 16 columns x 64 bytes: the
+// columns are the query heads of a K/V head (GP, the group rounded up to a
+// power of two) times RT rows, which share the pages' reads where they belong
+// to one sequence. Both operands are loaded where they are used: lane 16 g + c
+// reads 16 consecutive bytes of page c, and holds the same bytes of column c's
+// codes; it gets the sums of pages 4 g .. 4 g + 3 for column c.
+typedef int v4i_t __attribute__((ext_vector_type(4)));
+
+__device__ __forceinline__ float max_over_rows(float x) {  // over the four g of a column
+    x = fmaxf(x, __shfl_xor(x, 16));
+    return fmaxf(x, __shfl_xor(x, 32));
+}
+
 // order-preserving key of a score; 0 is kept for pages that cannot be taken
 __device__ __forceinline__ uint64_t score_key(double s) {
     if (s != s) return 1;
@@ -32,77 +45,318 @@ __device__ __forceinline__ uint64_t score_key(double s) {
     return b < 0 ? ~uint64_t(b) : uint64_t(b) | (uint64_t(1) << 63);
 }
 
-// a workgroup per (row, K/V head, 256 pages), a lane per page
-template <int DH>
-__global__ __launch_bounds__(256) void page_scores_kernel(SelectArgs a) {
-    const PagedRows& c = a.c;
-    const int tid = threadIdx.x, r = blockIdx.x / c.Hkv, g = blockIdx.x % c.Hkv, group = a.Hq / c.Hkv;
-    int seq;
-    const int pos = row_position(c, r, &seq);
-    if (pos < 0) return;
-    const int visible = pos / c.page_size + 1;
-    if (visible <= a.top || int(blockIdx.y) * 256 >= visible) return;
-    __shared__ int8_t q[8][DH];
-    __shared__ float step[8];
-    for (int h = tid >> 6; h < group; h += 4) {
-        const float* x = a.q_rot + (int64_t(r) * a.Hq + g * group + h) * DH;
-        float amax = 0.f;
-        for (int j = tid & 63; j < DH; j += 64) amax = fmaxf(amax, fabsf(x[j]));
-        for (int off = 32; off > 0; off >>= 1) amax = fmaxf(amax, __shfl_xor(amax, off));
-        const float d = amax / 127.f, id = d != 0.f ? 1.f / d : 0.f;
-        for (int j = tid & 63; j < DH; j += 64) q[h][j] = int8_t(int(roundf(x[j] * id)));
-        if ((tid & 63) == 0) step[h] = round11(d);
-    }
-    __syncthreads();
-    const int page = blockIdx.y * 256 + tid;
-    if (page >= visible) return;
-    const int64_t id = pool_page(c, seq, page);
-    double s = -INFINITY;
-    if (id >= 0) {
-        const int8_t* b = reinterpret_cast<const int8_t*>(c.summaries + id * kv_summary_page_bytes(c.Hkv, DH));
-        const float d = reinterpret_cast<const float*>(b + int64_t(c.Hkv) * 2 * DH)[g];
-        b += int64_t(g) * 2 * DH;
-        for (int h = 0; h < group; ++h) {
-            int sum = 0;
-            for (int j = 0; j < DH; ++j) sum += q[h][j] > 0 ? int(q[h][j]) * b[j] : -int(q[h][j]) * b[DH + j];
-            s = fmax(s, double(sum) * double(step[h]));
-        }
-        s *= double(d);
-    } else {
-        s = __longlong_as_double(0x7ff8000000000000ll);
-    }
-    a.keys[(int64_t(r) * c.Hkv + g) * c.max_pages + page] = score_key(s);
+template <int CTRL>
+__device__ __forceinline__ double max_with(double v) {  // with a lane of the same 16
+    const int2 x = __builtin_bit_cast(int2, v);
+    const int2 y = make_int2(__builtin_amdgcn_update_dpp(0, x.x, CTRL, 0xF, 0xF, false), __builtin_amdgcn_update_dpp(0, x.y, CTRL, 0xF, 0xF, false));
+    return fmax(v, __builtin_bit_cast(double, y));
 }
 
-// a wave per (row, K/V head): the top-th largest key bit by bit, then the
-// pages above it and the first of its equals, in order
-__global__ __launch_bounds__(64) void page_select_kernel(SelectArgs a) {
+// The scores of pages 64 k, k = first, first + stride, ..., for rows r0 .. r0 +
+// RT - 1 and K/V head g, by one wave; store(row, page, key) for every page the
+// row sees, of the rows that see more than `top`.
+template <int DH, int GP, int RT, class Store>
+__device__ __forceinline__ void score_pages(const SelectArgs& a, int g, int r0, int first, int stride, Store store) {
+    constexpr int H = DH / 64, KS = 2 * H;  // 64-byte steps: [max | -min]
     const PagedRows& c = a.c;
-    const int lane = threadIdx.x, r = blockIdx.x / c.Hkv, g = blockIdx.x % c.Hkv;
-    int32_t* out = a.selected + (int64_t(r) * c.Hkv + g) * a.top;
+    const int lane = threadIdx.x & 63, g4 = lane >> 4, c16 = lane & 15, sub = c16 % GP, rt = c16 / GP;
+    const int group = a.Hq / c.Hkv, r = r0 + min(rt, RT - 1);
+    int seq = -1, pos = -1;
+    if (r < c.rows) pos = row_position(c, r, &seq);
+    const int sees = pos < 0 ? 0 : pos / c.page_size + 1;
+    bool todo = rt < RT && sees > a.top;
+    if (!__any(todo)) return;
+
+    // the column's codes: a head's 16 channels 64 s + 16 g4 .., positive parts, then negative
+    v4i_t q[KS];
+    double step;
+    {
+        const float* x = a.q_rot + (int64_t(min(r, c.rows - 1)) * a.Hq + g * group + min(sub, group - 1)) * DH + 16 * g4;
+        float v[H][16], amax = 0.f;
+#pragma unroll
+        for (int s = 0; s < H; ++s)
+#pragma unroll
+            for (int j = 0; j < 16; j += 4) {
+                const float4 f = *reinterpret_cast<const float4*>(x + 64 * s + j);
+                v[s][j] = f.x, v[s][j + 1] = f.y, v[s][j + 2] = f.z, v[s][j + 3] = f.w;
+            }
+#pragma unroll
+        for (int s = 0; s < H; ++s)
+#pragma unroll
+            for (int j = 0; j < 16; ++j) amax = fmaxf(amax, fabsf(v[s][j]));
+        amax = max_over_rows(amax);
+        const float d = amax / 127.f, id = d != 0.f ? 1.f / d : 0.f;
+        step = double(round11(d));
+#pragma unroll
+        for (int s = 0; s < H; ++s)
+#pragma unroll
+            for (int w = 0; w < 4; ++w) {
+                int up = 0, down = 0;
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    const int code = int(roundf(v[s][4 * w + j] * id));
+                    up |= max(code, 0) << (8 * j);
+                    down |= max(-code, 0) << (8 * j);
+                }
+                q[s][w] = up;
+                q[H + s][w] = down;
+            }
+    }
+
+    const int64_t page_bytes = kv_summary_page_bytes(c.Hkv, DH), steps_at = int64_t(c.Hkv) * 2 * DH + 4 * g;
+    while (const uint64_t left = __ballot(todo)) {  // the rows of one sequence at a time
+        const int s0 = RT == 1 ? __builtin_amdgcn_readfirstlane(seq) : __shfl(seq, __ffsll((unsigned long long)left) - 1);
+        const bool mine = todo && seq == s0;
+        int most = mine ? sees : 0;
+        if constexpr (RT > 1)
+            for (int off = 8; off > 0; off >>= 1) most = max(most, __shfl_xor(most, off));
+        most = __builtin_amdgcn_readfirstlane(most);
+        todo = todo && !mine;
+        for (int k = first; 64 * k < most; k += stride) {
+            const int page = 64 * k + lane;
+            const int64_t id = page < most ? pool_page(c, s0, page) : -1;
+            const uint8_t* at = c.summaries + (id < 0 ? 0 : id) * page_bytes;  // page 0 for none: read, then ranked last
+            const float step_l = id < 0 ? __uint_as_float(0x7fc00000u) : *reinterpret_cast<const float*>(at + steps_at);
+            const int at_lo = int(reinterpret_cast<uintptr_t>(at)), at_hi = int(reinterpret_cast<uintptr_t>(at) >> 32);
+            constexpr int TT = DH == 128 ? 4 : 2;  // tiles of 16 pages in flight
+#pragma unroll
+            for (int t0 = 0; t0 < 4; t0 += TT) {
+                if (64 * k + 16 * t0 >= most) break;
+                v4i_t b[TT][KS];
+#pragma unroll
+                for (int t = 0; t < TT; ++t) {
+                    const int from = 16 * (t0 + t) + c16;
+                    const uintptr_t p = uint32_t(__shfl(at_lo, from)) | uint64_t(uint32_t(__shfl(at_hi, from))) << 32;
+                    const v4i_t* src = reinterpret_cast<const v4i_t*>(p + int64_t(g) * 2 * DH + 16 * g4);
+#pragma unroll
+                    for (int s = 0; s < KS; ++s) b[t][s] = src[4 * s];
+                }
+#pragma unroll
+                for (int t = 0; t < TT; ++t) {
+                    v4i_t sum = {0, 0, 0, 0};
+#pragma unroll
+                    for (int s = 0; s < KS; ++s) sum = __builtin_amdgcn_mfma_i32_16x16x64_i8(b[t][s], q[s], sum, 0, 0, 0);
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        double s = double(sum[i]) * step;
+                        if constexpr (GP >= 2) s = max_with<0xB1>(s);   // quad_perm [1,0,3,2]
+                        if constexpr (GP >= 4) s = max_with<0x4E>(s);   // quad_perm [2,3,0,1]
+                        if constexpr (GP >= 8) s = max_with<0x141>(s);  // row_half_mirror
+                        const int at_page = 16 * (t0 + t) + 4 * g4 + i;
+                        s *= double(__shfl(step_l, at_page));
+                        if (mine && (GP >= 4 ? sub == i : (i & (GP - 1)) == sub) && 64 * k + at_page < sees) store(rt, 64 * k + at_page, score_key(s));
+                    }
+                }
+            }
+        }
+    }
+}
+
+// NT lanes choose the pages of one (row, K/V head) that sees `sees` > top pages:
+// the first and last ones, and of the others the best by key, lane t holding
+// pages t, t + NT, ... (at most KPL). The smallest key that is taken is found
+// bit by bit, the upper 32 bits first; most searches end as soon as exactly
+// the wanted number of keys lies at or above.
+struct SelectShared {
+    int count[2][16];
+    int place[16 * 16];
+};
+template <int NT, int KPL>
+__device__ __forceinline__ void choose_pages(const uint64_t* keys, int sees, int top, int sink, int recent, int32_t* out, SelectShared* sh) {
+    constexpr int NW = NT / 64;
+    const int t = NT == 64 ? threadIdx.x & 63 : threadIdx.x, w = t >> 6, lane = t & 63;
+    const int lo_end = sink, hi_end = sees - recent, need = top - sink - recent;
+    uint32_t hi[KPL], lo[KPL];
+#pragma unroll
+    for (int i = 0; i < KPL; ++i) {
+        const int p = NT * i + t;
+        const uint64_t k = p >= lo_end && p < hi_end ? keys[p] : 0;
+        hi[i] = uint32_t(k >> 32);
+        lo[i] = uint32_t(k);
+    }
+    int turn = 0;
+    auto count = [&](auto pred) {
+        int n = 0;
+#pragma unroll
+        for (int i = 0; i < KPL; ++i)
+            if (NT * i < sees) n += __popcll(__ballot(pred(hi[i], lo[i])));
+        if constexpr (NW > 1) {
+            if (lane == 0) sh->count[turn][w] = n;
+            __syncthreads();
+            n = 0;
+            for (int k = 0; k < NW; ++k) n += sh->count[turn][k];
+            turn ^= 1;
+        }
+        return n;
+    };
+    uint32_t th = 0, tl = 0;
+    int equal = 0x7fffffff;  // how many of the keys equal to (th, tl) are taken
+    if (need > 0) {
+        bool exact = false;
+        for (int bit = 31; bit >= 0 && !exact; --bit) {
+            const uint32_t u = th | (1u << bit);
+            const int n = count([&](uint32_t h, uint32_t) { return h >= u; });
+            if (n >= need) th = u, exact = n == need;
+        }
+        if (!exact) {
+            const int rest = need - count([&](uint32_t h, uint32_t) { return h > th; });
+            for (int bit = 31; bit >= 0 && !exact; --bit) {
+                const uint32_t u = tl | (1u << bit);
+                const int n = count([&](uint32_t h, uint32_t l) { return h == th && l >= u; });
+                if (n >= rest) tl = u, exact = n == rest;
+            }
+            if (!exact) equal = rest - count([&](uint32_t h, uint32_t l) { return h == th && l > tl; });
+        }
+    } else {
+        th = tl = 0xffffffffu;
+        equal = 0;
+    }
+    // ascending pages: (i, wave, lane). Equal keys first, if they are not all taken
+    const uint64_t below = (uint64_t(1) << lane) - 1;
+    auto ranked = [&](auto pred, auto use) {  // use(i, rank of this lane's page among those with pred)
+        int at = 0;
+        if constexpr (NW > 1) {
+            __syncthreads();
+#pragma unroll
+            for (int i = 0; i < KPL; ++i) {
+                const int n = __popcll(__ballot(pred(i)));
+                if (lane == 0) sh->place[i * NW + w] = n;
+            }
+            __syncthreads();
+            if (w == 0) {  // exclusive sums of KPL * NW counts, four a lane
+                int v[4], s = 0;
+#pragma unroll
+                for (int k = 0; k < 4; ++k) v[k] = 4 * lane + k < KPL * NW ? sh->place[4 * lane + k] : 0;
+#pragma unroll
+                for (int k = 0; k < 4; ++k) s += v[k];
+                int x = s;
+                for (int off = 1; off < 64; off <<= 1) {
+                    const int y = __shfl_up(x, off);
+                    if (lane >= off) x += y;
+                }
+                x -= s;
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                    if (4 * lane + k < KPL * NW) sh->place[4 * lane + k] = x;
+                    x += v[k];
+                }
+            }
+            __syncthreads();
+        }
+#pragma unroll
+        for (int i = 0; i < KPL; ++i) {
+            if (NT * i >= sees) break;
+            const uint64_t m = __ballot(pred(i));
+            if constexpr (NW > 1) at = sh->place[i * NW + w];
+            use(i, at + __popcll(m & below));
+            at += __popcll(m);
+        }
+    };
+    uint32_t skip = 0;  // bit i: an equal key that is not taken
+    if (equal != 0x7fffffff)
+        ranked([&](int i) { return hi[i] == th && lo[i] == tl && NT * i + t >= lo_end && NT * i + t < hi_end; },
+               [&](int i, int rank) { skip |= rank >= equal ? 1u << i : 0u; });
+    auto taken = [&](int i) {
+        const int p = NT * i + t;
+        if (p >= sees) return false;
+        if (p < lo_end || p >= hi_end) return true;
+        return hi[i] > th || (hi[i] == th && (lo[i] > tl || (lo[i] == tl && !(skip >> i & 1))));
+    };
+    ranked(taken, [&](int i, int rank) {
+        if (taken(i)) out[rank] = NT * i + t;
+    });
+}
+
+// fewer pages than the list holds: all of them, -1 behind
+__device__ __forceinline__ void list_all(int32_t* out, int sees, int top, int t, int nt) {
+    for (int i = t; i < top; i += nt) out[i] = i < sees ? i : -1;
+}
+
+__device__ __forceinline__ int row_sees(const PagedRows& c, int r) {
     int seq;
     const int pos = row_position(c, r, &seq);
-    const int visible = pos < 0 ? 0 : pos / c.page_size + 1;
-    if (visible <= a.top) {
-        for (int i = lane; i < a.top; i += 64) out[i] = i < visible ? i : -1;
+    return pos < 0 ? 0 : pos / c.page_size + 1;
+}
+
+// Up to 1024 pages: four waves score them for RT rows into shared memory, then
+// a wave per row chooses.
+template <int DH, int GP, int RT>
+__global__ __launch_bounds__(256) void select_pages_kernel(SelectArgs a) {
+    const PagedRows& c = a.c;
+    const int w = threadIdx.x >> 6, g = blockIdx.x % c.Hkv, r0 = blockIdx.x / c.Hkv * RT;
+    extern __shared__ __align__(16) uint64_t sel_keys[];  // [RT][max_pages]
+    score_pages<DH, GP, RT>(a, g, r0, w, 4, [&](int rt, int page, uint64_t k) { sel_keys[rt * c.max_pages + page] = k; });
+    __syncthreads();
+    for (int rt = w; rt < RT && r0 + rt < c.rows; rt += 4) {
+        int32_t* out = a.selected + (int64_t(r0 + rt) * c.Hkv + g) * a.top;
+        const int sees = row_sees(c, r0 + rt);
+        if (sees <= a.top)
+            list_all(out, sees, a.top, threadIdx.x & 63, 64);
+        else if (sees <= 256)
+            choose_pages<64, 4>(sel_keys + rt * c.max_pages, sees, a.top, a.sink, a.recent, out, nullptr);
+        else
+            choose_pages<64, 16>(sel_keys + rt * c.max_pages, sees, a.top, a.sink, a.recent, out, nullptr);
+    }
+}
+
+// More pages: scores to the workspace, a wave per 64 pages at a time ...
+template <int DH, int GP, int RT>
+__global__ __launch_bounds__(256) void page_scores_kernel(SelectArgs a) {
+    const PagedRows& c = a.c;
+    const int w = threadIdx.x >> 6, g = blockIdx.x % c.Hkv, r0 = blockIdx.x / c.Hkv * RT;
+    score_pages<DH, GP, RT>(a, g, r0, blockIdx.y * 4 + w, gridDim.y * 4,
+                            [&](int rt, int page, uint64_t k) { a.keys[(int64_t(r0 + rt) * c.Hkv + g) * c.max_pages + page] = k; });
+}
+// ... then a workgroup per (row, K/V head) chooses among up to 16 NT pages
+template <int NT>
+__global__ __launch_bounds__(NT) void choose_pages_kernel(SelectArgs a) {
+    const PagedRows& c = a.c;
+    const int r = blockIdx.x / c.Hkv, g = blockIdx.x % c.Hkv;
+    int32_t* out = a.selected + (int64_t(r) * c.Hkv + g) * a.top;
+    __shared__ SelectShared sh;
+    const int sees = row_sees(c, r);
+    if (sees <= a.top)
+        list_all(out, sees, a.top, threadIdx.x, NT);
+    else
+        choose_pages<NT, 16>(a.keys + (int64_t(r) * c.Hkv + g) * c.max_pages, sees, a.top, a.sink, a.recent, out, &sh);
+}
+
+// any number of pages: the same search with the keys read again for every bit
+__global__ __launch_bounds__(1024) void choose_pages_long_kernel(SelectArgs a) {
+    const PagedRows& c = a.c;
+    const int t = threadIdx.x, lane = t & 63, w = t >> 6, r = blockIdx.x / c.Hkv, g = blockIdx.x % c.Hkv;
+    int32_t* out = a.selected + (int64_t(r) * c.Hkv + g) * a.top;
+    const int sees = row_sees(c, r);
+    if (sees <= a.top) {
+        list_all(out, sees, a.top, t, 1024);
         return;
     }
+    __shared__ int part[16];
     const uint64_t* keys = a.keys + (int64_t(r) * c.Hkv + g) * c.max_pages;
-    auto key = [&](int i) { return i >= visible ? 0 : i < a.sink || i >= visible - a.recent ? ~uint64_t(0) : keys[i]; };
-    uint64_t t = 0;  // the largest t with at least top keys >= t
+    auto key = [&](int i) { return i >= sees ? 0 : i < a.sink || i >= sees - a.recent ? ~uint64_t(0) : keys[i]; };
+    auto total = [&](int n) {  // of the waves' counts
+        __syncthreads();
+        if (lane == 0) part[w] = n;
+        __syncthreads();
+        n = 0;
+        for (int k = 0; k < 16; ++k) n += part[k];
+        return n;
+    };
+    uint64_t th = 0;  // the largest with at least top keys at or above
     for (int bit = 63; bit >= 0; --bit) {
-        const uint64_t u = t | (uint64_t(1) << bit);
+        const uint64_t u = th | (uint64_t(1) << bit);
         int n = 0;
-        for (int i = lane; i - lane < visible; i += 64) n += __popcll(__ballot(key(i) >= u));
-        if (n >= a.top) t = u;
+        for (int i = t; i - t < sees; i += 1024) n += __popcll(__ballot(key(i) >= u));
+        if (total(n) >= a.top) th = u;
     }
-    int above = 0;
-    for (int i = lane; i - lane < visible; i += 64) above += __popcll(__ballot(key(i) > t));
-    int equal = a.top - above, at = 0;
+    int n = 0;
+    for (int i = t; i - t < sees; i += 1024) n += __popcll(__ballot(key(i) > th));
+    int equal = a.top - total(n), at = 0;
     const uint64_t below = (uint64_t(1) << lane) - 1;
-    for (int i = lane; i - lane < visible && at < a.top; i += 64) {
-        const uint64_t k = key(i), eq = __ballot(k == t);
-        const bool take = k > t || (k == t && __popcll(eq & below) < equal);
+    if (w != 0) return;
+    for (int i = lane; i - lane < sees && at < a.top; i += 64) {
+        const uint64_t k = key(i), eq = __ballot(k == th);
+        const bool take = k > th || (k == th && __popcll(eq & below) < equal);
         const uint64_t m = __ballot(take);
         if (take) out[at + __popcll(m & below)] = i;
         at += __popcll(m);
@@ -150,10 +404,6 @@ constexpr float kPSlack = 2.f;   // m may lag the maximum by this: weights stay 
 
 __device__ __forceinline__ float column_other(float x) {  // the value of column c ^ 8
     return __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(x), 0x128, 0xF, 0xF, false));  // row_ror:8
-}
-__device__ __forceinline__ float max_over_rows(float x) {  // over the four g of a column
-    x = fmaxf(x, __shfl_xor(x, 16));
-    return fmaxf(x, __shfl_xor(x, 32));
 }
 __device__ __forceinline__ float sum_over_rows(float x) {
     x += __shfl_xor(x, 16);
@@ -558,16 +808,56 @@ void sparse_plan(int64_t rows, int64_t Hkv, int64_t ps, int64_t top, int* per, i
 
 }  // namespace
 
-void launch_attn_select(const SelectArgs& a, hipStream_t s) {
-    const unsigned heads = unsigned(a.c.rows * a.c.Hkv);
-    if (a.c.max_pages > a.top) {
-        const dim3 grid(heads, unsigned((a.c.max_pages + 255) / 256));
-        if (a.c.Dh == 256)
-            hipLaunchKernelGGL(page_scores_kernel<256>, grid, dim3(256), 0, s, a);
-        else
-            hipLaunchKernelGGL(page_scores_kernel<128>, grid, dim3(256), 0, s, a);
+namespace {
+constexpr int kSelectFused = 1024;  // pages: RT rows' keys are at most 32 KB of shared memory
+
+template <int DH, int GP, int RT>
+void select_rows(const SelectArgs& a, hipStream_t s) {
+    const PagedRows& c = a.c;
+    const unsigned tiles = unsigned((c.rows + RT - 1) / RT * c.Hkv), heads = unsigned(c.rows * c.Hkv);
+    if (c.max_pages <= kSelectFused) {
+        hipLaunchKernelGGL((select_pages_kernel<DH, GP, RT>), dim3(tiles), dim3(256), size_t(RT) * c.max_pages * 8, s, a);
+        return;
     }
-    hipLaunchKernelGGL(page_select_kernel, dim3(heads), dim3(64), 0, s, a);
+    // a workgroup's four waves take 64 pages each at a time; about four workgroups per CU
+    const unsigned most = unsigned((c.max_pages + 255) / 256), ranges = std::min(most, std::max(1u, 1024 / tiles));
+    hipLaunchKernelGGL((page_scores_kernel<DH, GP, RT>), dim3(tiles, ranges), dim3(256), 0, s, a);
+    if (c.max_pages <= 4096)
+        hipLaunchKernelGGL(choose_pages_kernel<256>, dim3(heads), dim3(256), 0, s, a);
+    else if (c.max_pages <= 16384)
+        hipLaunchKernelGGL(choose_pages_kernel<1024>, dim3(heads), dim3(1024), 0, s, a);
+    else
+        hipLaunchKernelGGL(choose_pages_long_kernel, dim3(heads), dim3(1024), 0, s, a);
+}
+
+// rows without row_seq belong to sequences of their own and share no page;
+// others are taken in tiles
+template <int DH, int GP>
+void select_group(const SelectArgs& a, hipStream_t s) {
+    constexpr int RT = GP == 8 ? 2 : 4;
+    if (a.c.row_seq && a.c.rows > 1)
+        select_rows<DH, GP, RT>(a, s);
+    else
+        select_rows<DH, GP, 1>(a, s);
+}
+
+template <int DH>
+void select_heads(const SelectArgs& a, hipStream_t s) {
+    switch (a.Hq / a.c.Hkv) {
+        case 1: select_group<DH, 1>(a, s); break;
+        case 2: select_group<DH, 2>(a, s); break;
+        case 3:
+        case 4: select_group<DH, 4>(a, s); break;
+        default: select_group<DH, 8>(a, s); break;
+    }
+}
+}  // namespace
+
+void launch_attn_select(const SelectArgs& a, hipStream_t s) {
+    if (a.c.Dh == 256)
+        select_heads<256>(a, s);
+    else
+        select_heads<128>(a, s);
 }
 
 int64_t attn_sparse_work_bytes(int64_t rows, int64_t Hq, int64_t Hkv, int64_t Dh, int64_t page_size, int64_t top) {
