@@ -45,6 +45,10 @@ __device__ __forceinline__ uint64_t score_key(double s) {
     return b < 0 ? ~uint64_t(b) : uint64_t(b) | (uint64_t(1) << 63);
 }
 
+// roundf(x) for |x| < 2^22 in three instructions: 0.5 less half an ulp carries
+// exactly the values whose nearest integer (halves away from zero) is one more
+__device__ __forceinline__ int round_code(float x) { return int(x + __builtin_copysignf(0.49999997f, x)); }
+
 template <int CTRL>
 __device__ __forceinline__ double max_with(double v) {  // with a lane of the same 16
     const int2 x = __builtin_bit_cast(int2, v);
@@ -52,58 +56,76 @@ __device__ __forceinline__ double max_with(double v) {  // with a lane of the sa
     return fmax(v, __builtin_bit_cast(double, y));
 }
 
-// The scores of pages 64 k, k = first, first + stride, ..., for rows r0 .. r0 +
-// RT - 1 and K/V head g, by one wave; store(row, page, key) for every page the
-// row sees, of the rows that see more than `top`.
+// maximum over the wave (in scalar registers)
+__device__ __forceinline__ uint32_t wave_max(uint32_t x) {
+    x = max(x, uint32_t(__builtin_amdgcn_update_dpp(0, int(x), 0xB1, 0xF, 0xF, false)));   // quad_perm [1,0,3,2]
+    x = max(x, uint32_t(__builtin_amdgcn_update_dpp(0, int(x), 0x4E, 0xF, 0xF, false)));   // quad_perm [2,3,0,1]
+    x = max(x, uint32_t(__builtin_amdgcn_update_dpp(0, int(x), 0x141, 0xF, 0xF, false)));  // row_half_mirror
+    x = max(x, uint32_t(__builtin_amdgcn_update_dpp(0, int(x), 0x140, 0xF, 0xF, false)));  // row_mirror
+    return max(max(uint32_t(__builtin_amdgcn_readlane(int(x), 0)), uint32_t(__builtin_amdgcn_readlane(int(x), 16))),
+               max(uint32_t(__builtin_amdgcn_readlane(int(x), 32)), uint32_t(__builtin_amdgcn_readlane(int(x), 48))));
+}
+
+// The codes of RT rows' query heads, by the whole workgroup (a wave per head):
+// positive parts, then negative, as the pages' [max | -min] go.
+template <int DH, int GP, int RT>
+struct QueryCodes {
+    alignas(16) uint8_t q[RT * GP][2 * DH];
+    float step[RT * GP];
+};
+template <int DH, int GP, int RT>
+__device__ __forceinline__ void form_codes(const SelectArgs& a, int g, int r0, QueryCodes<DH, GP, RT>& qc) {
+    const int lane = threadIdx.x & 63, group = a.Hq / a.c.Hkv;
+#pragma unroll 1
+    for (int h = threadIdx.x >> 6; h < RT * GP; h += blockDim.x >> 6) {
+        const float* x = a.q_rot + (int64_t(min(r0 + h / GP, a.c.rows - 1)) * a.Hq + g * group + min(h % GP, group - 1)) * DH;
+        float v[DH / 64];
+        uint32_t most = 0;  // of the magnitudes' bits
+#pragma unroll
+        for (int m = 0; m < DH / 64; ++m) v[m] = x[lane + 64 * m];
+#pragma unroll
+        for (int m = 0; m < DH / 64; ++m) most = max(most, __float_as_uint(v[m]) & 0x7fffffffu);
+        const float d = __uint_as_float(wave_max(most)) / 127.f, id = d != 0.f ? 1.f / d : 0.f;
+#pragma unroll
+        for (int m = 0; m < DH / 64; ++m) {
+            const int code = round_code(v[m] * id);
+            qc.q[h][lane + 64 * m] = uint8_t(max(code, 0));
+            qc.q[h][DH + lane + 64 * m] = uint8_t(max(-code, 0));
+        }
+        if (lane == 0) qc.step[h] = round11(d);
+    }
+}
+
+// The scores of pages 64 k .., k = first, first + stride, ..., for rows r0 .. r0
+// + RT - 1 and K/V head g, by one wave; store(row, page, key) for every page the
+// row sees, of the rows that see more than `top`. Contains the workgroup's
+// barrier between forming the codes and using them.
 template <int DH, int GP, int RT, class Store>
-__device__ __forceinline__ void score_pages(const SelectArgs& a, int g, int r0, int first, int stride, Store store) {
-    constexpr int H = DH / 64, KS = 2 * H;  // 64-byte steps: [max | -min]
+__device__ __forceinline__ void score_pages(const SelectArgs& a, int g, int r0, int first, int stride, QueryCodes<DH, GP, RT>& qc, Store store) {
+    constexpr int KS = DH / 32;                           // 64-byte steps of [max | -min]
+    constexpr int TT = DH == 128 ? 4 : 2;                 // tiles of 16 pages in flight
+    constexpr int CG = RT > 1 ? 1 : GP == 8 ? 2 : TT;     // a lone row's repeated columns finish this many tiles at once
     const PagedRows& c = a.c;
-    const int lane = threadIdx.x & 63, g4 = lane >> 4, c16 = lane & 15, sub = c16 % GP, rt = c16 / GP;
-    const int group = a.Hq / c.Hkv, r = r0 + min(rt, RT - 1);
+    const int lane = threadIdx.x & 63, g4 = lane >> 4, c16 = lane & 15, sub = c16 % GP, rt = RT > 1 ? c16 / GP : 0, cg = c16 / GP % CG;
+    const int r = r0 + min(rt, RT - 1);
     int seq = -1, pos = -1;
     if (r < c.rows) pos = row_position(c, r, &seq);
     const int sees = pos < 0 ? 0 : pos / c.page_size + 1;
-    bool todo = rt < RT && sees > a.top;
+    bool todo = rt < RT && sees > a.top && c16 < GP * CG * RT;
+    int64_t id0 = -1;  // the first pages, before the codes are formed
+    if (RT == 1 && 64 * first + lane < sees && sees > a.top) id0 = pool_page(c, seq, 64 * first + lane);
+    form_codes<DH, GP, RT>(a, g, r0, qc);
+    __syncthreads();
     if (!__any(todo)) return;
 
-    // the column's codes: a head's 16 channels 64 s + 16 g4 .., positive parts, then negative
+    const int col = RT > 1 ? min(c16, RT * GP - 1) : sub;
     v4i_t q[KS];
-    double step;
-    {
-        const float* x = a.q_rot + (int64_t(min(r, c.rows - 1)) * a.Hq + g * group + min(sub, group - 1)) * DH + 16 * g4;
-        float v[H][16], amax = 0.f;
 #pragma unroll
-        for (int s = 0; s < H; ++s)
-#pragma unroll
-            for (int j = 0; j < 16; j += 4) {
-                const float4 f = *reinterpret_cast<const float4*>(x + 64 * s + j);
-                v[s][j] = f.x, v[s][j + 1] = f.y, v[s][j + 2] = f.z, v[s][j + 3] = f.w;
-            }
-#pragma unroll
-        for (int s = 0; s < H; ++s)
-#pragma unroll
-            for (int j = 0; j < 16; ++j) amax = fmaxf(amax, fabsf(v[s][j]));
-        amax = max_over_rows(amax);
-        const float d = amax / 127.f, id = d != 0.f ? 1.f / d : 0.f;
-        step = double(round11(d));
-#pragma unroll
-        for (int s = 0; s < H; ++s)
-#pragma unroll
-            for (int w = 0; w < 4; ++w) {
-                int up = 0, down = 0;
-#pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    const int code = int(roundf(v[s][4 * w + j] * id));
-                    up |= max(code, 0) << (8 * j);
-                    down |= max(-code, 0) << (8 * j);
-                }
-                q[s][w] = up;
-                q[H + s][w] = down;
-            }
-    }
-
-    const int64_t page_bytes = kv_summary_page_bytes(c.Hkv, DH), steps_at = int64_t(c.Hkv) * 2 * DH + 4 * g;
+    for (int s = 0; s < KS; ++s) q[s] = *reinterpret_cast<const v4i_t*>(&qc.q[col][64 * s + 16 * g4]);
+    const double step = double(qc.step[col]);
+    const int64_t page_bytes = kv_summary_page_bytes(c.Hkv, DH);
+    const uint8_t* const steps_at = c.summaries + int64_t(c.Hkv) * 2 * DH + 4 * g;
+    const uint8_t* const codes_at = c.summaries + int64_t(g) * 2 * DH + 16 * g4;
     while (const uint64_t left = __ballot(todo)) {  // the rows of one sequence at a time
         const int s0 = RT == 1 ? __builtin_amdgcn_readfirstlane(seq) : __shfl(seq, __ffsll((unsigned long long)left) - 1);
         const bool mine = todo && seq == s0;
@@ -112,41 +134,43 @@ __device__ __forceinline__ void score_pages(const SelectArgs& a, int g, int r0, 
             for (int off = 8; off > 0; off >>= 1) most = max(most, __shfl_xor(most, off));
         most = __builtin_amdgcn_readfirstlane(most);
         todo = todo && !mine;
+#pragma unroll 1
         for (int k = first; 64 * k < most; k += stride) {
             const int page = 64 * k + lane;
-            const int64_t id = page < most ? pool_page(c, s0, page) : -1;
-            const uint8_t* at = c.summaries + (id < 0 ? 0 : id) * page_bytes;  // page 0 for none: read, then ranked last
-            const float step_l = id < 0 ? __uint_as_float(0x7fc00000u) : *reinterpret_cast<const float*>(at + steps_at);
-            const int at_lo = int(reinterpret_cast<uintptr_t>(at)), at_hi = int(reinterpret_cast<uintptr_t>(at) >> 32);
-            constexpr int TT = DH == 128 ? 4 : 2;  // tiles of 16 pages in flight
-#pragma unroll
+            const int64_t id = RT == 1 && k == first ? id0 : page < most ? pool_page(c, s0, page) : -1;
+            const int id_l = id < 0 ? 0 : int(id);  // page 0 for none: read, then ranked last
+            const float step_l = id < 0 ? __uint_as_float(0x7fc00000u) : *reinterpret_cast<const float*>(steps_at + id * page_bytes);
+#pragma unroll 1
             for (int t0 = 0; t0 < 4; t0 += TT) {
                 if (64 * k + 16 * t0 >= most) break;
-                v4i_t b[TT][KS];
+                v4i_t b[TT][KS], sum[TT];
 #pragma unroll
                 for (int t = 0; t < TT; ++t) {
-                    const int from = 16 * (t0 + t) + c16;
-                    const uintptr_t p = uint32_t(__shfl(at_lo, from)) | uint64_t(uint32_t(__shfl(at_hi, from))) << 32;
-                    const v4i_t* src = reinterpret_cast<const v4i_t*>(p + int64_t(g) * 2 * DH + 16 * g4);
+                    const v4i_t* src = reinterpret_cast<const v4i_t*>(codes_at + int64_t(uint32_t(__shfl(id_l, 16 * (t0 + t) + c16))) * page_bytes);
 #pragma unroll
                     for (int s = 0; s < KS; ++s) b[t][s] = src[4 * s];
                 }
 #pragma unroll
                 for (int t = 0; t < TT; ++t) {
-                    v4i_t sum = {0, 0, 0, 0};
+                    sum[t] = v4i_t{0, 0, 0, 0};
 #pragma unroll
-                    for (int s = 0; s < KS; ++s) sum = __builtin_amdgcn_mfma_i32_16x16x64_i8(b[t][s], q[s], sum, 0, 0, 0);
+                    for (int s = 0; s < KS; ++s) sum[t] = __builtin_amdgcn_mfma_i32_16x16x64_i8(b[t][s], q[s], sum[t], 0, 0, 0);
+                }
+#pragma unroll
+                for (int t = 0; t < TT; t += CG)
 #pragma unroll
                     for (int i = 0; i < 4; ++i) {
-                        double s = double(sum[i]) * step;
+                        int x = sum[t][i];
+#pragma unroll
+                        for (int u = 1; u < CG; ++u) x = cg == u ? sum[t + u][i] : x;
+                        double s = double(x) * step;
                         if constexpr (GP >= 2) s = max_with<0xB1>(s);   // quad_perm [1,0,3,2]
                         if constexpr (GP >= 4) s = max_with<0x4E>(s);   // quad_perm [2,3,0,1]
                         if constexpr (GP >= 8) s = max_with<0x141>(s);  // row_half_mirror
-                        const int at_page = 16 * (t0 + t) + 4 * g4 + i;
+                        const int at_page = 16 * (t0 + t + cg) + 4 * g4 + i;
                         s *= double(__shfl(step_l, at_page));
                         if (mine && (GP >= 4 ? sub == i : (i & (GP - 1)) == sub) && 64 * k + at_page < sees) store(rt, 64 * k + at_page, score_key(s));
                     }
-                }
             }
         }
     }
@@ -155,71 +179,103 @@ __device__ __forceinline__ void score_pages(const SelectArgs& a, int g, int r0, 
 // NT lanes choose the pages of one (row, K/V head) that sees `sees` > top pages:
 // the first and last ones, and of the others the best by key, lane t holding
 // pages t, t + NT, ... (at most KPL). The smallest key that is taken is found
-// bit by bit, the upper 32 bits first; most searches end as soon as exactly
-// the wanted number of keys lies at or above.
+// two bits at a time, in the upper 32 bits from the first bit in which the keys
+// differ; most searches end there, as soon as exactly the wanted number of keys
+// lies at or above. Otherwise the lower 32 bits of those equal so far decide,
+// then the order of the pages. All of it is latency, of the counts and of
+// fetching the instructions, which run once or a few times: one search serves
+// both halves.
 struct SelectShared {
-    int count[2][16];
+    int count[3][4];  // of the waves together: this count's, the last one's, the next one's (zero)
+    uint32_t ends[2];
     int place[16 * 16];
 };
 template <int NT, int KPL>
 __device__ __forceinline__ void choose_pages(const uint64_t* keys, int sees, int top, int sink, int recent, int32_t* out, SelectShared* sh) {
     constexpr int NW = NT / 64;
     const int t = NT == 64 ? threadIdx.x & 63 : threadIdx.x, w = t >> 6, lane = t & 63;
-    const int lo_end = sink, hi_end = sees - recent, need = top - sink - recent;
-    uint32_t hi[KPL], lo[KPL];
+    int need = top - sink - recent;
+    uint32_t cur[KPL], lo[KPL];
+    uint32_t in = 0, open = 0;  // bit i: page NT i + t is taken; may be taken
 #pragma unroll
     for (int i = 0; i < KPL; ++i) {
         const int p = NT * i + t;
-        const uint64_t k = p >= lo_end && p < hi_end ? keys[p] : 0;
-        hi[i] = uint32_t(k >> 32);
+        const bool may = p >= sink && p < sees - recent;
+        const uint64_t k = keys[min(p, sees - 1)];
+        cur[i] = may ? uint32_t(k >> 32) : 0;
         lo[i] = uint32_t(k);
+        open |= may ? 1u << i : 0u;
+        in |= p < sees && !may ? 1u << i : 0u;
     }
     int turn = 0;
-    auto count = [&](auto pred) {
-        int n = 0;
-#pragma unroll
-        for (int i = 0; i < KPL; ++i)
-            if (NT * i < sees) n += __popcll(__ballot(pred(hi[i], lo[i])));
+    auto over_waves = [&](int (&n)[3]) {  // sums of the waves' counts
         if constexpr (NW > 1) {
-            if (lane == 0) sh->count[turn][w] = n;
+            if (lane < 3) atomicAdd(&sh->count[turn][lane], lane == 0 ? n[0] : lane == 1 ? n[1] : n[2]);
             __syncthreads();
-            n = 0;
-            for (int k = 0; k < NW; ++k) n += sh->count[turn][k];
-            turn ^= 1;
+            const int4 x = *reinterpret_cast<const int4*>(sh->count[turn]);
+            turn = turn == 2 ? 0 : turn + 1;
+            // the counters after the next ones were last read before this barrier
+            if (t < 4) sh->count[turn == 2 ? 0 : turn + 1][t] = 0;
+            n[0] = __builtin_amdgcn_readfirstlane(x.x), n[1] = __builtin_amdgcn_readfirstlane(x.y), n[2] = __builtin_amdgcn_readfirstlane(x.z);
         }
-        return n;
     };
-    uint32_t th = 0, tl = 0;
-    int equal = 0x7fffffff;  // how many of the keys equal to (th, tl) are taken
-    if (need > 0) {
-        bool exact = false;
-        for (int bit = 31; bit >= 0 && !exact; --bit) {
-            const uint32_t u = th | (1u << bit);
-            const int n = count([&](uint32_t h, uint32_t) { return h >= u; });
-            if (n >= need) th = u, exact = n == need;
-        }
-        if (!exact) {
-            const int rest = need - count([&](uint32_t h, uint32_t) { return h > th; });
-            for (int bit = 31; bit >= 0 && !exact; --bit) {
-                const uint32_t u = tl | (1u << bit);
-                const int n = count([&](uint32_t h, uint32_t l) { return h == th && l >= u; });
-                if (n >= rest) tl = u, exact = n == rest;
-            }
-            if (!exact) equal = rest - count([&](uint32_t h, uint32_t l) { return h == th && l > tl; });
-        }
-    } else {
-        th = tl = 0xffffffffu;
-        equal = 0;
+    uint32_t most = 0, least = 0;  // of the upper halves (least: inverted)
+#pragma unroll
+    for (int i = 0; i < KPL; ++i)
+        most = max(most, cur[i]), least = max(least, open >> i & 1 ? ~cur[i] : 0u);
+    uint32_t both[2] = {wave_max(most), wave_max(least)};
+    if constexpr (NW > 1) {
+        if (t < 12) sh->count[t / 4][t % 4] = 0;
+        if (t < 2) sh->ends[t] = 0;
+        __syncthreads();
+        if (lane < 2) atomicMax(&sh->ends[lane], lane ? both[1] : both[0]);
+        __syncthreads();
+        both[0] = __builtin_amdgcn_readfirstlane(sh->ends[0]), both[1] = __builtin_amdgcn_readfirstlane(sh->ends[1]);
     }
-    // ascending pages: (i, wave, lane). Equal keys first, if they are not all taken
-    const uint64_t below = (uint64_t(1) << lane) - 1;
-    auto ranked = [&](auto pred, auto use) {  // use(i, rank of this lane's page among those with pred)
-        int at = 0;
+    const uint32_t differ = both[0] ^ ~both[1];
+    int bits = differ ? (33 - __builtin_clz(differ)) & ~1 : 0;  // an even number
+    uint32_t th = bits == 32 ? 0 : both[0] >> bits << bits;
+#pragma unroll 1
+    for (int half = 0; half < 2 && need > 0; ++half) {
+        bool exact = false;
+#pragma unroll 1
+        while (bits > 0 && !exact) {  // the largest th with at least `need` keys at or above
+            bits -= 2;
+            int n[3] = {0, 0, 0};
+#pragma unroll
+            for (int i = 0; i < KPL; ++i)
+#pragma unroll
+                for (int v = 0; v < 3; ++v) n[v] += __popcll(__ballot(cur[i] >= (th | uint32_t(v + 1) << bits)));
+            over_waves(n);
+            const int v = n[2] >= need ? 3 : n[1] >= need ? 2 : n[0] >= need ? 1 : 0;
+            th |= uint32_t(v) << bits;
+            exact = (v == 3 ? n[2] : v == 2 ? n[1] : v == 1 ? n[0] : 0) == need;
+        }
+        int above[3] = {0, 0, 0};
+#pragma unroll
+        for (int i = 0; i < KPL; ++i) {
+            const bool up = (open >> i & 1) && (cur[i] > th || (exact && cur[i] == th));
+            above[0] += __popcll(__ballot(up));
+            const bool still = (open >> i & 1) && !up && cur[i] == th;
+            in |= up ? 1u << i : 0u;
+            open = (open & ~(1u << i)) | (still ? 1u << i : 0u);
+            cur[i] = still ? lo[i] : 0;
+        }
+        over_waves(above);
+        need -= above[0];
+        bits = 32;
+        th = 0;
+    }
+    // ascending pages are (i, wave, lane): each chosen page's place, and before it
+    // that of the equal keys, of which the first `need` are taken
+#pragma unroll 1
+    for (int last = need > 0 ? 0 : 1; last < 2; ++last) {
+        const uint32_t set = last ? in : open;
         if constexpr (NW > 1) {
             __syncthreads();
 #pragma unroll
             for (int i = 0; i < KPL; ++i) {
-                const int n = __popcll(__ballot(pred(i)));
+                const int n = __popcll(__ballot(set >> i & 1));
                 if (lane == 0) sh->place[i * NW + w] = n;
             }
             __syncthreads();
@@ -243,28 +299,21 @@ __device__ __forceinline__ void choose_pages(const uint64_t* keys, int sees, int
             }
             __syncthreads();
         }
+        int at = 0;
 #pragma unroll
         for (int i = 0; i < KPL; ++i) {
-            if (NT * i >= sees) break;
-            const uint64_t m = __ballot(pred(i));
+            const uint64_t m = __ballot(set >> i & 1);
             if constexpr (NW > 1) at = sh->place[i * NW + w];
-            use(i, at + __popcll(m & below));
+            const int place = at + __popcll(m & ((uint64_t(1) << lane) - 1));
+            if (set >> i & 1) {
+                if (last)
+                    out[place] = NT * i + t;
+                else if (place < need)
+                    in |= 1u << i;
+            }
             at += __popcll(m);
         }
-    };
-    uint32_t skip = 0;  // bit i: an equal key that is not taken
-    if (equal != 0x7fffffff)
-        ranked([&](int i) { return hi[i] == th && lo[i] == tl && NT * i + t >= lo_end && NT * i + t < hi_end; },
-               [&](int i, int rank) { skip |= rank >= equal ? 1u << i : 0u; });
-    auto taken = [&](int i) {
-        const int p = NT * i + t;
-        if (p >= sees) return false;
-        if (p < lo_end || p >= hi_end) return true;
-        return hi[i] > th || (hi[i] == th && (lo[i] > tl || (lo[i] == tl && !(skip >> i & 1))));
-    };
-    ranked(taken, [&](int i, int rank) {
-        if (taken(i)) out[rank] = NT * i + t;
-    });
+    }
 }
 
 // fewer pages than the list holds: all of them, -1 behind
@@ -278,37 +327,44 @@ __device__ __forceinline__ int row_sees(const PagedRows& c, int r) {
     return pos < 0 ? 0 : pos / c.page_size + 1;
 }
 
-// Up to 1024 pages: four waves score them for RT rows into shared memory, then
-// a wave per row chooses.
+// Up to 1024 pages: the waves of a workgroup score them for RT rows into shared
+// memory, then a wave per row chooses (a wave's counts need no barrier).
+template <int RT>
+constexpr int kSelThreads = RT == 1 ? 512 : 256;
 template <int DH, int GP, int RT>
-__global__ __launch_bounds__(256) void select_pages_kernel(SelectArgs a) {
+__global__ __launch_bounds__(kSelThreads<RT>, 4) void select_pages_kernel(SelectArgs a) {
     const PagedRows& c = a.c;
     const int w = threadIdx.x >> 6, g = blockIdx.x % c.Hkv, r0 = blockIdx.x / c.Hkv * RT;
     extern __shared__ __align__(16) uint64_t sel_keys[];  // [RT][max_pages]
-    score_pages<DH, GP, RT>(a, g, r0, w, 4, [&](int rt, int page, uint64_t k) { sel_keys[rt * c.max_pages + page] = k; });
+    __shared__ QueryCodes<DH, GP, RT> qc;
+    score_pages<DH, GP, RT>(a, g, r0, w, kSelThreads<RT> / 64, qc, [&](int rt, int page, uint64_t k) { sel_keys[rt * c.max_pages + page] = k; });
     __syncthreads();
-    for (int rt = w; rt < RT && r0 + rt < c.rows; rt += 4) {
-        int32_t* out = a.selected + (int64_t(r0 + rt) * c.Hkv + g) * a.top;
-        const int sees = row_sees(c, r0 + rt);
-        if (sees <= a.top)
-            list_all(out, sees, a.top, threadIdx.x & 63, 64);
-        else if (sees <= 256)
-            choose_pages<64, 4>(sel_keys + rt * c.max_pages, sees, a.top, a.sink, a.recent, out, nullptr);
-        else
-            choose_pages<64, 16>(sel_keys + rt * c.max_pages, sees, a.top, a.sink, a.recent, out, nullptr);
-    }
+    const int r = r0 + w;
+    if (w >= RT || r >= c.rows) return;
+    int32_t* out = a.selected + (int64_t(r) * c.Hkv + g) * a.top;
+    const uint64_t* keys = sel_keys + w * c.max_pages;
+    const int sees = row_sees(c, r);
+    if (sees <= a.top)
+        list_all(out, sees, a.top, threadIdx.x & 63, 64);
+    else if (sees <= 320)
+        choose_pages<64, 5>(keys, sees, a.top, a.sink, a.recent, out, nullptr);
+    else if (sees <= 512)
+        choose_pages<64, 8>(keys, sees, a.top, a.sink, a.recent, out, nullptr);
+    else
+        choose_pages<64, 16>(keys, sees, a.top, a.sink, a.recent, out, nullptr);
 }
 
 // More pages: scores to the workspace, a wave per 64 pages at a time ...
 template <int DH, int GP, int RT>
-__global__ __launch_bounds__(256) void page_scores_kernel(SelectArgs a) {
+__global__ __launch_bounds__(256, 4) void page_scores_kernel(SelectArgs a) {
     const PagedRows& c = a.c;
     const int w = threadIdx.x >> 6, g = blockIdx.x % c.Hkv, r0 = blockIdx.x / c.Hkv * RT;
-    score_pages<DH, GP, RT>(a, g, r0, blockIdx.y * 4 + w, gridDim.y * 4,
+    __shared__ QueryCodes<DH, GP, RT> qc;
+    score_pages<DH, GP, RT>(a, g, r0, blockIdx.y * 4 + w, gridDim.y * 4, qc,
                             [&](int rt, int page, uint64_t k) { a.keys[(int64_t(r0 + rt) * c.Hkv + g) * c.max_pages + page] = k; });
 }
-// ... then a workgroup per (row, K/V head) chooses among up to 16 NT pages
-template <int NT>
+// ... then a workgroup per (row, K/V head) chooses among up to KPL NT pages
+template <int NT, int KPL>
 __global__ __launch_bounds__(NT) void choose_pages_kernel(SelectArgs a) {
     const PagedRows& c = a.c;
     const int r = blockIdx.x / c.Hkv, g = blockIdx.x % c.Hkv;
@@ -318,7 +374,7 @@ __global__ __launch_bounds__(NT) void choose_pages_kernel(SelectArgs a) {
     if (sees <= a.top)
         list_all(out, sees, a.top, threadIdx.x, NT);
     else
-        choose_pages<NT, 16>(a.keys + (int64_t(r) * c.Hkv + g) * c.max_pages, sees, a.top, a.sink, a.recent, out, &sh);
+        choose_pages<NT, KPL>(a.keys + (int64_t(r) * c.Hkv + g) * c.max_pages, sees, a.top, a.sink, a.recent, out, &sh);
 }
 
 // any number of pages: the same search with the keys read again for every bit
@@ -816,16 +872,18 @@ void select_rows(const SelectArgs& a, hipStream_t s) {
     const PagedRows& c = a.c;
     const unsigned tiles = unsigned((c.rows + RT - 1) / RT * c.Hkv), heads = unsigned(c.rows * c.Hkv);
     if (c.max_pages <= kSelectFused) {
-        hipLaunchKernelGGL((select_pages_kernel<DH, GP, RT>), dim3(tiles), dim3(256), size_t(RT) * c.max_pages * 8, s, a);
+        hipLaunchKernelGGL((select_pages_kernel<DH, GP, RT>), dim3(tiles), dim3(kSelThreads<RT>), size_t(RT) * c.max_pages * 8, s, a);
         return;
     }
     // a workgroup's four waves take 64 pages each at a time; about four workgroups per CU
     const unsigned most = unsigned((c.max_pages + 255) / 256), ranges = std::min(most, std::max(1u, 1024 / tiles));
     hipLaunchKernelGGL((page_scores_kernel<DH, GP, RT>), dim3(tiles, ranges), dim3(256), 0, s, a);
-    if (c.max_pages <= 4096)
-        hipLaunchKernelGGL(choose_pages_kernel<256>, dim3(heads), dim3(256), 0, s, a);
+    if (c.max_pages <= 2048)
+        hipLaunchKernelGGL((choose_pages_kernel<256, 8>), dim3(heads), dim3(256), 0, s, a);
+    else if (c.max_pages <= 4096)
+        hipLaunchKernelGGL((choose_pages_kernel<512, 8>), dim3(heads), dim3(512), 0, s, a);
     else if (c.max_pages <= 16384)
-        hipLaunchKernelGGL(choose_pages_kernel<1024>, dim3(heads), dim3(1024), 0, s, a);
+        hipLaunchKernelGGL((choose_pages_kernel<1024, 16>), dim3(heads), dim3(1024), 0, s, a);
     else
         hipLaunchKernelGGL(choose_pages_long_kernel, dim3(heads), dim3(1024), 0, s, a);
 }
