@@ -134,10 +134,12 @@ __device__ __forceinline__ void score_pages(const SelectArgs& a, int g, int r0, 
             for (int off = 8; off > 0; off >>= 1) most = max(most, __shfl_xor(most, off));
         most = __builtin_amdgcn_readfirstlane(most);
         todo = todo && !mine;
+        auto page_of = [&](int k) { return 64 * k + lane < most ? pool_page(c, s0, 64 * k + lane) : int64_t(-1); };
+        int64_t next = RT == 1 ? id0 : page_of(first);
 #pragma unroll 1
         for (int k = first; 64 * k < most; k += stride) {
-            const int page = 64 * k + lane;
-            const int64_t id = RT == 1 && k == first ? id0 : page < most ? pool_page(c, s0, page) : -1;
+            const int64_t id = next;
+            next = page_of(k + stride);
             const int id_l = id < 0 ? 0 : int(id);  // page 0 for none: read, then ranked last
             const float step_l = id < 0 ? __uint_as_float(0x7fc00000u) : *reinterpret_cast<const float*>(steps_at + id * page_bytes);
 #pragma unroll 1
@@ -327,8 +329,11 @@ __device__ __forceinline__ int row_sees(const PagedRows& c, int r) {
     return pos < 0 ? 0 : pos / c.page_size + 1;
 }
 
-// Up to 1024 pages: the waves of a workgroup score them for RT rows into shared
-// memory, then a wave per row chooses (a wave's counts need no barrier).
+// The waves of a workgroup score up to 512 (a lone row) or 1024 pages for RT rows
+// into shared memory, then a wave per row chooses: its counts need no barrier.
+// Longer lists of a lone row are faster over many workgroups in two launches:
+// 1000 pages 12 against 15 us, 4000 pages 15 against 40 us (one sequence; the
+// same times for sixteen).
 template <int RT>
 constexpr int kSelThreads = RT == 1 ? 512 : 256;
 template <int DH, int GP, int RT>
@@ -346,11 +351,11 @@ __global__ __launch_bounds__(kSelThreads<RT>, 4) void select_pages_kernel(Select
     const int sees = row_sees(c, r);
     if (sees <= a.top)
         list_all(out, sees, a.top, threadIdx.x & 63, 64);
-    else if (sees <= 320)
+    else if (RT > 1 && sees <= 320)
         choose_pages<64, 5>(keys, sees, a.top, a.sink, a.recent, out, nullptr);
-    else if (sees <= 512)
+    else if (RT == 1 || sees <= 512)
         choose_pages<64, 8>(keys, sees, a.top, a.sink, a.recent, out, nullptr);
-    else
+    else if constexpr (RT > 1)
         choose_pages<64, 16>(keys, sees, a.top, a.sink, a.recent, out, nullptr);
 }
 
@@ -865,22 +870,18 @@ void sparse_plan(int64_t rows, int64_t Hkv, int64_t ps, int64_t top, int* per, i
 }  // namespace
 
 namespace {
-constexpr int kSelectFused = 1024;  // pages: RT rows' keys are at most 32 KB of shared memory
-
 template <int DH, int GP, int RT>
 void select_rows(const SelectArgs& a, hipStream_t s) {
     const PagedRows& c = a.c;
     const unsigned tiles = unsigned((c.rows + RT - 1) / RT * c.Hkv), heads = unsigned(c.rows * c.Hkv);
-    if (c.max_pages <= kSelectFused) {
+    if (c.max_pages <= (RT == 1 ? 512 : 1024)) {
         hipLaunchKernelGGL((select_pages_kernel<DH, GP, RT>), dim3(tiles), dim3(kSelThreads<RT>), size_t(RT) * c.max_pages * 8, s, a);
         return;
     }
     // a workgroup's four waves take 64 pages each at a time; about four workgroups per CU
     const unsigned most = unsigned((c.max_pages + 255) / 256), ranges = std::min(most, std::max(1u, 1024 / tiles));
     hipLaunchKernelGGL((page_scores_kernel<DH, GP, RT>), dim3(tiles, ranges), dim3(256), 0, s, a);
-    if (c.max_pages <= 2048)
-        hipLaunchKernelGGL((choose_pages_kernel<256, 8>), dim3(heads), dim3(256), 0, s, a);
-    else if (c.max_pages <= 4096)
+    if (c.max_pages <= 4096)
         hipLaunchKernelGGL((choose_pages_kernel<512, 8>), dim3(heads), dim3(512), 0, s, a);
     else if (c.max_pages <= 16384)
         hipLaunchKernelGGL((choose_pages_kernel<1024, 16>), dim3(heads), dim3(1024), 0, s, a);
