@@ -14,7 +14,8 @@
 // pool, so the summary needs no second launch, no atomics and nothing kept
 // from earlier calls. The chain of a row's squares is as long as the row (one
 // dependent add per channel); lanes of one wave run the chains of up to 64
-// rows side by side.
+// rows side by side. Everything else is 32 lanes per row, four neighbouring
+// channels each, so that a row is read and written in whole words.
 #include "hero/device.hpp"
 #include "hero/kernels.hpp"
 #include "hero/paged.hpp"
@@ -23,8 +24,7 @@ namespace hero {
 
 namespace {
 
-constexpr int kApRows = 64;  // rows per pass of the K/V part
-constexpr int kApQ = 32;     // (row, query head) items per workgroup of the q part
+constexpr int kApRows = 64;  // rows (of the K/V part) or (row, query head) items a pass
 
 // x rounded to fp32 by whatever formed it, then to fp16 (the compiler may not
 // round a product to fp16 at once)
@@ -36,14 +36,31 @@ __device__ __forceinline__ uint16_t f16_bits(float x) {
     return b;
 }
 
-// quantize_row_q8_0 of a 32-value block held one value per lane by 32 lanes
-__device__ __forceinline__ int q8_code(float x, uint16_t* dh) {
-    float amax = fabsf(x);
-    for (int off = 16; off > 0; off >>= 1) amax = fmaxf(amax, __shfl_xor(amax, off, 32));
+__device__ __forceinline__ float4 load4(const float* p) {  // at any float's address
+    float4 v;
+    __builtin_memcpy(&v, p, 16);
+    return v;
+}
+
+// roundf(x) for |x| < 2^22: 0.5 less half an ulp carries exactly the values
+// whose nearest integer (halves away from zero) is one more
+__device__ __forceinline__ int round_code(float x) { return int(x + __builtin_copysignf(0.49999997f, x)); }
+
+// quantize_row_q8_0 of a 32-value block held four values per lane by 8 lanes:
+// the four codes packed; *dh the block's fp16 step
+__device__ __forceinline__ uint32_t q8_codes(const float (&x)[4], uint16_t* dh) {
+    float amax = fmaxf(fmaxf(fabsf(x[0]), fabsf(x[1])), fmaxf(fabsf(x[2]), fabsf(x[3])));
+    auto with = [](float v, int bits) { return fmaxf(v, __int_as_float(bits)); };
+    amax = with(amax, __builtin_amdgcn_update_dpp(0, __float_as_int(amax), 0xB1, 0xF, 0xF, false));   // quad_perm [1,0,3,2]
+    amax = with(amax, __builtin_amdgcn_update_dpp(0, __float_as_int(amax), 0x4E, 0xF, 0xF, false));   // quad_perm [2,3,0,1]
+    amax = with(amax, __builtin_amdgcn_update_dpp(0, __float_as_int(amax), 0x141, 0xF, 0xF, false));  // row_half_mirror
     const float d = amax / 127.f;
     const float id = d != 0.f ? 1.f / d : 0.f;
     *dh = fp32_to_fp16_ref(d);
-    return int(int8_t(int(roundf(x * id))));
+    uint32_t w = 0;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) w |= uint32_t(round_code(x[k] * id) & 0xFF) << (8 * k);
+    return w;
 }
 
 // 1 / rms of a row of DH values in shared memory, squares added in order
@@ -62,67 +79,95 @@ __device__ __forceinline__ float row_scale(const float* row, float eps) {
     return 1.f / sqrtf(ss / float(DH) + eps);
 }
 
-// norm and rotation of a row held by 32 lanes, lane l channels l + 32 m
+// A head's weights and rotation for lane l of 32: channels 4 l + 128 m + k and
+// their partners, half a head away (the same lane's for 256 channels)
 template <int DH>
-__device__ __forceinline__ void norm_rotate(const float* row, const float* gamma, float scale, const float* cs, int l, float (&y)[DH / 32]) {
-    float n[DH / 32];
+struct HeadLane {
+    float g[2][4];  // of the lane's channels, and of their partners (DH 128) or channels + 128 (DH 256)
+    __device__ __forceinline__ HeadLane(const float* gamma, int l) {
+        const int a = 4 * l, b = DH == 128 ? (4 * l + 64) & 127 : 4 * l + 128;
 #pragma unroll
-    for (int m = 0; m < DH / 32; ++m) n[m] = gamma[l + 32 * m] * row[l + 32 * m] * scale;
-#pragma unroll
-    for (int m = 0; m < DH / 64; ++m) {
-        const float2 t = reinterpret_cast<const float2*>(cs)[l + 32 * m];
-        const float xx = n[m], yy = n[m + DH / 64];
-        y[m] = xx * t.x - yy * t.y;
-        y[m + DH / 64] = yy * t.x + xx * t.y;
+        for (int k = 0; k < 4; ++k) g[0][k] = gamma[a + k], g[1][k] = gamma[b + k];
     }
-}
+    // norm and rotation of a row in shared memory; cs: the position's (cos, sin) per plane
+    __device__ __forceinline__ void rotate(const float* row, float scale, const float* cs, int l, float (&y)[DH / 128][4]) const {
+        const int a = 4 * l, b = DH == 128 ? (4 * l + 64) & 127 : 4 * l + 128;
+        const float4 xa = *reinterpret_cast<const float4*>(row + a), xb = *reinterpret_cast<const float4*>(row + b);
+        const float4* c4 = reinterpret_cast<const float4*>(cs + 2 * (a % (DH / 2)));
+        const float4 c0 = c4[0], c1 = c4[1];
+        const float na[4] = {g[0][0] * xa.x * scale, g[0][1] * xa.y * scale, g[0][2] * xa.z * scale, g[0][3] * xa.w * scale};
+        const float nb[4] = {g[1][0] * xb.x * scale, g[1][1] * xb.y * scale, g[1][2] * xb.z * scale, g[1][3] * xb.w * scale};
+        const float co[4] = {c0.x, c0.z, c1.x, c1.z}, si[4] = {c0.y, c0.w, c1.y, c1.w};
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            if constexpr (DH == 128) {  // (lo, hi) = (own, partner) for the lower half's lanes, else the other way
+                y[0][k] = l < 16 ? na[k] * co[k] - nb[k] * si[k] : na[k] * co[k] + nb[k] * si[k];
+            } else {
+                y[0][k] = na[k] * co[k] - nb[k] * si[k];
+                y[DH / 128 - 1][k] = nb[k] * co[k] + na[k] * si[k];
+            }
+        }
+    }
+};
 
-template <int DH, bool Q8>
-__global__ __launch_bounds__(256) void kv_append_kernel(KvAppendArgs a, int kv_blocks) {
-    constexpr int M = DH / 32, kStride = DH + 4;
-    constexpr int kBuf = kApRows * kStride > 16 * DH ? kApRows * kStride : 16 * DH;
+// NT lanes; a workgroup of the K/V part works off the runs that start in its
+// ROWS rows. Rows that come one per sequence: 256 lanes, one row. Chunks: 512
+// lanes (a page's 64 rows are four turns of the 16 half-waves), eight rows, so
+// that few workgroups are launched for nothing (of 1000 rows' 8000, most of
+// which start no run, the launching alone took 50 us).
+template <int DH, bool Q8, int NT, int ROWS>
+__global__ __launch_bounds__(NT) void kv_append_kernel(KvAppendArgs a, int kv_blocks, int q_items) {
+    constexpr int V = DH / 128, kStride = DH + 4, HW = NT / 32;
+    constexpr int kBuf = kApRows * kStride > HW * 2 * DH ? kApRows * kStride : HW * 2 * DH;
     const PagedRows& c = a.c;
     const int tid = threadIdx.x, hw = tid >> 5, l = tid & 31;
     __shared__ __align__(16) float buf[kBuf];
     __shared__ float scale[kApRows];
+    __shared__ int run;
     if (int(blockIdx.x) >= kv_blocks) {  // queries
-        const int64_t items = int64_t(c.rows) * a.Hq, i0 = int64_t(blockIdx.x - kv_blocks) * kApQ;
-        const int n = int(min(int64_t(kApQ), items - i0));
-        for (int e = tid; e < n * DH; e += 256) {
-            const int64_t it = i0 + e / DH;
-            buf[(e / DH) * kStride + e % DH] = a.proj[it / a.Hq * a.proj_stride + it % a.Hq * 2 * DH + e % DH];
+        const int64_t items = int64_t(c.rows) * a.Hq, i0 = int64_t(blockIdx.x - kv_blocks) * q_items;
+        const int n = int(min(int64_t(q_items), items - i0));
+        for (int e = tid; e < n * (DH / 4); e += NT) {
+            const int64_t it = i0 + e / (DH / 4);
+            *reinterpret_cast<float4*>(buf + (e / (DH / 4)) * kStride + e % (DH / 4) * 4) = load4(a.proj + it / a.Hq * a.proj_stride + it % a.Hq * 2 * DH + e % (DH / 4) * 4);
         }
+        const HeadLane<DH> lane(a.q_gamma, l);
         __syncthreads();
         if (tid < n) scale[tid] = row_scale<DH>(buf + tid * kStride, a.eps);
         __syncthreads();
-        for (int i = hw; i < n; i += 8) {
+        for (int i = hw; i < n; i += HW) {
             const int64_t it = i0 + i;
             int seq;
             const int pos = row_position(c, int(it / a.Hq), &seq);
             if (pos < 0 || pos >= a.rope_positions) continue;
-            float y[M];
-            norm_rotate<DH>(buf + i * kStride, a.q_gamma, scale[i], a.rope_cs + int64_t(pos) * DH, l, y);
+            float y[V][4];
+            lane.rotate(buf + i * kStride, scale[i], a.rope_cs + int64_t(pos) * DH, l, y);
 #pragma unroll
-            for (int m = 0; m < M; ++m) a.q_rot[it * DH + l + 32 * m] = y[m];
+            for (int v = 0; v < V; ++v) *reinterpret_cast<float4*>(a.q_rot + it * DH + 128 * v + 4 * l) = make_float4(y[v][0], y[v][1], y[v][2], y[v][3]);
         }
         return;
     }
-    const int r0 = blockIdx.x / c.Hkv, g = blockIdx.x % c.Hkv, ps = c.page_size;
-    int seq, prev_seq;
-    const int pos = row_position(c, r0, &seq);
-    if (pos < 0 || pos >= a.rope_positions) return;
-    const int slot0 = pos % ps;
-    if (r0 > 0 && slot0 > 0) {  // inside the run of an earlier row
-        const int prev = row_position(c, r0 - 1, &prev_seq);
-        if (prev == pos - 1 && prev_seq == seq) return;
+    const int g = blockIdx.x % c.Hkv, ps = c.page_size, first = int(blockIdx.x / c.Hkv) * ROWS;
+    // which of this workgroup's rows start a run: a lane each
+    const HeadLane<DH> lane(a.k_gamma, l);
+    bool starts = false;
+    if (const int r = first + (tid & 63); (tid & 63) < ROWS && r < c.rows) {
+        int s, before;
+        const int p = row_position(c, r, &s);
+        starts = p >= 0 && p < a.rope_positions && !(r > 0 && p % ps > 0 && row_position(c, r - 1, &before) == p - 1 && before == s);
     }
+    for (uint64_t left = __ballot(starts); left; left &= left - 1) {
+    const int r0 = first + __ffsll((unsigned long long)left) - 1;
+    int seq;
+    const int pos = row_position(c, r0, &seq), slot0 = pos % ps;
     const int64_t page = pool_page(c, seq, pos / ps);
-    if (page < 0) return;
+    if (page < 0) continue;
     // the run: rows r0 + i at pos + i in this page
-    __shared__ int run;
-    if (tid == 0) run = min(ps - slot0, c.rows - r0);
+    const int room = min(ps - slot0, c.rows - r0);
     __syncthreads();
-    if (tid > 0 && tid < ps - slot0 && r0 + tid < c.rows) {
+    if (tid == 0) run = room;
+    __syncthreads();
+    if (tid > 0 && tid < room) {
         int s2;
         const int p2 = row_position(c, r0 + tid, &s2);
         if (p2 != pos + tid || s2 != seq || p2 >= a.rope_positions) atomicMin(&run, tid);
@@ -130,79 +175,104 @@ __global__ __launch_bounds__(256) void kv_append_kernel(KvAppendArgs a, int kv_b
     __syncthreads();
     const int n = run;
 
-    float hi[M], lo[M];
+    float hi[V][4], lo[V][4];
 #pragma unroll
-    for (int m = 0; m < M; ++m) hi[m] = -INFINITY, lo[m] = INFINITY;
-    auto bound = [&](int m, float x) {
-        hi[m] = fmaxf(hi[m], x);
-        lo[m] = fminf(lo[m], x);
+    for (int v = 0; v < V; ++v)
+#pragma unroll
+        for (int k = 0; k < 4; ++k) hi[v][k] = -INFINITY, lo[v][k] = INFINITY;
+    auto bound = [&](int v, int k, float x) {
+        hi[v][k] = fmaxf(hi[v][k], x);
+        lo[v][k] = fminf(lo[v][k], x);
     };
     uint16_t* const fpage = const_cast<uint16_t*>(reinterpret_cast<const uint16_t*>(f16_page<DH>(c, page)));
     uint8_t* const qpage = q8_page<DH>(c, page);
     uint16_t* const qscales = reinterpret_cast<uint16_t*>(qpage + q8_scales_at<DH>(c));
-    for (int t = hw; t < slot0; t += 8) {  // keys of earlier calls
-        const int64_t row = page_row_index(c, 0, g, t);
-#pragma unroll
-        for (int m = 0; m < M; ++m) {
-            if constexpr (Q8)
-                bound(m, half_bits_to_f32(qscales[row * M + m]) * float(int8_t(qpage[row * DH + l + 32 * m])));
-            else
-                bound(m, half_bits_to_f32(fpage[row * DH + l + 32 * m]));
-        }
-    }
     for (int c0 = 0; c0 < n; c0 += kApRows) {
         const int nr = min(kApRows, n - c0);
-        __syncthreads();
-        for (int e = tid; e < nr * DH; e += 256)
-            buf[(e / DH) * kStride + e % DH] = a.proj[int64_t(r0 + c0 + e / DH) * a.proj_stride + a.k_off + int64_t(g) * DH + e % DH];
+        const float* rows = a.proj + int64_t(r0 + c0) * a.proj_stride + int64_t(g) * DH;
+        if (c0 > 0) __syncthreads();
+        for (int e = tid; e < nr * (DH / 4); e += NT)
+            *reinterpret_cast<float4*>(buf + (e / (DH / 4)) * kStride + e % (DH / 4) * 4) = load4(rows + int64_t(e / (DH / 4)) * a.proj_stride + a.k_off + e % (DH / 4) * 4);
+        if (c0 == 0) {  // keys of earlier calls
+            for (int t = hw; t < slot0; t += HW) {
+                const int64_t row = page_row_index(c, 0, g, t);
+#pragma unroll
+                for (int v = 0; v < V; ++v) {
+                    if constexpr (Q8) {
+                        const uint32_t q = *reinterpret_cast<const uint32_t*>(qpage + row * DH + 4 * l);
+                        const float d = half_bits_to_f32(qscales[row * 4 + l / 8]);
+#pragma unroll
+                        for (int k = 0; k < 4; ++k) bound(v, k, d * float(int8_t(q >> (8 * k))));
+                    } else {
+                        const ushort4 h = *reinterpret_cast<const ushort4*>(fpage + row * DH + 128 * v + 4 * l);
+                        bound(v, 0, half_bits_to_f32(h.x)), bound(v, 1, half_bits_to_f32(h.y)), bound(v, 2, half_bits_to_f32(h.z)), bound(v, 3, half_bits_to_f32(h.w));
+                    }
+                }
+            }
+        }
         __syncthreads();
         if (tid < nr) scale[tid] = row_scale<DH>(buf + tid * kStride, a.eps);
         __syncthreads();
-        for (int i = hw; i < nr; i += 8) {
+        for (int i = hw; i < nr; i += HW) {
             const int t = slot0 + c0 + i;
-            const float* v = a.proj + int64_t(r0 + c0 + i) * a.proj_stride + a.v_off + int64_t(g) * DH;
             const int64_t krow = page_row_index(c, 0, g, t), vrow = page_row_index(c, 1, g, t);
-            float y[M];
-            norm_rotate<DH>(buf + i * kStride, a.k_gamma, scale[i], a.rope_cs + int64_t(pos + c0 + i) * DH, l, y);
+            float x[V][4], y[V][4];
 #pragma unroll
-            for (int m = 0; m < M; ++m) {
-                const float vm = v[l + 32 * m];
+            for (int v = 0; v < V; ++v) {
+                const float4 f = load4(rows + int64_t(i) * a.proj_stride + a.v_off + 128 * v + 4 * l);
+                x[v][0] = f.x, x[v][1] = f.y, x[v][2] = f.z, x[v][3] = f.w;
+            }
+            lane.rotate(buf + i * kStride, scale[i], a.rope_cs + int64_t(pos + c0 + i) * DH, l, y);
+#pragma unroll
+            for (int v = 0; v < V; ++v) {
                 if constexpr (Q8) {
                     uint16_t dk, dv;
-                    const int qk = q8_code(y[m], &dk), qv = q8_code(vm, &dv);
-                    qpage[krow * DH + l + 32 * m] = uint8_t(qk);
-                    qpage[vrow * DH + l + 32 * m] = uint8_t(qv);
-                    if (l == 0) qscales[krow * M + m] = dk, qscales[vrow * M + m] = dv;
-                    bound(m, half_bits_to_f32(dk) * float(qk));
+                    const uint32_t qk = q8_codes(y[v], &dk), qv = q8_codes(x[v], &dv);
+                    *reinterpret_cast<uint32_t*>(qpage + krow * DH + 4 * l) = qk;
+                    *reinterpret_cast<uint32_t*>(qpage + vrow * DH + 4 * l) = qv;
+                    if (l % 8 == 0) qscales[krow * 4 + l / 8] = dk, qscales[vrow * 4 + l / 8] = dv;
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) bound(v, k, half_bits_to_f32(dk) * float(int8_t(qk >> (8 * k))));
                 } else {
-                    const uint16_t kb = f16_bits(y[m]);
-                    fpage[krow * DH + l + 32 * m] = kb;
-                    fpage[vrow * DH + l + 32 * m] = f16_bits(vm);
-                    bound(m, half_bits_to_f32(kb));
+                    const ushort4 kb = make_ushort4(f16_bits(y[v][0]), f16_bits(y[v][1]), f16_bits(y[v][2]), f16_bits(y[v][3]));
+                    *reinterpret_cast<ushort4*>(fpage + krow * DH + 128 * v + 4 * l) = kb;
+                    *reinterpret_cast<ushort4*>(fpage + vrow * DH + 128 * v + 4 * l) =
+                        make_ushort4(f16_bits(x[v][0]), f16_bits(x[v][1]), f16_bits(x[v][2]), f16_bits(x[v][3]));
+                    bound(v, 0, half_bits_to_f32(kb.x)), bound(v, 1, half_bits_to_f32(kb.y)), bound(v, 2, half_bits_to_f32(kb.z)), bound(v, 3, half_bits_to_f32(kb.w));
                 }
             }
         }
     }
-    // the eight half-waves' bounds, then the codes: lane j < DH channel j
+    // the half-waves' bounds, then the codes: lane j < DH channel j
     __syncthreads();
 #pragma unroll
-    for (int m = 0; m < M; ++m) buf[hw * 2 * DH + l + 32 * m] = hi[m], buf[hw * 2 * DH + DH + l + 32 * m] = lo[m];
+    for (int v = 0; v < V; ++v) {
+        *reinterpret_cast<float4*>(buf + hw * 2 * DH + 128 * v + 4 * l) = make_float4(hi[v][0], hi[v][1], hi[v][2], hi[v][3]);
+        *reinterpret_cast<float4*>(buf + hw * 2 * DH + DH + 128 * v + 4 * l) = make_float4(lo[v][0], lo[v][1], lo[v][2], lo[v][3]);
+    }
     __syncthreads();
     float mx = -INFINITY, mn = INFINITY;
-    if (tid < DH)
-        for (int w = 0; w < 8; ++w) mx = fmaxf(mx, buf[w * 2 * DH + tid]), mn = fminf(mn, buf[w * 2 * DH + DH + tid]);
-    float amax = tid < DH ? fmaxf(fabsf(mx), fabsf(mn)) : 0.f;
-    for (int off = 32; off > 0; off >>= 1) amax = fmaxf(amax, __shfl_xor(amax, off));
-    if ((tid & 63) == 0) scale[tid >> 6] = amax;
-    __syncthreads();
-    amax = fmaxf(fmaxf(scale[0], scale[1]), fmaxf(scale[2], scale[3]));
-    const float d = amax / 127.f, id = d != 0.f ? 1.f / d : 0.f;
-    uint8_t* sum = c.summaries + page * kv_summary_page_bytes(c.Hkv, DH);
     if (tid < DH) {
-        sum[int64_t(g) * 2 * DH + tid] = uint8_t(int8_t(int(roundf(mx * id))));
-        sum[int64_t(g) * 2 * DH + DH + tid] = uint8_t(int8_t(int(roundf(-mn * id))));
+#pragma unroll 8
+        for (int w = 0; w < HW; ++w) mx = fmaxf(mx, buf[w * 2 * DH + tid]), mn = fminf(mn, buf[w * 2 * DH + DH + tid]);
     }
-    if (tid == 0) reinterpret_cast<float*>(sum + int64_t(c.Hkv) * 2 * DH)[g] = round11(d);
+    if (tid < DH) {
+        float amax = fmaxf(fabsf(mx), fabsf(mn));
+        for (int off = 32; off > 0; off >>= 1) amax = fmaxf(amax, __shfl_xor(amax, off));
+        if ((tid & 63) == 0) scale[tid >> 6] = amax;
+    }
+    __syncthreads();
+    if (tid < DH) {
+        float amax = scale[0];
+#pragma unroll
+        for (int w = 1; w < DH / 64; ++w) amax = fmaxf(amax, scale[w]);
+        const float d = amax / 127.f, id = d != 0.f ? 1.f / d : 0.f;
+        uint8_t* sum = c.summaries + page * kv_summary_page_bytes(c.Hkv, DH);
+        sum[int64_t(g) * 2 * DH + tid] = uint8_t(round_code(mx * id));
+        sum[int64_t(g) * 2 * DH + DH + tid] = uint8_t(round_code(-mn * id));
+        if (tid == 0) reinterpret_cast<float*>(sum + int64_t(c.Hkv) * 2 * DH)[g] = round11(d);
+    }
+    }
 }
 
 // eight channels a lane: a row's K (or V, or bounds) of all heads is one
@@ -252,15 +322,26 @@ __global__ __launch_bounds__(256) void kv_read_kernel(KvReadArgs a) {
 
 }  // namespace
 
+namespace {
+template <int DH, bool Q8>
+void kv_append_typed(const KvAppendArgs& a, hipStream_t s) {
+    const int64_t kv = int64_t(a.c.rows) * a.c.Hkv, items = int64_t(a.c.rows) * a.Hq;
+    if (!a.c.row_seq || a.c.rows == 1) {  // runs of one row
+        hipLaunchKernelGGL((kv_append_kernel<DH, Q8, 256, 1>), dim3(unsigned(kv + (items + 15) / 16)), dim3(256), 0, s, a, int(kv), 16);
+    } else {
+        const int64_t some = int64_t(a.c.rows + 7) / 8 * a.c.Hkv;
+        hipLaunchKernelGGL((kv_append_kernel<DH, Q8, 512, 8>), dim3(unsigned(some + (items + kApRows - 1) / kApRows)), dim3(512), 0, s, a, int(some), kApRows);
+    }
+}
+}  // namespace
+
 void launch_kv_append(const KvAppendArgs& a, hipStream_t s) {
-    const int64_t kv = int64_t(a.c.rows) * a.c.Hkv, q = (int64_t(a.c.rows) * a.Hq + kApQ - 1) / kApQ;
-    const dim3 grid(unsigned(kv + q));
     if (a.c.Dh == 256)
-        hipLaunchKernelGGL((kv_append_kernel<256, false>), grid, dim3(256), 0, s, a, int(kv));
+        kv_append_typed<256, false>(a, s);
     else if (a.c.q8)
-        hipLaunchKernelGGL((kv_append_kernel<128, true>), grid, dim3(256), 0, s, a, int(kv));
+        kv_append_typed<128, true>(a, s);
     else
-        hipLaunchKernelGGL((kv_append_kernel<128, false>), grid, dim3(256), 0, s, a, int(kv));
+        kv_append_typed<128, false>(a, s);
 }
 
 namespace {
