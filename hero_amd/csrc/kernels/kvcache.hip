@@ -24,7 +24,7 @@ namespace hero {
 
 namespace {
 
-constexpr int kApRows = 64;  // rows (of the K/V part) or (row, query head) items a pass
+constexpr int kApSpread = 61;  // chunks: workgroups per K/V head
 
 // x rounded to fp32 by whatever formed it, then to fp16 (the compiler may not
 // round a product to fp16 at once)
@@ -89,15 +89,13 @@ struct HeadLane {
 #pragma unroll
         for (int k = 0; k < 4; ++k) g[0][k] = gamma[a + k], g[1][k] = gamma[b + k];
     }
-    // norm and rotation of a row in shared memory; cs: the position's (cos, sin) per plane
-    __device__ __forceinline__ void rotate(const float* row, float scale, const float* cs, int l, float (&y)[DH / 128][4]) const {
-        const int a = 4 * l, b = DH == 128 ? (4 * l + 64) & 127 : 4 * l + 128;
-        const float4 xa = *reinterpret_cast<const float4*>(row + a), xb = *reinterpret_cast<const float4*>(row + b);
-        const float4* c4 = reinterpret_cast<const float4*>(cs + 2 * (a % (DH / 2)));
-        const float4 c0 = c4[0], c1 = c4[1];
+    // norm and rotation: the lane's own values x, its partners' in the row in
+    // shared memory, cs the (cos, sin) of its four planes
+    __device__ __forceinline__ void rotate(const float4 (&x)[DH / 128], const float* row, float scale, const float4 (&cs)[2], int l, float (&y)[DH / 128][4]) const {
+        const float4 xa = x[0], xb = DH == 128 ? *reinterpret_cast<const float4*>(row + ((4 * l + 64) & 127)) : x[DH / 128 - 1];
         const float na[4] = {g[0][0] * xa.x * scale, g[0][1] * xa.y * scale, g[0][2] * xa.z * scale, g[0][3] * xa.w * scale};
         const float nb[4] = {g[1][0] * xb.x * scale, g[1][1] * xb.y * scale, g[1][2] * xb.z * scale, g[1][3] * xb.w * scale};
-        const float co[4] = {c0.x, c0.z, c1.x, c1.z}, si[4] = {c0.y, c0.w, c1.y, c1.w};
+        const float co[4] = {cs[0].x, cs[0].z, cs[1].x, cs[1].z}, si[4] = {cs[0].y, cs[0].w, cs[1].y, cs[1].w};
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
             if constexpr (DH == 128) {  // (lo, hi) = (own, partner) for the lower half's lanes, else the other way
@@ -109,72 +107,23 @@ struct HeadLane {
         }
     }
 };
+template <int DH>
+__device__ __forceinline__ void load_cs(const float* rope_cs, int pos, int l, float4 (&cs)[2]) {
+    const float4* c4 = reinterpret_cast<const float4*>(rope_cs + int64_t(pos) * DH + 2 * (4 * l % (DH / 2)));
+    cs[0] = c4[0];
+    cs[1] = c4[1];
+}
 
-// NT lanes; a workgroup of the K/V part works off the runs that start in its
-// ROWS rows. Rows that come one per sequence: 256 lanes, one row. Chunks: 512
-// lanes (a page's 64 rows are four turns of the 16 half-waves), eight rows, so
-// that few workgroups are launched for nothing (of 1000 rows' 8000, most of
-// which start no run, the launching alone took 50 us).
-template <int DH, bool Q8, int NT, int ROWS>
-__global__ __launch_bounds__(NT) void kv_append_kernel(KvAppendArgs a, int kv_blocks, int q_items) {
-    constexpr int V = DH / 128, kStride = DH + 4, HW = NT / 32;
-    constexpr int kBuf = kApRows * kStride > HW * 2 * DH ? kApRows * kStride : HW * 2 * DH;
+// One K/V head of the run that starts in row r0, by the whole workgroup.
+template <int DH, bool Q8, int NT, int T>
+__device__ __forceinline__ void append_run(const KvAppendArgs& a, int g, int r0, const HeadLane<DH>& lane, float* buf, float* scale, int* run) {
+    constexpr int V = DH / 128, kStride = DH + 4, HW = NT / 32, kRows = HW * T;
     const PagedRows& c = a.c;
-    const int tid = threadIdx.x, hw = tid >> 5, l = tid & 31;
-    __shared__ __align__(16) float buf[kBuf];
-    __shared__ float scale[kApRows];
-    __shared__ int run;
-    if (int(blockIdx.x) >= kv_blocks) {  // queries
-        const int64_t items = int64_t(c.rows) * a.Hq, i0 = int64_t(blockIdx.x - kv_blocks) * q_items;
-        const int n = int(min(int64_t(q_items), items - i0));
-        for (int e = tid; e < n * (DH / 4); e += NT) {
-            const int64_t it = i0 + e / (DH / 4);
-            *reinterpret_cast<float4*>(buf + (e / (DH / 4)) * kStride + e % (DH / 4) * 4) = load4(a.proj + it / a.Hq * a.proj_stride + it % a.Hq * 2 * DH + e % (DH / 4) * 4);
-        }
-        const HeadLane<DH> lane(a.q_gamma, l);
-        __syncthreads();
-        if (tid < n) scale[tid] = row_scale<DH>(buf + tid * kStride, a.eps);
-        __syncthreads();
-        for (int i = hw; i < n; i += HW) {
-            const int64_t it = i0 + i;
-            int seq;
-            const int pos = row_position(c, int(it / a.Hq), &seq);
-            if (pos < 0 || pos >= a.rope_positions) continue;
-            float y[V][4];
-            lane.rotate(buf + i * kStride, scale[i], a.rope_cs + int64_t(pos) * DH, l, y);
-#pragma unroll
-            for (int v = 0; v < V; ++v) *reinterpret_cast<float4*>(a.q_rot + it * DH + 128 * v + 4 * l) = make_float4(y[v][0], y[v][1], y[v][2], y[v][3]);
-        }
-        return;
-    }
-    const int g = blockIdx.x % c.Hkv, ps = c.page_size, first = int(blockIdx.x / c.Hkv) * ROWS;
-    // which of this workgroup's rows start a run: a lane each
-    const HeadLane<DH> lane(a.k_gamma, l);
-    bool starts = false;
-    if (const int r = first + (tid & 63); (tid & 63) < ROWS && r < c.rows) {
-        int s, before;
-        const int p = row_position(c, r, &s);
-        starts = p >= 0 && p < a.rope_positions && !(r > 0 && p % ps > 0 && row_position(c, r - 1, &before) == p - 1 && before == s);
-    }
-    for (uint64_t left = __ballot(starts); left; left &= left - 1) {
-    const int r0 = first + __ffsll((unsigned long long)left) - 1;
+    const int tid = threadIdx.x, hw = tid >> 5, l = tid & 31, ps = c.page_size;
     int seq;
-    const int pos = row_position(c, r0, &seq), slot0 = pos % ps;
+    const int pos = row_position(c, r0, &seq), slot0 = pos % ps, room = min(ps - slot0, c.rows - r0);
     const int64_t page = pool_page(c, seq, pos / ps);
-    if (page < 0) continue;
-    // the run: rows r0 + i at pos + i in this page
-    const int room = min(ps - slot0, c.rows - r0);
-    __syncthreads();
-    if (tid == 0) run = room;
-    __syncthreads();
-    if (tid > 0 && tid < room) {
-        int s2;
-        const int p2 = row_position(c, r0 + tid, &s2);
-        if (p2 != pos + tid || s2 != seq || p2 >= a.rope_positions) atomicMin(&run, tid);
-    }
-    __syncthreads();
-    const int n = run;
-
+    if (page < 0) return;
     float hi[V][4], lo[V][4];
 #pragma unroll
     for (int v = 0; v < V; ++v)
@@ -187,12 +136,34 @@ __global__ __launch_bounds__(NT) void kv_append_kernel(KvAppendArgs a, int kv_bl
     uint16_t* const fpage = const_cast<uint16_t*>(reinterpret_cast<const uint16_t*>(f16_page<DH>(c, page)));
     uint8_t* const qpage = q8_page<DH>(c, page);
     uint16_t* const qscales = reinterpret_cast<uint16_t*>(qpage + q8_scales_at<DH>(c));
-    for (int c0 = 0; c0 < n; c0 += kApRows) {
-        const int nr = min(kApRows, n - c0);
-        const float* rows = a.proj + int64_t(r0 + c0) * a.proj_stride + int64_t(g) * DH;
-        if (c0 > 0) __syncthreads();
-        for (int e = tid; e < nr * (DH / 4); e += NT)
-            *reinterpret_cast<float4*>(buf + (e / (DH / 4)) * kStride + e % (DH / 4) * 4) = load4(rows + int64_t(e / (DH / 4)) * a.proj_stride + a.k_off + e % (DH / 4) * 4);
+    // the run: rows r0 + i at pos + i in this page
+    int n = 1;
+    if (NT > 256 || c.row_seq) {
+        __syncthreads();
+        if (tid == 0) *run = room;
+        __syncthreads();
+        if (tid > 0 && tid < room) {
+            int s2;
+            const int p2 = row_position(c, r0 + tid, &s2);
+            if (p2 != pos + tid || s2 != seq || p2 >= a.rope_positions) atomicMin(run, tid);
+        }
+        __syncthreads();
+        n = *run;
+    }
+    for (int c0 = 0; c0 < n; c0 += kRows) {
+        const int nr = min(kRows, n - c0);
+        const float* rows = a.proj + int64_t(r0 + c0) * a.proj_stride + int64_t(g) * DH + 4 * l;
+        float4 kx[T][V], vx[T][V], cs[T][2];
+#pragma unroll
+        for (int j = 0; j < T; ++j) {
+            const int i = min(hw + HW * j, nr - 1);
+#pragma unroll
+            for (int v = 0; v < V; ++v) {
+                kx[j][v] = load4(rows + int64_t(i) * a.proj_stride + a.k_off + 128 * v);
+                vx[j][v] = load4(rows + int64_t(i) * a.proj_stride + a.v_off + 128 * v);
+            }
+            load_cs<DH>(a.rope_cs, pos + c0 + i, l, cs[j]);
+        }
         if (c0 == 0) {  // keys of earlier calls
             for (int t = hw; t < slot0; t += HW) {
                 const int64_t row = page_row_index(c, 0, g, t);
@@ -211,23 +182,26 @@ __global__ __launch_bounds__(NT) void kv_append_kernel(KvAppendArgs a, int kv_bl
             }
         }
         __syncthreads();
+#pragma unroll
+        for (int j = 0; j < T; ++j)
+#pragma unroll
+            for (int v = 0; v < V; ++v) *reinterpret_cast<float4*>(buf + (hw + HW * j) * kStride + 128 * v + 4 * l) = kx[j][v];
+        __syncthreads();
         if (tid < nr) scale[tid] = row_scale<DH>(buf + tid * kStride, a.eps);
         __syncthreads();
-        for (int i = hw; i < nr; i += HW) {
-            const int t = slot0 + c0 + i;
+#pragma unroll
+        for (int j = 0; j < T; ++j) {
+            const int i = hw + HW * j, t = slot0 + c0 + i;
+            if (i >= nr) continue;
             const int64_t krow = page_row_index(c, 0, g, t), vrow = page_row_index(c, 1, g, t);
-            float x[V][4], y[V][4];
+            float y[V][4];
+            lane.rotate(kx[j], buf + i * kStride, scale[i], cs[j], l, y);
 #pragma unroll
             for (int v = 0; v < V; ++v) {
-                const float4 f = load4(rows + int64_t(i) * a.proj_stride + a.v_off + 128 * v + 4 * l);
-                x[v][0] = f.x, x[v][1] = f.y, x[v][2] = f.z, x[v][3] = f.w;
-            }
-            lane.rotate(buf + i * kStride, scale[i], a.rope_cs + int64_t(pos + c0 + i) * DH, l, y);
-#pragma unroll
-            for (int v = 0; v < V; ++v) {
+                const float x[4] = {vx[j][v].x, vx[j][v].y, vx[j][v].z, vx[j][v].w};
                 if constexpr (Q8) {
                     uint16_t dk, dv;
-                    const uint32_t qk = q8_codes(y[v], &dk), qv = q8_codes(x[v], &dv);
+                    const uint32_t qk = q8_codes(y[v], &dk), qv = q8_codes(x, &dv);
                     *reinterpret_cast<uint32_t*>(qpage + krow * DH + 4 * l) = qk;
                     *reinterpret_cast<uint32_t*>(qpage + vrow * DH + 4 * l) = qv;
                     if (l % 8 == 0) qscales[krow * 4 + l / 8] = dk, qscales[vrow * 4 + l / 8] = dv;
@@ -236,8 +210,7 @@ __global__ __launch_bounds__(NT) void kv_append_kernel(KvAppendArgs a, int kv_bl
                 } else {
                     const ushort4 kb = make_ushort4(f16_bits(y[v][0]), f16_bits(y[v][1]), f16_bits(y[v][2]), f16_bits(y[v][3]));
                     *reinterpret_cast<ushort4*>(fpage + krow * DH + 128 * v + 4 * l) = kb;
-                    *reinterpret_cast<ushort4*>(fpage + vrow * DH + 128 * v + 4 * l) =
-                        make_ushort4(f16_bits(x[v][0]), f16_bits(x[v][1]), f16_bits(x[v][2]), f16_bits(x[v][3]));
+                    *reinterpret_cast<ushort4*>(fpage + vrow * DH + 128 * v + 4 * l) = make_ushort4(f16_bits(x[0]), f16_bits(x[1]), f16_bits(x[2]), f16_bits(x[3]));
                     bound(v, 0, half_bits_to_f32(kb.x)), bound(v, 1, half_bits_to_f32(kb.y)), bound(v, 2, half_bits_to_f32(kb.z)), bound(v, 3, half_bits_to_f32(kb.w));
                 }
             }
@@ -255,8 +228,6 @@ __global__ __launch_bounds__(NT) void kv_append_kernel(KvAppendArgs a, int kv_bl
     if (tid < DH) {
 #pragma unroll 8
         for (int w = 0; w < HW; ++w) mx = fmaxf(mx, buf[w * 2 * DH + tid]), mn = fminf(mn, buf[w * 2 * DH + DH + tid]);
-    }
-    if (tid < DH) {
         float amax = fmaxf(fabsf(mx), fabsf(mn));
         for (int off = 32; off > 0; off >>= 1) amax = fmaxf(amax, __shfl_xor(amax, off));
         if ((tid & 63) == 0) scale[tid >> 6] = amax;
@@ -272,6 +243,73 @@ __global__ __launch_bounds__(NT) void kv_append_kernel(KvAppendArgs a, int kv_bl
         sum[int64_t(g) * 2 * DH + DH + tid] = uint8_t(round_code(-mn * id));
         if (tid == 0) reinterpret_cast<float*>(sum + int64_t(c.Hkv) * 2 * DH)[g] = round11(d);
     }
+}
+
+// NT lanes, T rows (or (row, query head) items) for each of their half-waves a
+// pass, everything a pass reads in flight before the chains run. Rows that come
+// one per sequence: 256 lanes, T = 1. Chunks: 512 lanes, T = 4, so that a page of
+// 64 positions is one pass. A workgroup of the K/V part works off the runs that
+// start in rows b, b + spread, ...: neighbouring rows of different sequences
+// go to different workgroups, and so do the pages of one chunk, whose starts
+// are a page size apart, as `spread` is odd; there are few of them, as most find no
+// start (one per row and head cost 50 us of launching alone at 1000 rows).
+template <int DH, bool Q8, int NT, int T>
+__global__ __launch_bounds__(NT, NT / 128) void kv_append_kernel(KvAppendArgs a, int spread) {
+    constexpr int V = DH / 128, kStride = DH + 4, HW = NT / 32, kRows = HW * T;
+    constexpr int kBuf = kRows * kStride > HW * 2 * DH ? kRows * kStride : HW * 2 * DH;
+    const PagedRows& c = a.c;
+    const int tid = threadIdx.x, hw = tid >> 5, l = tid & 31;
+    __shared__ __align__(16) float buf[kBuf];
+    __shared__ float scale[kRows];
+    __shared__ int run;
+    const int kv_blocks = spread * c.Hkv;
+    if (int(blockIdx.x) >= kv_blocks) {  // queries
+        const int64_t items = int64_t(c.rows) * a.Hq, i0 = int64_t(blockIdx.x - kv_blocks) * kRows;
+        const int n = int(min(int64_t(kRows), items - i0));
+        const HeadLane<DH> lane(a.q_gamma, l);
+        float4 x[T][V], cs[T][2];
+        int pos[T];
+#pragma unroll
+        for (int j = 0; j < T; ++j) {
+            const int64_t it = i0 + min(hw + HW * j, n - 1);
+            int seq;
+            pos[j] = row_position(c, int(it / a.Hq), &seq);
+            if (pos[j] >= a.rope_positions || hw + HW * j >= n) pos[j] = -1;
+            load_cs<DH>(a.rope_cs, max(pos[j], 0), l, cs[j]);
+            const float* q = a.proj + it / a.Hq * a.proj_stride + it % a.Hq * 2 * DH + 4 * l;
+#pragma unroll
+            for (int v = 0; v < V; ++v) x[j][v] = load4(q + 128 * v);
+        }
+#pragma unroll
+        for (int j = 0; j < T; ++j)
+#pragma unroll
+            for (int v = 0; v < V; ++v) *reinterpret_cast<float4*>(buf + (hw + HW * j) * kStride + 128 * v + 4 * l) = x[j][v];
+        __syncthreads();
+        if (tid < n) scale[tid] = row_scale<DH>(buf + tid * kStride, a.eps);
+        __syncthreads();
+#pragma unroll
+        for (int j = 0; j < T; ++j) {
+            if (pos[j] < 0) continue;
+            float y[V][4];
+            lane.rotate(x[j], buf + (hw + HW * j) * kStride, scale[hw + HW * j], cs[j], l, y);
+#pragma unroll
+            for (int v = 0; v < V; ++v)
+                *reinterpret_cast<float4*>(a.q_rot + (i0 + hw + HW * j) * DH + 128 * v + 4 * l) = make_float4(y[v][0], y[v][1], y[v][2], y[v][3]);
+        }
+        return;
+    }
+    const int g = blockIdx.x % c.Hkv, b = blockIdx.x / c.Hkv, ps = c.page_size;
+    const HeadLane<DH> lane(a.k_gamma, l);
+    for (int64_t first = b; first < c.rows; first += 64 * int64_t(spread)) {
+        // which of the next 64 rows start a run: a lane each
+        bool starts = false;
+        if (const int64_t r = first + int64_t(tid & 63) * spread; r < c.rows) {
+            int s, before;
+            const int p = row_position(c, int(r), &s);
+            starts = p >= 0 && p < a.rope_positions && !(r > 0 && p % ps > 0 && row_position(c, int(r) - 1, &before) == p - 1 && before == s);
+        }
+        for (uint64_t left = __ballot(starts); left; left &= left - 1)
+            append_run<DH, Q8, NT, T>(a, g, int(first + (__ffsll((unsigned long long)left) - 1) * int64_t(spread)), lane, buf, scale, &run);
     }
 }
 
@@ -323,15 +361,17 @@ __global__ __launch_bounds__(256) void kv_read_kernel(KvReadArgs a) {
 }  // namespace
 
 namespace {
+template <int DH, bool Q8, int NT, int T>
+void kv_append_sized(const KvAppendArgs& a, int spread, hipStream_t s) {
+    const int64_t per = NT / 32 * T, q = (int64_t(a.c.rows) * a.Hq + per - 1) / per;
+    hipLaunchKernelGGL((kv_append_kernel<DH, Q8, NT, T>), dim3(unsigned(int64_t(spread) * a.c.Hkv + q)), dim3(NT), 0, s, a, spread);
+}
 template <int DH, bool Q8>
 void kv_append_typed(const KvAppendArgs& a, hipStream_t s) {
-    const int64_t kv = int64_t(a.c.rows) * a.c.Hkv, items = int64_t(a.c.rows) * a.Hq;
-    if (!a.c.row_seq || a.c.rows == 1) {  // runs of one row
-        hipLaunchKernelGGL((kv_append_kernel<DH, Q8, 256, 1>), dim3(unsigned(kv + (items + 15) / 16)), dim3(256), 0, s, a, int(kv), 16);
-    } else {
-        const int64_t some = int64_t(a.c.rows + 7) / 8 * a.c.Hkv;
-        hipLaunchKernelGGL((kv_append_kernel<DH, Q8, 512, 8>), dim3(unsigned(some + (items + kApRows - 1) / kApRows)), dim3(512), 0, s, a, int(some), kApRows);
-    }
+    if (!a.c.row_seq || a.c.rows == 1)  // runs of one row
+        kv_append_sized<DH, Q8, 256, 1>(a, a.c.rows, s);
+    else
+        kv_append_sized<DH, Q8, 512, 4>(a, std::min(a.c.rows, kApSpread), s);
 }
 }  // namespace
 
