@@ -247,8 +247,8 @@ __device__ __forceinline__ void append_run(const KvAppendArgs& a, int g, int r0,
 
 // NT lanes, T rows (or (row, query head) items) for each of their half-waves a
 // pass, everything a pass reads in flight before the chains run. Rows that come
-// one per sequence: 256 lanes, T = 1. Chunks: 512 lanes, T = 4, so that a page of
-// 64 positions is one pass. A workgroup of the K/V part works off the runs that
+// one per sequence: 256 lanes, T = 1. Chunks: 512 lanes, T = 2: half a page of
+// 64 positions a pass (T = 4, a whole one, is 6% slower: fewer waves fit). A workgroup of the K/V part works off the runs that
 // start in rows b, b + spread, ...: neighbouring rows of different sequences
 // go to different workgroups, and so do the pages of one chunk, whose starts
 // are a page size apart, as `spread` is odd; there are few of them, as most find no
@@ -371,7 +371,7 @@ void kv_append_typed(const KvAppendArgs& a, hipStream_t s) {
     if (!a.c.row_seq || a.c.rows == 1)  // runs of one row
         kv_append_sized<DH, Q8, 256, 1>(a, a.c.rows, s);
     else
-        kv_append_sized<DH, Q8, 512, 4>(a, std::min(a.c.rows, kApSpread), s);
+        kv_append_sized<DH, Q8, 512, 2>(a, std::min(a.c.rows, kApSpread), s);
 }
 }  // namespace
 

@@ -836,24 +836,49 @@ __global__ __launch_bounds__(256) void attn_sparse_kernel(SparseAttnArgs a, int 
     }
 }
 
-// a workgroup per (row, query head), a lane per channel: the ranges' results
+// a workgroup per (row, query head), a lane per channel: the ranges' results,
+// their maxima and sums read once by a lane each
 template <int DH>
 __global__ __launch_bounds__(DH) void attn_sparse_combine_kernel(SparseAttnArgs a, int nsplit) {
-    const int r = blockIdx.x / a.Hq, h = blockIdx.x % a.Hq, ch = threadIdx.x;
+    constexpr int kRec = DH + 4, kPass = 16;
+    const int r = blockIdx.x / a.Hq, h = blockIdx.x % a.Hq, t = threadIdx.x;
     int seq;
     if (row_position(a.c, r, &seq) < 0) return;
-    const float* rec = a.work + (int64_t(r) * a.Hq + h) * nsplit * (DH + 4);
+    extern __shared__ float share[];  // [nsplit], a multiple of kPass: a range's share of the result, 0 behind
+    __shared__ float part[2][DH / 64];
+    const float* rec = a.work + (int64_t(r) * a.Hq + h) * nsplit * kRec;
+    const int padded = (nsplit + kPass - 1) / kPass * kPass;
+    auto over_waves = [&](float v, int k, auto f) {
+        for (int off = 32; off > 0; off >>= 1) v = f(v, __shfl_xor(v, off));
+        if ((t & 63) == 0) part[k][t >> 6] = v;
+        __syncthreads();
+        v = part[k][0];
+#pragma unroll
+        for (int w = 1; w < DH / 64; ++w) v = f(v, part[k][w]);
+        return v;
+    };
     float mx = -INFINITY;
-    for (int s = 0; s < nsplit; ++s) mx = fmaxf(mx, rec[s * (DH + 4)]);
-    float o = 0.f, l = 0.f;
-    for (int s = 0; s < nsplit; ++s) {
-        const float m = rec[s * (DH + 4)], ls = rec[s * (DH + 4) + 1];
-        if (m == -INFINITY && ls == 0.f) continue;
-        const float f = exp2_hw(m - mx);
-        l += f * ls;
-        o += f * rec[s * (DH + 4) + 4 + ch];
+    for (int s = t; s < nsplit; s += DH) mx = fmaxf(mx, rec[int64_t(s) * kRec]);
+    mx = over_waves(mx, 0, [](float x, float y) { return fmaxf(x, y); });
+    float l = 0.f;
+    for (int s = t; s < padded; s += DH) {
+        float f = 0.f;
+        if (s < nsplit) {
+            const float m = rec[int64_t(s) * kRec], ls = rec[int64_t(s) * kRec + 1];
+            if (m != -INFINITY || ls != 0.f) f = exp2_hw(m - mx), l += f * ls;  // a range without keys has neither
+        }
+        share[s] = f;
     }
-    sparse_store<DH>(a, r, h, ch, o, l);
+    l = over_waves(l, 1, [](float x, float y) { return x + y; });
+    float o = 0.f;
+    for (int s = 0; s < nsplit; s += kPass) {
+        float v[kPass];
+#pragma unroll
+        for (int k = 0; k < kPass; ++k) v[k] = rec[int64_t(min(s + k, nsplit - 1)) * kRec + 4 + t];
+#pragma unroll
+        for (int k = 0; k < kPass; ++k) o += share[s + k] * v[k];
+    }
+    sparse_store<DH>(a, r, h, t, o, l);
 }
 
 // Ranges of a row's list: about four workgroups per CU over all rows and heads,
@@ -941,9 +966,9 @@ void launch_attn_sparse(const SparseAttnArgs& a, hipStream_t s) {
     if (nsplit == 1) return;
     const dim3 heads(unsigned(a.c.rows * a.Hq));
     if (a.c.Dh == 256)
-        hipLaunchKernelGGL(attn_sparse_combine_kernel<256>, heads, dim3(256), 0, s, a, nsplit);
+        hipLaunchKernelGGL(attn_sparse_combine_kernel<256>, heads, dim3(256), size_t(nsplit + 15) / 16 * 64, s, a, nsplit);
     else
-        hipLaunchKernelGGL(attn_sparse_combine_kernel<128>, heads, dim3(128), 0, s, a, nsplit);
+        hipLaunchKernelGGL(attn_sparse_combine_kernel<128>, heads, dim3(128), size_t(nsplit + 15) / 16 * 64, s, a, nsplit);
 }
 
 }  // namespace hero
