@@ -551,39 +551,59 @@ __global__ __launch_bounds__(256) void attn_sparse_kernel(SparseAttnArgs a, int 
     }
 
     // the column's head and its query terms: fp16 pages take term c / 8 of head
-    // c % 8; Q8_0 pages both terms of head 4 quad + c % 4
+    // c % 8; Q8_0 pages both terms of head 4 quad + c % 4. A wave forms its share
+    // of the 32-channel blocks for all four.
+    constexpr int TERMS = Q8 ? 2 : 1, PER = KB / 4;
+    __shared__ h8_t terms[GQ][TERMS][KB][64];
+    __shared__ float biggest[GQ][4][16];
     const float* q_row = a.q_rot + (int64_t(r) * a.Hq + int64_t(g) * group) * DH;
-    h8_t qf[GQ][Q8 ? 2 : 1][KB];
-    float qscale[GQ];
+    float qv[GQ][PER][8];
 #pragma unroll
     for (int x = 0; x < GQ; ++x) {
         const int h = Q8 ? 4 * x + (c16 & 3) : c16 & 7;
-        const bool have = h < group;
-        float q[KB][8], amax = 0.f;
+        float amax = 0.f;
 #pragma unroll
-        for (int k = 0; k < KB; ++k)
+        for (int y = 0; y < PER; ++y) {
+            const float4* p = reinterpret_cast<const float4*>(q_row + min(h, group - 1) * DH + 32 * (PER * w + y) + 8 * g4);
+            const float4 lo = p[0], hi = p[1];
+            qv[x][y][0] = lo.x, qv[x][y][1] = lo.y, qv[x][y][2] = lo.z, qv[x][y][3] = lo.w;
+            qv[x][y][4] = hi.x, qv[x][y][5] = hi.y, qv[x][y][6] = hi.z, qv[x][y][7] = hi.w;
 #pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                q[k][j] = have ? q_row[h * DH + 32 * k + 8 * g4 + j] : 0.f;
-                amax = fmaxf(amax, fabsf(q[k][j]));
-            }
+            for (int j = 0; j < 8; ++j) amax = fmaxf(amax, fabsf(qv[x][y][j]));
+        }
         amax = max_over_rows(amax);
+        if (g4 == 0) biggest[x][w][c16] = amax;
+    }
+    __syncthreads();
+    float qscale[GQ];
+#pragma unroll
+    for (int x = 0; x < GQ; ++x) {
+        const bool have = (Q8 ? 4 * x + (c16 & 3) : c16 & 7) < group;
+        const float amax = fmaxf(fmaxf(biggest[x][0][c16], biggest[x][1][c16]), fmaxf(biggest[x][2][c16], biggest[x][3][c16]));
         const int e = __builtin_amdgcn_frexp_expf(amax);  // amax <= 2^e
         qscale[x] = ldexpf(a.score_scale * kLog2e, e);
 #pragma unroll
-        for (int k = 0; k < KB; ++k)
+        for (int y = 0; y < PER; ++y) {
+            h8_t f[2];
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
                 _Float16 hi, lo;
-                split_f16(ldexpf(q[k][j], -e), hi, lo);
-                if constexpr (Q8) {
-                    qf[x][0][k][j] = hi;
-                    qf[x][1][k][j] = lo;
-                } else {
-                    qf[x][0][k][j] = c16 < 8 ? hi : lo;
-                }
+                split_f16(have ? ldexpf(qv[x][y][j], -e) : 0.f, hi, lo);
+                f[0][j] = Q8 || c16 < 8 ? hi : lo;
+                f[1][j] = lo;
             }
+#pragma unroll
+            for (int k = 0; k < TERMS; ++k) terms[x][k][PER * w + y][lane] = f[k];
+        }
     }
+    __syncthreads();
+    h8_t qf[GQ][TERMS][KB];
+#pragma unroll
+    for (int x = 0; x < GQ; ++x)
+#pragma unroll
+        for (int k = 0; k < TERMS; ++k)
+#pragma unroll
+            for (int y = 0; y < KB; ++y) qf[x][k][y] = terms[x][k][y][lane];
     float m[GQ], l[GQ];
     f4_t o[GQ][8 * VH];
 #pragma unroll
@@ -594,18 +614,27 @@ __global__ __launch_bounds__(256) void attn_sparse_kernel(SparseAttnArgs a, int 
         for (int e = 0; e < 8 * VH; ++e) o[x][e] = f4_t{0.f, 0.f, 0.f, 0.f};
     }
     int ve = -200;  // Q8_0: the column's accumulators are in units of 2^ve
-    __syncthreads();
 
-    const int hp = ps / 16, halves = ne * hp;
-    for (int u = w; 2 * u < halves; u += 4) {
+    // the wave's halves: entry and 16-key block of 2 (w + 4 n) and the next one
+    const int hp = ps / 16, halves = ne * hp, step_e = 8 / hp, step_b = 8 % hp;
+    const int wu = __builtin_amdgcn_readfirstlane(w);
+    int entry[2], block[2];
+#pragma unroll
+    for (int s = 0; s < 2; ++s) entry[s] = (2 * wu + s) / hp, block[s] = (2 * wu + s) % hp;
+    const int64_t page_stride = Q8 ? 2 * int64_t(c.Hkv) * ps * (DH + DH / 16) : 4 * int64_t(c.Hkv) * ps * DH;
+    const int64_t krow0 = int64_t(g) * ps, vrow0 = (int64_t(c.Hkv) + g) * ps;
+    const char* const pool = reinterpret_cast<const char*>(c.pages);
+    for (int u = wu; 2 * u < halves; u += 4) {
         int page[2], off[2], nv[2];
 #pragma unroll
         for (int s = 0; s < 2; ++s) {
-            const int hf = min(2 * u + s, halves - 1), e = hf / hp;
-            const ListEntry le = list[e];
-            off[s] = (hf - e * hp) * 16;
+            const ListEntry le = list[min(entry[s], ne - 1)];
+            off[s] = 16 * block[s];
             page[s] = __builtin_amdgcn_readfirstlane(le.page);
             nv[s] = 2 * u + s < halves ? __builtin_amdgcn_readfirstlane(max(0, min(16, le.keys - off[s]))) : 0;
+            entry[s] += step_e;
+            block[s] += step_b;
+            if (block[s] >= hp) block[s] -= hp, ++entry[s];
         }
         if (nv[0] + nv[1] == 0) continue;
         if (nv[0] == 0) page[0] = page[1], off[0] = off[1];  // an entry of none names no page: read what is there, use nothing
@@ -617,17 +646,17 @@ __global__ __launch_bounds__(256) void attn_sparse_kernel(SparseAttnArgs a, int 
             h8_t kf[2][KB], vf[VH][8];
 #pragma unroll
             for (int hf = 0; hf < 2; ++hf) {
-                const _Float16* p = f16_page<DH>(c, page[hf]) + page_row_index(c, 0, g, off[hf] + c16) * DH + 8 * g4;
+                const char* p = pool + page[hf] * page_stride + (krow0 + off[hf]) * (2 * DH);
 #pragma unroll
-                for (int k = 0; k < KB; ++k) kf[hf][k] = *reinterpret_cast<const h8_t*>(p + 32 * k);
+                for (int k = 0; k < KB; ++k) kf[hf][k] = *reinterpret_cast<const h8_t*>(p + uint32_t(2 * DH * c16 + 16 * g4 + 64 * k));
             }
 #pragma unroll
             for (int hf = 0; hf < 2; ++hf) {
-                const _Float16* p = f16_page<DH>(c, page[hf]) + page_row_index(c, 1, g, off[hf] + 4 * g4) * DH + 8 * c16;
+                const char* p = pool + page[hf] * page_stride + (vrow0 + off[hf]) * (2 * DH);
 #pragma unroll
                 for (int i = 0; i < 4; ++i)
 #pragma unroll
-                    for (int v = 0; v < VH; ++v) vf[v][4 * hf + i] = *reinterpret_cast<const h8_t*>(p + i * DH + 128 * v);
+                    for (int v = 0; v < VH; ++v) vf[v][4 * hf + i] = *reinterpret_cast<const h8_t*>(p + uint32_t(8 * DH * g4 + 16 * c16 + 2 * DH * i + 256 * v));
             }
 #pragma unroll
             for (int hf = 0; hf < 2; ++hf) {
@@ -682,20 +711,17 @@ __global__ __launch_bounds__(256) void attn_sparse_kernel(SparseAttnArgs a, int 
             uint4 kd[2][2], vd[2][2];
 #pragma unroll
             for (int hf = 0; hf < 2; ++hf) {
-                const uint8_t* pg = q8_page<DH>(c, page[hf]);
-                const int64_t kr = page_row_index(c, 0, g, off[hf]), vr = page_row_index(c, 1, g, off[hf]);
-                const uint8_t* kp = pg + (kr + c16) * DH + 8 * g4;
+                const char* pg = pool + page[hf] * page_stride;
+                const char *kp = pg + (krow0 + off[hf]) * DH, *vp = pg + (vrow0 + off[hf]) * DH, *steps = pg + q8_scales_at<DH>(c);
+                const char *kd_at = steps + (krow0 + off[hf]) * (2 * KB), *vd_at = steps + (vrow0 + off[hf]) * (2 * KB);
 #pragma unroll
-                for (int k = 0; k < KB; ++k) kq[hf][k] = *reinterpret_cast<const uint2*>(kp + 32 * k);
-                const uint4* kdp = reinterpret_cast<const uint4*>(pg + q8_scales_at<DH>(c) + (kr + 4 * g4) * (2 * KB));
-                kd[hf][0] = kdp[0];
-                kd[hf][1] = kdp[1];
-                const uint8_t* vp = pg + (vr + 4 * g4) * DH + 8 * c16;
+                for (int k = 0; k < KB; ++k) kq[hf][k] = *reinterpret_cast<const uint2*>(kp + uint32_t(DH * c16 + 8 * g4 + 32 * k));
 #pragma unroll
-                for (int i = 0; i < 4; ++i) vq[4 * hf + i] = *reinterpret_cast<const uint2*>(vp + i * DH);
-                const uint4* vdp = reinterpret_cast<const uint4*>(pg + q8_scales_at<DH>(c) + (vr + 4 * g4) * (2 * KB));
-                vd[hf][0] = vdp[0];
-                vd[hf][1] = vdp[1];
+                for (int n = 0; n < 2; ++n) kd[hf][n] = *reinterpret_cast<const uint4*>(kd_at + uint32_t(8 * KB * g4 + 16 * n));
+#pragma unroll
+                for (int i = 0; i < 4; ++i) vq[4 * hf + i] = *reinterpret_cast<const uint2*>(vp + uint32_t(4 * DH * g4 + 8 * c16 + DH * i));
+#pragma unroll
+                for (int n = 0; n < 2; ++n) vd[hf][n] = *reinterpret_cast<const uint4*>(vd_at + uint32_t(8 * KB * g4 + 16 * n));
             }
             // scores: a block's product, then the key's step of that block
 #pragma unroll
