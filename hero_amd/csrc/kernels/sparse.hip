@@ -498,16 +498,105 @@ __device__ __forceinline__ h8_t codes8_to_half(uint2 w) {
     return r;
 }
 
-// rows of the lists of a range, in shared memory: the pool page and how many of
-// its keys the row sees (0: none)
+// A workgroup's pages, in shared memory: the pool page, how many of its keys each
+// row sees (0: none, or not selected), and the most of them.
+template <int R>
 struct ListEntry {
-    int32_t page, keys;
+    int32_t page;
+    uint16_t most, keys[R];
 };
 
-template <int DH>
-struct SparseMerge {  // the four waves' results
-    float m[4][8], l[4][8], o[4][8][DH];
+template <int DH, int SLOTS>
+struct SparseMerge {  // the four waves' results; a slot per (row, head)
+    float m[4][SLOTS], l[4][SLOTS], o[4][SLOTS][DH];
 };
+
+// The pages of R rows' lists, each once with the rows' key counts: a page that
+// several rows of one sequence select is read once for all of them. `top`
+// entries a row, at most 128; a page's second place in one list stays an entry
+// of its own. Entries in the order of row 0's list, then what row 1 adds, ...;
+// returns their number.
+struct UnionScratch {
+    int32_t lp[512], page[512], count[512], sums[2][4];
+    uint16_t keys[512][4];
+};
+template <int R>
+__device__ __forceinline__ int build_union(const SparseAttnArgs& a, int g, int r0, const int (&seq)[R], const int (&pos)[R], ListEntry<R>* list, UnionScratch& u) {
+    const PagedRows& c = a.c;
+    const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6, top = a.top, ps = c.page_size, n = R * top;
+    for (int x = tid; x < n; x += 256) {
+        const int j = x / top;
+        int lp = -1, count = 0, page = 0;
+#pragma unroll
+        for (int k = 0; k < R; ++k)
+            if (k == j && pos[k] >= 0) {
+                lp = a.selected[(int64_t(r0 + k) * c.Hkv + g) * top + x - j * top];
+                if (lp >= 0 && lp <= pos[k] / ps) {
+                    const int64_t id = pool_page(c, seq[k], lp);
+                    if (id >= 0) page = int32_t(id), count = min(ps, pos[k] + 1 - lp * ps);
+                }
+            }
+        u.lp[x] = count ? lp : -1;
+        u.page[x] = page;
+        u.count[x] = count;
+#pragma unroll
+        for (int k = 0; k < R; ++k) u.keys[x][k] = 0;
+    }
+    __syncthreads();
+    bool own[2] = {false, false};
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+        const int x = tid + 256 * k;
+        if (x >= n || u.lp[x] < 0) continue;
+        const int j = x / top, lp = u.lp[x];
+        int owner = x;
+        bool again = false;
+        for (int y = j * top; y < x; ++y) again |= u.lp[y] == lp;
+        if (!again) {
+            int s = 0;
+#pragma unroll
+            for (int q = 0; q < R; ++q) s = q == j ? seq[q] : s;
+#pragma unroll
+            for (int q = R - 2; q >= 0; --q) {  // the earliest row's first place wins
+                if (q >= j || seq[q] != s) continue;
+                for (int y = (q + 1) * top - 1; y >= q * top; --y) owner = u.lp[y] == lp ? y : owner;
+            }
+        }
+        own[k] = owner == x;
+        u.keys[owner][j] = uint16_t(u.count[x]);
+    }
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+        const int s = __popcll(__ballot(own[k]));
+        if (lane == 0) u.sums[k][w] = s;
+    }
+    __syncthreads();
+    int total = 0;
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+        int at = total;
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+            at += q < w ? u.sums[k][q] : 0;
+            total += u.sums[k][q];
+        }
+        const uint64_t m = __ballot(own[k]);
+        at += __popcll(m & ((uint64_t(1) << lane) - 1));
+        if (own[k]) {
+            const int x = tid + 256 * k;
+            ListEntry<R> e;
+            e.page = u.page[x];
+            e.most = 0;
+#pragma unroll
+            for (int q = 0; q < R; ++q) {
+                e.keys[q] = u.keys[x][q];
+                e.most = max(e.most, e.keys[q]);
+            }
+            list[at] = e;
+        }
+    }
+    return total;
+}
 
 template <int DH>
 __device__ __forceinline__ void sparse_store(const SparseAttnArgs& a, int r, int h, int ch, float o, float l) {
@@ -525,46 +614,74 @@ __device__ __forceinline__ void sparse_store(const SparseAttnArgs& a, int r, int
     }
 }
 
-// GQ: quads of query heads (Q8_0 pages), 1 otherwise
-template <int DH, bool Q8, int GQ>
+// R rows by GP heads each (fp16 pages: GP a power of two, in GQ sets of eight
+// columns times two terms; Q8_0 pages: GP 4 or 8, in GQ quads). R > 1: the rows
+// of a chunk, which mostly select the same pages. A row's columns get weight 0
+// for the pages of other rows; should those hold values that are not finite, 0
+// times them would reach the row, so a workgroup whose sums are not finite
+// works its rows off again one by one, over their own keys alone.
+template <int DH, bool Q8, int GQ, int R, int GP>
 __global__ __launch_bounds__(256) void attn_sparse_kernel(SparseAttnArgs a, int per, int nsplit) {
     constexpr int KB = DH / 32, VH = DH / 128;  // 32-channel blocks, 128-channel halves
+    constexpr int SLOTS = Q8 ? 4 * GQ : 8 * GQ, RS = 8 / GP, QPR = GP / 4;
     const PagedRows& c = a.c;
     const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6, g4 = lane >> 4, c16 = lane & 15;
     // K/V head fastest: with eight of them each XCD's L2 holds one head's pages
-    const int g = blockIdx.x % c.Hkv, r = blockIdx.x / c.Hkv % c.rows, split = blockIdx.x / c.Hkv / c.rows;
+    const int tiles = R > 1 ? (c.rows + R - 1) / R : c.rows;
+    const int g = blockIdx.x % c.Hkv, r0 = int(blockIdx.x / c.Hkv % tiles) * R, split = blockIdx.x / c.Hkv / tiles;
     const int group = a.Hq / c.Hkv, ps = c.page_size;
-    int seq;
-    const int pos = row_position(c, r, &seq);
-    if (pos < 0) return;
-    extern __shared__ __align__(16) ListEntry list[];
-    __shared__ __align__(16) SparseMerge<DH> mg;
-    const int e0 = split * per, ne = min(per, a.top - e0);
-    for (int i = tid; i < ne; i += 256) {
-        const int lp = a.selected[(int64_t(r) * c.Hkv + g) * a.top + e0 + i];
-        ListEntry e{0, 0};
-        if (lp >= 0 && lp <= pos / ps) {
-            const int64_t page = pool_page(c, seq, lp);
-            if (page >= 0) e = {int32_t(page), min(ps, pos + 1 - lp * ps)};
+    int seq[R], pos[R];
+    bool some = false;
+#pragma unroll
+    for (int k = 0; k < R; ++k) {
+        pos[k] = seq[k] = -1;
+        if (R == 1 || r0 + k < c.rows) pos[k] = row_position(c, r0 + k, &seq[k]);
+        some |= pos[k] >= 0;
+    }
+    if (!some) return;
+    // the row and head of a column of set x, and its slot
+    auto row_of = [&](int x) { return R == 1 ? 0 : Q8 ? x / (QPR ? QPR : 1) : min(RS * x + (c16 & 7) / GP, R - 1); };
+    auto head_of = [&](int x) { return Q8 ? 4 * (x % (QPR ? QPR : 1)) + (c16 & 3) : c16 & (GP - 1); };
+    auto used = [&](int x) {  // columns that stand for a row and head
+        bool live = head_of(x) < group && (Q8 || RS * x + (c16 & 7) / GP < R);
+#pragma unroll
+        for (int k = 0; k < R; ++k) live = live && (row_of(x) != k || pos[k] >= 0);
+        return live;
+    };
+    extern __shared__ __align__(16) char list_mem[];
+    ListEntry<R>* const list = reinterpret_cast<ListEntry<R>*>(list_mem);
+    __shared__ __align__(16) SparseMerge<DH, SLOTS> mg;
+    int ne;
+    if constexpr (R > 1) {
+        static_assert(sizeof(UnionScratch) <= sizeof(mg));
+        ne = __builtin_amdgcn_readfirstlane(build_union<R>(a, g, r0, seq, pos, list, *reinterpret_cast<UnionScratch*>(&mg)));
+    } else {
+        const int e0 = split * per;
+        ne = min(per, a.top - e0);
+        for (int i = tid; i < ne; i += 256) {
+            const int lp = a.selected[(int64_t(r0) * c.Hkv + g) * a.top + e0 + i];
+            ListEntry<R> e{0, 0, {0}};
+            if (lp >= 0 && lp <= pos[0] / ps) {
+                const int64_t page = pool_page(c, seq[0], lp);
+                if (page >= 0) e.page = int32_t(page), e.most = e.keys[0] = uint16_t(min(ps, pos[0] + 1 - lp * ps));
+            }
+            list[i] = e;
         }
-        list[i] = e;
     }
 
-    // the column's head and its query terms: fp16 pages take term c / 8 of head
-    // c % 8; Q8_0 pages both terms of head 4 quad + c % 4. A wave forms its share
-    // of the 32-channel blocks for all four.
+    // the columns' query terms: fp16 pages take term c / 8, Q8_0 pages both. A wave
+    // forms its share of the 32-channel blocks for all four.
     constexpr int TERMS = Q8 ? 2 : 1, PER = KB / 4;
     __shared__ h8_t terms[GQ][TERMS][KB][64];
     __shared__ float biggest[GQ][4][16];
-    const float* q_row = a.q_rot + (int64_t(r) * a.Hq + int64_t(g) * group) * DH;
     float qv[GQ][PER][8];
 #pragma unroll
     for (int x = 0; x < GQ; ++x) {
-        const int h = Q8 ? 4 * x + (c16 & 3) : c16 & 7;
+        const float* q_row = a.q_rot + (int64_t(min(r0 + row_of(x), c.rows - 1)) * a.Hq + g * group + min(head_of(x), group - 1)) * DH;
         float amax = 0.f;
 #pragma unroll
         for (int y = 0; y < PER; ++y) {
-            const float4* p = reinterpret_cast<const float4*>(q_row + min(h, group - 1) * DH + 32 * (PER * w + y) + 8 * g4);
+            const float4* p = reinterpret_cast<const float4*>(q_row + 32 * (PER * w + y) + 8 * g4);
             const float4 lo = p[0], hi = p[1];
             qv[x][y][0] = lo.x, qv[x][y][1] = lo.y, qv[x][y][2] = lo.z, qv[x][y][3] = lo.w;
             qv[x][y][4] = hi.x, qv[x][y][5] = hi.y, qv[x][y][6] = hi.z, qv[x][y][7] = hi.w;
@@ -578,7 +695,7 @@ __global__ __launch_bounds__(256) void attn_sparse_kernel(SparseAttnArgs a, int 
     float qscale[GQ];
 #pragma unroll
     for (int x = 0; x < GQ; ++x) {
-        const bool have = (Q8 ? 4 * x + (c16 & 3) : c16 & 7) < group;
+        const bool have = used(x);
         const float amax = fmaxf(fmaxf(biggest[x][0][c16], biggest[x][1][c16]), fmaxf(biggest[x][2][c16], biggest[x][3][c16]));
         const int e = __builtin_amdgcn_frexp_expf(amax);  // amax <= 2^e
         qscale[x] = ldexpf(a.score_scale * kLog2e, e);
@@ -604,261 +721,300 @@ __global__ __launch_bounds__(256) void attn_sparse_kernel(SparseAttnArgs a, int 
         for (int k = 0; k < TERMS; ++k)
 #pragma unroll
             for (int y = 0; y < KB; ++y) qf[x][k][y] = terms[x][k][y][lane];
-    float m[GQ], l[GQ];
-    f4_t o[GQ][8 * VH];
-#pragma unroll
-    for (int x = 0; x < GQ; ++x) {
-        m[x] = -INFINITY;
-        l[x] = 0.f;
-#pragma unroll
-        for (int e = 0; e < 8 * VH; ++e) o[x][e] = f4_t{0.f, 0.f, 0.f, 0.f};
-    }
-    int ve = -200;  // Q8_0: the column's accumulators are in units of 2^ve
 
-    // the wave's halves: entry and 16-key block of 2 (w + 4 n) and the next one
     const int hp = ps / 16, halves = ne * hp, step_e = 8 / hp, step_b = 8 % hp;
     const int wu = __builtin_amdgcn_readfirstlane(w);
-    int entry[2], block[2];
-#pragma unroll
-    for (int s = 0; s < 2; ++s) entry[s] = (2 * wu + s) / hp, block[s] = (2 * wu + s) % hp;
     const int64_t page_stride = Q8 ? 2 * int64_t(c.Hkv) * ps * (DH + DH / 16) : 4 * int64_t(c.Hkv) * ps * DH;
     const int64_t krow0 = int64_t(g) * ps, vrow0 = (int64_t(c.Hkv) + g) * ps;
     const char* const pool = reinterpret_cast<const char*>(c.pages);
-    for (int u = wu; 2 * u < halves; u += 4) {
-        int page[2], off[2], nv[2];
+    float m[GQ], l[GQ];
+    f4_t o[GQ][8 * VH];
+#pragma unroll 1
+    for (int only = -1; only < R; ++only) {  // -1: all rows; the others run only if that was not finite
 #pragma unroll
-        for (int s = 0; s < 2; ++s) {
-            const ListEntry le = list[min(entry[s], ne - 1)];
-            off[s] = 16 * block[s];
-            page[s] = __builtin_amdgcn_readfirstlane(le.page);
-            nv[s] = 2 * u + s < halves ? __builtin_amdgcn_readfirstlane(max(0, min(16, le.keys - off[s]))) : 0;
-            entry[s] += step_e;
-            block[s] += step_b;
-            if (block[s] >= hp) block[s] -= hp, ++entry[s];
+        for (int x = 0; x < GQ; ++x) {
+            m[x] = -INFINITY;
+            l[x] = 0.f;
+#pragma unroll
+            for (int e = 0; e < 8 * VH; ++e) o[x][e] = f4_t{0.f, 0.f, 0.f, 0.f};
         }
-        if (nv[0] + nv[1] == 0) continue;
-        if (nv[0] == 0) page[0] = page[1], off[0] = off[1];  // an entry of none names no page: read what is there, use nothing
-        if (nv[1] == 0) page[1] = page[0], off[1] = off[0];
-        const bool full = nv[0] + nv[1] == 32;
+        int ve = -200;  // Q8_0: the column's accumulators are in units of 2^ve
 
-        f4_t s[GQ][2];
-        if constexpr (!Q8) {
-            h8_t kf[2][KB], vf[VH][8];
+        // the wave's halves: entry and 16-key block of 2 (w + 4 n) and the next one
+        int entry[2], block[2];
 #pragma unroll
-            for (int hf = 0; hf < 2; ++hf) {
-                const char* p = pool + page[hf] * page_stride + (krow0 + off[hf]) * (2 * DH);
+        for (int s = 0; s < 2; ++s) entry[s] = (2 * wu + s) / hp, block[s] = (2 * wu + s) % hp;
+        for (int u = wu; 2 * u < halves; u += 4) {
+            int page[2], off[2], nv[2], mine[GQ][2];  // keys of the half that any row, the set's column sees
 #pragma unroll
-                for (int k = 0; k < KB; ++k) kf[hf][k] = *reinterpret_cast<const h8_t*>(p + uint32_t(2 * DH * c16 + 16 * g4 + 64 * k));
-            }
+            for (int s = 0; s < 2; ++s) {
+                const ListEntry<R>& le = list[min(entry[s], ne - 1)];
+                off[s] = 16 * block[s];
+                page[s] = __builtin_amdgcn_readfirstlane(le.page);
+                const bool real = 2 * u + s < halves;
+                nv[s] = real ? __builtin_amdgcn_readfirstlane(max(0, min(16, int(R > 1 && only >= 0 ? le.keys[max(only, 0)] : le.most) - off[s]))) : 0;
 #pragma unroll
-            for (int hf = 0; hf < 2; ++hf) {
-                const char* p = pool + page[hf] * page_stride + (vrow0 + off[hf]) * (2 * DH);
-#pragma unroll
-                for (int i = 0; i < 4; ++i)
-#pragma unroll
-                    for (int v = 0; v < VH; ++v) vf[v][4 * hf + i] = *reinterpret_cast<const h8_t*>(p + uint32_t(8 * DH * g4 + 16 * c16 + 2 * DH * i + 256 * v));
-            }
-#pragma unroll
-            for (int hf = 0; hf < 2; ++hf) {
-                f4_t acc = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-                for (int k = 0; k < KB; ++k) acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf[hf][k], qf[0][0][k], acc, 0, 0, 0);
-#pragma unroll
-                for (int i = 0; i < 4; ++i) s[0][hf][i] = (acc[i] + column_other(acc[i])) * qscale[0];
-            }
-            if (!full) {
-#pragma unroll
-                for (int hf = 0; hf < 2; ++hf)
-#pragma unroll
-                    for (int i = 0; i < 4; ++i)
-                        if (4 * g4 + i >= nv[hf]) {
-                            s[0][hf][i] = -INFINITY;
-#pragma unroll
-                            for (int v = 0; v < VH; ++v) vf[v][4 * hf + i] = h8_t{};
-                        }
-            }
-            float top = s[0][0][0];
-#pragma unroll
-            for (int i = 1; i < 8; ++i) top = fmaxf(top, s[0][i >> 2][i & 3]);
-            if (__any(top > m[0] + kPSlack)) {
-                const float m2 = fmaxf(m[0], max_over_rows(top)), f = m2 == -INFINITY ? 1.f : exp2_hw(m[0] - m2);
-                m[0] = m2;
-                l[0] *= f;
-#pragma unroll
-                for (int e = 0; e < 8 * VH; ++e) o[0][e] *= f;
-            }
-            const float base = m[0] - kPShift;
-            h8_t pf;
-#pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                const float p = exp2_hw(s[0][i >> 2][i & 3] - base);
-                l[0] += p;
-                _Float16 hi, lo;
-                split_f16(p, hi, lo);
-                pf[i] = c16 < 8 ? hi : lo;
-            }
-#pragma unroll
-            for (int v = 0; v < VH; ++v)
-#pragma unroll
-                for (int e = 0; e < 8; ++e) {
-                    h8_t x;
-#pragma unroll
-                    for (int i = 0; i < 8; ++i) x[i] = vf[v][i][e];
-                    o[0][8 * v + e] = __builtin_amdgcn_mfma_f32_16x16x32_f16(x, pf, o[0][8 * v + e], 0, 0, 0);
+                for (int x = 0; x < GQ; ++x) {
+                    mine[x][s] = nv[s];
+                    if constexpr (R > 1) mine[x][s] = min(nv[s], max(0, int(le.keys[row_of(x)]) - off[s]));
                 }
-        } else {
-            uint2 kq[2][KB], vq[8];
-            uint4 kd[2][2], vd[2][2];
-#pragma unroll
-            for (int hf = 0; hf < 2; ++hf) {
-                const char* pg = pool + page[hf] * page_stride;
-                const char *kp = pg + (krow0 + off[hf]) * DH, *vp = pg + (vrow0 + off[hf]) * DH, *steps = pg + q8_scales_at<DH>(c);
-                const char *kd_at = steps + (krow0 + off[hf]) * (2 * KB), *vd_at = steps + (vrow0 + off[hf]) * (2 * KB);
-#pragma unroll
-                for (int k = 0; k < KB; ++k) kq[hf][k] = *reinterpret_cast<const uint2*>(kp + uint32_t(DH * c16 + 8 * g4 + 32 * k));
-#pragma unroll
-                for (int n = 0; n < 2; ++n) kd[hf][n] = *reinterpret_cast<const uint4*>(kd_at + uint32_t(8 * KB * g4 + 16 * n));
-#pragma unroll
-                for (int i = 0; i < 4; ++i) vq[4 * hf + i] = *reinterpret_cast<const uint2*>(vp + uint32_t(4 * DH * g4 + 8 * c16 + DH * i));
-#pragma unroll
-                for (int n = 0; n < 2; ++n) vd[hf][n] = *reinterpret_cast<const uint4*>(vd_at + uint32_t(8 * KB * g4 + 16 * n));
+                entry[s] += step_e;
+                block[s] += step_b;
+                if (block[s] >= hp) block[s] -= hp, ++entry[s];
             }
-            // scores: a block's product, then the key's step of that block
+            if (nv[0] + nv[1] == 0) continue;
+            if (nv[0] == 0) page[0] = page[1], off[0] = off[1];  // an entry of none names no page: read what is there, use nothing
+            if (nv[1] == 0) page[1] = page[0], off[1] = off[0];
+            const bool full = nv[0] + nv[1] == 32;
+            auto weights_base = [&](int x, const f4_t (&s)[2], auto rescale) {
+                float top = s[0][0];
 #pragma unroll
-            for (int hf = 0; hf < 2; ++hf) {
-                h8_t steps[2] = {__builtin_bit_cast(h8_t, kd[hf][0]), __builtin_bit_cast(h8_t, kd[hf][1])};  // [key][block]
-#pragma unroll
-                for (int x = 0; x < GQ; ++x) s[x][hf] = f4_t{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-                for (int k = 0; k < KB; ++k) {
-                    const h8_t kf = codes8_to_half(kq[hf][k]);
-#pragma unroll
-                    for (int x = 0; x < GQ; ++x) {
-                        f4_t acc = {0.f, 0.f, 0.f, 0.f};
-                        acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf, qf[x][1][k], acc, 0, 0, 0);
-                        acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf, qf[x][0][k], acc, 0, 0, 0);
-#pragma unroll
-                        for (int i = 0; i < 4; ++i) s[x][hf][i] = __builtin_fmaf(float(steps[i >> 1][4 * (i & 1) + k]), acc[i], s[x][hf][i]);
-                    }
-                }
-#pragma unroll
-                for (int x = 0; x < GQ; ++x)
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) s[x][hf][i] = 4 * g4 + i < nv[hf] ? s[x][hf][i] * qscale[x] : -INFINITY;
-            }
-            // the column's value steps, 2^-ve times, 0 past the keys
-            float d[8], dmax = 0.f;
-#pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                const uint4 two = vd[i >> 2][(i & 3) >> 1];
-                const uint64_t four = (i & 1) ? uint64_t(two.w) << 32 | two.z : uint64_t(two.y) << 32 | two.x;
-                d[i] = 4 * g4 + (i & 3) < nv[i >> 2] ? half_bits_to_f32(uint16_t(four >> (16 * (c16 >> 2)))) : 0.f;
-                dmax = fmaxf(dmax, d[i]);
-            }
-            const int top_e = __builtin_amdgcn_frexp_expf(dmax);
-            if (__any(dmax > 0.f && top_e > ve)) {
-                int e = dmax > 0.f ? top_e : -200;
-                e = max(e, __shfl_xor(e, 16));
-                e = max(e, __shfl_xor(e, 32));
-                e = max(e, ve);
-#pragma unroll
-                for (int x = 0; x < GQ; ++x)
-#pragma unroll
-                    for (int n = 0; n < 8; ++n)
-#pragma unroll
-                        for (int i = 0; i < 4; ++i) o[x][n][i] = ldexpf(o[x][n][i], ve - e);
-                ve = e;
-            }
-#pragma unroll
-            for (int i = 0; i < 8; ++i) d[i] = ldexpf(d[i], -ve);
-            h8_t ph[GQ], pl[GQ];
-#pragma unroll
-            for (int x = 0; x < GQ; ++x) {
-                float top = s[x][0][0];
-#pragma unroll
-                for (int i = 1; i < 8; ++i) top = fmaxf(top, s[x][i >> 2][i & 3]);
+                for (int i = 1; i < 8; ++i) top = fmaxf(top, s[i >> 2][i & 3]);
                 if (__any(top > m[x] + kPSlack)) {
                     const float m2 = fmaxf(m[x], max_over_rows(top)), f = m2 == -INFINITY ? 1.f : exp2_hw(m[x] - m2);
                     m[x] = m2;
                     l[x] *= f;
-#pragma unroll
-                    for (int e = 0; e < 8; ++e) o[x][e] *= f;
+                    rescale(f);
                 }
-                const float base = m[x] - kPShift;
+                return fmaxf(m[x], -3e38f) - kPShift;  // a column that has seen no key: 2^-inf, not NaN
+            };
+
+            if constexpr (!Q8) {
+                h8_t kf[2][KB], vf[VH][8];
 #pragma unroll
-                for (int i = 0; i < 8; ++i) {
-                    const float p = exp2_hw(s[x][i >> 2][i & 3] - base);
-                    l[x] += p;
-                    _Float16 hi, lo;
-                    split_f16(p * d[i], hi, lo);
-                    ph[x][i] = hi;
-                    pl[x][i] = lo;
+                for (int hf = 0; hf < 2; ++hf) {
+                    const char* p = pool + page[hf] * page_stride + (krow0 + off[hf]) * (2 * DH);
+#pragma unroll
+                    for (int k = 0; k < KB; ++k) kf[hf][k] = *reinterpret_cast<const h8_t*>(p + uint32_t(2 * DH * c16 + 16 * g4 + 64 * k));
                 }
-            }
 #pragma unroll
-            for (int e = 0; e < 8; ++e) {
-                h8_t v;
+                for (int hf = 0; hf < 2; ++hf) {
+                    const char* p = pool + page[hf] * page_stride + (vrow0 + off[hf]) * (2 * DH);
 #pragma unroll
-                for (int i = 0; i < 8; i += 2) {
-                    const uint32_t lo = e < 4 ? vq[i].x : vq[i].y, hi = e < 4 ? vq[i + 1].x : vq[i + 1].y;
-                    const h2_t t = codes_to_half(__builtin_amdgcn_perm(hi, lo, 0x0c040c00u + 0x00010001u * (e & 3)));
-                    v[i] = t[0];
-                    v[i + 1] = t[1];
+                    for (int i = 0; i < 4; ++i)
+#pragma unroll
+                        for (int v = 0; v < VH; ++v) vf[v][4 * hf + i] = *reinterpret_cast<const h8_t*>(p + uint32_t(8 * DH * g4 + 16 * c16 + 2 * DH * i + 256 * v));
                 }
+                h8_t pf[GQ];
 #pragma unroll
                 for (int x = 0; x < GQ; ++x) {
-                    o[x][e] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, pl[x], o[x][e], 0, 0, 0);
-                    o[x][e] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, ph[x], o[x][e], 0, 0, 0);
+                    f4_t s[2];
+#pragma unroll
+                    for (int hf = 0; hf < 2; ++hf) {
+                        f4_t acc = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                        for (int k = 0; k < KB; ++k) acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf[hf][k], qf[x][0][k], acc, 0, 0, 0);
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) s[hf][i] = (acc[i] + column_other(acc[i])) * qscale[x];
+                    }
+                    if (R > 1 || !full) {
+#pragma unroll
+                        for (int i = 0; i < 8; ++i)
+                            if (4 * g4 + (i & 3) >= mine[x][i >> 2]) s[i >> 2][i & 3] = -INFINITY;
+                    }
+                    const float base = weights_base(x, s, [&](float f) {
+#pragma unroll
+                        for (int e = 0; e < 8 * VH; ++e) o[x][e] *= f;
+                    });
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) {
+                        const float p = exp2_hw(s[i >> 2][i & 3] - base);
+                        l[x] += p;
+                        _Float16 hi, lo;
+                        split_f16(p, hi, lo);
+                        pf[x][i] = c16 < 8 ? hi : lo;
+                    }
+                }
+                if (!full) {
+#pragma unroll
+                    for (int i = 0; i < 8; ++i)
+                        if (4 * g4 + (i & 3) >= nv[i >> 2]) {
+#pragma unroll
+                            for (int v = 0; v < VH; ++v) vf[v][i] = h8_t{};
+                        }
+                }
+#pragma unroll
+                for (int v = 0; v < VH; ++v)
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) {
+                        h8_t y;
+#pragma unroll
+                        for (int i = 0; i < 8; ++i) y[i] = vf[v][i][e];
+#pragma unroll
+                        for (int x = 0; x < GQ; ++x) o[x][8 * v + e] = __builtin_amdgcn_mfma_f32_16x16x32_f16(y, pf[x], o[x][8 * v + e], 0, 0, 0);
+                    }
+            } else {
+                uint2 kq[2][KB], vq[8];
+                uint4 kd[2][2], vd[2][2];
+#pragma unroll
+                for (int hf = 0; hf < 2; ++hf) {
+                    const char* pg = pool + page[hf] * page_stride;
+                    const char *kp = pg + (krow0 + off[hf]) * DH, *vp = pg + (vrow0 + off[hf]) * DH, *steps = pg + q8_scales_at<DH>(c);
+                    const char *kd_at = steps + (krow0 + off[hf]) * (2 * KB), *vd_at = steps + (vrow0 + off[hf]) * (2 * KB);
+#pragma unroll
+                    for (int k = 0; k < KB; ++k) kq[hf][k] = *reinterpret_cast<const uint2*>(kp + uint32_t(DH * c16 + 8 * g4 + 32 * k));
+#pragma unroll
+                    for (int n = 0; n < 2; ++n) kd[hf][n] = *reinterpret_cast<const uint4*>(kd_at + uint32_t(8 * KB * g4 + 16 * n));
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) vq[4 * hf + i] = *reinterpret_cast<const uint2*>(vp + uint32_t(4 * DH * g4 + 8 * c16 + DH * i));
+#pragma unroll
+                    for (int n = 0; n < 2; ++n) vd[hf][n] = *reinterpret_cast<const uint4*>(vd_at + uint32_t(8 * KB * g4 + 16 * n));
+                }
+                // scores: a block's product, then the key's step of that block
+                f4_t s[GQ][2];
+#pragma unroll
+                for (int hf = 0; hf < 2; ++hf) {
+                    h8_t steps[2] = {__builtin_bit_cast(h8_t, kd[hf][0]), __builtin_bit_cast(h8_t, kd[hf][1])};  // [key][block]
+#pragma unroll
+                    for (int x = 0; x < GQ; ++x) s[x][hf] = f4_t{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                    for (int k = 0; k < KB; ++k) {
+                        const h8_t kf = codes8_to_half(kq[hf][k]);
+#pragma unroll
+                        for (int x = 0; x < GQ; ++x) {
+                            f4_t acc = {0.f, 0.f, 0.f, 0.f};
+                            acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf, qf[x][1][k], acc, 0, 0, 0);
+                            acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf, qf[x][0][k], acc, 0, 0, 0);
+#pragma unroll
+                            for (int i = 0; i < 4; ++i) s[x][hf][i] = __builtin_fmaf(float(steps[i >> 1][4 * (i & 1) + k]), acc[i], s[x][hf][i]);
+                        }
+                    }
+#pragma unroll
+                    for (int x = 0; x < GQ; ++x)
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) s[x][hf][i] = 4 * g4 + i < mine[x][hf] ? s[x][hf][i] * qscale[x] : -INFINITY;
+                }
+                // the column's value steps, 2^-ve times, 0 past the keys
+                float d[8], dmax = 0.f;
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    const uint4 two = vd[i >> 2][(i & 3) >> 1];
+                    const uint64_t four = (i & 1) ? uint64_t(two.w) << 32 | two.z : uint64_t(two.y) << 32 | two.x;
+                    d[i] = 4 * g4 + (i & 3) < nv[i >> 2] ? half_bits_to_f32(uint16_t(four >> (16 * (c16 >> 2)))) : 0.f;
+                    dmax = fmaxf(dmax, d[i]);
+                }
+                const int top_e = __builtin_amdgcn_frexp_expf(dmax);
+                if (__any(dmax > 0.f && top_e > ve)) {
+                    int e = dmax > 0.f ? top_e : -200;
+                    e = max(e, __shfl_xor(e, 16));
+                    e = max(e, __shfl_xor(e, 32));
+                    e = max(e, ve);
+#pragma unroll
+                    for (int x = 0; x < GQ; ++x)
+#pragma unroll
+                        for (int n = 0; n < 8; ++n)
+#pragma unroll
+                            for (int i = 0; i < 4; ++i) o[x][n][i] = ldexpf(o[x][n][i], ve - e);
+                    ve = e;
+                }
+#pragma unroll
+                for (int i = 0; i < 8; ++i) d[i] = ldexpf(d[i], -ve);
+                h8_t ph[GQ], pl[GQ];
+#pragma unroll
+                for (int x = 0; x < GQ; ++x) {
+                    const float base = weights_base(x, s[x], [&](float f) {
+#pragma unroll
+                        for (int e = 0; e < 8; ++e) o[x][e] *= f;
+                    });
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) {
+                        const float p = exp2_hw(s[x][i >> 2][i & 3] - base);
+                        l[x] += p;
+                        _Float16 hi, lo;
+                        split_f16(p * d[i], hi, lo);
+                        ph[x][i] = hi;
+                        pl[x][i] = lo;
+                    }
+                }
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    h8_t v;
+#pragma unroll
+                    for (int i = 0; i < 8; i += 2) {
+                        const uint32_t lo = e < 4 ? vq[i].x : vq[i].y, hi = e < 4 ? vq[i + 1].x : vq[i + 1].y;
+                        const h2_t t = codes_to_half(__builtin_amdgcn_perm(hi, lo, 0x0c040c00u + 0x00010001u * (e & 3)));
+                        v[i] = t[0];
+                        v[i + 1] = t[1];
+                    }
+#pragma unroll
+                    for (int x = 0; x < GQ; ++x) {
+                        o[x][e] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, pl[x], o[x][e], 0, 0, 0);
+                        o[x][e] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, ph[x], o[x][e], 0, 0, 0);
+                    }
                 }
             }
         }
-    }
 
-    // merge: a lane holds channels 128 v + 32 g4 + 8 i + e of its column's head
+        // merge: a lane holds channels 128 v + 32 g4 + 8 i + e of its column's head
+        float bad = 0.f;  // NaN if a sum of a row is not finite
 #pragma unroll
-    for (int x = 0; x < GQ; ++x) {
-        const float sum = sum_over_rows(l[x]);
-        const int h = Q8 ? 4 * x + (c16 & 3) : c16 & 7;
+        for (int x = 0; x < GQ; ++x) {
+            const float sum = sum_over_rows(l[x]);
+            const int slot = Q8 ? 4 * x + (c16 & 3) : 8 * x + (c16 & 7);
 #pragma unroll
-        for (int n = 0; n < 8 * VH; ++n)
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                if constexpr (Q8)
-                    o[x][n][i] = ldexpf(o[x][n][i], ve);
-                else
-                    o[x][n][i] += column_other(o[x][n][i]);
-            }
-        if (h < group && (Q8 ? (c16 >> 2) == g4 : c16 < 8)) {
-            if (Q8 || g4 == 0) mg.m[w][h] = m[x], mg.l[w][h] = sum;
-#pragma unroll
-            for (int v = 0; v < VH; ++v)
+            for (int n = 0; n < 8 * VH; ++n)
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
-                    float4* to = reinterpret_cast<float4*>(&mg.o[w][h][128 * v + 32 * g4 + 8 * i]);
-                    to[0] = make_float4(o[x][8 * v][i], o[x][8 * v + 1][i], o[x][8 * v + 2][i], o[x][8 * v + 3][i]);
-                    to[1] = make_float4(o[x][8 * v + 4][i], o[x][8 * v + 5][i], o[x][8 * v + 6][i], o[x][8 * v + 7][i]);
+                    if constexpr (Q8)
+                        o[x][n][i] = ldexpf(o[x][n][i], ve);
+                    else
+                        o[x][n][i] += column_other(o[x][n][i]);
                 }
-        }
-    }
-    __syncthreads();
-    for (int e = tid; e < group * DH; e += 256) {
-        const int h = e / DH, ch = e % DH;
-        const float mx = fmaxf(fmaxf(mg.m[0][h], mg.m[1][h]), fmaxf(mg.m[2][h], mg.m[3][h]));
-        float ov = 0.f, lv = 0.f;
+            if (used(x) && (Q8 ? (c16 >> 2) == g4 : c16 < 8)) {
+                if (Q8 || g4 == 0) mg.m[w][slot] = m[x], mg.l[w][slot] = sum;
+                if constexpr (R > 1) {
+                    bad = __builtin_fmaf(sum, 0.f, bad);
 #pragma unroll
-        for (int k = 0; k < 4; ++k) {
-            if (mg.m[k][h] == -INFINITY && mg.l[k][h] == 0.f) continue;  // a wave without keys
-            const float f = exp2_hw(mg.m[k][h] - mx);
-            ov += f * mg.o[k][h][ch];
-            lv += f * mg.l[k][h];
+                    for (int n = 0; n < 8 * VH; ++n)
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) bad = __builtin_fmaf(o[x][n][i], 0.f, bad);
+                }
+#pragma unroll
+                for (int v = 0; v < VH; ++v)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        float4* to = reinterpret_cast<float4*>(&mg.o[w][slot][128 * v + 32 * g4 + 8 * i]);
+                        to[0] = make_float4(o[x][8 * v][i], o[x][8 * v + 1][i], o[x][8 * v + 2][i], o[x][8 * v + 3][i]);
+                        to[1] = make_float4(o[x][8 * v + 4][i], o[x][8 * v + 5][i], o[x][8 * v + 6][i], o[x][8 * v + 7][i]);
+                    }
+            }
         }
-        if (nsplit == 1) {
-            sparse_store<DH>(a, r, g * group + h, ch, ov, lv);
-        } else {
-            float* rec = a.work + ((int64_t(r) * a.Hq + g * group + h) * nsplit + split) * (DH + 4);
-            rec[4 + ch] = ov;
-            if (ch == 0) rec[0] = mx, rec[1] = lv;
+        bool again = false;
+        if constexpr (R > 1)
+            again = __syncthreads_or(only < 0 && bad != 0.f);
+        else
+            __syncthreads();
+        if (!again) {
+            const int first = R > 1 && only >= 0 ? only : 0, last = R > 1 && only < 0 ? R : first + 1;
+            for (int e = first * group * DH + tid; e < last * group * DH; e += 256) {
+                const int k = R == 1 ? 0 : e / (group * DH), h = e / DH - k * group, ch = e % DH;
+                if (R > 1) {
+                    bool live = true;
+#pragma unroll
+                    for (int q = 0; q < R; ++q) live = live && (q != k || pos[q] >= 0);
+                    if (!live) continue;
+                }
+                const int slot = R == 1 ? h : Q8 ? k * GP + h : 8 * (k / RS) + k % RS * GP + h;
+                const float mx = fmaxf(fmaxf(mg.m[0][slot], mg.m[1][slot]), fmaxf(mg.m[2][slot], mg.m[3][slot]));
+                float ov = 0.f, lv = 0.f;
+#pragma unroll
+                for (int q = 0; q < 4; ++q) {
+                    if (mg.m[q][slot] == -INFINITY && mg.l[q][slot] == 0.f) continue;  // a wave without keys
+                    const float f = exp2_hw(mg.m[q][slot] - mx);
+                    ov += f * mg.o[q][slot][ch];
+                    lv += f * mg.l[q][slot];
+                }
+                if (nsplit == 1) {
+                    sparse_store<DH>(a, r0 + k, g * group + h, ch, ov, lv);
+                } else {
+                    float* rec = a.work + ((int64_t(r0) * a.Hq + g * group + h) * nsplit + split) * (DH + 4);
+                    rec[4 + ch] = ov;
+                    if (ch == 0) rec[0] = mx, rec[1] = lv;
+                }
+            }
+            if (R == 1 || only < 0) return;
         }
+        __syncthreads();
     }
 }
 
@@ -976,19 +1132,40 @@ int64_t attn_sparse_work_bytes(int64_t rows, int64_t Hq, int64_t Hkv, int64_t Dh
     return nsplit == 1 ? 0 : rows * Hq * nsplit * (Dh + 4) * 4;
 }
 
+namespace {
+template <int DH, bool Q8, int GQ, int R, int GP>
+void sparse_rows(const SparseAttnArgs& a, int per, int nsplit, hipStream_t s) {
+    const int64_t tiles = (a.c.rows + R - 1) / R;
+    hipLaunchKernelGGL((attn_sparse_kernel<DH, Q8, GQ, R, GP>), dim3(unsigned(tiles * a.c.Hkv * nsplit)), dim3(256), size_t(R > 1 ? R * a.top : per) * sizeof(ListEntry<R>),
+                       s, a, per, nsplit);
+}
+
+// Chunks with enough rows to fill the chip take several rows a workgroup, so
+// that a page which neighbouring rows select is read once for them.
+bool sparse_shares(const SparseAttnArgs& a) {
+    return a.c.row_seq && !a.c.q8 && a.top <= 128 && a.Hq / a.c.Hkv <= 4 && int64_t(a.c.rows) * a.c.Hkv >= 1024;
+}
+}  // namespace
+
 void launch_attn_sparse(const SparseAttnArgs& a, hipStream_t s) {
     int per, nsplit;
     sparse_plan(a.c.rows, a.c.Hkv, a.c.page_size, a.top, &per, &nsplit);
-    const dim3 grid(unsigned(int64_t(a.c.rows) * a.c.Hkv * nsplit));
-    const size_t smem = size_t(per) * sizeof(ListEntry);
+    const int group = a.Hq / a.c.Hkv;
+    if (sparse_shares(a)) {
+        if (a.c.Dh == 256)
+            group <= 2 ? sparse_rows<256, false, 1, 4, 2>(a, per, 1, s) : sparse_rows<256, false, 1, 2, 4>(a, per, 1, s);
+        else
+            group <= 2 ? sparse_rows<128, false, 1, 4, 2>(a, per, 1, s) : sparse_rows<128, false, 1, 2, 4>(a, per, 1, s);
+        return;
+    }
     if (a.c.Dh == 256)
-        hipLaunchKernelGGL((attn_sparse_kernel<256, false, 1>), grid, dim3(256), smem, s, a, per, nsplit);
+        sparse_rows<256, false, 1, 1, 8>(a, per, nsplit, s);
     else if (!a.c.q8)
-        hipLaunchKernelGGL((attn_sparse_kernel<128, false, 1>), grid, dim3(256), smem, s, a, per, nsplit);
-    else if (a.Hq / a.c.Hkv <= 4)
-        hipLaunchKernelGGL((attn_sparse_kernel<128, true, 1>), grid, dim3(256), smem, s, a, per, nsplit);
+        sparse_rows<128, false, 1, 1, 8>(a, per, nsplit, s);
+    else if (group <= 4)
+        sparse_rows<128, true, 1, 1, 4>(a, per, nsplit, s);
     else
-        hipLaunchKernelGGL((attn_sparse_kernel<128, true, 2>), grid, dim3(256), smem, s, a, per, nsplit);
+        sparse_rows<128, true, 2, 1, 8>(a, per, nsplit, s);
     if (nsplit == 1) return;
     const dim3 heads(unsigned(a.c.rows * a.Hq));
     if (a.c.Dh == 256)

@@ -596,6 +596,80 @@ def test_rows_of_a_chunk_equal_single_tokens(lib):
     check_attend(c, 32, q, proj, [0] * n, pos, sel, got, act, rows=[0, 1, 5, 6, 33, 69])
 
 
+def chunk_lists(rng, seq, pos, ps, hkv, top):
+    """lists of neighbouring rows that mostly agree, as a chunk's do"""
+    shared = rng.standard_normal((max(seq) + 1, hkv, max(pos) // ps + 1))
+    sel = np.full((len(pos), hkv, top), -1, np.int32)
+    for r in range(len(pos)):
+        if pos[r] < 0:
+            continue
+        seen = pos[r] // ps + 1
+        score = shared[seq[r], :, :seen] + 0.5 * rng.standard_normal((hkv, seen))
+        n = min(top, seen)
+        sel[r, :, :n] = np.sort(np.argsort(-score, axis=1)[:, :n], axis=1)
+    return sel
+
+
+CHUNKS = [(False, 128, 64, 32, 8, 6), (False, 128, 16, 24, 8, 20), (False, 128, 32, 16, 8, 9), (False, 128, 64, 8, 8, 5), (False, 256, 64, 32, 8, 4), (False, 256, 16, 16, 8, 11),
+          (False, 128, 48, 64, 8, 7), (True, 128, 64, 32, 8, 6), (True, 128, 16, 16, 8, 20), (True, 128, 64, 64, 8, 5), (False, 128, 64, 32, 8, 128), (False, 128, 64, 32, 8, 129)]
+
+
+@pytest.mark.parametrize("q8,dh,ps,hq,hkv,top", CHUNKS)
+def test_attend_of_large_chunks(lib, q8, dh, ps, hq, hkv, top):
+    """Chunks of three sequences of many rows, which share page reads between
+    rows: rows of two sequences in one tile, padding inside tiles, empty lists,
+    lists in any order, pages twice, out of range and holding nothing."""
+    rng = np.random.default_rng(ps + hq + top + dh)
+    c = Cache(rng, 3, max(9, min(top, 40) + 2), hkv, dh, ps, q8)
+    span = c.max_pages * ps
+    seq = [0] * 71 + [1] * 33 + [2] * 40
+    pos = list(range(span - 71, span)) + list(range(ps - 3, ps + 30)) + list(range(0, 40))
+    pos[5] = pos[70] = -1
+    seq[100] = 3
+    sel = chunk_lists(rng, [0 if s > 2 else s for s in seq], pos, ps, hkv, top)
+    sel[2], sel[20, 1] = -1, -1
+    sel[8] = sel[8][:, ::-1]
+    sel[9, :, 1] = sel[9, :, 0]
+    sel[10, 0, :3], sel[11, 0, :2] = sel[10, 0, 0], sel[10, 0, 0]
+    sel[12, 1, 0], sel[13, 2, 1] = 1 << 30, -9
+    table = c.table.copy()
+    table[0, 1], table[2, 0] = -1, c.n
+    q = (rng.standard_normal((len(pos), hq, dh)) * 1.5).astype(np.float32)
+    proj = rng.standard_normal((len(pos), 2 * hq * dh)).astype(np.float32)
+    got, act = run_attend(lib, c, hq, q, proj, seq, pos, sel, fill=3.0, table=table)
+    check_attend(c, hq, q, proj, seq, pos, sel, got, act, fill=3.0, table=table, rows=[0, 1, 2, 3, 4, 5, 8, 9, 10, 11, 12, 13, 20, 21, 69, 70, 71, 72, 99, 100, 101, 103, 104, 105, 143])
+
+
+@pytest.mark.parametrize("q8,hq", [(False, 32), (False, 16), (True, 32)])
+def test_rows_of_a_chunk_do_not_reach_each_other(lib, q8, hq):
+    """A page that only some rows of a tile select, and keys behind some rows'
+    positions, hold infinities and NaNs: they reach the rows that see them and
+    no other."""
+    rng = np.random.default_rng(50 + hq)
+    hkv, dh, ps, n = 8, 128, 64, 140
+    c = Cache(rng, 1, 6, hkv, dh, ps, q8)
+    pos = list(range(6 * ps - n, 6 * ps))
+    sel = np.zeros((n, hkv, 2), np.int32)
+    sel[:, :, 1] = np.array(pos)[:, None] // ps
+    sel[::3, :, 0] = 1
+    bad = copy_of(c)
+    for value, page, slots in ((np.nan, 1, slice(None)), (np.inf, 5, slice(40, 64)), (-np.inf, 4, slice(50, 52))):
+        at = c.table[0, page]
+        if q8:
+            bad.d[at, :, :, slots] = value
+        else:
+            bad.kv[at, 1, :, slots] = value
+    q, proj = rng.standard_normal((n, hq, dh)).astype(np.float32), rng.standard_normal((n, 2 * hq * dh)).astype(np.float32)
+    got, act = run_attend(lib, bad, hq, q, proj, [0] * n, pos, sel)
+    first_bad = {5: 5 * ps + 40, 4: 4 * ps + 50}
+    clean = [r for r in range(n) if r % 3 and not any(pos[r] >= f and page == pos[r] // ps for page, f in first_bad.items())]
+    assert len(clean) > 30
+    assert np.all(np.isfinite(got[clean])) and not np.any(np.isfinite(got[::3]))
+    hit = [r for r in range(n) if pos[r] // ps == 5 and pos[r] >= first_bad[5]]
+    assert not np.any(np.isfinite(got[hit]))
+    check_attend(c, hq, q, proj, [0] * n, pos, sel, got, rows=clean[:12] + clean[-12:])
+
+
 @pytest.mark.parametrize("q8", [False, True])
 def test_offsets_past_32_bits(lib, q8):
     """Pages whose byte offset in the pool passes 2^32: appended, read, selected
