@@ -442,6 +442,8 @@ __global__ __launch_bounds__(1024) void choose_pages_long_kernel(SelectArgs a) {
 //            channels 8 c .. 8 c + 7: whole rows per load, transposed in the
 //            lane's registers. Product e covers channels 8 c + e, and a lane
 //            ends with 32 consecutive channels of its column's head.
+// (Keys alone pass through shared memory first: a load whose neighbouring lanes
+// read different rows takes several times as long.)
 // The matrix cores multiply fp16; queries and weights are fp32. Each is split
 // into two fp16 terms (22 bits). A head's query is scaled by a power of two to
 // at most 1 first, and a weight is 2^13 e^(s - m) with m at most 2 (base 2) below
@@ -650,11 +652,19 @@ __global__ __launch_bounds__(256) void attn_sparse_kernel(SparseAttnArgs a, int 
     };
     extern __shared__ __align__(16) char list_mem[];
     ListEntry<R>* const list = reinterpret_cast<ListEntry<R>*>(list_mem);
-    __shared__ __align__(16) SparseMerge<DH, SLOTS> mg;
+    // the waves' key tiles (32 keys each); before, what the list is built in, and
+    // behind, the waves' results
+    constexpr int ROW = Q8 ? DH : 2 * DH, TILE = 32 * ROW, CH = ROW / 16;
+    using Merge = SparseMerge<DH, SLOTS>;
+    __shared__ __align__(16) char shared_mem[sizeof(Merge) > 4 * TILE ? sizeof(Merge) : 4 * TILE];
+    Merge& mg = *reinterpret_cast<Merge*>(shared_mem);
+    char* const tile = shared_mem + w * TILE;
+    // 16-byte chunk k of a tile's row: rows of one bank go to different ones
+    auto chunk_at = [&](int row, int k) { return row * ROW + ((k ^ (Q8 ? (row >> 1) & 7 : row & 15)) * 16); };
     int ne;
     if constexpr (R > 1) {
-        static_assert(sizeof(UnionScratch) <= sizeof(mg));
-        ne = __builtin_amdgcn_readfirstlane(build_union<R>(a, g, r0, seq, pos, list, *reinterpret_cast<UnionScratch*>(&mg)));
+        static_assert(sizeof(UnionScratch) <= sizeof(shared_mem));
+        ne = __builtin_amdgcn_readfirstlane(build_union<R>(a, g, r0, seq, pos, list, *reinterpret_cast<UnionScratch*>(shared_mem)));
     } else {
         const int e0 = split * per;
         ne = min(per, a.top - e0);
@@ -779,14 +789,19 @@ __global__ __launch_bounds__(256) void attn_sparse_kernel(SparseAttnArgs a, int 
                 return fmaxf(m[x], -3e38f) - kPShift;  // a column that has seen no key: 2^-inf, not NaN
             };
 
+            // the keys through the wave's tile: read as whole rows, lane by lane on (16
+            // lanes on 16 rows, as the product wants them, are 64 requests a load:
+            // 118 us of 146 for 500 rows' loads alone), 16 bytes each
+            constexpr int LOADS = 2 * CH / 4;  // of 1024 bytes, half of them a half
+            uint4 staged[LOADS];
+#pragma unroll
+            for (int hf = 0; hf < 2; ++hf) {
+                const char* p = pool + page[hf] * page_stride + (krow0 + off[hf]) * ROW;
+#pragma unroll
+                for (int k = 0; k < LOADS / 2; ++k) staged[hf * (LOADS / 2) + k] = *reinterpret_cast<const uint4*>(p + uint32_t(1024 * k + 16 * lane));
+            }
             if constexpr (!Q8) {
-                h8_t kf[2][KB], vf[VH][8];
-#pragma unroll
-                for (int hf = 0; hf < 2; ++hf) {
-                    const char* p = pool + page[hf] * page_stride + (krow0 + off[hf]) * (2 * DH);
-#pragma unroll
-                    for (int k = 0; k < KB; ++k) kf[hf][k] = *reinterpret_cast<const h8_t*>(p + uint32_t(2 * DH * c16 + 16 * g4 + 64 * k));
-                }
+                h8_t vf[VH][8];
 #pragma unroll
                 for (int hf = 0; hf < 2; ++hf) {
                     const char* p = pool + page[hf] * page_stride + (vrow0 + off[hf]) * (2 * DH);
@@ -795,18 +810,28 @@ __global__ __launch_bounds__(256) void attn_sparse_kernel(SparseAttnArgs a, int 
 #pragma unroll
                         for (int v = 0; v < VH; ++v) vf[v][4 * hf + i] = *reinterpret_cast<const h8_t*>(p + uint32_t(8 * DH * g4 + 16 * c16 + 2 * DH * i + 256 * v));
                 }
+#pragma unroll
+                for (int k = 0; k < LOADS; ++k) *reinterpret_cast<uint4*>(tile + chunk_at((64 * k + lane) / CH, (64 * k + lane) % CH)) = staged[k];
+                f4_t acc[GQ][2];
+#pragma unroll
+                for (int hf = 0; hf < 2; ++hf) {
+#pragma unroll
+                    for (int x = 0; x < GQ; ++x) acc[x][hf] = f4_t{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                    for (int k = 0; k < KB; ++k) {
+                        const h8_t kf = *reinterpret_cast<const h8_t*>(tile + chunk_at(16 * hf + c16, 4 * k + g4));
+#pragma unroll
+                        for (int x = 0; x < GQ; ++x) acc[x][hf] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf, qf[x][0][k], acc[x][hf], 0, 0, 0);
+                    }
+                }
                 h8_t pf[GQ];
 #pragma unroll
                 for (int x = 0; x < GQ; ++x) {
                     f4_t s[2];
 #pragma unroll
-                    for (int hf = 0; hf < 2; ++hf) {
-                        f4_t acc = {0.f, 0.f, 0.f, 0.f};
+                    for (int hf = 0; hf < 2; ++hf)
 #pragma unroll
-                        for (int k = 0; k < KB; ++k) acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf[hf][k], qf[x][0][k], acc, 0, 0, 0);
-#pragma unroll
-                        for (int i = 0; i < 4; ++i) s[hf][i] = (acc[i] + column_other(acc[i])) * qscale[x];
-                    }
+                        for (int i = 0; i < 4; ++i) s[hf][i] = (acc[x][hf][i] + column_other(acc[x][hf][i])) * qscale[x];
                     if (R > 1 || !full) {
 #pragma unroll
                         for (int i = 0; i < 8; ++i)
@@ -844,15 +869,13 @@ __global__ __launch_bounds__(256) void attn_sparse_kernel(SparseAttnArgs a, int 
                         for (int x = 0; x < GQ; ++x) o[x][8 * v + e] = __builtin_amdgcn_mfma_f32_16x16x32_f16(y, pf[x], o[x][8 * v + e], 0, 0, 0);
                     }
             } else {
-                uint2 kq[2][KB], vq[8];
+                uint2 vq[8];
                 uint4 kd[2][2], vd[2][2];
 #pragma unroll
                 for (int hf = 0; hf < 2; ++hf) {
                     const char* pg = pool + page[hf] * page_stride;
-                    const char *kp = pg + (krow0 + off[hf]) * DH, *vp = pg + (vrow0 + off[hf]) * DH, *steps = pg + q8_scales_at<DH>(c);
+                    const char *vp = pg + (vrow0 + off[hf]) * DH, *steps = pg + q8_scales_at<DH>(c);
                     const char *kd_at = steps + (krow0 + off[hf]) * (2 * KB), *vd_at = steps + (vrow0 + off[hf]) * (2 * KB);
-#pragma unroll
-                    for (int k = 0; k < KB; ++k) kq[hf][k] = *reinterpret_cast<const uint2*>(kp + uint32_t(DH * c16 + 8 * g4 + 32 * k));
 #pragma unroll
                     for (int n = 0; n < 2; ++n) kd[hf][n] = *reinterpret_cast<const uint4*>(kd_at + uint32_t(8 * KB * g4 + 16 * n));
 #pragma unroll
@@ -860,6 +883,8 @@ __global__ __launch_bounds__(256) void attn_sparse_kernel(SparseAttnArgs a, int 
 #pragma unroll
                     for (int n = 0; n < 2; ++n) vd[hf][n] = *reinterpret_cast<const uint4*>(vd_at + uint32_t(8 * KB * g4 + 16 * n));
                 }
+#pragma unroll
+                for (int k = 0; k < LOADS; ++k) *reinterpret_cast<uint4*>(tile + chunk_at((64 * k + lane) / CH, (64 * k + lane) % CH)) = staged[k];
                 // scores: a block's product, then the key's step of that block
                 f4_t s[GQ][2];
 #pragma unroll
@@ -869,7 +894,7 @@ __global__ __launch_bounds__(256) void attn_sparse_kernel(SparseAttnArgs a, int 
                     for (int x = 0; x < GQ; ++x) s[x][hf] = f4_t{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
                     for (int k = 0; k < KB; ++k) {
-                        const h8_t kf = codes8_to_half(kq[hf][k]);
+                        const h8_t kf = codes8_to_half(*reinterpret_cast<const uint2*>(tile + chunk_at(16 * hf + c16, 2 * k + g4 / 2) + 8 * (g4 & 1)));
 #pragma unroll
                         for (int x = 0; x < GQ; ++x) {
                             f4_t acc = {0.f, 0.f, 0.f, 0.f};
@@ -946,6 +971,7 @@ __global__ __launch_bounds__(256) void attn_sparse_kernel(SparseAttnArgs a, int 
         }
 
         // merge: a lane holds channels 128 v + 32 g4 + 8 i + e of its column's head
+        __syncthreads();
         float bad = 0.f;  // NaN if a sum of a row is not finite
 #pragma unroll
         for (int x = 0; x < GQ; ++x) {
