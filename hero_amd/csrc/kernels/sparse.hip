@@ -793,25 +793,37 @@ __global__ __launch_bounds__(256) void attn_sparse_kernel(SparseAttnArgs a, int 
             // lanes on 16 rows, as the product wants them, are 64 requests a load:
             // 118 us of 146 for 500 rows' loads alone), 16 bytes each
             constexpr int LOADS = 2 * CH / 4;  // of 1024 bytes, half of them a half
-            uint4 staged[LOADS];
+            v4i_t staged[LOADS];
 #pragma unroll
             for (int hf = 0; hf < 2; ++hf) {
                 const char* p = pool + page[hf] * page_stride + (krow0 + off[hf]) * ROW;
 #pragma unroll
-                for (int k = 0; k < LOADS / 2; ++k) staged[hf * (LOADS / 2) + k] = *reinterpret_cast<const uint4*>(p + uint32_t(1024 * k + 16 * lane));
+                for (int k = 0; k < LOADS / 2; ++k) staged[hf * (LOADS / 2) + k] = *reinterpret_cast<const v4i_t*>(p + uint32_t(1024 * k + 16 * lane));
             }
+            __builtin_amdgcn_sched_barrier(0);  // all of a unit's loads in flight before the first is waited for
             if constexpr (!Q8) {
                 h8_t vf[VH][8];
+                // 256 channels: the values take the keys' registers once those are in the
+                // tile, so that two workgroups fit a compute unit
+                constexpr bool LATE = DH == 256;
 #pragma unroll
-                for (int hf = 0; hf < 2; ++hf) {
-                    const char* p = pool + page[hf] * page_stride + (vrow0 + off[hf]) * (2 * DH);
+                for (int turn = 0; turn < 2; ++turn) {
+                    if (turn == (LATE ? 1 : 0)) {
 #pragma unroll
-                    for (int i = 0; i < 4; ++i)
+                        for (int hf = 0; hf < 2; ++hf) {
+                            const char* p = pool + page[hf] * page_stride + (vrow0 + off[hf]) * (2 * DH);
 #pragma unroll
-                        for (int v = 0; v < VH; ++v) vf[v][4 * hf + i] = *reinterpret_cast<const h8_t*>(p + uint32_t(8 * DH * g4 + 16 * c16 + 2 * DH * i + 256 * v));
+                            for (int i = 0; i < 4; ++i)
+#pragma unroll
+                                for (int v = 0; v < VH; ++v) vf[v][4 * hf + i] = *reinterpret_cast<const h8_t*>(p + uint32_t(8 * DH * g4 + 16 * c16 + 2 * DH * i + 256 * v));
+                        }
+                        __builtin_amdgcn_sched_barrier(0);
+                    } else {
+#pragma unroll
+                        for (int k = 0; k < LOADS; ++k) *reinterpret_cast<v4i_t*>(tile + chunk_at((64 * k + lane) / CH, (64 * k + lane) % CH)) = staged[k];
+                        __builtin_amdgcn_sched_barrier(0);
+                    }
                 }
-#pragma unroll
-                for (int k = 0; k < LOADS; ++k) *reinterpret_cast<uint4*>(tile + chunk_at((64 * k + lane) / CH, (64 * k + lane) % CH)) = staged[k];
                 f4_t acc[GQ][2];
 #pragma unroll
                 for (int hf = 0; hf < 2; ++hf) {
@@ -883,8 +895,9 @@ __global__ __launch_bounds__(256) void attn_sparse_kernel(SparseAttnArgs a, int 
 #pragma unroll
                     for (int n = 0; n < 2; ++n) vd[hf][n] = *reinterpret_cast<const uint4*>(vd_at + uint32_t(8 * KB * g4 + 16 * n));
                 }
+                __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-                for (int k = 0; k < LOADS; ++k) *reinterpret_cast<uint4*>(tile + chunk_at((64 * k + lane) / CH, (64 * k + lane) % CH)) = staged[k];
+                for (int k = 0; k < LOADS; ++k) *reinterpret_cast<v4i_t*>(tile + chunk_at((64 * k + lane) / CH, (64 * k + lane) % CH)) = staged[k];
                 // scores: a block's product, then the key's step of that block
                 f4_t s[GQ][2];
 #pragma unroll
