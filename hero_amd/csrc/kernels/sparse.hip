@@ -737,6 +737,7 @@ __global__ __launch_bounds__(256) void attn_sparse_kernel(SparseAttnArgs a, int 
     const int64_t page_stride = Q8 ? 2 * int64_t(c.Hkv) * ps * (DH + DH / 16) : 4 * int64_t(c.Hkv) * ps * DH;
     const int64_t krow0 = int64_t(g) * ps, vrow0 = (int64_t(c.Hkv) + g) * ps;
     const char* const pool = reinterpret_cast<const char*>(c.pages);
+    const float is_lo = c16 < 8 ? 0.f : 1.f;
     float m[GQ], l[GQ];
     f4_t o[GQ][8 * VH];
 #pragma unroll 1
@@ -776,10 +777,13 @@ __global__ __launch_bounds__(256) void attn_sparse_kernel(SparseAttnArgs a, int 
             if (nv[0] == 0) page[0] = page[1], off[0] = off[1];  // an entry of none names no page: read what is there, use nothing
             if (nv[1] == 0) page[1] = page[0], off[1] = off[0];
             const bool full = nv[0] + nv[1] == 32;
-            auto weights_base = [&](int x, const f4_t (&s)[2], auto rescale) {
-                float top = s[0][0];
+            auto weights_base = [&](int x, const f4_t (&s)[2], const int (&sees)[2], auto rescale) {
+                float top = -INFINITY;
 #pragma unroll
-                for (int i = 1; i < 8; ++i) top = fmaxf(top, s[i >> 2][i & 3]);
+                for (int hf = 0; hf < 2; ++hf) {
+                    const float of = fmaxf(fmaxf(s[hf][0], s[hf][1]), fmaxf(s[hf][2], s[hf][3]));
+                    top = fmaxf(top, R > 1 && sees[hf] == 0 ? -INFINITY : of);
+                }
                 if (__any(top > m[x] + kPSlack)) {
                     const float m2 = fmaxf(m[x], max_over_rows(top)), f = m2 == -INFINITY ? 1.f : exp2_hw(m[x] - m2);
                     m[x] = m2;
@@ -844,22 +848,30 @@ __global__ __launch_bounds__(256) void attn_sparse_kernel(SparseAttnArgs a, int 
                     for (int hf = 0; hf < 2; ++hf)
 #pragma unroll
                         for (int i = 0; i < 4; ++i) s[hf][i] = (acc[x][hf][i] + column_other(acc[x][hf][i])) * qscale[x];
-                    if (R > 1 || !full) {
+                    // halves that a column sees in part are masked key by key, halves
+                    // that it does not see as a whole
+                    const bool partly = R == 1 ? !full : __any((mine[x][0] & 15) + (mine[x][1] & 15));
+                    if (partly) {
 #pragma unroll
                         for (int i = 0; i < 8; ++i)
                             if (4 * g4 + (i & 3) >= mine[x][i >> 2]) s[i >> 2][i & 3] = -INFINITY;
                     }
-                    const float base = weights_base(x, s, [&](float f) {
+                    const float base = weights_base(x, s, mine[x], [&](float f) {
 #pragma unroll
                         for (int e = 0; e < 8 * VH; ++e) o[x][e] *= f;
                     });
 #pragma unroll
-                    for (int i = 0; i < 8; ++i) {
-                        const float p = exp2_hw(s[i >> 2][i & 3] - base);
-                        l[x] += p;
-                        _Float16 hi, lo;
-                        split_f16(p, hi, lo);
-                        pf[x][i] = c16 < 8 ? hi : lo;
+                    for (int hf = 0; hf < 2; ++hf) {
+                        const float less = R > 1 && mine[x][hf] == 0 ? INFINITY : base;
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) {
+                            float p = exp2_hw(s[hf][i] - less);
+                            asm("" : "+v"(p));
+                            l[x] += p;
+                            // the column's term: fp16(p), or of the rest (is_lo 1)
+                            const float rest = __builtin_fmaf(-float(_Float16(p)), is_lo, p);
+                            pf[x][4 * hf + i] = _Float16(rest);
+                        }
                     }
                 }
                 if (!full) {
@@ -950,7 +962,7 @@ __global__ __launch_bounds__(256) void attn_sparse_kernel(SparseAttnArgs a, int 
                 h8_t ph[GQ], pl[GQ];
 #pragma unroll
                 for (int x = 0; x < GQ; ++x) {
-                    const float base = weights_base(x, s[x], [&](float f) {
+                    const float base = weights_base(x, s[x], mine[x], [&](float f) {
 #pragma unroll
                         for (int e = 0; e < 8; ++e) o[x][e] *= f;
                     });
