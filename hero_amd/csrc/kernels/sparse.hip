@@ -659,8 +659,15 @@ __global__ __launch_bounds__(256) void attn_sparse_kernel(SparseAttnArgs a, int 
     __shared__ __align__(16) char shared_mem[sizeof(Merge) > 4 * TILE ? sizeof(Merge) : 4 * TILE];
     Merge& mg = *reinterpret_cast<Merge*>(shared_mem);
     char* const tile = shared_mem + w * TILE;
-    // 16-byte chunk k of a tile's row: rows of one bank go to different ones
-    auto chunk_at = [&](int row, int k) { return row * ROW + ((k ^ (Q8 ? (row >> 1) & 7 : row & 15)) * 16); };
+    // Chunk k (16 bytes) of a tile's row is kept at k ^ row % 16 (Q8_0: row / 2 % 8),
+    // so that neither the stores (whole rows) nor the reads (one chunk of 16 rows)
+    // meet in a bank. Load n of a unit's keys is rows 64 n / CH ..: its place, and
+    // that of the 64-byte step k of row c16, differ from lane constants by the
+    // exclusive or of a constant (formed at each use: kept, they cost ten registers)
+    int put = (lane / CH) * ROW + ((lane % CH) ^ (Q8 ? lane / CH >> 1 & 7 : lane / CH)) * 16;
+    int get = c16 * ROW + (Q8 ? ((g4 >> 1) ^ (c16 >> 1 & 7)) * 16 + (g4 & 1) * 8 : (g4 ^ c16) * 16);
+    auto put_at = [&](int n) { return 1024 * n + (put ^ ((64 / CH * n % 16 >> (Q8 ? 1 : 0)) * 16)); };
+    auto get_at = [&](int hf, int k) { return 16 * hf * ROW + (get ^ (Q8 ? 32 * k : 64 * k)); };
     int ne;
     if constexpr (R > 1) {
         static_assert(sizeof(UnionScratch) <= sizeof(shared_mem));
@@ -751,31 +758,63 @@ __global__ __launch_bounds__(256) void attn_sparse_kernel(SparseAttnArgs a, int 
         }
         int ve = -200;  // Q8_0: the column's accumulators are in units of 2^ve
 
-        // the wave's halves: entry and 16-key block of 2 (w + 4 n) and the next one
-        int entry[2], block[2];
+        // the wave's units: halves 2 (w + 4 n) and the one behind, as entry and 16-key
+        // block; `next` finds the following one that holds keys
+        int entry[2], block[2], at = wu;
 #pragma unroll
         for (int s = 0; s < 2; ++s) entry[s] = (2 * wu + s) / hp, block[s] = (2 * wu + s) % hp;
-        for (int u = wu; 2 * u < halves; u += 4) {
+        int next_page[2], next_off[2], next_nv[2], next_mine[GQ][2];
+        auto next = [&] {
+            while (2 * at < halves) {
+#pragma unroll
+                for (int s = 0; s < 2; ++s) {
+                    const ListEntry<R>& le = list[min(entry[s], ne - 1)];
+                    next_off[s] = 16 * block[s];
+                    next_page[s] = __builtin_amdgcn_readfirstlane(le.page);
+                    const bool real = 2 * at + s < halves;
+                    next_nv[s] = real ? __builtin_amdgcn_readfirstlane(max(0, min(16, int(R > 1 && only >= 0 ? le.keys[max(only, 0)] : le.most) - next_off[s]))) : 0;
+#pragma unroll
+                    for (int x = 0; x < GQ; ++x) {
+                        next_mine[x][s] = next_nv[s];
+                        if constexpr (R > 1) next_mine[x][s] = min(next_nv[s], max(0, int(le.keys[row_of(x)]) - next_off[s]));
+                    }
+                    entry[s] += step_e;
+                    block[s] += step_b;
+                    if (block[s] >= hp) block[s] -= hp, ++entry[s];
+                }
+                at += 4;
+                if (next_nv[0] + next_nv[1] == 0) continue;
+                if (next_nv[0] == 0) next_page[0] = next_page[1], next_off[0] = next_off[1];  // an entry of none names no page: read what is there, use nothing
+                if (next_nv[1] == 0) next_page[1] = next_page[0], next_off[1] = next_off[0];
+                return true;
+            }
+            return false;
+        };
+        // the keys through the wave's tile: read as whole rows, lane by lane on (16
+        // lanes on 16 rows, as the product wants them, are 64 requests a load: 118 us
+        // of 146 for 500 rows' loads alone), 16 bytes each; of heads of 128 channels
+        // a unit ahead, for 256 there are not the registers
+        constexpr int LOADS = 2 * CH / 4;  // of 1024 bytes, half of them a half
+        constexpr bool AHEAD = DH == 128 && R == 1;
+        v4i_t staged[LOADS];
+        auto stage = [&](const int (&page)[2], const int (&off)[2]) {
+#pragma unroll
+            for (int hf = 0; hf < 2; ++hf) {
+                const __amdgpu_buffer_rsrc_t b = buffer_of(pool + page[hf] * page_stride + (krow0 + off[hf]) * ROW, 16 * ROW);
+#pragma unroll
+                for (int k = 0; k < LOADS / 2; ++k) staged[hf * (LOADS / 2) + k] = __builtin_amdgcn_raw_buffer_load_b128(b, 16 * lane + 1024 * k, 0, 0);
+            }
+        };
+        bool more = next();
+        if (AHEAD && more) stage(next_page, next_off);
+        while (more) {
             int page[2], off[2], nv[2], mine[GQ][2];  // keys of the half that any row, the set's column sees
 #pragma unroll
             for (int s = 0; s < 2; ++s) {
-                const ListEntry<R>& le = list[min(entry[s], ne - 1)];
-                off[s] = 16 * block[s];
-                page[s] = __builtin_amdgcn_readfirstlane(le.page);
-                const bool real = 2 * u + s < halves;
-                nv[s] = real ? __builtin_amdgcn_readfirstlane(max(0, min(16, int(R > 1 && only >= 0 ? le.keys[max(only, 0)] : le.most) - off[s]))) : 0;
+                page[s] = next_page[s], off[s] = next_off[s], nv[s] = next_nv[s];
 #pragma unroll
-                for (int x = 0; x < GQ; ++x) {
-                    mine[x][s] = nv[s];
-                    if constexpr (R > 1) mine[x][s] = min(nv[s], max(0, int(le.keys[row_of(x)]) - off[s]));
-                }
-                entry[s] += step_e;
-                block[s] += step_b;
-                if (block[s] >= hp) block[s] -= hp, ++entry[s];
+                for (int x = 0; x < GQ; ++x) mine[x][s] = next_mine[x][s];
             }
-            if (nv[0] + nv[1] == 0) continue;
-            if (nv[0] == 0) page[0] = page[1], off[0] = off[1];  // an entry of none names no page: read what is there, use nothing
-            if (nv[1] == 0) page[1] = page[0], off[1] = off[0];
             const bool full = nv[0] + nv[1] == 32;
             auto weights_base = [&](int x, const f4_t (&s)[2], const int (&sees)[2], auto rescale) {
                 float top = -INFINITY;
@@ -793,18 +832,9 @@ __global__ __launch_bounds__(256) void attn_sparse_kernel(SparseAttnArgs a, int 
                 return fmaxf(m[x], -3e38f) - kPShift;  // a column that has seen no key: 2^-inf, not NaN
             };
 
-            // the keys through the wave's tile: read as whole rows, lane by lane on (16
-            // lanes on 16 rows, as the product wants them, are 64 requests a load:
-            // 118 us of 146 for 500 rows' loads alone), 16 bytes each
-            constexpr int LOADS = 2 * CH / 4;  // of 1024 bytes, half of them a half
-            v4i_t staged[LOADS];
-#pragma unroll
-            for (int hf = 0; hf < 2; ++hf) {
-                const char* p = pool + page[hf] * page_stride + (krow0 + off[hf]) * ROW;
-#pragma unroll
-                for (int k = 0; k < LOADS / 2; ++k) staged[hf * (LOADS / 2) + k] = *reinterpret_cast<const v4i_t*>(p + uint32_t(1024 * k + 16 * lane));
-            }
-            __builtin_amdgcn_sched_barrier(0);  // all of a unit's loads in flight before the first is waited for
+            if (!AHEAD) stage(page, off);
+            asm volatile("" : "+v"(put), "+v"(get));  // see put_at
+            __builtin_amdgcn_sched_barrier(0);  // a unit's loads are all in flight before the first is waited for
             if constexpr (!Q8) {
                 h8_t vf[VH][8];
                 // 256 channels: the values take the keys' registers once those are in the
@@ -815,16 +845,22 @@ __global__ __launch_bounds__(256) void attn_sparse_kernel(SparseAttnArgs a, int 
                     if (turn == (LATE ? 1 : 0)) {
 #pragma unroll
                         for (int hf = 0; hf < 2; ++hf) {
-                            const char* p = pool + page[hf] * page_stride + (vrow0 + off[hf]) * (2 * DH);
+                            const __amdgpu_buffer_rsrc_t b = buffer_of(pool + page[hf] * page_stride + (vrow0 + off[hf]) * ROW, 16 * ROW);
 #pragma unroll
                             for (int i = 0; i < 4; ++i)
 #pragma unroll
-                                for (int v = 0; v < VH; ++v) vf[v][4 * hf + i] = *reinterpret_cast<const h8_t*>(p + uint32_t(8 * DH * g4 + 16 * c16 + 2 * DH * i + 256 * v));
+                                for (int v = 0; v < VH; ++v)
+                                    vf[v][4 * hf + i] = __builtin_bit_cast(h8_t, __builtin_amdgcn_raw_buffer_load_b128(b, 8 * DH * g4 + 16 * c16 + 2 * DH * i + 256 * v, 0, 0));
                         }
                         __builtin_amdgcn_sched_barrier(0);
                     } else {
 #pragma unroll
-                        for (int k = 0; k < LOADS; ++k) *reinterpret_cast<v4i_t*>(tile + chunk_at((64 * k + lane) / CH, (64 * k + lane) % CH)) = staged[k];
+                        for (int k = 0; k < LOADS; ++k) *reinterpret_cast<v4i_t*>(tile + put_at(k)) = staged[k];
+                        __builtin_amdgcn_sched_barrier(0);
+                        if (AHEAD) {
+                            more = next();
+                            if (more) stage(next_page, next_off);
+                        }
                         __builtin_amdgcn_sched_barrier(0);
                     }
                 }
@@ -835,7 +871,7 @@ __global__ __launch_bounds__(256) void attn_sparse_kernel(SparseAttnArgs a, int 
                     for (int x = 0; x < GQ; ++x) acc[x][hf] = f4_t{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
                     for (int k = 0; k < KB; ++k) {
-                        const h8_t kf = *reinterpret_cast<const h8_t*>(tile + chunk_at(16 * hf + c16, 4 * k + g4));
+                        const h8_t kf = *reinterpret_cast<const h8_t*>(tile + get_at(hf, k));
 #pragma unroll
                         for (int x = 0; x < GQ; ++x) acc[x][hf] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf, qf[x][0][k], acc[x][hf], 0, 0, 0);
                     }
@@ -894,22 +930,28 @@ __global__ __launch_bounds__(256) void attn_sparse_kernel(SparseAttnArgs a, int 
                     }
             } else {
                 uint2 vq[8];
-                uint4 kd[2][2], vd[2][2];
+                v4i_t kd[2][2], vd[2][2];
 #pragma unroll
                 for (int hf = 0; hf < 2; ++hf) {
-                    const char* pg = pool + page[hf] * page_stride;
-                    const char *vp = pg + (vrow0 + off[hf]) * DH, *steps = pg + q8_scales_at<DH>(c);
-                    const char *kd_at = steps + (krow0 + off[hf]) * (2 * KB), *vd_at = steps + (vrow0 + off[hf]) * (2 * KB);
+                    const char *pg = pool + page[hf] * page_stride, *steps = pg + q8_scales_at<DH>(c);
+                    const __amdgpu_buffer_rsrc_t vb = buffer_of(pg + (vrow0 + off[hf]) * ROW, 16 * ROW);
+                    const __amdgpu_buffer_rsrc_t kd_b = buffer_of(steps + (krow0 + off[hf]) * (2 * KB), 32 * KB), vd_b = buffer_of(steps + (vrow0 + off[hf]) * (2 * KB), 32 * KB);
 #pragma unroll
-                    for (int n = 0; n < 2; ++n) kd[hf][n] = *reinterpret_cast<const uint4*>(kd_at + uint32_t(8 * KB * g4 + 16 * n));
+                    for (int n = 0; n < 2; ++n) kd[hf][n] = __builtin_amdgcn_raw_buffer_load_b128(kd_b, 8 * KB * g4 + 16 * n, 0, 0);
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) vq[4 * hf + i] = *reinterpret_cast<const uint2*>(vp + uint32_t(4 * DH * g4 + 8 * c16 + DH * i));
+                    for (int i = 0; i < 4; ++i) vq[4 * hf + i] = __builtin_bit_cast(uint2, __builtin_amdgcn_raw_buffer_load_b64(vb, 4 * DH * g4 + 8 * c16 + DH * i, 0, 0));
 #pragma unroll
-                    for (int n = 0; n < 2; ++n) vd[hf][n] = *reinterpret_cast<const uint4*>(vd_at + uint32_t(8 * KB * g4 + 16 * n));
+                    for (int n = 0; n < 2; ++n) vd[hf][n] = __builtin_amdgcn_raw_buffer_load_b128(vd_b, 8 * KB * g4 + 16 * n, 0, 0);
                 }
                 __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-                for (int k = 0; k < LOADS; ++k) *reinterpret_cast<v4i_t*>(tile + chunk_at((64 * k + lane) / CH, (64 * k + lane) % CH)) = staged[k];
+                for (int k = 0; k < LOADS; ++k) *reinterpret_cast<v4i_t*>(tile + put_at(k)) = staged[k];
+                __builtin_amdgcn_sched_barrier(0);
+                if (AHEAD) {
+                    more = next();
+                    if (more) stage(next_page, next_off);
+                }
+                __builtin_amdgcn_sched_barrier(0);
                 // scores: a block's product, then the key's step of that block
                 f4_t s[GQ][2];
 #pragma unroll
@@ -919,7 +961,7 @@ __global__ __launch_bounds__(256) void attn_sparse_kernel(SparseAttnArgs a, int 
                     for (int x = 0; x < GQ; ++x) s[x][hf] = f4_t{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
                     for (int k = 0; k < KB; ++k) {
-                        const h8_t kf = codes8_to_half(*reinterpret_cast<const uint2*>(tile + chunk_at(16 * hf + c16, 2 * k + g4 / 2) + 8 * (g4 & 1)));
+                        const h8_t kf = codes8_to_half(*reinterpret_cast<const uint2*>(tile + get_at(hf, k)));
 #pragma unroll
                         for (int x = 0; x < GQ; ++x) {
                             f4_t acc = {0.f, 0.f, 0.f, 0.f};
@@ -938,8 +980,8 @@ __global__ __launch_bounds__(256) void attn_sparse_kernel(SparseAttnArgs a, int 
                 float d[8], dmax = 0.f;
 #pragma unroll
                 for (int i = 0; i < 8; ++i) {
-                    const uint4 two = vd[i >> 2][(i & 3) >> 1];
-                    const uint64_t four = (i & 1) ? uint64_t(two.w) << 32 | two.z : uint64_t(two.y) << 32 | two.x;
+                    const v4i_t two = vd[i >> 2][(i & 3) >> 1];
+                    const uint64_t four = (i & 1) ? uint64_t(uint32_t(two.w)) << 32 | uint32_t(two.z) : uint64_t(uint32_t(two.y)) << 32 | uint32_t(two.x);
                     d[i] = 4 * g4 + (i & 3) < nv[i >> 2] ? half_bits_to_f32(uint16_t(four >> (16 * (c16 >> 2)))) : 0.f;
                     dmax = fmaxf(dmax, d[i]);
                 }
@@ -993,6 +1035,7 @@ __global__ __launch_bounds__(256) void attn_sparse_kernel(SparseAttnArgs a, int 
                     }
                 }
             }
+            if (!AHEAD) more = next();
         }
 
         // merge: a lane holds channels 128 v + 32 g4 + 8 i + e of its column's head
