@@ -601,9 +601,8 @@ __device__ __forceinline__ int build_union(const SparseAttnArgs& a, int g, int r
 }
 
 template <int DH>
-__device__ __forceinline__ void sparse_store(const SparseAttnArgs& a, int r, int h, int ch, float o, float l) {
+__device__ __forceinline__ void sparse_store(const SparseAttnArgs& a, int r, int h, int ch, float o, float l, float gate) {
     const int64_t width = int64_t(a.Hq) * DH, idx = int64_t(r) * width + int64_t(h) * DH + ch;
-    const float gate = a.proj[int64_t(r) * a.proj_stride + int64_t(h) * 2 * DH + DH + ch];
     const float out = l == 0.f ? 0.f : (o / l) * sigmoid_f32(gate);
     if (a.out_f32) a.out_f32[idx] = out;
     if (a.act_out) {
@@ -1080,7 +1079,21 @@ __global__ __launch_bounds__(256) void attn_sparse_kernel(SparseAttnArgs a, int 
             __syncthreads();
         if (!again) {
             const int first = R > 1 && only >= 0 ? only : 0, last = R > 1 && only < 0 ? R : first + 1;
-            for (int e = first * group * DH + tid; e < last * group * DH; e += 256) {
+            // up to NI results a lane, all their gates on the way at once
+            constexpr int NI = (R * (R == 1 ? 8 : GP) * DH + 255) / 256;
+            const int from = first * group * DH + tid, to = last * group * DH;
+            float gate[NI];
+            if (nsplit == 1) {
+#pragma unroll
+                for (int n = 0; n < NI; ++n) {
+                    const int e = min(from + 256 * n, to - 1), k = R == 1 ? 0 : e / (group * DH);
+                    gate[n] = a.proj[int64_t(min(r0 + k, c.rows - 1)) * a.proj_stride + (g * group + e / DH - k * group) * 2 * DH + DH + e % DH];
+                }
+            }
+#pragma unroll
+            for (int n = 0; n < NI; ++n) {
+                const int e = from + 256 * n;
+                if (e >= to) break;
                 const int k = R == 1 ? 0 : e / (group * DH), h = e / DH - k * group, ch = e % DH;
                 if (R > 1) {
                     bool live = true;
@@ -1089,17 +1102,19 @@ __global__ __launch_bounds__(256) void attn_sparse_kernel(SparseAttnArgs a, int 
                     if (!live) continue;
                 }
                 const int slot = R == 1 ? h : Q8 ? k * GP + h : 8 * (k / RS) + k % RS * GP + h;
-                const float mx = fmaxf(fmaxf(mg.m[0][slot], mg.m[1][slot]), fmaxf(mg.m[2][slot], mg.m[3][slot]));
+                float mw[4], lw[4];
+#pragma unroll
+                for (int q = 0; q < 4; ++q) mw[q] = mg.m[q][slot], lw[q] = mg.l[q][slot];
+                const float mx = fmaxf(fmaxf(mw[0], mw[1]), fmaxf(mw[2], mw[3]));
                 float ov = 0.f, lv = 0.f;
 #pragma unroll
                 for (int q = 0; q < 4; ++q) {
-                    if (mg.m[q][slot] == -INFINITY && mg.l[q][slot] == 0.f) continue;  // a wave without keys
-                    const float f = exp2_hw(mg.m[q][slot] - mx);
-                    ov += f * mg.o[q][slot][ch];
-                    lv += f * mg.l[q][slot];
+                    const float f = mw[q] == -INFINITY && lw[q] == 0.f ? 0.f : exp2_hw(mw[q] - mx);  // a wave without keys: 0
+                    ov = __builtin_fmaf(f, mg.o[q][slot][ch], ov);
+                    lv = __builtin_fmaf(f, lw[q], lv);
                 }
                 if (nsplit == 1) {
-                    sparse_store<DH>(a, r0 + k, g * group + h, ch, ov, lv);
+                    sparse_store<DH>(a, r0 + k, g * group + h, ch, ov, lv, gate[n]);
                 } else {
                     float* rec = a.work + ((int64_t(r0) * a.Hq + g * group + h) * nsplit + split) * (DH + 4);
                     rec[4 + ch] = ov;
@@ -1133,6 +1148,7 @@ __global__ __launch_bounds__(DH) void attn_sparse_combine_kernel(SparseAttnArgs 
         for (int w = 1; w < DH / 64; ++w) v = f(v, part[k][w]);
         return v;
     };
+    const float gate = a.proj[int64_t(r) * a.proj_stride + int64_t(h) * 2 * DH + DH + t];
     float mx = -INFINITY;
     for (int s = t; s < nsplit; s += DH) mx = fmaxf(mx, rec[int64_t(s) * kRec]);
     mx = over_waves(mx, 0, [](float x, float y) { return fmaxf(x, y); });
@@ -1154,14 +1170,15 @@ __global__ __launch_bounds__(DH) void attn_sparse_combine_kernel(SparseAttnArgs 
 #pragma unroll
         for (int k = 0; k < kPass; ++k) o += share[s + k] * v[k];
     }
-    sparse_store<DH>(a, r, h, t, o, l);
+    sparse_store<DH>(a, r, h, t, o, l, gate);
 }
 
-// Ranges of a row's list: about four workgroups per CU over all rows and heads,
+// Ranges of a row's list: about two workgroups per CU over all rows and heads (as many
+// as fit; with four the sixteen Q8_0 sequences take 28 us instead of 24),
 // whole pages, at least 32 key slots for each wave, at most 2048 list entries
 // (16 KB of shared memory).
 void sparse_plan(int64_t rows, int64_t Hkv, int64_t ps, int64_t top, int* per, int* nsplit) {
-    const int64_t want = std::max<int64_t>(1, 1024 / (rows * Hkv));
+    const int64_t want = std::max<int64_t>(1, 512 / (rows * Hkv));
     const int64_t most = std::max<int64_t>(1, top * ps / 128);
     const int64_t n = std::max(std::min(std::min(want, most), top), (top + 2047) / 2048);
     *per = int((top + n - 1) / n);
@@ -1220,10 +1237,13 @@ void launch_attn_select(const SelectArgs& a, hipStream_t s) {
         select_heads<128>(a, s);
 }
 
+// Room for any call of up to `rows` rows: rows * Hkv * ranges is at most 512 where
+// the plan takes several ranges to fill the chip, twice rows * Hkv where it
+// does for the list's length.
 int64_t attn_sparse_work_bytes(int64_t rows, int64_t Hq, int64_t Hkv, int64_t Dh, int64_t page_size, int64_t top) {
-    int per, nsplit;
-    sparse_plan(rows, Hkv, page_size, top, &per, &nsplit);
-    return nsplit == 1 ? 0 : rows * Hq * nsplit * (Dh + 4) * 4;
+    const int64_t most = std::min(top, std::max<int64_t>(1, top * page_size / 128));
+    const int64_t parts = std::max(most > 1 ? std::min<int64_t>(512, rows * Hkv * most) : 0, top > 2048 ? 2 * rows * Hkv : 0);
+    return parts * (Hq / Hkv) * (Dh + 4) * 4;
 }
 
 namespace {

@@ -367,7 +367,8 @@ int hero_attn_decode_paged(const hero_attn_paged_args* args, void* stream);
  * 16; heads of 128 channels (fp16 and Q8_0) or 256 (fp16), at most 8 query
  * heads per K/V head, at most 2^23 (row, query head) pairs a call. Full
  * attention only: p.a.window must be 0. All calls of a stream may share one
- * workspace; calls that may overlap need one each. */
+ * workspace (the sizes grow with the rows: one for the largest call serves all);
+ * calls that may overlap need one each. */
 typedef struct hero_attn_sparse_args {
     hero_attn_paged_args p;      /* p.a.k_cache, v_cache, scores, max_ctx unused */
     int64_t pool_pages;          /* pages in the pool (and in summaries) */
