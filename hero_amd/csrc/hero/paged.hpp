@@ -43,4 +43,8 @@ __device__ __forceinline__ int64_t q8_scales_at(const PagedRows& c) { return 2 *
 // such values are exact in 64 bits
 __device__ __forceinline__ float round11(float x) { return __uint_as_float((__float_as_uint(x) + 0x1000u) & ~0x1FFFu); }
 
+// roundf(x) for |x| < 2^22 in three instructions: 0.5 less half an ulp carries
+// exactly the values whose nearest integer (halves away from zero) is one more
+__device__ __forceinline__ int round_code(float x) { return int(x + __builtin_copysignf(0.49999997f, x)); }
+
 }  // namespace hero

@@ -570,7 +570,7 @@ int hero_attn_decode_paged(const hero_attn_paged_args* p, void* stream) {
 
 // ---- long contexts over the paged cache
 namespace {
-constexpr int64_t kMaxRowHeads = int64_t(1) << 23;  // (row, query head) pairs: grids stay below 2^32 lanes
+constexpr int64_t kMaxRowHeads = int64_t(1) << 21;  // (row, query head) pairs: grids of up to 1024 lanes for each stay below 2^32
 
 void check_paged_rows(const PagedRows& c, const int32_t* row_seq) {
     require(c.Dh == 128 || (c.Dh == 256 && c.q8 == 0), "heads of 128 channels, or of 256 in fp16 pages");
@@ -578,7 +578,7 @@ void check_paged_rows(const PagedRows& c, const int32_t* row_seq) {
     require(c.page_size >= 16 && c.page_size <= 256 && c.page_size % 16 == 0, "page_size must be a multiple of 16, 16 .. 256");
     require(c.max_pages > 0 && int64_t(c.page_size) * c.max_pages <= (int64_t(1) << 24), "bad page geometry");
     require(c.pool_pages > 0 && c.pool_pages <= (int64_t(1) << 31), "pool_pages out of range");
-    require(c.rows > 0 && c.seqs > 0 && c.Hkv > 0 && c.Hkv <= 1024 && c.rows <= kMaxRowHeads / c.Hkv, "bad row, sequence or head count");
+    require(c.rows > 0 && c.seqs > 0 && c.Hkv > 0 && c.Hkv <= 1024 && c.rows <= kMaxRowHeads / c.Hkv, "bad count of rows, sequences or heads");
     require(row_seq || c.rows <= c.seqs, "without row_seq every row needs a sequence of its own");
     require(c.positions && c.page_table, "null pointer");
     require(aligned(c.positions, 4) && aligned(c.page_table, 4) && aligned(row_seq, 4), "positions, page_table and row_seq must be 4-byte aligned");

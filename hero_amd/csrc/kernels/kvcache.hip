@@ -42,10 +42,6 @@ __device__ __forceinline__ float4 load4(const float* p) {  // at any float's add
     return v;
 }
 
-// roundf(x) for |x| < 2^22: 0.5 less half an ulp carries exactly the values
-// whose nearest integer (halves away from zero) is one more
-__device__ __forceinline__ int round_code(float x) { return int(x + __builtin_copysignf(0.49999997f, x)); }
-
 // quantize_row_q8_0 of a 32-value block held four values per lane by 8 lanes:
 // the four codes packed; *dh the block's fp16 step
 __device__ __forceinline__ uint32_t q8_codes(const float (&x)[4], uint16_t* dh) {

@@ -45,10 +45,6 @@ __device__ __forceinline__ uint64_t score_key(double s) {
     return b < 0 ? ~uint64_t(b) : uint64_t(b) | (uint64_t(1) << 63);
 }
 
-// roundf(x) for |x| < 2^22 in three instructions: 0.5 less half an ulp carries
-// exactly the values whose nearest integer (halves away from zero) is one more
-__device__ __forceinline__ int round_code(float x) { return int(x + __builtin_copysignf(0.49999997f, x)); }
-
 template <int CTRL>
 __device__ __forceinline__ double max_with(double v) {  // with a lane of the same 16
     const int2 x = __builtin_bit_cast(int2, v);

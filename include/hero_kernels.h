@@ -365,7 +365,7 @@ int hero_attn_decode_paged(const hero_attn_paged_args* args, void* stream);
  * key that is not at or before a row's position has no influence on the row,
  * whatever the pool holds there. Pages of 16 to 256 positions, a multiple of
  * 16; heads of 128 channels (fp16 and Q8_0) or 256 (fp16), at most 8 query
- * heads per K/V head, at most 2^23 (row, query head) pairs a call. Full
+ * heads per K/V head, at most 2^21 (row, query head) pairs a call. Full
  * attention only: p.a.window must be 0. All calls of a stream may share one
  * workspace (the sizes grow with the rows: one for the largest call serves all);
  * calls that may overlap need one each. */

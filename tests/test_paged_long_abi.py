@@ -88,7 +88,7 @@ def test_size_helpers():
 @pytest.mark.parametrize("hq,hkv,dh,ps,top", [(32, 8, 128, 64, 32), (8, 8, 128, 16, 5), (16, 2, 128, 256, 1), (16, 4, 256, 64, 4096), (8, 1, 128, 16, 2049)])
 def test_workspaces_grow_with_the_rows(hq, hkv, dh, ps, top):
     """one workspace for the largest call serves every smaller one"""
-    sizes = [lib.hero_attn_sparse_work_bytes(r, hq, hkv, dh, ps, top) for r in list(range(1, 300)) + [1000, 100000]]
+    sizes = [lib.hero_attn_sparse_work_bytes(r, hq, hkv, dh, ps, top) for r in list(range(1, 300)) + [1000, 60000]]
     assert sizes == sorted(sizes) and sizes[0] >= 0
     sizes = [lib.hero_attn_select_work_bytes(r, hkv, 700) for r in range(1, 300)]
     assert sizes == sorted(sizes)
