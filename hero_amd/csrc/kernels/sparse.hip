@@ -681,10 +681,11 @@ __global__ __launch_bounds__(256) void attn_sparse_kernel(SparseAttnArgs a, int 
         }
     }
 
-    // the columns' query terms: fp16 pages take term c / 8, Q8_0 pages both. A wave
-    // forms its share of the 32-channel blocks for all four.
-    constexpr int TERMS = Q8 ? 2 : 1, PER = KB / 4;
-    __shared__ h8_t terms[GQ][TERMS][KB][64];
+    // the columns' query terms: the first in columns 0 .. 7, the second in 8 .. 15
+    // (of the same heads). A wave forms its share of the 32-channel blocks for all
+    // four.
+    constexpr int PER = KB / 4;
+    __shared__ h8_t terms[GQ][KB][64];
     __shared__ float biggest[GQ][4][16];
     float qv[GQ][PER][8];
 #pragma unroll
@@ -713,26 +714,22 @@ __global__ __launch_bounds__(256) void attn_sparse_kernel(SparseAttnArgs a, int 
         qscale[x] = ldexpf(a.score_scale * kLog2e, e);
 #pragma unroll
         for (int y = 0; y < PER; ++y) {
-            h8_t f[2];
+            h8_t f;
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
                 _Float16 hi, lo;
                 split_f16(have ? ldexpf(qv[x][y][j], -e) : 0.f, hi, lo);
-                f[0][j] = Q8 || c16 < 8 ? hi : lo;
-                f[1][j] = lo;
+                f[j] = c16 < 8 ? hi : lo;
             }
-#pragma unroll
-            for (int k = 0; k < TERMS; ++k) terms[x][k][PER * w + y][lane] = f[k];
+            terms[x][PER * w + y][lane] = f;
         }
     }
     __syncthreads();
-    h8_t qf[GQ][TERMS][KB];
+    h8_t qf[GQ][KB];
 #pragma unroll
     for (int x = 0; x < GQ; ++x)
 #pragma unroll
-        for (int k = 0; k < TERMS; ++k)
-#pragma unroll
-            for (int y = 0; y < KB; ++y) qf[x][k][y] = terms[x][k][y][lane];
+        for (int y = 0; y < KB; ++y) qf[x][y] = terms[x][y][lane];
 
     const int hp = ps / 16, halves = ne * hp, step_e = 8 / hp, step_b = 8 % hp;
     const int wu = __builtin_amdgcn_readfirstlane(w);
@@ -790,7 +787,7 @@ __global__ __launch_bounds__(256) void attn_sparse_kernel(SparseAttnArgs a, int 
         // of 146 for 500 rows' loads alone), 16 bytes each; of heads of 128 channels
         // a unit ahead, for 256 there are not the registers
         constexpr int LOADS = 2 * CH / 4;  // of 1024 bytes, half of them a half
-        constexpr bool AHEAD = DH == 128 && R == 1;
+        constexpr bool AHEAD = DH == 128 && R == 1 && !Q8;
         v4i_t staged[LOADS];
         auto stage = [&](const int (&page)[2], const int (&off)[2]) {
 #pragma unroll
@@ -868,7 +865,7 @@ __global__ __launch_bounds__(256) void attn_sparse_kernel(SparseAttnArgs a, int 
                     for (int k = 0; k < KB; ++k) {
                         const h8_t kf = *reinterpret_cast<const h8_t*>(tile + get_at(hf, k));
 #pragma unroll
-                        for (int x = 0; x < GQ; ++x) acc[x][hf] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf, qf[x][0][k], acc[x][hf], 0, 0, 0);
+                        for (int x = 0; x < GQ; ++x) acc[x][hf] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf, qf[x][k], acc[x][hf], 0, 0, 0);
                     }
                 }
                 h8_t pf[GQ];
@@ -960,8 +957,7 @@ __global__ __launch_bounds__(256) void attn_sparse_kernel(SparseAttnArgs a, int 
 #pragma unroll
                         for (int x = 0; x < GQ; ++x) {
                             f4_t acc = {0.f, 0.f, 0.f, 0.f};
-                            acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf, qf[x][1][k], acc, 0, 0, 0);
-                            acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf, qf[x][0][k], acc, 0, 0, 0);
+                            acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf, qf[x][k], acc, 0, 0, 0);
 #pragma unroll
                             for (int i = 0; i < 4; ++i) s[x][hf][i] = __builtin_fmaf(float(steps[i >> 1][4 * (i & 1) + k]), acc[i], s[x][hf][i]);
                         }
@@ -969,7 +965,7 @@ __global__ __launch_bounds__(256) void attn_sparse_kernel(SparseAttnArgs a, int 
 #pragma unroll
                     for (int x = 0; x < GQ; ++x)
 #pragma unroll
-                        for (int i = 0; i < 4; ++i) s[x][hf][i] = 4 * g4 + i < mine[x][hf] ? s[x][hf][i] * qscale[x] : -INFINITY;
+                        for (int i = 0; i < 4; ++i) s[x][hf][i] = 4 * g4 + i < mine[x][hf] ? (s[x][hf][i] + column_other(s[x][hf][i])) * qscale[x] : -INFINITY;
                 }
                 // the column's value steps, 2^-ve times, 0 past the keys
                 float d[8], dmax = 0.f;
