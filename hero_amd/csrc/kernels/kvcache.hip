@@ -13,9 +13,16 @@
 // page that this call writes, and reads the page's earlier keys back from the
 // pool, so the summary needs no second launch, no atomics and nothing kept
 // from earlier calls. The chain of a row's squares is as long as the row (one
-// dependent add per channel); lanes of one wave run the chains of up to 64
+// dependent add per channel); lanes of one wave run the chains of up to 32
 // rows side by side. Everything else is 32 lanes per row, four neighbouring
 // channels each, so that a row is read and written in whole words.
+//
+// Bound: for single tokens the dependent reads (position, page id, row), the chain
+// (0.4 us) and the exchange of the bounds: 5.1 us for one row of 32 + 8 heads of
+// 128, 6.7 us for sixteen rows into Q8_0 pages that hold 32 keys on average. For
+// chunks the same latencies and HBM: 1000 rows (41 MB) 15 to 16 us, 8.6 us at a
+// large copy's 4.76 TB/s. Reading back 8192 Q8_0 rows as fp32 (85 MB): 18.3 us,
+// 4.6 TB/s, as a copy.
 #include "hero/device.hpp"
 #include "hero/kernels.hpp"
 #include "hero/paged.hpp"

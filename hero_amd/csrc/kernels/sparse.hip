@@ -30,7 +30,16 @@ namespace {
 // power of two) times RT rows, which share the pages' reads where they belong
 // to one sequence. Both operands are loaded where they are used: lane 16 g + c
 // reads 16 consecutive bytes of page c, and holds the same bytes of column c's
-// codes; it gets the sums of pages 4 g .. 4 g + 3 for column c.
+// codes; it gets the sums of pages 4 g .. 4 g + 3 for column c. The codes are
+// formed once per workgroup, a wave per head.
+//
+// Bound: one token over 500 pages (1 MB of summaries): latency, 9 us in one
+// launch -- three dependent reads, some 600 instructions that run once, and five
+// to seven rounds of the search. Sixteen tokens over 2047 pages each (67 MB): 20
+// us for the scores, 3.3 TB/s of reads that are 256 bytes apart from each other
+// in no order, and 9 us for the choice; 14.4 us at a copy's rate. 500 rows of a
+// chunk over 251 to 258 pages: 18 us, vector instructions (the exact scores take
+// 64-bit products and maxima, about 45 instructions for four pages and rows).
 typedef int v4i_t __attribute__((ext_vector_type(4)));
 
 __device__ __forceinline__ float max_over_rows(float x) {  // over the four g of a column
@@ -425,12 +434,14 @@ __global__ __launch_bounds__(1024) void choose_pages_long_kernel(SelectArgs a) {
 // A workgroup of four waves per (row, K/V head, range of its list); a wave
 // takes 32 key slots at a time, two halves of 16 that each lie in one page.
 //
-// Both products run on the matrix cores with every operand where its load or
-// the product before put it, nothing through shared memory and no lane
-// exchanged (lane = 16 g + c below):
+// Both products run on the matrix cores, and no lane exchanges anything between
+// them (lane = 16 g + c below):
 //   scores   S^T[key][column] = K Q^T, 16 keys x 16 columns x 32 channels. Lane
-//            (g, c) loads 16 bytes of key c, and gets the scores of keys 4 g ..
-//            4 g + 3 for column c.
+//            (g, c) brings 16 bytes of key c, and gets the scores of keys 4 g ..
+//            4 g + 3 for column c. A load whose neighbouring lanes read
+//            different rows takes several times as long as one of whole rows, so
+//            the keys are read as whole rows and pass through a tile of shared
+//            memory that is the wave's own.
 //   values   O^T[channel][column] += V^T P^T, 16 channels x 16 columns x 32
 //            keys. The order of the 32 keys is free as long as both operands
 //            agree, so a lane's eight scores (keys 4 g .. 4 g + 3 of both
@@ -438,21 +449,28 @@ __global__ __launch_bounds__(1024) void choose_pages_long_kernel(SelectArgs a) {
 //            channels 8 c .. 8 c + 7: whole rows per load, transposed in the
 //            lane's registers. Product e covers channels 8 c + e, and a lane
 //            ends with 32 consecutive channels of its column's head.
-// (Keys alone pass through shared memory first: a load whose neighbouring lanes
-// read different rows takes several times as long.)
 // The matrix cores multiply fp16; queries and weights are fp32. Each is split
 // into two fp16 terms (22 bits). A head's query is scaled by a power of two to
 // at most 1 first, and a weight is 2^13 e^(s - m) with m at most 2 (base 2) below
 // the running maximum, so that neither term leaves fp16's range: terms are
-// dropped below 2^-38 of the largest. Keys and values of fp16 pages are exact, and
-// the up to eight heads of a group times two terms are the 16 columns (head h
-// in columns h and h + 8, added at the end).
+// dropped below 2^-38 of the largest. The up to eight heads of a group (or of
+// several rows) times two terms are the 16 columns: head h in columns h and h +
+// 8, added where both are done.
+// fp16 pages: keys and values are exact.
 // Q8_0 pages: codes are exact in fp16. A key block's product is scaled by the
 // block's step afterwards. A value block's step goes into the weights: column
 // (block, head) holds weights times that block's steps, for four heads at a
 // time, and of its result the 32 channels of that block count. The steps'
 // power of two is kept apart per column (`ve`), as theirs range as widely as
 // fp16 does.
+//
+// Bound: few tokens, latency (one token over 2048 keys 6.3 us, and 3.9 for
+// merging the ranges); batches of tokens, HBM: sixteen over 2048 Q8_0 keys each
+// (71 MB) 19 us, eight over 48 pages of 256-wide heads (101 MB) 22 us, sixteen
+// over 32 fp16 pages (134 MB) 30 us, 3.7 to 4.6 TB/s of a copy's 4.76, and the
+// merge 4 us. Chunks, what L2 gives and the vector instructions around the
+// products: 500 rows over 16 pages each read 1.5 GB through L2 for 92 MB of
+// distinct bytes, 89 us (Q8_0 pages 140 us, vector instructions).
 typedef _Float16 h8_t __attribute__((ext_vector_type(8)));
 typedef _Float16 h2_t __attribute__((ext_vector_type(2)));
 typedef float f4_t __attribute__((ext_vector_type(4)));
@@ -511,7 +529,7 @@ struct SparseMerge {  // the four waves' results; a slot per (row, head)
 
 // The pages of R rows' lists, each once with the rows' key counts: a page that
 // several rows of one sequence select is read once for all of them. `top`
-// entries a row, at most 128; a page's second place in one list stays an entry
+// entries a row, at most 512 together; a page's second place in one list stays an entry
 // of its own. Entries in the order of row 0's list, then what row 1 adds, ...;
 // returns their number.
 struct UnionScratch {
@@ -1247,9 +1265,15 @@ void sparse_rows(const SparseAttnArgs& a, int per, int nsplit, hipStream_t s) {
 }
 
 // Chunks with enough rows to fill the chip take several rows a workgroup, so
-// that a page which neighbouring rows select is read once for them.
+// that a page which neighbouring rows select is read once for them: lists of 16
+// pages of 32 query heads break even at 128 rows (34 us; 64 rows 29 against 20 us
+// alone), lists of 128 pages take 137 against 180 us there and 433 against 600 us
+// at 500 rows. 512 list entries a workgroup are what its scratch holds. Groups of
+// more than four heads fill the columns by themselves, and Q8_0 pages, whose
+// values and weights cost more instructions than their reads time, gain nothing.
 bool sparse_shares(const SparseAttnArgs& a) {
-    return a.c.row_seq && !a.c.q8 && a.top <= 128 && a.Hq / a.c.Hkv <= 4 && int64_t(a.c.rows) * a.c.Hkv >= 1024;
+    const int group = a.Hq / a.c.Hkv;
+    return a.c.row_seq && !a.c.q8 && group <= 4 && a.top <= (group <= 2 ? 128 : 256) && int64_t(a.c.rows) * a.c.Hkv >= 1024;
 }
 }  // namespace
 

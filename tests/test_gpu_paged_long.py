@@ -611,7 +611,8 @@ def chunk_lists(rng, seq, pos, ps, hkv, top):
 
 
 CHUNKS = [(False, 128, 64, 32, 8, 6), (False, 128, 16, 24, 8, 20), (False, 128, 32, 16, 8, 9), (False, 128, 64, 8, 8, 5), (False, 256, 64, 32, 8, 4), (False, 256, 16, 16, 8, 11),
-          (False, 128, 48, 64, 8, 7), (True, 128, 64, 32, 8, 6), (True, 128, 16, 16, 8, 20), (True, 128, 64, 64, 8, 5), (False, 128, 64, 32, 8, 128), (False, 128, 64, 32, 8, 129)]
+          (False, 128, 48, 64, 8, 7), (True, 128, 64, 32, 8, 6), (True, 128, 16, 16, 8, 20), (True, 128, 64, 64, 8, 5), (False, 128, 64, 32, 8, 128), (False, 128, 64, 16, 8, 129),
+          (False, 128, 16, 32, 8, 256), (False, 128, 16, 24, 8, 257)]
 
 
 @pytest.mark.parametrize("q8,dh,ps,hq,hkv,top", CHUNKS)
