@@ -200,6 +200,18 @@ def test_append_ignores_bad_pages_and_positions_past_the_rope_table(lib, q8):
     check_append(before, c, 4, seq, pos, table, ran, rope=75)
 
 
+def test_append_of_thousands_of_rows(lib):
+    """More rows than one look of the workgroups that search for runs takes in:
+    a long chunk, then rows of many sequences."""
+    rng = np.random.default_rng(61)
+    c = Cache(rng, 130, 66, 1, 128, 64)
+    n = 4100
+    seq, pos = [0] * n + list(range(1, 130)), list(range(63, 63 + n)) + [int(p) for p in rng.integers(0, 66 * 64, 129)]
+    before = copy_of(c)
+    ran = run_append(lib, rng, c, 1, seq, pos)
+    check_append(before, c, 1, seq, pos, c.table, ran)
+
+
 @pytest.mark.parametrize("q8,dh,ps", [(False, 128, 16), (False, 128, 64), (True, 128, 16), (True, 128, 64), (False, 256, 64)])
 def test_append_stores_what_the_decode_attention_stores(lib, q8, dh, ps):
     """Token by token through hero_attn_decode_paged and in one chunk through
@@ -346,6 +358,41 @@ def test_select_of_single_tokens_over_short_and_long_contexts(lib, pages, ps, to
     assert np.array_equal(got, select_reference(q, codes, steps, table, [0, 1], pos, ps, 2048, top, 1, 2))
 
 
+@pytest.mark.parametrize("hq,hkv,dh,pages,ps,top", [(8, 2, 128, 600, 64, 20), (8, 2, 128, 1030, 64, 40), (16, 2, 256, 1100, 16, 30), (4, 2, 128, 4200, 16, 64), (8, 1, 128, 16500, 16, 100),
+                                                    (2, 2, 128, 1024, 16, 500)])
+def test_select_of_chunks_over_long_contexts(lib, hq, hkv, dh, pages, ps, top):
+    """Rows of two sequences in one tile, at the ends of long lists."""
+    rng = np.random.default_rng(pages + top)
+    codes, steps, q = select_inputs(rng, 3000, hkv, hq, dh, 9)
+    table = rng.integers(0, 3000, (2, pages)).astype(np.int32)
+    seq, pos = [0] * 6 + [1] * 3, [pages * ps - 6 + i for i in range(6)] + [pages * ps // 2 + i for i in range(3)]
+    got = run_select(lib, q, codes, steps, table, seq, pos, ps, 3000, top, 1, 2)
+    assert np.array_equal(got, select_reference(q, codes, steps, table, seq, pos, ps, 3000, top, 1, 2))
+
+
+@pytest.mark.parametrize("pages", [100, 700, 5000])
+@pytest.mark.parametrize("good", [0, 3])
+def test_select_where_hardly_a_page_holds_anything(lib, pages, good):
+    """Pages that hold nothing rank behind those that do, and among themselves by
+    number; NaN steps and queries stay inside their rows."""
+    rng = np.random.default_rng(pages)
+    codes, steps, q = select_inputs(rng, 200, 2, 8, 128, 3)
+    table = np.full((3, pages), -1, np.int32)
+    for s in range(3):
+        table[s, rng.permutation(pages)[:good]] = np.arange(good)
+    pos = [pages * 16 - 1] * 3
+    got = run_select(lib, q, codes, steps, table, range(3), pos, 16, 200, 12, 1, 2, row_seq=False)
+    want = select_reference(q, codes, steps, table, range(3), pos, 16, 200, 12, 1, 2)
+    assert np.array_equal(got, want)
+    steps[7] = np.nan
+    q[1, 2, 5], q[1, 6, 0] = np.nan, np.inf
+    table[0, 5] = 7
+    again = run_select(lib, q, codes, steps, table, range(3), pos, 16, 200, 12, 1, 2, row_seq=False)
+    assert np.array_equal(again[2], want[2])
+    for r in (0, 1):  # some choice, in range, ascending, with the pages that are always there
+        assert np.all(np.diff(again[r], axis=1) > 0) and again[r].min() == 0 and again[r].max() == pages - 1
+
+
 def test_select_breaks_ties_to_the_lowest_page(lib):
     """All pages alike, zero queries and zero steps: the first pages are taken;
     two values of the score: the larger first, then the first of the smaller."""
@@ -480,6 +527,26 @@ def test_attend_of_single_tokens(lib, q8, dh, ps, hq, hkv, top, b):
     sel = random_lists(rng, b, hkv, top, [p // ps + 1 for p in pos])
     got, act = run_attend(lib, c, hq, q, proj, range(b), pos, sel, row_seq=False)
     check_attend(c, hq, q, proj, range(b), pos, sel, got, act, rows=[0, b // 2, b - 1])
+
+
+@pytest.mark.parametrize("q8,dh,rows,top", [(False, 128, 70, 2100), (True, 128, 3, 4096), (False, 256, 66, 4096), (True, 128, 66, 2049)])
+def test_attend_of_very_long_lists(lib, q8, dh, rows, top):
+    """Lists longer than one workgroup takes in, of pages that are mostly not
+    there: in front, behind, and one here and there."""
+    rng = np.random.default_rng(top + rows)
+    hq, hkv, ps = 16, 8, 16
+    c = Cache(rng, 1, 40, hkv, dh, ps, q8)
+    pos = [int(p) for p in rng.integers(300, 640, rows)]
+    sel = np.full((rows, hkv, top), -1, np.int32)
+    for r in range(rows):
+        for g in range(hkv):
+            n = int(rng.integers(1, 19))
+            sel[r, g, rng.permutation(top)[:n]] = rng.permutation(19)[:n]
+    sel[0, 0] = -1
+    sel[1, 0, :] = np.where(np.arange(top) == top - 1, 3, -1)
+    q, proj = rng.standard_normal((rows, hq, dh)).astype(np.float32), rng.standard_normal((rows, 2 * hq * dh)).astype(np.float32)
+    got, act = run_attend(lib, c, hq, q, proj, [0] * rows, pos, sel)
+    check_attend(c, hq, q, proj, [0] * rows, pos, sel, got, act, rows=[0, 1, 2, rows // 2, rows - 1])
 
 
 @pytest.mark.parametrize("q8", [False, True])
