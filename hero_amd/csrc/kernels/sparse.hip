@@ -567,6 +567,7 @@ __device__ __forceinline__ int build_union(const SparseAttnArgs& a, int g, int r
         const int j = x / top, lp = u.lp[x];
         int owner = x;
         bool again = false;
+#pragma unroll 8
         for (int y = j * top; y < x; ++y) again |= u.lp[y] == lp;
         if (!again) {
             int s = 0;
@@ -575,6 +576,7 @@ __device__ __forceinline__ int build_union(const SparseAttnArgs& a, int g, int r
 #pragma unroll
             for (int q = R - 2; q >= 0; --q) {  // the earliest row's first place wins
                 if (q >= j || seq[q] != s) continue;
+#pragma unroll 8
                 for (int y = (q + 1) * top - 1; y >= q * top; --y) owner = u.lp[y] == lp ? y : owner;
             }
         }
@@ -681,6 +683,24 @@ __global__ __launch_bounds__(256) void attn_sparse_kernel(SparseAttnArgs a, int 
     int get = c16 * ROW + (Q8 ? ((g4 >> 1) ^ (c16 >> 1 & 7)) * 16 + (g4 & 1) * 8 : (g4 ^ c16) * 16);
     auto put_at = [&](int n) { return 1024 * n + (put ^ ((64 / CH * n % 16 >> (Q8 ? 1 : 0)) * 16)); };
     auto get_at = [&](int hf, int k) { return 16 * hf * ROW + (get ^ (Q8 ? 32 * k : 64 * k)); };
+    // the columns' query terms: the first in columns 0 .. 7, the second in 8 .. 15
+    // (of the same heads). A wave forms its share of the 32-channel blocks for all
+    // four.
+    constexpr int PER = KB / 4;
+    __shared__ h8_t terms[GQ][KB][64];
+    __shared__ float biggest[GQ][4][16];
+    float qv[GQ][PER][8];  // on the way while the list is built
+#pragma unroll
+    for (int x = 0; x < GQ; ++x) {
+        const float* q_row = a.q_rot + (int64_t(min(r0 + row_of(x), c.rows - 1)) * a.Hq + g * group + min(head_of(x), group - 1)) * DH;
+#pragma unroll
+        for (int y = 0; y < PER; ++y) {
+            const float4* p = reinterpret_cast<const float4*>(q_row + 32 * (PER * w + y) + 8 * g4);
+            const float4 lo = p[0], hi = p[1];
+            qv[x][y][0] = lo.x, qv[x][y][1] = lo.y, qv[x][y][2] = lo.z, qv[x][y][3] = lo.w;
+            qv[x][y][4] = hi.x, qv[x][y][5] = hi.y, qv[x][y][6] = hi.z, qv[x][y][7] = hi.w;
+        }
+    }
     int ne;
     if constexpr (R > 1) {
         static_assert(sizeof(UnionScratch) <= sizeof(shared_mem));
@@ -699,26 +719,13 @@ __global__ __launch_bounds__(256) void attn_sparse_kernel(SparseAttnArgs a, int 
         }
     }
 
-    // the columns' query terms: the first in columns 0 .. 7, the second in 8 .. 15
-    // (of the same heads). A wave forms its share of the 32-channel blocks for all
-    // four.
-    constexpr int PER = KB / 4;
-    __shared__ h8_t terms[GQ][KB][64];
-    __shared__ float biggest[GQ][4][16];
-    float qv[GQ][PER][8];
 #pragma unroll
     for (int x = 0; x < GQ; ++x) {
-        const float* q_row = a.q_rot + (int64_t(min(r0 + row_of(x), c.rows - 1)) * a.Hq + g * group + min(head_of(x), group - 1)) * DH;
         float amax = 0.f;
 #pragma unroll
-        for (int y = 0; y < PER; ++y) {
-            const float4* p = reinterpret_cast<const float4*>(q_row + 32 * (PER * w + y) + 8 * g4);
-            const float4 lo = p[0], hi = p[1];
-            qv[x][y][0] = lo.x, qv[x][y][1] = lo.y, qv[x][y][2] = lo.z, qv[x][y][3] = lo.w;
-            qv[x][y][4] = hi.x, qv[x][y][5] = hi.y, qv[x][y][6] = hi.z, qv[x][y][7] = hi.w;
+        for (int y = 0; y < PER; ++y)
 #pragma unroll
             for (int j = 0; j < 8; ++j) amax = fmaxf(amax, fabsf(qv[x][y][j]));
-        }
         amax = max_over_rows(amax);
         if (g4 == 0) biggest[x][w][c16] = amax;
     }
