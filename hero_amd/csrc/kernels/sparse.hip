@@ -28,18 +28,18 @@ namespace {
 // Scores are int8 matrix products of 16 pages x 16 columns x 64 bytes: the
 // columns are the query heads of a K/V head (GP, the group rounded up to a
 // power of two) times RT rows, which share the pages' reads where they belong
-// to one sequence. Both operands are loaded where they are used: lane 16 g + c
-// reads 16 consecutive bytes of page c, and holds the same bytes of column c's
-// codes; it gets the sums of pages 4 g .. 4 g + 3 for column c. The codes are
-// formed once per workgroup, a wave per head.
+// to one sequence. Lane 16 g + c brings 16 bytes of page c and the same bytes of
+// column c's codes, and gets the sums of pages 4 g .. 4 g + 3 for column c. The
+// codes are formed once per workgroup, a wave per head.
 //
-// Bound: one token over 500 pages (1 MB of summaries): latency, 9 us in one
+// Bound: one token over 500 pages (1 MB of summaries): latency, 8.4 us in one
 // launch -- three dependent reads, some 600 instructions that run once, and five
-// to seven rounds of the search. Sixteen tokens over 2047 pages each (67 MB): 20
-// us for the scores, 3.3 TB/s of reads that are 256 bytes apart from each other
-// in no order, and 9 us for the choice; 14.4 us at a copy's rate. 500 rows of a
-// chunk over 251 to 258 pages: 18 us, vector instructions (the exact scores take
-// 64-bit products and maxima, about 45 instructions for four pages and rows).
+// to seven rounds of the search. Sixteen tokens over 2047 pages each (67 MB): 18
+// to 20 us for the scores, 3.5 TB/s of records that lie 256 bytes at a time in no
+// order (sixty-four tokens: 3.7 TB/s), and 8 us for the choice; 14.4 us at a
+// copy's rate. 500 rows of a chunk over 251 to 258 pages: 18 us, vector
+// instructions (the exact scores take 64-bit products and maxima, about 45
+// instructions for four pages and rows).
 typedef int v4i_t __attribute__((ext_vector_type(4)));
 
 __device__ __forceinline__ float max_over_rows(float x) {  // over the four g of a column
@@ -106,9 +106,10 @@ __device__ __forceinline__ void form_codes(const SelectArgs& a, int g, int r0, Q
 // row sees, of the rows that see more than `top`. Contains the workgroup's
 // barrier between forming the codes and using them.
 template <int DH, int GP, int RT, class Store>
-__device__ __forceinline__ void score_pages(const SelectArgs& a, int g, int r0, int first, int stride, QueryCodes<DH, GP, RT>& qc, Store store) {
+__device__ __forceinline__ void score_pages(const SelectArgs& a, int g, int r0, int first, int stride, QueryCodes<DH, GP, RT>& qc, char* tile, Store store) {
     constexpr int KS = DH / 32;                           // 64-byte steps of [max | -min]
-    constexpr int TT = DH == 128 ? 4 : 2;                 // tiles of 16 pages in flight
+    constexpr int ROW = 2 * DH, CH = ROW / 16;            // a page's bounds, and its 16-byte chunks
+    constexpr int TT = DH == 128 && RT == 1 ? 4 : 2;      // tiles of 16 pages in flight (four of several rows spill)
     constexpr int CG = RT > 1 ? 1 : GP == 8 ? 2 : TT;     // a lone row's repeated columns finish this many tiles at once
     const PagedRows& c = a.c;
     const int lane = threadIdx.x & 63, g4 = lane >> 4, c16 = lane & 15, sub = c16 % GP, rt = RT > 1 ? c16 / GP : 0, cg = c16 / GP % CG;
@@ -130,7 +131,8 @@ __device__ __forceinline__ void score_pages(const SelectArgs& a, int g, int r0, 
     const double step = double(qc.step[col]);
     const int64_t page_bytes = kv_summary_page_bytes(c.Hkv, DH);
     const uint8_t* const steps_at = c.summaries + int64_t(c.Hkv) * 2 * DH + 4 * g;
-    const uint8_t* const codes_at = c.summaries + int64_t(g) * 2 * DH + 16 * g4;
+    const uint8_t* const codes_at = c.summaries + int64_t(g) * 2 * DH;
+    const int put = lane / CH * ROW + (lane % CH ^ lane / CH) * 16, get = c16 * ROW + (g4 ^ c16) * 16;
     while (const uint64_t left = __ballot(todo)) {  // the rows of one sequence at a time
         const int s0 = RT == 1 ? __builtin_amdgcn_readfirstlane(seq) : __shfl(seq, __ffsll((unsigned long long)left) - 1);
         const bool mine = todo && seq == s0;
@@ -150,18 +152,24 @@ __device__ __forceinline__ void score_pages(const SelectArgs& a, int g, int r0, 
 #pragma unroll 1
             for (int t0 = 0; t0 < 4; t0 += TT) {
                 if (64 * k + 16 * t0 >= most) break;
+                // whole records are read (KS loads a tile, 1024 bytes each) and pass
+                // through the wave's tile, chunk k of record r at k ^ r: the product
+                // wants 16 lanes on 16 records, which a load does as 64 requests
                 v4i_t b[TT][KS], sum[TT];
 #pragma unroll
-                for (int t = 0; t < TT; ++t) {
-                    const v4i_t* src = reinterpret_cast<const v4i_t*>(codes_at + int64_t(uint32_t(__shfl(id_l, 16 * (t0 + t) + c16))) * page_bytes);
+                for (int t = 0; t < TT; ++t)
 #pragma unroll
-                    for (int s = 0; s < KS; ++s) b[t][s] = src[4 * s];
-                }
+                    for (int n = 0; n < KS; ++n) {
+                        const int from = 16 * (t0 + t) + (64 * n + lane) / CH;
+                        b[t][n] = *reinterpret_cast<const v4i_t*>(codes_at + int64_t(uint32_t(__shfl(id_l, from))) * page_bytes + lane % CH * 16);
+                    }
 #pragma unroll
                 for (int t = 0; t < TT; ++t) {
+#pragma unroll
+                    for (int n = 0; n < KS; ++n) *reinterpret_cast<v4i_t*>(tile + 1024 * n + (put ^ (64 / CH * n % 16 * 16))) = b[t][n];
                     sum[t] = v4i_t{0, 0, 0, 0};
 #pragma unroll
-                    for (int s = 0; s < KS; ++s) sum[t] = __builtin_amdgcn_mfma_i32_16x16x64_i8(b[t][s], q[s], sum[t], 0, 0, 0);
+                    for (int s = 0; s < KS; ++s) sum[t] = __builtin_amdgcn_mfma_i32_16x16x64_i8(*reinterpret_cast<const v4i_t*>(tile + (get ^ 64 * s)), q[s], sum[t], 0, 0, 0);
                 }
 #pragma unroll
                 for (int t = 0; t < TT; t += CG)
@@ -337,8 +345,8 @@ __device__ __forceinline__ int row_sees(const PagedRows& c, int r) {
 // The waves of a workgroup score up to 512 (a lone row) or 1024 pages for RT rows
 // into shared memory, then a wave per row chooses: its counts need no barrier.
 // Longer lists of a lone row are faster over many workgroups in two launches:
-// 1000 pages 12 against 15 us, 4000 pages 15 against 40 us (one sequence; the
-// same times for sixteen).
+// 1000 pages 11 to 12 against 15 us, 4000 pages 15 against 40 us (one sequence;
+// the same times for sixteen).
 template <int RT>
 constexpr int kSelThreads = RT == 1 ? 512 : 256;
 template <int DH, int GP, int RT>
@@ -347,7 +355,8 @@ __global__ __launch_bounds__(kSelThreads<RT>, 4) void select_pages_kernel(Select
     const int w = threadIdx.x >> 6, g = blockIdx.x % c.Hkv, r0 = blockIdx.x / c.Hkv * RT;
     extern __shared__ __align__(16) uint64_t sel_keys[];  // [RT][max_pages]
     __shared__ QueryCodes<DH, GP, RT> qc;
-    score_pages<DH, GP, RT>(a, g, r0, w, kSelThreads<RT> / 64, qc, [&](int rt, int page, uint64_t k) { sel_keys[rt * c.max_pages + page] = k; });
+    __shared__ __align__(16) char tiles[kSelThreads<RT> / 64][32 * DH];
+    score_pages<DH, GP, RT>(a, g, r0, w, kSelThreads<RT> / 64, qc, tiles[w], [&](int rt, int page, uint64_t k) { sel_keys[rt * c.max_pages + page] = k; });
     __syncthreads();
     const int r = r0 + w;
     if (w >= RT || r >= c.rows) return;
@@ -370,7 +379,8 @@ __global__ __launch_bounds__(256, 4) void page_scores_kernel(SelectArgs a) {
     const PagedRows& c = a.c;
     const int w = threadIdx.x >> 6, g = blockIdx.x % c.Hkv, r0 = blockIdx.x / c.Hkv * RT;
     __shared__ QueryCodes<DH, GP, RT> qc;
-    score_pages<DH, GP, RT>(a, g, r0, blockIdx.y * 4 + w, gridDim.y * 4, qc,
+    __shared__ __align__(16) char tiles[4][32 * DH];
+    score_pages<DH, GP, RT>(a, g, r0, blockIdx.y * 4 + w, gridDim.y * 4, qc, tiles[w],
                             [&](int rt, int page, uint64_t k) { a.keys[(int64_t(r0 + rt) * c.Hkv + g) * c.max_pages + page] = k; });
 }
 // ... then a workgroup per (row, K/V head) chooses among up to KPL NT pages
@@ -1216,7 +1226,9 @@ void select_rows(const SelectArgs& a, hipStream_t s) {
     // a workgroup's four waves take 64 pages each at a time; about four workgroups per CU
     const unsigned most = unsigned((c.max_pages + 255) / 256), ranges = std::min(most, std::max(1u, 1024 / tiles));
     hipLaunchKernelGGL((page_scores_kernel<DH, GP, RT>), dim3(tiles, ranges), dim3(256), 0, s, a);
-    if (c.max_pages <= 4096)
+    if (c.max_pages <= 2048)
+        hipLaunchKernelGGL((choose_pages_kernel<256, 8>), dim3(heads), dim3(256), 0, s, a);
+    else if (c.max_pages <= 4096)
         hipLaunchKernelGGL((choose_pages_kernel<512, 8>), dim3(heads), dim3(512), 0, s, a);
     else if (c.max_pages <= 16384)
         hipLaunchKernelGGL((choose_pages_kernel<1024, 16>), dim3(heads), dim3(1024), 0, s, a);
