@@ -393,8 +393,8 @@ int64_t hero_kv_summary_bytes(int64_t pool_pages, int32_t hkv, int32_t head_dim)
  * over the page's slots up to the row's. Uses p.a.proj, proj_stride, k_off,
  * v_off, q_gamma, k_gamma, eps, rope_cs, positions, q_rot, b, hq, hkv, dh, the
  * page fields and everything above but selected, top, sink and recent. The rows
- * of one sequence stand together, positions ascending by one; a page belongs
- * to one sequence of the call. */
+ * of one sequence stand together, positions ascending by one and no left-out
+ * row between them; a page belongs to one sequence of the call. */
 int hero_kv_append_paged(const hero_attn_sparse_args* args, void* stream);
 
 /* Rows of the cache back as fp32 (exact) or fp16 (rounded once; exact for fp16
@@ -440,7 +440,10 @@ int hero_attn_select_pages(const hero_attn_sparse_args* args, void* stream);
  * one. Uses p.a.q_rot, proj (the gates), proj_stride, positions, score_scale, b,
  * hq, hkv, dh, the page fields and work (hero_attn_sparse_work_bytes, 16-byte
  * aligned). Results agree with the sequential reference over the stored keys
- * and values to fp32 rounding. */
+ * and values to fp32 rounding, save that a query's channels are kept to 2^-25 of
+ * the head's largest and weights to 2^-38 of the row's largest (Q8_0: weight
+ * times value step, to 2^-37 of the largest weight times the largest step the
+ * row meets in that block). */
 int64_t hero_attn_sparse_work_bytes(int64_t rows, int32_t hq, int32_t hkv, int32_t head_dim, int32_t page_size, int32_t top);
 int hero_attn_sparse_paged(const hero_attn_sparse_args* args, void* stream);
 

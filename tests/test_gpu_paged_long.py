@@ -450,7 +450,9 @@ def run_attend(lib, c, hq, q_rot, proj, seq, pos, sel, row_seq=True, act=True, o
     return host(d_out, np.float32, (rows, hq * c.dh)), host(d_act, np.uint8)
 
 
-def check_attend(c, hq, q_rot, proj, seq, pos, sel, got, act=None, table=None, rows=None, fill=0.0):
+def check_attend(c, hq, q_rot, proj, seq, pos, sel, got, act=None, table=None, rows=None, fill=0.0, dropped=0.0):
+    """`dropped`: what a weight may lose, as a part of the largest weight, per key, where the value
+    block's step is the largest of the row's keys."""
     values, dh, grp = c.values(), c.dh, hq // c.hkv
     table = c.table if table is None else table
     scale = float(np.float32(1 / np.sqrt(dh)))
@@ -469,6 +471,9 @@ def check_attend(c, hq, q_rot, proj, seq, pos, sel, got, act=None, table=None, r
             k, v = np.concatenate(ks), np.concatenate(vs)
             for h in range(g * grp, (g + 1) * grp):
                 want, bound = attend_reference(q_rot[r, h].astype(np.float64), proj[r, h * 2 * dh + dh:(h + 1) * 2 * dh].astype(np.float64), k, v, scale)
+                if dropped:
+                    largest = np.repeat(np.abs(v).reshape(len(v), dh // 32, 32).max((0, 2)), 32)
+                    bound = bound + dropped * len(k) * largest
                 d = np.abs(got[r, h * dh:(h + 1) * dh] - want)
                 assert np.all(d <= bound), f"row {r} head {h}: {np.max(d / bound):.3g} of the bound"
         if act is not None:
@@ -646,6 +651,29 @@ def test_attend_of_values_of_every_size(lib):
     q, proj, sel = rng.standard_normal((1, 4, 128)).astype(np.float32), rng.standard_normal((1, 1024)).astype(np.float32), np.array([[[0, 1, 2]]], np.int32)
     got, act = run_attend(lib, c, 4, q, proj, [0], [180], sel)
     check_attend(c, 4, q, proj, [0], [180], sel, got, act)
+
+
+@pytest.mark.parametrize("rows", [1, 2, 5])
+@pytest.mark.parametrize("hq,hkv,ps", [(8, 2, 64), (8, 1, 16), (2, 1, 32)])
+def test_attend_over_steps_of_every_size(lib, rows, hq, hkv, ps):
+    """Q8_0 blocks whose steps run from fp16's smallest to 2^9, zeros among them. A
+    weight of at most 2^15 (the largest at least 2^13), times its step over a power of
+    two at most twice the largest step, is two fp16 terms, so off by at most 2^-25
+    where it is small: by 2 2^-25 / 2^13 = 2^-37 of the largest weight in units of the
+    largest step, or of codes up to 127 times it."""
+    rng = np.random.default_rng(90 + rows + hq)
+    c = Cache(rng, 1, 5, hkv, 128, ps, True)
+    shape = c.d[:, 0].shape
+    c.codes[..., ::32] = 127  # a block's largest value is 127 of its steps
+    c.d[:, 0] = (2.0 ** rng.integers(-18, -5, shape)).astype(np.float16)
+    c.d[:, 1] = (rng.integers(1, 4, shape) * 2.0 ** rng.integers(-24, 9, shape)).astype(np.float16)
+    c.d[:, 1][rng.random(shape) < 0.1] = 0
+    c.d[1::2, 1] *= np.float16(2.0 ** -6)
+    pos = [5 * ps - 9 + i for i in range(rows)]
+    q, proj = rng.standard_normal((rows, hq, 128)).astype(np.float32), rng.standard_normal((rows, 2 * hq * 128)).astype(np.float32)
+    sel = np.array([[[0, 2, 4] if (r + g) % 2 else [1, 3, 4] for g in range(hkv)] for r in range(rows)], np.int32)
+    got, act = run_attend(lib, c, hq, q, proj, [0] * rows, pos, sel)
+    check_attend(c, hq, q, proj, [0] * rows, pos, sel, got, act, dropped=2.0 ** -37)
 
 
 def test_rows_of_a_chunk_equal_single_tokens(lib):
