@@ -487,6 +487,7 @@ typedef float f4_t __attribute__((ext_vector_type(4)));
 
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kPShift = 13.f;  // weights are 2^13 2^(s - m)
+constexpr float kPOne = 8192.f;  // 2^kPShift
 constexpr float kPSlack = 2.f;   // m may lag the maximum by this: weights stay below 2^15
 
 __device__ __forceinline__ float column_other(float x) {  // the value of column c ^ 8
@@ -641,12 +642,91 @@ __device__ __forceinline__ void sparse_store(const SparseAttnArgs& a, int r, int
     }
 }
 
+// A (row, query head) over the keys of a workgroup's list that the row (its k-th)
+// sees, in plain fp32 by one wave: a lane per key for the scores, a lane per
+// channel, of 64 from `ch0` on, for the sum. A key of score -inf has weight 0;
+// where every key does, m is -inf and `any` true.
+template <int DH, bool Q8, int R>
+__device__ __forceinline__ void attend_plain(const SparseAttnArgs& a, int r, int k, int g, int h, int ch0, const ListEntry<R>* list, int ne, float& m, float& l, float& o,
+                                             bool& any) {
+    const PagedRows& c = a.c;
+    const int lane = threadIdx.x & 63;
+    const float* const q = a.q_rot + (int64_t(r) * a.Hq + h) * DH;
+    const float scale = a.score_scale * kLog2e;
+    m = -INFINITY, l = o = 0.f, any = false;
+#pragma unroll 1
+    for (int e = 0; e < ne; ++e) {
+        const int64_t page = list[e].page;
+        const int n = list[e].keys[k];
+        const _Float16* const fpage = f16_page<DH>(c, page);
+        const uint8_t* const qpage = q8_page<DH>(c, page);
+        const _Float16* const steps = reinterpret_cast<const _Float16*>(qpage + q8_scales_at<DH>(c));
+        any |= n > 0;
+#pragma unroll 1
+        for (int t0 = 0; t0 < n; t0 += 64) {
+            const bool mine = t0 + lane < n;
+            const int64_t krow = page_row_index(c, 0, g, mine ? t0 + lane : t0);
+            float s = 0.f;
+#pragma unroll 1
+            for (int ch = 0; ch < DH; ch += 8) {
+                float x[8];
+                if constexpr (Q8) {
+                    const int2 w = *reinterpret_cast<const int2*>(qpage + krow * DH + ch);
+                    const float d = float(steps[krow * (DH / 32) + ch / 32]);
+#pragma unroll
+                    for (int u = 0; u < 8; ++u) x[u] = d * float(int8_t((u < 4 ? w.x : w.y) >> (8 * (u & 3))));
+                } else {
+                    const h8_t w = *reinterpret_cast<const h8_t*>(fpage + krow * DH + ch);
+#pragma unroll
+                    for (int u = 0; u < 8; ++u) x[u] = float(w[u]);
+                }
+#pragma unroll
+                for (int u = 0; u < 8; ++u) s += q[ch + u] * x[u];
+            }
+            s = mine ? s * scale : -INFINITY;
+            float m2 = s;
+            for (int off = 32; off > 0; off >>= 1) m2 = fmaxf(m2, __shfl_xor(m2, off));
+            m2 = fmaxf(m, m2);
+            const float p = mine ? exp2_hw(s - (m2 == -INFINITY ? 0.f : m2)) : 0.f, f = m == -INFINITY ? 1.f : exp2_hw(m - m2);
+            m = m2;
+            float sum = p;
+            for (int off = 32; off > 0; off >>= 1) sum += __shfl_xor(sum, off);
+            l = l * f + sum;
+            o *= f;
+            const int last = min(64, n - t0);
+#pragma unroll 1
+            for (int j0 = 0; j0 < last; j0 += 8) {
+                float v[8];
+#pragma unroll
+                for (int j = 0; j < 8; ++j) {
+                    const int64_t at = page_row_index(c, 1, g, t0 + min(j0 + j, last - 1)) * DH + ch0 + lane;
+                    if constexpr (Q8)
+                        v[j] = float(steps[at / 32]) * float(int8_t(qpage[at]));
+                    else
+                        v[j] = float(fpage[at]);
+                }
+#pragma unroll
+                for (int j = 0; j < 8; ++j) o += __shfl(p, j0 + j) * (j0 + j < last ? v[j] : 0.f);
+            }
+        }
+    }
+}
+
 // R rows by GP heads each (fp16 pages: GP a power of two, in GQ sets of eight
 // columns times two terms; Q8_0 pages: GP 4 or 8, in GQ quads). R > 1: the rows
-// of a chunk, which mostly select the same pages. A row's columns get weight 0
-// for the pages of other rows; should those hold values that are not finite, 0
-// times them would reach the row, so a workgroup whose sums are not finite
-// works its rows off again one by one, over their own keys alone.
+// of a chunk, which mostly select the same pages.
+//
+// Infinities and NaNs: the two terms of a query or weight may differ in sign, or
+// one be 0, so that an infinite key or value turns a score or sum to NaN which
+// the definition has infinite; and a row's columns, of weight 0 for the pages of
+// other rows, get 0 times whatever those hold. All of it leaves a result that is
+// not finite. What leaves none is marked: a column all of whose keys score -inf
+// (NaN by the definition), and with Q8_0 any score of -inf (a block's infinite
+// step times the sum of its products, where products may be infinite of both
+// signs). A wave among whose 64 results (channels of one row and head) some are
+// not finite forms them again in plain fp32, over the row's own keys: sixteen Q8_0
+// sequences 219 us instead of 38 if every page holds such keys and values, 500
+// fp16 rows 1.8 ms instead of 0.11 (one call, waited for).
 template <int DH, bool Q8, int GQ, int R, int GP>
 __global__ __launch_bounds__(256) void attn_sparse_kernel(SparseAttnArgs a, int per, int nsplit) {
     constexpr int KB = DH / 32, VH = DH / 128;  // 32-channel blocks, 128-channel halves
@@ -772,385 +852,407 @@ __global__ __launch_bounds__(256) void attn_sparse_kernel(SparseAttnArgs a, int 
     const int64_t krow0 = int64_t(g) * ps, vrow0 = (int64_t(c.Hkv) + g) * ps;
     const char* const pool = reinterpret_cast<const char*>(c.pages);
     const float is_lo = c16 < 8 ? 0.f : 1.f;
-    float m[GQ], l[GQ];
+    float m[GQ], l[GQ], low[GQ];  // low: Q8_0, the smallest score, or 0
+    int saw[GQ];                  // whether the column has seen a key
     f4_t o[GQ][8 * VH];
-#pragma unroll 1
-    for (int only = -1; only < R; ++only) {  // -1: all rows; the others run only if that was not finite
 #pragma unroll
-        for (int x = 0; x < GQ; ++x) {
-            m[x] = -INFINITY;
-            l[x] = 0.f;
+    for (int x = 0; x < GQ; ++x) {
+        m[x] = -INFINITY;
+        l[x] = low[x] = 0.f;
+        saw[x] = 0;
 #pragma unroll
-            for (int e = 0; e < 8 * VH; ++e) o[x][e] = f4_t{0.f, 0.f, 0.f, 0.f};
-        }
-        int ve = -200;  // Q8_0: the column's accumulators are in units of 2^ve
+        for (int e = 0; e < 8 * VH; ++e) o[x][e] = f4_t{0.f, 0.f, 0.f, 0.f};
+    }
+    int ve = -200;  // Q8_0: the column's accumulators are in units of 2^ve
 
-        // the wave's units: halves 2 (w + 4 n) and the one behind, as entry and 16-key
-        // block; `next` finds the following one that holds keys
-        int entry[2], block[2], at = wu;
+    // the wave's units: halves 2 (w + 4 n) and the one behind, as entry and 16-key
+    // block; `next` finds the following one that holds keys
+    int entry[2], block[2], at = wu;
 #pragma unroll
-        for (int s = 0; s < 2; ++s) entry[s] = (2 * wu + s) / hp, block[s] = (2 * wu + s) % hp;
-        int next_page[2], next_off[2], next_nv[2], next_mine[GQ][2];
-        auto next = [&] {
-            while (2 * at < halves) {
-#pragma unroll
-                for (int s = 0; s < 2; ++s) {
-                    const ListEntry<R>& le = list[min(entry[s], ne - 1)];
-                    next_off[s] = 16 * block[s];
-                    next_page[s] = __builtin_amdgcn_readfirstlane(le.page);
-                    const bool real = 2 * at + s < halves;
-                    next_nv[s] = real ? __builtin_amdgcn_readfirstlane(max(0, min(16, int(R > 1 && only >= 0 ? le.keys[max(only, 0)] : le.most) - next_off[s]))) : 0;
-#pragma unroll
-                    for (int x = 0; x < GQ; ++x) {
-                        next_mine[x][s] = next_nv[s];
-                        if constexpr (R > 1) next_mine[x][s] = min(next_nv[s], max(0, int(le.keys[row_of(x)]) - next_off[s]));
-                    }
-                    entry[s] += step_e;
-                    block[s] += step_b;
-                    if (block[s] >= hp) block[s] -= hp, ++entry[s];
-                }
-                at += 4;
-                if (next_nv[0] + next_nv[1] == 0) continue;
-                if (next_nv[0] == 0) next_page[0] = next_page[1], next_off[0] = next_off[1];  // an entry of none names no page: read what is there, use nothing
-                if (next_nv[1] == 0) next_page[1] = next_page[0], next_off[1] = next_off[0];
-                return true;
-            }
-            return false;
-        };
-        // the keys through the wave's tile: read as whole rows, lane by lane on (16
-        // lanes on 16 rows, as the product wants them, are 64 requests a load: 118 us
-        // of 146 for 500 rows' loads alone), 16 bytes each; of heads of 128 channels
-        // a unit ahead, for 256 there are not the registers
-        constexpr int LOADS = 2 * CH / 4;  // of 1024 bytes, half of them a half
-        constexpr bool AHEAD = DH == 128 && R == 1 && !Q8;
-        v4i_t staged[LOADS];
-        auto stage = [&](const int (&page)[2], const int (&off)[2]) {
-#pragma unroll
-            for (int hf = 0; hf < 2; ++hf) {
-                const __amdgpu_buffer_rsrc_t b = buffer_of(pool + page[hf] * page_stride + (krow0 + off[hf]) * ROW, 16 * ROW);
-#pragma unroll
-                for (int k = 0; k < LOADS / 2; ++k) staged[hf * (LOADS / 2) + k] = __builtin_amdgcn_raw_buffer_load_b128(b, 16 * lane + 1024 * k, 0, 0);
-            }
-        };
-        bool more = next();
-        if (AHEAD && more) stage(next_page, next_off);
-        while (more) {
-            int page[2], off[2], nv[2], mine[GQ][2];  // keys of the half that any row, the set's column sees
+    for (int s = 0; s < 2; ++s) entry[s] = (2 * wu + s) / hp, block[s] = (2 * wu + s) % hp;
+    int next_page[2], next_off[2], next_nv[2], next_mine[GQ][2];
+    auto next = [&] {
+        while (2 * at < halves) {
 #pragma unroll
             for (int s = 0; s < 2; ++s) {
-                page[s] = next_page[s], off[s] = next_off[s], nv[s] = next_nv[s];
-#pragma unroll
-                for (int x = 0; x < GQ; ++x) mine[x][s] = next_mine[x][s];
-            }
-            const bool full = nv[0] + nv[1] == 32;
-            auto weights_base = [&](int x, const f4_t (&s)[2], const int (&sees)[2], auto rescale) {
-                float top = -INFINITY;
-#pragma unroll
-                for (int hf = 0; hf < 2; ++hf) {
-                    const float of = fmaxf(fmaxf(s[hf][0], s[hf][1]), fmaxf(s[hf][2], s[hf][3]));
-                    top = fmaxf(top, R > 1 && sees[hf] == 0 ? -INFINITY : of);
-                }
-                if (__any(top > m[x] + kPSlack)) {
-                    const float m2 = fmaxf(m[x], max_over_rows(top)), f = m2 == -INFINITY ? 1.f : exp2_hw(m[x] - m2);
-                    m[x] = m2;
-                    l[x] *= f;
-                    rescale(f);
-                }
-                return fmaxf(m[x], -3e38f) - kPShift;  // a column that has seen no key: 2^-inf, not NaN
-            };
-
-            if (!AHEAD) stage(page, off);
-            asm volatile("" : "+v"(put), "+v"(get));  // see put_at
-            __builtin_amdgcn_sched_barrier(0);  // a unit's loads are all in flight before the first is waited for
-            if constexpr (!Q8) {
-                h8_t vf[VH][8];
-                // 256 channels: the values take the keys' registers once those are in the
-                // tile, so that two workgroups fit a compute unit
-                constexpr bool LATE = DH == 256;
-#pragma unroll
-                for (int turn = 0; turn < 2; ++turn) {
-                    if (turn == (LATE ? 1 : 0)) {
-#pragma unroll
-                        for (int hf = 0; hf < 2; ++hf) {
-                            const __amdgpu_buffer_rsrc_t b = buffer_of(pool + page[hf] * page_stride + (vrow0 + off[hf]) * ROW, 16 * ROW);
-#pragma unroll
-                            for (int i = 0; i < 4; ++i)
-#pragma unroll
-                                for (int v = 0; v < VH; ++v)
-                                    vf[v][4 * hf + i] = __builtin_bit_cast(h8_t, __builtin_amdgcn_raw_buffer_load_b128(b, 8 * DH * g4 + 16 * c16 + 2 * DH * i + 256 * v, 0, 0));
-                        }
-                        __builtin_amdgcn_sched_barrier(0);
-                    } else {
-#pragma unroll
-                        for (int k = 0; k < LOADS; ++k) *reinterpret_cast<v4i_t*>(tile + put_at(k)) = staged[k];
-                        __builtin_amdgcn_sched_barrier(0);
-                        if (AHEAD) {
-                            more = next();
-                            if (more) stage(next_page, next_off);
-                        }
-                        __builtin_amdgcn_sched_barrier(0);
-                    }
-                }
-                f4_t acc[GQ][2];
-#pragma unroll
-                for (int hf = 0; hf < 2; ++hf) {
-#pragma unroll
-                    for (int x = 0; x < GQ; ++x) acc[x][hf] = f4_t{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-                    for (int k = 0; k < KB; ++k) {
-                        const h8_t kf = *reinterpret_cast<const h8_t*>(tile + get_at(hf, k));
-#pragma unroll
-                        for (int x = 0; x < GQ; ++x) acc[x][hf] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf, qf[x][k], acc[x][hf], 0, 0, 0);
-                    }
-                }
-                h8_t pf[GQ];
+                const ListEntry<R>& le = list[min(entry[s], ne - 1)];
+                next_off[s] = 16 * block[s];
+                next_page[s] = __builtin_amdgcn_readfirstlane(le.page);
+                const bool real = 2 * at + s < halves;
+                next_nv[s] = real ? __builtin_amdgcn_readfirstlane(max(0, min(16, int(le.most) - next_off[s]))) : 0;
 #pragma unroll
                 for (int x = 0; x < GQ; ++x) {
-                    f4_t s[2];
+                    next_mine[x][s] = next_nv[s];
+                    if constexpr (R > 1) next_mine[x][s] = min(next_nv[s], max(0, int(le.keys[row_of(x)]) - next_off[s]));
+                }
+                entry[s] += step_e;
+                block[s] += step_b;
+                if (block[s] >= hp) block[s] -= hp, ++entry[s];
+            }
+            at += 4;
+            if (next_nv[0] + next_nv[1] == 0) continue;
+            if (next_nv[0] == 0) next_page[0] = next_page[1], next_off[0] = next_off[1];  // an entry of none names no page: read what is there, use nothing
+            if (next_nv[1] == 0) next_page[1] = next_page[0], next_off[1] = next_off[0];
+            return true;
+        }
+        return false;
+    };
+    // the keys through the wave's tile: read as whole rows, lane by lane on (16
+    // lanes on 16 rows, as the product wants them, are 64 requests a load: 118 us
+    // of 146 for 500 rows' loads alone), 16 bytes each; of heads of 128 channels
+    // a unit ahead, for 256 there are not the registers
+    constexpr int LOADS = 2 * CH / 4;  // of 1024 bytes, half of them a half
+    constexpr bool AHEAD = DH == 128 && R == 1 && !Q8;
+    v4i_t staged[LOADS];
+    auto stage = [&](const int (&page)[2], const int (&off)[2]) {
 #pragma unroll
-                    for (int hf = 0; hf < 2; ++hf)
+        for (int hf = 0; hf < 2; ++hf) {
+            const __amdgpu_buffer_rsrc_t b = buffer_of(pool + page[hf] * page_stride + (krow0 + off[hf]) * ROW, 16 * ROW);
 #pragma unroll
-                        for (int i = 0; i < 4; ++i) s[hf][i] = (acc[x][hf][i] + column_other(acc[x][hf][i])) * qscale[x];
-                    // halves that a column sees in part are masked key by key, halves
-                    // that it does not see as a whole
-                    const bool partly = R == 1 ? !full : __any((mine[x][0] & 15) + (mine[x][1] & 15));
-                    if (partly) {
+            for (int k = 0; k < LOADS / 2; ++k) staged[hf * (LOADS / 2) + k] = __builtin_amdgcn_raw_buffer_load_b128(b, 16 * lane + 1024 * k, 0, 0);
+        }
+    };
+    bool more = next();
+    if (AHEAD && more) stage(next_page, next_off);
+    while (more) {
+        int page[2], off[2], nv[2], mine[GQ][2];  // keys of the half that any row, the set's column sees
 #pragma unroll
-                        for (int i = 0; i < 8; ++i)
-                            if (4 * g4 + (i & 3) >= mine[x][i >> 2]) s[i >> 2][i & 3] = -INFINITY;
-                    }
-                    const float base = weights_base(x, s, mine[x], [&](float f) {
+        for (int s = 0; s < 2; ++s) {
+            page[s] = next_page[s], off[s] = next_off[s], nv[s] = next_nv[s];
 #pragma unroll
-                        for (int e = 0; e < 8 * VH; ++e) o[x][e] *= f;
-                    });
+            for (int x = 0; x < GQ; ++x) mine[x][s] = next_mine[x][s], saw[x] |= mine[x][s];
+        }
+        const bool full = nv[0] + nv[1] == 32;
+        auto weights_base = [&](int x, const f4_t (&s)[2], const int (&sees)[2], auto rescale) {
+            float top = -INFINITY;
+#pragma unroll
+            for (int hf = 0; hf < 2; ++hf) {
+                const float of = fmaxf(fmaxf(s[hf][0], s[hf][1]), fmaxf(s[hf][2], s[hf][3]));
+                top = fmaxf(top, R > 1 && sees[hf] == 0 ? -INFINITY : of);
+            }
+            if (__any(top > m[x] + kPSlack)) {
+                const float m2 = fmaxf(m[x], max_over_rows(top)), f = m2 == -INFINITY ? 1.f : exp2_hw(m[x] - m2);
+                m[x] = m2;
+                l[x] *= f;
+                rescale(f);
+            }
+            return fmaxf(m[x], -3e38f) - kPShift;  // a column that has seen no key: 2^-inf, not NaN
+        };
+
+        if (!AHEAD) stage(page, off);
+        asm volatile("" : "+v"(put), "+v"(get));  // see put_at
+        __builtin_amdgcn_sched_barrier(0);  // a unit's loads are all in flight before the first is waited for
+        if constexpr (!Q8) {
+            h8_t vf[VH][8];
+            // 256 channels: the values take the keys' registers once those are in the
+            // tile, so that two workgroups fit a compute unit
+            constexpr bool LATE = DH == 256;
+#pragma unroll
+            for (int turn = 0; turn < 2; ++turn) {
+                if (turn == (LATE ? 1 : 0)) {
 #pragma unroll
                     for (int hf = 0; hf < 2; ++hf) {
-                        const float less = R > 1 && mine[x][hf] == 0 ? INFINITY : base;
+                        const __amdgpu_buffer_rsrc_t b = buffer_of(pool + page[hf] * page_stride + (vrow0 + off[hf]) * ROW, 16 * ROW);
 #pragma unroll
-                        for (int i = 0; i < 4; ++i) {
-                            float p = exp2_hw(s[hf][i] - less);
-                            asm("" : "+v"(p));
-                            l[x] += p;
-                            // the column's term: fp16(p), or of the rest (is_lo 1)
-                            const float rest = __builtin_fmaf(-float(_Float16(p)), is_lo, p);
-                            pf[x][4 * hf + i] = _Float16(rest);
-                        }
+                        for (int i = 0; i < 4; ++i)
+#pragma unroll
+                            for (int v = 0; v < VH; ++v)
+                                vf[v][4 * hf + i] = __builtin_bit_cast(h8_t, __builtin_amdgcn_raw_buffer_load_b128(b, 8 * DH * g4 + 16 * c16 + 2 * DH * i + 256 * v, 0, 0));
                     }
+                    __builtin_amdgcn_sched_barrier(0);
+                } else {
+#pragma unroll
+                    for (int k = 0; k < LOADS; ++k) *reinterpret_cast<v4i_t*>(tile + put_at(k)) = staged[k];
+                    __builtin_amdgcn_sched_barrier(0);
+                    if (AHEAD) {
+                        more = next();
+                        if (more) stage(next_page, next_off);
+                    }
+                    __builtin_amdgcn_sched_barrier(0);
                 }
-                if (!full) {
+            }
+            f4_t acc[GQ][2];
+#pragma unroll
+            for (int hf = 0; hf < 2; ++hf) {
+#pragma unroll
+                for (int x = 0; x < GQ; ++x) acc[x][hf] = f4_t{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                for (int k = 0; k < KB; ++k) {
+                    const h8_t kf = *reinterpret_cast<const h8_t*>(tile + get_at(hf, k));
+#pragma unroll
+                    for (int x = 0; x < GQ; ++x) acc[x][hf] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf, qf[x][k], acc[x][hf], 0, 0, 0);
+                }
+            }
+            h8_t pf[GQ];
+#pragma unroll
+            for (int x = 0; x < GQ; ++x) {
+                f4_t s[2];
+#pragma unroll
+                for (int hf = 0; hf < 2; ++hf)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) s[hf][i] = (acc[x][hf][i] + column_other(acc[x][hf][i])) * qscale[x];
+                // halves that a column sees in part are masked key by key, halves
+                // that it does not see as a whole
+                const bool partly = R == 1 ? !full : __any((mine[x][0] & 15) + (mine[x][1] & 15));
+                if (partly) {
 #pragma unroll
                     for (int i = 0; i < 8; ++i)
-                        if (4 * g4 + (i & 3) >= nv[i >> 2]) {
-#pragma unroll
-                            for (int v = 0; v < VH; ++v) vf[v][i] = h8_t{};
-                        }
+                        if (4 * g4 + (i & 3) >= mine[x][i >> 2]) s[i >> 2][i & 3] = -INFINITY;
                 }
+                const float base = weights_base(x, s, mine[x], [&](float f) {
 #pragma unroll
-                for (int v = 0; v < VH; ++v)
-#pragma unroll
-                    for (int e = 0; e < 8; ++e) {
-                        h8_t y;
-#pragma unroll
-                        for (int i = 0; i < 8; ++i) y[i] = vf[v][i][e];
-#pragma unroll
-                        for (int x = 0; x < GQ; ++x) o[x][8 * v + e] = __builtin_amdgcn_mfma_f32_16x16x32_f16(y, pf[x], o[x][8 * v + e], 0, 0, 0);
-                    }
-            } else {
-                uint2 vq[8];
-                v4i_t kd[2][2], vd[2][2];
+                    for (int e = 0; e < 8 * VH; ++e) o[x][e] *= f;
+                });
 #pragma unroll
                 for (int hf = 0; hf < 2; ++hf) {
-                    const char *pg = pool + page[hf] * page_stride, *steps = pg + q8_scales_at<DH>(c);
-                    const __amdgpu_buffer_rsrc_t vb = buffer_of(pg + (vrow0 + off[hf]) * ROW, 16 * ROW);
-                    const __amdgpu_buffer_rsrc_t kd_b = buffer_of(steps + (krow0 + off[hf]) * (2 * KB), 32 * KB), vd_b = buffer_of(steps + (vrow0 + off[hf]) * (2 * KB), 32 * KB);
-#pragma unroll
-                    for (int n = 0; n < 2; ++n) kd[hf][n] = __builtin_amdgcn_raw_buffer_load_b128(kd_b, 8 * KB * g4 + 16 * n, 0, 0);
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) vq[4 * hf + i] = __builtin_bit_cast(uint2, __builtin_amdgcn_raw_buffer_load_b64(vb, 4 * DH * g4 + 8 * c16 + DH * i, 0, 0));
-#pragma unroll
-                    for (int n = 0; n < 2; ++n) vd[hf][n] = __builtin_amdgcn_raw_buffer_load_b128(vd_b, 8 * KB * g4 + 16 * n, 0, 0);
-                }
-                __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-                for (int k = 0; k < LOADS; ++k) *reinterpret_cast<v4i_t*>(tile + put_at(k)) = staged[k];
-                __builtin_amdgcn_sched_barrier(0);
-                if (AHEAD) {
-                    more = next();
-                    if (more) stage(next_page, next_off);
-                }
-                __builtin_amdgcn_sched_barrier(0);
-                // scores: a block's product, then the key's step of that block
-                f4_t s[GQ][2];
-#pragma unroll
-                for (int hf = 0; hf < 2; ++hf) {
-                    h8_t steps[2] = {__builtin_bit_cast(h8_t, kd[hf][0]), __builtin_bit_cast(h8_t, kd[hf][1])};  // [key][block]
-#pragma unroll
-                    for (int x = 0; x < GQ; ++x) s[x][hf] = f4_t{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-                    for (int k = 0; k < KB; ++k) {
-                        const h8_t kf = codes8_to_half(*reinterpret_cast<const uint2*>(tile + get_at(hf, k)));
-#pragma unroll
-                        for (int x = 0; x < GQ; ++x) {
-                            f4_t acc = {0.f, 0.f, 0.f, 0.f};
-                            acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf, qf[x][k], acc, 0, 0, 0);
-#pragma unroll
-                            for (int i = 0; i < 4; ++i) s[x][hf][i] = __builtin_fmaf(float(steps[i >> 1][4 * (i & 1) + k]), acc[i], s[x][hf][i]);
-                        }
-                    }
-#pragma unroll
-                    for (int x = 0; x < GQ; ++x)
-#pragma unroll
-                        for (int i = 0; i < 4; ++i) s[x][hf][i] = 4 * g4 + i < mine[x][hf] ? (s[x][hf][i] + column_other(s[x][hf][i])) * qscale[x] : -INFINITY;
-                }
-                // the column's value steps, 2^-ve times, 0 past the keys
-                float d[8], dmax = 0.f;
-#pragma unroll
-                for (int i = 0; i < 8; ++i) {
-                    const v4i_t two = vd[i >> 2][(i & 3) >> 1];
-                    const uint64_t four = (i & 1) ? uint64_t(uint32_t(two.w)) << 32 | uint32_t(two.z) : uint64_t(uint32_t(two.y)) << 32 | uint32_t(two.x);
-                    d[i] = 4 * g4 + (i & 3) < nv[i >> 2] ? half_bits_to_f32(uint16_t(four >> (16 * (c16 >> 2)))) : 0.f;
-                    dmax = fmaxf(dmax, d[i]);
-                }
-                const int top_e = __builtin_amdgcn_frexp_expf(dmax);
-                if (__any(dmax > 0.f && top_e > ve)) {
-                    int e = dmax > 0.f ? top_e : -200;
-                    e = max(e, __shfl_xor(e, 16));
-                    e = max(e, __shfl_xor(e, 32));
-                    e = max(e, ve);
-#pragma unroll
-                    for (int x = 0; x < GQ; ++x)
-#pragma unroll
-                        for (int n = 0; n < 8; ++n)
-#pragma unroll
-                            for (int i = 0; i < 4; ++i) o[x][n][i] = ldexpf(o[x][n][i], ve - e);
-                    ve = e;
-                }
-#pragma unroll
-                for (int i = 0; i < 8; ++i) d[i] = ldexpf(d[i], -ve);
-                h8_t ph[GQ], pl[GQ];
-#pragma unroll
-                for (int x = 0; x < GQ; ++x) {
-                    const float base = weights_base(x, s[x], mine[x], [&](float f) {
-#pragma unroll
-                        for (int e = 0; e < 8; ++e) o[x][e] *= f;
-                    });
-#pragma unroll
-                    for (int i = 0; i < 8; ++i) {
-                        const float p = exp2_hw(s[x][i >> 2][i & 3] - base);
-                        l[x] += p;
-                        _Float16 hi, lo;
-                        split_f16(p * d[i], hi, lo);
-                        ph[x][i] = hi;
-                        pl[x][i] = lo;
-                    }
-                }
-#pragma unroll
-                for (int e = 0; e < 8; ++e) {
-                    h8_t v;
-#pragma unroll
-                    for (int i = 0; i < 8; i += 2) {
-                        const uint32_t lo = e < 4 ? vq[i].x : vq[i].y, hi = e < 4 ? vq[i + 1].x : vq[i + 1].y;
-                        const h2_t t = codes_to_half(__builtin_amdgcn_perm(hi, lo, 0x0c040c00u + 0x00010001u * (e & 3)));
-                        v[i] = t[0];
-                        v[i + 1] = t[1];
-                    }
-#pragma unroll
-                    for (int x = 0; x < GQ; ++x) {
-                        o[x][e] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, pl[x], o[x][e], 0, 0, 0);
-                        o[x][e] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, ph[x], o[x][e], 0, 0, 0);
-                    }
-                }
-            }
-            if (!AHEAD) more = next();
-        }
-
-        // merge: a lane holds channels 128 v + 32 g4 + 8 i + e of its column's head
-        __syncthreads();
-        float bad = 0.f;  // NaN if a sum of a row is not finite
-#pragma unroll
-        for (int x = 0; x < GQ; ++x) {
-            const float sum = sum_over_rows(l[x]);
-            const int slot = Q8 ? 4 * x + (c16 & 3) : 8 * x + (c16 & 7);
-#pragma unroll
-            for (int n = 0; n < 8 * VH; ++n)
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    if constexpr (Q8)
-                        o[x][n][i] = ldexpf(o[x][n][i], ve);
-                    else
-                        o[x][n][i] += column_other(o[x][n][i]);
-                }
-            if (used(x) && (Q8 ? (c16 >> 2) == g4 : c16 < 8)) {
-                if (Q8 || g4 == 0) mg.m[w][slot] = m[x], mg.l[w][slot] = sum;
-                if constexpr (R > 1) {
-                    bad = __builtin_fmaf(sum, 0.f, bad);
-#pragma unroll
-                    for (int n = 0; n < 8 * VH; ++n)
-#pragma unroll
-                        for (int i = 0; i < 4; ++i) bad = __builtin_fmaf(o[x][n][i], 0.f, bad);
-                }
-#pragma unroll
-                for (int v = 0; v < VH; ++v)
+                    const float less = R > 1 && mine[x][hf] == 0 ? INFINITY : base;
 #pragma unroll
                     for (int i = 0; i < 4; ++i) {
-                        float4* to = reinterpret_cast<float4*>(&mg.o[w][slot][128 * v + 32 * g4 + 8 * i]);
-                        to[0] = make_float4(o[x][8 * v][i], o[x][8 * v + 1][i], o[x][8 * v + 2][i], o[x][8 * v + 3][i]);
-                        to[1] = make_float4(o[x][8 * v + 4][i], o[x][8 * v + 5][i], o[x][8 * v + 6][i], o[x][8 * v + 7][i]);
+                        float p = exp2_hw(s[hf][i] - less);
+                        asm("" : "+v"(p));
+                        l[x] += p;
+                        // the column's term: fp16(p), or of the rest (is_lo 1)
+                        const float rest = __builtin_fmaf(-float(_Float16(p)), is_lo, p);
+                        pf[x][4 * hf + i] = _Float16(rest);
+                    }
+                }
+            }
+            if (!full) {
+#pragma unroll
+                for (int i = 0; i < 8; ++i)
+                    if (4 * g4 + (i & 3) >= nv[i >> 2]) {
+#pragma unroll
+                        for (int v = 0; v < VH; ++v) vf[v][i] = h8_t{};
                     }
             }
-        }
-        bool again = false;
-        if constexpr (R > 1)
-            again = __syncthreads_or(only < 0 && bad != 0.f);
-        else
-            __syncthreads();
-        if (!again) {
-            const int first = R > 1 && only >= 0 ? only : 0, last = R > 1 && only < 0 ? R : first + 1;
-            // up to NI results a lane, all their gates on the way at once
-            constexpr int NI = (R * (R == 1 ? 8 : GP) * DH + 255) / 256;
-            const int from = first * group * DH + tid, to = last * group * DH;
-            float gate[NI];
-            if (nsplit == 1) {
 #pragma unroll
-                for (int n = 0; n < NI; ++n) {
-                    const int e = min(from + 256 * n, to - 1), k = R == 1 ? 0 : e / (group * DH);
-                    gate[n] = a.proj[int64_t(min(r0 + k, c.rows - 1)) * a.proj_stride + (g * group + e / DH - k * group) * 2 * DH + DH + e % DH];
+            for (int v = 0; v < VH; ++v)
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    h8_t y;
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) y[i] = vf[v][i][e];
+#pragma unroll
+                    for (int x = 0; x < GQ; ++x) o[x][8 * v + e] = __builtin_amdgcn_mfma_f32_16x16x32_f16(y, pf[x], o[x][8 * v + e], 0, 0, 0);
+                }
+        } else {
+            uint2 vq[8];
+            v4i_t kd[2][2], vd[2][2];
+#pragma unroll
+            for (int hf = 0; hf < 2; ++hf) {
+                const char *pg = pool + page[hf] * page_stride, *steps = pg + q8_scales_at<DH>(c);
+                const __amdgpu_buffer_rsrc_t vb = buffer_of(pg + (vrow0 + off[hf]) * ROW, 16 * ROW);
+                const __amdgpu_buffer_rsrc_t kd_b = buffer_of(steps + (krow0 + off[hf]) * (2 * KB), 32 * KB), vd_b = buffer_of(steps + (vrow0 + off[hf]) * (2 * KB), 32 * KB);
+#pragma unroll
+                for (int n = 0; n < 2; ++n) kd[hf][n] = __builtin_amdgcn_raw_buffer_load_b128(kd_b, 8 * KB * g4 + 16 * n, 0, 0);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) vq[4 * hf + i] = __builtin_bit_cast(uint2, __builtin_amdgcn_raw_buffer_load_b64(vb, 4 * DH * g4 + 8 * c16 + DH * i, 0, 0));
+#pragma unroll
+                for (int n = 0; n < 2; ++n) vd[hf][n] = __builtin_amdgcn_raw_buffer_load_b128(vd_b, 8 * KB * g4 + 16 * n, 0, 0);
+            }
+            __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+            for (int k = 0; k < LOADS; ++k) *reinterpret_cast<v4i_t*>(tile + put_at(k)) = staged[k];
+            __builtin_amdgcn_sched_barrier(0);
+            if (AHEAD) {
+                more = next();
+                if (more) stage(next_page, next_off);
+            }
+            __builtin_amdgcn_sched_barrier(0);
+            // scores: a block's product, then the key's step of that block
+            f4_t s[GQ][2];
+#pragma unroll
+            for (int hf = 0; hf < 2; ++hf) {
+                h8_t steps[2] = {__builtin_bit_cast(h8_t, kd[hf][0]), __builtin_bit_cast(h8_t, kd[hf][1])};  // [key][block]
+#pragma unroll
+                for (int x = 0; x < GQ; ++x) s[x][hf] = f4_t{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                for (int k = 0; k < KB; ++k) {
+                    const h8_t kf = codes8_to_half(*reinterpret_cast<const uint2*>(tile + get_at(hf, k)));
+#pragma unroll
+                    for (int x = 0; x < GQ; ++x) {
+                        f4_t acc = {0.f, 0.f, 0.f, 0.f};
+                        acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf, qf[x][k], acc, 0, 0, 0);
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) s[x][hf][i] = __builtin_fmaf(float(steps[i >> 1][4 * (i & 1) + k]), acc[i], s[x][hf][i]);
+                    }
+                }
+#pragma unroll
+                for (int x = 0; x < GQ; ++x)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const bool sees = 4 * g4 + i < mine[x][hf];
+                        const float sum = (s[x][hf][i] + column_other(s[x][hf][i])) * qscale[x];
+                        low[x] = fminf(low[x], sees ? sum : 0.f);
+                        s[x][hf][i] = sees ? sum : -INFINITY;
+                    }
+            }
+            // the column's value steps, 2^-ve times, 0 past the keys
+            float d[8], dmax = 0.f;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const v4i_t two = vd[i >> 2][(i & 3) >> 1];
+                const uint64_t four = (i & 1) ? uint64_t(uint32_t(two.w)) << 32 | uint32_t(two.z) : uint64_t(uint32_t(two.y)) << 32 | uint32_t(two.x);
+                d[i] = 4 * g4 + (i & 3) < nv[i >> 2] ? half_bits_to_f32(uint16_t(four >> (16 * (c16 >> 2)))) : 0.f;
+                dmax = fmaxf(dmax, d[i]);
+            }
+            const int top_e = __builtin_amdgcn_frexp_expf(dmax);
+            if (__any(dmax > 0.f && top_e > ve)) {
+                int e = dmax > 0.f ? top_e : -200;
+                e = max(e, __shfl_xor(e, 16));
+                e = max(e, __shfl_xor(e, 32));
+                e = max(e, ve);
+#pragma unroll
+                for (int x = 0; x < GQ; ++x)
+#pragma unroll
+                    for (int n = 0; n < 8; ++n)
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) o[x][n][i] = ldexpf(o[x][n][i], ve - e);
+                ve = e;
+            }
+#pragma unroll
+            for (int i = 0; i < 8; ++i) d[i] = ldexpf(d[i], -ve);
+            h8_t ph[GQ], pl[GQ];
+#pragma unroll
+            for (int x = 0; x < GQ; ++x) {
+                const float base = weights_base(x, s[x], mine[x], [&](float f) {
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) o[x][e] *= f;
+                });
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    const float p = exp2_hw(s[x][i >> 2][i & 3] - base);
+                    l[x] += p;
+                    _Float16 hi, lo;
+                    split_f16(p * d[i], hi, lo);
+                    ph[x][i] = hi;
+                    pl[x][i] = lo;
                 }
             }
 #pragma unroll
-            for (int n = 0; n < NI; ++n) {
-                const int e = from + 256 * n;
-                if (e >= to) break;
-                const int k = R == 1 ? 0 : e / (group * DH), h = e / DH - k * group, ch = e % DH;
-                if (R > 1) {
-                    bool live = true;
+            for (int e = 0; e < 8; ++e) {
+                h8_t v;
 #pragma unroll
-                    for (int q = 0; q < R; ++q) live = live && (q != k || pos[q] >= 0);
-                    if (!live) continue;
+                for (int i = 0; i < 8; i += 2) {
+                    const uint32_t lo = e < 4 ? vq[i].x : vq[i].y, hi = e < 4 ? vq[i + 1].x : vq[i + 1].y;
+                    const h2_t t = codes_to_half(__builtin_amdgcn_perm(hi, lo, 0x0c040c00u + 0x00010001u * (e & 3)));
+                    v[i] = t[0];
+                    v[i + 1] = t[1];
                 }
-                const int slot = R == 1 ? h : Q8 ? k * GP + h : 8 * (k / RS) + k % RS * GP + h;
-                float mw[4], lw[4];
 #pragma unroll
-                for (int q = 0; q < 4; ++q) mw[q] = mg.m[q][slot], lw[q] = mg.l[q][slot];
-                const float mx = fmaxf(fmaxf(mw[0], mw[1]), fmaxf(mw[2], mw[3]));
-                float ov = 0.f, lv = 0.f;
-#pragma unroll
-                for (int q = 0; q < 4; ++q) {
-                    const float f = mw[q] == -INFINITY && lw[q] == 0.f ? 0.f : exp2_hw(mw[q] - mx);  // a wave without keys: 0
-                    ov = __builtin_fmaf(f, mg.o[q][slot][ch], ov);
-                    lv = __builtin_fmaf(f, lw[q], lv);
-                }
-                if (nsplit == 1) {
-                    sparse_store<DH>(a, r0 + k, g * group + h, ch, ov, lv, gate[n]);
-                } else {
-                    float* rec = a.work + ((int64_t(r0) * a.Hq + g * group + h) * nsplit + split) * (DH + 4);
-                    rec[4 + ch] = ov;
-                    if (ch == 0) rec[0] = mx, rec[1] = lv;
+                for (int x = 0; x < GQ; ++x) {
+                    o[x][e] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, pl[x], o[x][e], 0, 0, 0);
+                    o[x][e] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, ph[x], o[x][e], 0, 0, 0);
                 }
             }
-            if (R == 1 || only < 0) return;
         }
-        __syncthreads();
+        if (!AHEAD) more = next();
+    }
+
+    // merge: a lane holds channels 128 v + 32 g4 + 8 i + e of its column's head
+    __syncthreads();
+#pragma unroll
+    for (int x = 0; x < GQ; ++x) {
+        const bool marked = (Q8 && low[x] == -INFINITY) || (saw[x] && m[x] == -INFINITY);
+        const float sum = sum_over_rows(marked ? NAN : l[x]);
+        const int slot = Q8 ? 4 * x + (c16 & 3) : 8 * x + (c16 & 7);
+#pragma unroll
+        for (int n = 0; n < 8 * VH; ++n)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                if constexpr (Q8)
+                    o[x][n][i] = ldexpf(o[x][n][i], ve);
+                else
+                    o[x][n][i] += column_other(o[x][n][i]);
+            }
+        if (used(x) && (Q8 ? (c16 >> 2) == g4 : c16 < 8)) {
+            if (Q8 || g4 == 0) mg.m[w][slot] = m[x], mg.l[w][slot] = sum;
+#pragma unroll
+            for (int v = 0; v < VH; ++v)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    float4* to = reinterpret_cast<float4*>(&mg.o[w][slot][128 * v + 32 * g4 + 8 * i]);
+                    to[0] = make_float4(o[x][8 * v][i], o[x][8 * v + 1][i], o[x][8 * v + 2][i], o[x][8 * v + 3][i]);
+                    to[1] = make_float4(o[x][8 * v + 4][i], o[x][8 * v + 5][i], o[x][8 * v + 6][i], o[x][8 * v + 7][i]);
+                }
+        }
+    }
+    __syncthreads();
+    // up to NI results a lane, all their gates on the way at once
+    constexpr int NI = (R * (R == 1 ? 8 : GP) * DH + 255) / 256;
+    const int to = R * group * DH;
+    auto record = [&](int h) { return a.work + ((int64_t(r0) * a.Hq + g * group + h) * nsplit + split) * (DH + 4); };
+    auto live = [&](int k) {
+        bool yes = R == 1;
+#pragma unroll
+        for (int q = 0; q < R && R > 1; ++q) yes = yes || (q == k && pos[q] >= 0);
+        return yes;
+    };
+    // the maximum of the four waves' parts of a result, their shares and total
+    auto parts = [&](int slot, float (&f)[4], float& lv) {
+        float mw[4], lw[4];
+#pragma unroll
+        for (int q = 0; q < 4; ++q) mw[q] = mg.m[q][slot], lw[q] = mg.l[q][slot];
+        const float mx = fmaxf(fmaxf(mw[0], mw[1]), fmaxf(mw[2], mw[3]));
+        lv = 0.f;
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+            f[q] = mw[q] == -INFINITY && lw[q] == 0.f ? 0.f : exp2_hw(mw[q] - mx);  // a wave without keys: 0
+            lv = __builtin_fmaf(f[q], lw[q], lv);
+        }
+        return mx;
+    };
+    auto slot_of = [&](int k, int h) { return R == 1 ? h : Q8 ? k * GP + h : 8 * (k / RS) + k % RS * GP + h; };
+    float gate[NI];
+    if (nsplit == 1) {
+#pragma unroll
+        for (int n = 0; n < NI; ++n) {
+            const int e = min(tid + 256 * n, to - 1), k = R == 1 ? 0 : e / (group * DH);
+            gate[n] = a.proj[int64_t(min(r0 + k, c.rows - 1)) * a.proj_stride + (g * group + e / DH - k * group) * 2 * DH + DH + e % DH];
+        }
+    }
+    uint32_t again = 0;  // bit n: the wave's results n are not all finite
+#pragma unroll
+    for (int n = 0; n < NI; ++n) {
+        const int e = tid + 256 * n;
+        if (e >= to) break;
+        const int k = R == 1 ? 0 : e / (group * DH), h = e / DH - k * group, ch = e % DH;
+        if (!live(k)) continue;
+        const int slot = slot_of(k, h);
+        float f[4], lv, ov = 0.f;
+        const float mx = parts(slot, f, lv);
+#pragma unroll
+        for (int q = 0; q < 4; ++q) ov = __builtin_fmaf(f[q], mg.o[q][slot][ch], ov);
+        again |= __any(__builtin_fmaf(ov, 0.f, lv * 0.f) != 0.f) ? 1u << n : 0u;
+        if (nsplit == 1) {
+            sparse_store<DH>(a, r0 + k, g * group + h, ch, ov, lv, gate[n]);
+        } else {
+            float* rec = record(h);
+            rec[4 + ch] = ov;
+            if (ch == 0) rec[0] = mx, rec[1] = lv;
+        }
+    }
+    // a wave's 64 results are channels of one (row, head)
+#pragma unroll 1
+    for (int n = 0; again >> n; ++n) {
+        if (!(again >> n & 1)) continue;
+        const int e = 64 * wu + 256 * n, k = R == 1 ? 0 : e / (group * DH), h = e / DH - k * group, ch0 = e % DH, ch = ch0 + lane;
+        float m1, l1, o1, f[4], lv;
+        bool any;
+        attend_plain<DH, Q8, R>(a, r0 + k, k, g, g * group + h, ch0, list, ne, m1, l1, o1, any);
+        if (nsplit == 1) {
+            const float of = a.proj[int64_t(r0 + k) * a.proj_stride + int64_t(g * group + h) * 2 * DH + DH + ch];
+            sparse_store<DH>(a, r0 + k, g * group + h, ch, o1, any && m1 == -INFINITY ? NAN : l1, of);
+        } else {
+            float* rec = record(h);
+            const float mx = parts(slot_of(k, h), f, lv);
+            if (lv * 0.f == 0.f) {  // the values alone: beside the total that is there
+                rec[4 + ch] = kPOne * exp2_hw(m1 - mx) * o1;
+            } else {  // a total of 1 beside m = -inf: keys, but none with a weight
+                rec[4 + ch] = kPOne * o1;
+                if (ch == 0) rec[0] = m1, rec[1] = any && m1 == -INFINITY ? 1.f : kPOne * l1;
+            }
+        }
     }
 }
 

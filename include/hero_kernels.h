@@ -443,7 +443,11 @@ int hero_attn_select_pages(const hero_attn_sparse_args* args, void* stream);
  * and values to fp32 rounding, save that a query's channels are kept to 2^-25 of
  * the head's largest and weights to 2^-38 of the row's largest (Q8_0: weight
  * times value step, to 2^-37 of the largest weight times the largest step the
- * row meets in that block). */
+ * row meets in that block). Infinities and NaNs among the stored keys and values
+ * that a row sees give what the formulas give in IEEE fp32: a key of score -inf has
+ * weight 0, one of +inf makes the row's head NaN, and so does a softmax over
+ * nothing but -inf; weights below 2^-126 of the largest are 0. Rows that meet any
+ * take several times as long. */
 int64_t hero_attn_sparse_work_bytes(int64_t rows, int32_t hq, int32_t hkv, int32_t head_dim, int32_t page_size, int32_t top);
 int hero_attn_sparse_paged(const hero_attn_sparse_args* args, void* stream);
 

@@ -1,0 +1,171 @@
+"""The long-context paged-cache operators at the edges of their definitions:
+infinities among the stored keys and values, queries near the end of fp32's
+range, a few keys of nearly equal weight, forms of single tokens, workspaces."""
+import numpy as np
+import pytest
+
+import oracle
+from gpu_util import bits, check, dev, empty, host, ptr, stream
+from test_gpu_paged_long import (Cache, check_append, check_attend, copy_of, lib, quantize, random_lists, round11, run_append, run_attend, run_select, select_inputs,  # noqa: F401
+                                 select_reference, sparse_args)
+
+pytestmark = pytest.mark.gpu
+
+U = 2.0 ** -24  # half a step of fp32, relative
+
+
+# ---- infinities among what a row sees -----------------------------------------------------
+def attend_ieee(q, gate, k, v, scale):
+    """The definition in float64 with IEEE infinities, and the bound on an fp32
+    evaluation's error where the result is finite: that of attend_reference over the
+    keys of a score that is finite (the others have weight 0, or there is no finite result)."""
+    from test_gpu_paged_long import attend_reference
+
+    with np.errstate(all="ignore"):
+        s = scale * (k * q).sum(1)
+        w = np.exp(s - s.max())
+        out = (w[:, None] * v).sum(0) / w.sum() / (1 + np.exp(-gate))
+        near = np.isfinite(s)
+        bound = np.zeros_like(out)
+        if near.any():
+            _, bound = attend_reference(q, gate, k[near], np.where(np.isfinite(v[near]), v[near], 0), scale)
+    return out, bound
+
+
+def check_ieee(c, hq, q, proj, seq, pos, sel, got):
+    """every result, kind by kind; returns how many of each there were: finite ones,
+    infinities, NaNs"""
+    values, dh, grp = c.values().astype(np.float64), c.dh, hq // c.hkv
+    scale, count = float(np.float32(1 / np.sqrt(dh))), np.zeros(3, int)
+    for r in range(len(pos)):
+        for g in range(c.hkv):
+            at = [(c.table[seq[r], lp], min(c.ps, pos[r] + 1 - lp * c.ps)) for lp in sel[r, g] if lp >= 0]
+            k, v = (np.concatenate([values[page, what, g, :n] for page, n in at]) for what in (0, 1))
+            for h in range(g * grp, (g + 1) * grp):
+                want, bound = attend_ieee(q[r, h].astype(np.float64), proj[r, h * 2 * dh + dh:(h + 1) * 2 * dh].astype(np.float64), k, v, scale)
+                x, fin = got[r, h * dh:(h + 1) * dh], np.isfinite(want)
+                name = f"row {r} head {h}"
+                assert np.array_equal(np.isnan(x), np.isnan(want)), f"{name}: NaNs {np.isnan(x).sum()}, wanted {np.isnan(want).sum()}"
+                assert np.array_equal(x[np.isinf(want)], want[np.isinf(want)]), f"{name}: infinities"
+                assert np.all(np.abs(x[fin] - want[fin]) <= bound[fin]), f"{name}: {np.max(np.abs(x[fin] - want[fin]) / bound[fin]):.3g} of the bound"
+                count += [fin.sum(), np.isinf(want).sum(), np.isnan(want).sum()]
+    return count
+
+
+# (q8, dh, ps, hq, hkv, rows, top, row_seq): single tokens over split and whole lists, chunks
+# whose rows share pages (two rows a workgroup, four) and chunks whose rows do not
+SEES = [(False, 128, 64, 8, 2, 2, 12, False), (True, 128, 64, 8, 2, 2, 12, False), (False, 256, 16, 4, 2, 3, 9, False), (True, 128, 16, 8, 1, 2, 3, False),
+        (False, 128, 64, 16, 8, 130, 3, True), (False, 128, 16, 32, 8, 129, 4, True), (False, 256, 16, 16, 8, 130, 3, True), (True, 128, 16, 32, 8, 66, 2, True)]
+
+
+def chunk_of(rng, q8, dh, ps, hq, hkv, rows, top, row_seq):
+    seqs = 1 if row_seq else rows
+    c = Cache(rng, seqs, top + 2 + -(-rows // ps), hkv, dh, ps, q8)
+    span = c.max_pages * ps
+    seq = [0] * rows if row_seq else list(range(rows))
+    pos = [span - rows + r if row_seq else span - 1 - 5 * r for r in range(rows)]
+    q = rng.standard_normal((rows, hq, dh)).astype(np.float32)
+    proj = rng.standard_normal((rows, 2 * hq * dh)).astype(np.float32)
+    sel = np.empty((rows, hkv, top), np.int32)
+    for r in range(rows):
+        for g in range(hkv):
+            sel[r, g] = np.sort(np.concatenate([rng.permutation(top)[: top - 1], [pos[r] // ps]]))  # pages 0 .. top - 1, and the row's own
+    return c, seq, pos, q, proj, sel
+
+
+@pytest.mark.parametrize("q8,dh,ps,hq,hkv,rows,top,row_seq", SEES)
+def test_an_infinite_key_gives_what_the_definition_gives(lib, q8, dh, ps, hq, hkv, rows, top, row_seq):
+    """A key whose score is -inf has weight 0, one of +inf makes the result NaN: in
+    one page of each sequence an infinite channel (Q8_0: a block of an infinite
+    step), of either sign to the heads of a group."""
+    rng = np.random.default_rng(dh + ps + rows + hq)
+    c, seq, pos, q, proj, sel = chunk_of(rng, q8, dh, ps, hq, hkv, rows, top, row_seq)
+    for s in range(c.seqs):
+        at = c.table[s, 1]
+        if q8:
+            c.d[at, 0, :, 3, 1] = np.inf
+            c.codes[at, 0, :, 3, 32:64] = rng.integers(1, 128, (c.hkv, 32))
+        else:
+            c.kv[at, 0, :, 3, 5], c.kv[at, 0, 0, 7, 9] = np.inf, -np.inf
+    if q8:  # of one sign, so that the block's products have one
+        sign = rng.integers(0, 2, q.shape[:2]) * 2 - 1
+        q[..., 32:64] = np.abs(q[..., 32:64]) * sign[..., None]
+        q[0, 0, 40] *= -1  # of both
+    got, _ = run_attend(lib, c, hq, q, proj, seq, pos, sel, row_seq=row_seq)
+    fin, inf, nan = check_ieee(c, hq, q, proj, seq, pos, sel, got)
+    assert fin and not inf and (nan or rows == 2)  # the lists of two rows may miss the page
+
+
+@pytest.mark.parametrize("q8,dh,ps,hq,hkv,rows,top,row_seq", SEES)
+def test_an_infinite_value_gives_what_the_definition_gives(lib, q8, dh, ps, hq, hkv, rows, top, row_seq):
+    """Values of both infinities: the channels that hold one are infinite, those that
+    hold both NaN (Q8_0: and where a code of 0 meets an infinite step), the others
+    finite."""
+    rng = np.random.default_rng(1 + dh + ps + rows + hq)
+    c, seq, pos, q, proj, sel = chunk_of(rng, q8, dh, ps, hq, hkv, rows, top, row_seq)
+    for s in range(c.seqs):
+        at = c.table[s, 1]
+        if q8:
+            c.d[at, 1, :, 3, 1] = c.d[at, 1, :, 9, 3] = np.inf
+            c.codes[at, 1, :, 3, 40] = 0
+        else:
+            c.kv[at, 1, :, 3, 5], c.kv[at, 1, :, 4, 100], c.kv[at, 1, :, 6, 77] = np.inf, -np.inf, np.inf
+            c.kv[at, 1, :, 11, 77], c.kv[at, 1, 0, 12, dh - 1] = -np.inf, np.nan
+    got, _ = run_attend(lib, c, hq, q, proj, seq, pos, sel, row_seq=row_seq)
+    fin, inf, nan = check_ieee(c, hq, q, proj, seq, pos, sel, got)
+    assert fin and (inf and nan or rows == 2)
+
+
+@pytest.mark.parametrize("q8,dh,ps,hq,hkv,rows,top,row_seq", SEES)
+def test_keys_of_weight_zero(lib, q8, dh, ps, hq, hkv, rows, top, row_seq):
+    """A page whose keys all score -inf beside others: it takes no part, also where
+    a range of a list or a wave of a workgroup holds nothing else. Alone it leaves a
+    softmax over nothing but -inf: NaN, unlike a list without a page, which gives 0."""
+    rng = np.random.default_rng(2 + dh + ps + rows + hq)
+    c, seq, pos, q, proj, sel = chunk_of(rng, q8, dh, ps, hq, hkv, rows, top, row_seq)
+    q[..., :32] = np.abs(q[..., :32]) + np.float32(0.01)
+    for s in range(c.seqs):
+        at = c.table[s, 1]
+        if q8:
+            c.d[at, 0, :, :, 0] = np.inf
+            c.codes[at, 0, :, :, :32] = -rng.integers(1, 128, (hkv, ps, 32))
+        else:
+            c.kv[at, 0, :, :, 7] = -np.inf
+    sel[rows // 2] = -1
+    sel[rows // 2, :, 0] = 1
+    none = rows // 2 + 1 if rows > 2 else None
+    if none:
+        sel[none] = -1
+    got, _ = run_attend(lib, c, hq, q, proj, seq, pos, sel, row_seq=row_seq)
+    assert np.all(np.isnan(got[rows // 2]))
+    keep = [r for r in range(rows) if r != none]
+    if none:
+        assert np.all(got[none] == 0)
+    pick = lambda x: [x[r] for r in keep]  # noqa: E731
+    fin, inf, nan = check_ieee(c, hq, q[keep], proj[keep], pick(seq), pick(pos), sel[keep], got[keep])
+    assert fin and not inf and nan == hq * dh
+
+
+@pytest.mark.parametrize("q8,dh,hq,hkv,row_seq,rows", [(False, 128, 8, 2, False, 3), (True, 128, 8, 2, False, 3), (False, 256, 4, 2, False, 3), (False, 128, 32, 8, True, 130)])
+def test_a_cache_of_nans_but_for_what_is_seen(lib, q8, dh, hq, hkv, row_seq, rows):
+    """Every value and step of the pool is NaN but the keys that some row sees."""
+    rng = np.random.default_rng(dh + rows)
+    ps, top = 16, 4
+    c = Cache(rng, 1 if row_seq else rows, 20, hkv, dh, ps, q8, poison=True)
+    seq = [0] * rows if row_seq else list(range(rows))
+    pos = [20 * ps - rows - 3 + r if row_seq else 150 - 37 * r for r in range(rows)]
+    sel = np.empty((rows, hkv, top), np.int32)
+    clean = Cache(rng, c.seqs, 20, hkv, dh, ps, q8)
+    for r in range(rows):
+        own = pos[r] // ps
+        sel[r] = [0, 2, own - 1, own]
+        for lp in sel[r, 0]:
+            at, n = c.table[seq[r], lp], min(ps, max(p for p, s in zip(pos, seq) if s == seq[r]) + 1 - lp * ps) if lp == own else ps
+            if q8:
+                c.d[at, :, :, :n] = clean.d[at, :, :, :n]
+            else:
+                c.kv[at, :, :, :n] = clean.kv[at, :, :, :n]
+    q, proj = rng.standard_normal((rows, hq, dh)).astype(np.float32), rng.standard_normal((rows, 2 * hq * dh)).astype(np.float32)
+    got, act = run_attend(lib, c, hq, q, proj, seq, pos, sel, row_seq=row_seq)
+    check_attend(c, hq, q, proj, seq, pos, sel, got, act, rows=list(range(rows))[:: max(1, rows // 12)])
+    assert np.all(np.isfinite(got))
