@@ -72,11 +72,13 @@ __device__ __forceinline__ uint32_t wave_max(uint32_t x) {
 }
 
 // The codes of RT rows' query heads, by the whole workgroup (a wave per head):
-// positive parts, then negative, as the pages' [max | -min] go.
+// positive parts, then negative, as the pages' [max | -min] go. A head below 2^-80,
+// whose step or the step's reciprocal may leave fp32's normal range, is scaled by
+// 2^64 first, which changes no code, and its step back in 64 bits.
 template <int DH, int GP, int RT>
 struct QueryCodes {
     alignas(16) uint8_t q[RT * GP][2 * DH];
-    float step[RT * GP];
+    double step[RT * GP];
 };
 template <int DH, int GP, int RT>
 __device__ __forceinline__ void form_codes(const SelectArgs& a, int g, int r0, QueryCodes<DH, GP, RT>& qc) {
@@ -90,14 +92,16 @@ __device__ __forceinline__ void form_codes(const SelectArgs& a, int g, int r0, Q
         for (int m = 0; m < DH / 64; ++m) v[m] = x[lane + 64 * m];
 #pragma unroll
         for (int m = 0; m < DH / 64; ++m) most = max(most, __float_as_uint(v[m]) & 0x7fffffffu);
-        const float d = __uint_as_float(wave_max(most)) / 127.f, id = d != 0.f ? 1.f / d : 0.f;
+        const float amax = __uint_as_float(wave_max(most));
+        const bool small = amax < 0x1p-80f;
+        const float up = small ? 0x1p64f : 1.f, d = amax * up / 127.f, id = d != 0.f ? 1.f / d : 0.f;
 #pragma unroll
         for (int m = 0; m < DH / 64; ++m) {
-            const int code = round_code(v[m] * id);
+            const int code = round_code(v[m] * up * id);
             qc.q[h][lane + 64 * m] = uint8_t(max(code, 0));
             qc.q[h][DH + lane + 64 * m] = uint8_t(max(-code, 0));
         }
-        if (lane == 0) qc.step[h] = round11(d);
+        if (lane == 0) qc.step[h] = double(round11(d)) * (small ? 0x1p-64 : 1.);
     }
 }
 
@@ -128,7 +132,7 @@ __device__ __forceinline__ void score_pages(const SelectArgs& a, int g, int r0, 
     v4i_t q[KS];
 #pragma unroll
     for (int s = 0; s < KS; ++s) q[s] = *reinterpret_cast<const v4i_t*>(&qc.q[col][64 * s + 16 * g4]);
-    const double step = double(qc.step[col]);
+    const double step = qc.step[col];
     const int64_t page_bytes = kv_summary_page_bytes(c.Hkv, DH);
     const uint8_t* const steps_at = c.summaries + int64_t(c.Hkv) * 2 * DH + 4 * g;
     const uint8_t* const codes_at = c.summaries + int64_t(g) * 2 * DH;

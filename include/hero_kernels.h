@@ -423,7 +423,7 @@ int hero_kv_read_paged(const hero_kv_read_args* args, void* stream);
  * page: score = max over the group's query heads of
  *   step_q * step_page * sum_c max(q8_c max8_c, q8_c min8_c),
  * q8 = the head of p.a.q_rot as round(q / (amax / 127)), step_q = amax / 127 at
- * 11 bits, max8, min8 and step_page the page's summary. The integer sum and
+ * 11 bits (of subnormal heads too), max8, min8 and step_page the page's summary. The integer sum and
  * both steps make the score exact in 64 bits, so the lists do not depend on an
  * order of summation. With non-finite queries or keys the choice among pages is
  * unspecified. Uses p.a.q_rot, positions, b, hq, hkv, dh, page_table, page_size,

@@ -169,3 +169,48 @@ def test_a_cache_of_nans_but_for_what_is_seen(lib, q8, dh, hq, hkv, row_seq, row
     got, act = run_attend(lib, c, hq, q, proj, seq, pos, sel, row_seq=row_seq)
     check_attend(c, hq, q, proj, seq, pos, sel, got, act, rows=list(range(rows))[:: max(1, rows // 12)])
     assert np.all(np.isfinite(got))
+
+
+# ---- selection by queries near the end of fp32's range ------------------------------------
+def tiny_reference(q, codes, steps, table, seq, pos, ps, n_pool, top, sink, recent):
+    """the selection's definition with a step q / 127 of any size: heads are brought to fp32's
+    normal range by a power of two first, which changes no code, and the step is taken back in 64 bits"""
+    rows, hq, _ = q.shape
+    hkv = codes.shape[1]
+    small = np.abs(q).max(-1) < 2.0 ** -80
+    x = np.where(small[..., None], q.astype(np.float64) * 2.0 ** 64, q).astype(np.float32)
+    k, d = quantize(x)
+    d = d.astype(np.float64) * np.where(small, 2.0 ** -64, 1)
+    split = np.concatenate([np.maximum(k, 0), np.maximum(-k, 0)], -1).reshape(rows, hkv, hq // hkv, -1)
+    d = d.reshape(rows, hkv, -1)
+    out = np.full((rows, hkv, top), -1, np.int32)
+    for r in range(rows):
+        vis = pos[r] // ps + 1
+        page = table[seq[r], :vis]
+        for g in range(hkv):
+            score = ((codes[page, g].reshape(vis, -1).astype(np.int64) @ split[r, g].T).astype(np.float64) * d[r, g]).max(1) * steps[page, g].astype(np.float64)
+            score[:sink] = score[vis - recent:] = np.inf
+            take = np.sort(np.argsort(-score, kind="stable")[:top])
+            out[r, g, : len(take)] = take
+    return out
+
+
+@pytest.mark.parametrize("hq,hkv,dh", [(8, 2, 128), (4, 1, 256), (2, 2, 128), (8, 1, 128)])
+@pytest.mark.parametrize("pages", [40, 700])
+@pytest.mark.parametrize("row_seq", [False, True])
+def test_select_by_tiny_queries(lib, hq, hkv, dh, pages, row_seq):
+    """Heads whose step's reciprocal passes fp32's range, heads of subnormals, zeros and
+    ordinary heads: the codes and the order of the pages are the definition's. Every score
+    of a tiny head has a sign of its own: bounds of either sign, some pages negative."""
+    rng = np.random.default_rng(pages + hq)
+    rows = 6
+    codes, steps, q = select_inputs(rng, pages, hkv, hq, dh, rows)
+    size = np.array([1e-36, 3e-37, 1e-38, 2e-40, 3e-43, 1.0])
+    q = (q * size[:, None, None]).astype(np.float32)
+    q[5, ::2] = (q[5, ::2] * np.float32(1e-39))
+    q[1, 0] = 0
+    table = np.stack([rng.permutation(pages) for _ in range(rows)]).astype(np.int32)
+    seq = [0, 0, 0, 1, 1, 2] if row_seq else list(range(rows))
+    pos = [pages * 16 - 6 + r for r in range(rows)]
+    got = run_select(lib, q, codes, steps, table, seq, pos, 16, pages, 12, 1, 2, row_seq=row_seq)
+    assert np.array_equal(got, tiny_reference(q, codes, steps, table, seq, pos, 16, pages, 12, 1, 2))
