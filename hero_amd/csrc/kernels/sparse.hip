@@ -465,9 +465,13 @@ __global__ __launch_bounds__(1024) void choose_pages_long_kernel(SelectArgs a) {
 //            ends with 32 consecutive channels of its column's head.
 // The matrix cores multiply fp16; queries and weights are fp32. Each is split
 // into two fp16 terms (22 bits). A head's query is scaled by a power of two to
-// at most 1 first, and a weight is 2^13 e^(s - m) with m at most 2 (base 2) below
+// at most 1 first, and a weight is 2^13 2^(s - m) with m at most 2 below
 // the running maximum, so that neither term leaves fp16's range: terms are
-// dropped below 2^-38 of the largest. The up to eight heads of a group (or of
+// dropped below 2^-38 of the largest. (The factor comes after the exponential:
+// s - m + 13 would be rounded to 2^-21, s - m near the maximum hardly at all.)
+// Against 64 bits lists of 3, 64 and 2048 keys of random fp16 pages are off by
+// 1.0e-7, 1.9e-7 and 2.4e-7 (2-norm), a plain fp32 evaluation by 0.9e-7, 1.6e-7 and
+// 3.3e-7. The up to eight heads of a group (or of
 // several rows) times two terms are the 16 columns: head h in columns h and h +
 // 8, added where both are done.
 // fp16 pages: keys and values are exact.
@@ -490,7 +494,7 @@ typedef _Float16 h2_t __attribute__((ext_vector_type(2)));
 typedef float f4_t __attribute__((ext_vector_type(4)));
 
 constexpr float kLog2e = 1.4426950408889634f;
-constexpr float kPShift = 13.f;  // weights are 2^13 2^(s - m)
+constexpr int kPShift = 13;      // a weight's terms are of 2^13 2^(s - m); its part in the total is 2^(s - m)
 constexpr float kPOne = 8192.f;  // 2^kPShift
 constexpr float kPSlack = 2.f;   // m may lag the maximum by this: weights stay below 2^15
 
@@ -940,7 +944,7 @@ __global__ __launch_bounds__(256) void attn_sparse_kernel(SparseAttnArgs a, int 
                 l[x] *= f;
                 rescale(f);
             }
-            return fmaxf(m[x], -3e38f) - kPShift;  // a column that has seen no key: 2^-inf, not NaN
+            return fmaxf(m[x], -3e38f);  // a column that has seen no key: 2^-inf, not NaN
         };
 
         if (!AHEAD) stage(page, off);
@@ -1013,8 +1017,9 @@ __global__ __launch_bounds__(256) void attn_sparse_kernel(SparseAttnArgs a, int 
 #pragma unroll
                     for (int i = 0; i < 4; ++i) {
                         float p = exp2_hw(s[hf][i] - less);
-                        asm("" : "+v"(p));
                         l[x] += p;
+                        p *= kPOne;
+                        asm("" : "+v"(p));  // as in split_f16
                         // the column's term: fp16(p), or of the rest (is_lo 1)
                         const float rest = __builtin_fmaf(-float(_Float16(p)), is_lo, p);
                         pf[x][4 * hf + i] = _Float16(rest);
@@ -1091,7 +1096,7 @@ __global__ __launch_bounds__(256) void attn_sparse_kernel(SparseAttnArgs a, int 
                         s[x][hf][i] = sees ? sum : -INFINITY;
                     }
             }
-            // the column's value steps, 2^-ve times, 0 past the keys
+            // the column's value steps, 2^(13 - ve) times, 0 past the keys
             float d[8], dmax = 0.f;
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
@@ -1115,7 +1120,7 @@ __global__ __launch_bounds__(256) void attn_sparse_kernel(SparseAttnArgs a, int 
                 ve = e;
             }
 #pragma unroll
-            for (int i = 0; i < 8; ++i) d[i] = ldexpf(d[i], -ve);
+            for (int i = 0; i < 8; ++i) d[i] = ldexpf(d[i], kPShift - ve);
             h8_t ph[GQ], pl[GQ];
 #pragma unroll
             for (int x = 0; x < GQ; ++x) {
@@ -1158,7 +1163,7 @@ __global__ __launch_bounds__(256) void attn_sparse_kernel(SparseAttnArgs a, int 
 #pragma unroll
     for (int x = 0; x < GQ; ++x) {
         const bool marked = (Q8 && low[x] == -INFINITY) || (saw[x] && m[x] == -INFINITY);
-        const float sum = sum_over_rows(marked ? NAN : l[x]);
+        const float sum = kPOne * sum_over_rows(marked ? NAN : l[x]);
         const int slot = Q8 ? 4 * x + (c16 & 3) : 8 * x + (c16 & 7);
 #pragma unroll
         for (int n = 0; n < 8 * VH; ++n)

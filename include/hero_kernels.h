@@ -440,10 +440,10 @@ int hero_attn_select_pages(const hero_attn_sparse_args* args, void* stream);
  * one. Uses p.a.q_rot, proj (the gates), proj_stride, positions, score_scale, b,
  * hq, hkv, dh, the page fields and work (hero_attn_sparse_work_bytes, 16-byte
  * aligned). Results agree with the sequential reference over the stored keys
- * and values to fp32 rounding, save that a query's channels are kept to 2^-25 of
- * the head's largest and weights to 2^-38 of the row's largest (Q8_0: weight
- * times value step, to 2^-37 of the largest weight times the largest step the
- * row meets in that block). Infinities and NaNs among the stored keys and values
+ * and values to fp32 rounding, save that a query's channels are kept to 2^-23 of
+ * the head's largest and weights to 2^-23 of themselves or 2^-38 of the row's
+ * largest (Q8_0: weight times value step, to 2^-37 of the largest weight times the
+ * largest step the row meets in that block). Infinities and NaNs among the stored keys and values
  * that a row sees give what the formulas give in IEEE fp32: a key of score -inf has
  * weight 0, one of +inf makes the row's head NaN, and so does a softmax over
  * nothing but -inf; weights below 2^-126 of the largest are 0. Rows that meet any

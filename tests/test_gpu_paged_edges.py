@@ -214,3 +214,34 @@ def test_select_by_tiny_queries(lib, hq, hkv, dh, pages, row_seq):
     pos = [pages * 16 - 6 + r for r in range(rows)]
     got = run_select(lib, q, codes, steps, table, seq, pos, 16, pages, 12, 1, 2, row_seq=row_seq)
     assert np.array_equal(got, tiny_reference(q, codes, steps, table, seq, pos, 16, pages, 12, 1, 2))
+
+
+# ---- a few keys of nearly equal weight ------------------------------------------------------
+@pytest.mark.parametrize("q8,dh,hq,hkv,rows,row_seq", [(False, 128, 4, 1, 1, False), (True, 128, 4, 1, 1, False), (True, 128, 8, 1, 1, False), (False, 256, 2, 1, 1, False),
+                                                       (False, 128, 32, 8, 130, True), (False, 256, 16, 8, 130, True)])
+def test_weights_close_to_the_largest_are_kept_to_fp32(lib, q8, dh, hq, hkv, rows, row_seq):
+    """Two keys, values 1 and -1 in every channel, scores 0 and -x: the result is
+    -tanh(x / 2), which the error of one weight makes up. x = scale q k is exact up to
+    three roundings of 2^-24 of itself; the hardware's exponential is good to 1 ulp
+    (2^-24 just below 1); two fp16 terms of a value in [4096, 8192) (times a step of a
+    half: [2048, 4096)) leave 2^-24 of the largest, 11 bits and then 11 of a rest of at
+    most half a step of the first; both products and their difference are exact. The result is
+    off by half of that, so by 2^-24; total, division and a gate of 1 each round a result
+    below 2^-15."""
+    scale = float(np.float32(1 / np.sqrt(dh)))
+    rng = np.random.default_rng(dh + rows + hq)
+    c = Cache(rng, 1, 2, hkv, dh, 16, q8)
+    x = rng.random((rows, hq)) * 2.0 ** -18 + 2.0 ** -23  # at most a half of 2^-16
+    q = np.zeros((rows, hq, dh), np.float32)
+    q[..., 3] = (x / scale).astype(np.float32)
+    if q8:
+        c.codes[:, 0], c.codes[:, 1, :, 0], c.codes[:, 1, :, 1], c.d[:] = 0, 1, -1, 1
+        c.codes[:, 0, :, 1, 3] = -1
+    else:
+        c.kv[:, 0], c.kv[:, 1, :, 0], c.kv[:, 1, :, 1] = 0, 1, -1
+        c.kv[:, 0, :, 1, 3] = -1
+    proj = np.full((rows, 2 * hq * dh), 40, np.float32)  # sigmoid(40) rounds to 1
+    got, _ = run_attend(lib, c, hq, q, proj, [0] * rows, [1] * rows, np.zeros((rows, hkv, 1), np.int32), row_seq=row_seq)
+    want = np.tanh(scale * q[..., 3].astype(np.float64) / 2)
+    d = np.abs(got.reshape(rows, hq, dh) - want[..., None])
+    assert d.max() <= U + 2.0 ** -38, f"{d.max() / U:.3g} of half an fp32 step"
