@@ -38,6 +38,15 @@ __device__ __forceinline__ uint8_t* q8_page(const PagedRows& c, int64_t page) {
 template <int DH>
 __device__ __forceinline__ int64_t q8_scales_at(const PagedRows& c) { return 2 * int64_t(c.Hkv) * c.page_size * DH; }
 
+// Between the stores and the reads by which the lanes of one wave exchange values
+// through shared memory that is the wave's own, and before it is written again.
+// The hardware keeps a wave's shared-memory operations in order; to the compiler
+// the lanes are threads, and this is what keeps it from moving them.
+__device__ __forceinline__ void wave_exchange() {
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+}
+
 // x >= 0 to 11 significant bits, halves away from zero (the fp16 encoder's
 // rounding without fp16's range): products of an integer below 2^24 and two
 // such values are exact in 64 bits

@@ -136,7 +136,13 @@ __device__ __forceinline__ void score_pages(const SelectArgs& a, int g, int r0, 
     const int64_t page_bytes = kv_summary_page_bytes(c.Hkv, DH);
     const uint8_t* const steps_at = c.summaries + int64_t(c.Hkv) * 2 * DH + 4 * g;
     const uint8_t* const codes_at = c.summaries + int64_t(g) * 2 * DH;
-    const int put = lane / CH * ROW + (lane % CH ^ lane / CH) * 16, get = c16 * ROW + (g4 ^ c16) * 16;
+    int put = lane / CH * ROW + (lane % CH ^ lane / CH) * 16, get = c16 * ROW + (g4 ^ c16) * 16;
+    // The lanes exchange rows through the tile, whose stores and reads the hardware
+    // keeps in order. The compiler does too, as long as a lane's read may be of
+    // what the lane itself stored: it is not to know either place. (wave_exchange
+    // would hold the global reads as well: 2% of one token's time, 7% of a chunk's
+    // over heads of 256 channels.)
+    asm volatile("" : "+v"(put), "+v"(get));
     while (const uint64_t left = __ballot(todo)) {  // the rows of one sequence at a time
         const int s0 = RT == 1 ? __builtin_amdgcn_readfirstlane(seq) : __shfl(seq, __ffsll((unsigned long long)left) - 1);
         const bool mine = todo && seq == s0;
@@ -205,7 +211,7 @@ __device__ __forceinline__ void score_pages(const SelectArgs& a, int g, int r0, 
 // fetching the instructions, which run once or a few times: one search serves
 // both halves.
 struct SelectShared {
-    int count[3][4];  // of the waves together: this count's, the last one's, the next one's (zero)
+    alignas(16) int count[3][4];  // of the waves together: this count's, the last one's, the next one's (zero)
     uint32_t ends[2];
     int place[16 * 16];
 };
@@ -971,6 +977,7 @@ __global__ __launch_bounds__(256) void attn_sparse_kernel(SparseAttnArgs a, int 
                 } else {
 #pragma unroll
                     for (int k = 0; k < LOADS; ++k) *reinterpret_cast<v4i_t*>(tile + put_at(k)) = staged[k];
+                    wave_exchange();
                     __builtin_amdgcn_sched_barrier(0);
                     if (AHEAD) {
                         more = next();
@@ -1062,6 +1069,7 @@ __global__ __launch_bounds__(256) void attn_sparse_kernel(SparseAttnArgs a, int 
             __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
             for (int k = 0; k < LOADS; ++k) *reinterpret_cast<v4i_t*>(tile + put_at(k)) = staged[k];
+            wave_exchange();
             __builtin_amdgcn_sched_barrier(0);
             if (AHEAD) {
                 more = next();
@@ -1156,6 +1164,7 @@ __global__ __launch_bounds__(256) void attn_sparse_kernel(SparseAttnArgs a, int 
             }
         }
         if (!AHEAD) more = next();
+        wave_exchange();  // the tile's reads, before the next unit's stores
     }
 
     // merge: a lane holds channels 128 v + 32 g4 + 8 i + e of its column's head
