@@ -328,7 +328,7 @@ __global__ __launch_bounds__(256) void kv_read_kernel(KvReadArgs a) {
     const int64_t page = pool_page(c, seq, pos / c.page_size);
     if (page < 0) return;
     const int t = pos % c.page_size;
-    for (int e = blockIdx.y * 256 + threadIdx.x; e < 4 * kw8; e += 256 * gridDim.y) {
+    for (int e = threadIdx.x; e < 4 * kw8; e += 256) {
         const int what = e / kw8, ch = e % kw8 * 8, g = ch / DH, j = ch % DH;
         T* out = static_cast<T*>(a.out[what]);
         if (!out) continue;

@@ -375,7 +375,7 @@ __global__ __launch_bounds__(kSelThreads<RT>, 4) void select_pages_kernel(Select
     const int sees = row_sees(c, r);
     if (sees <= a.top)
         list_all(out, sees, a.top, threadIdx.x & 63, 64);
-    else if (RT > 1 && sees <= 320)
+    else if (RT > 1 && sees <= 320)  // five keys a lane instead of eight: 500 rows over 250 pages 17.8 us instead of 19.0, over 100 pages 13.5 instead of 15.0
         choose_pages<64, 5>(keys, sees, a.top, a.sink, a.recent, out, nullptr);
     else if (RT == 1 || sees <= 512)
         choose_pages<64, 8>(keys, sees, a.top, a.sink, a.recent, out, nullptr);
@@ -726,9 +726,9 @@ __device__ __forceinline__ void attend_plain(const SparseAttnArgs& a, int r, int
     }
 }
 
-// R rows by GP heads each (fp16 pages: GP a power of two, in GQ sets of eight
-// columns times two terms; Q8_0 pages: GP 4 or 8, in GQ quads). R > 1: the rows
-// of a chunk, which mostly select the same pages.
+// R rows by GP heads each, in GQ sets of 16 columns. fp16 pages: one set, R GP <= 8
+// of GP a power of two, times two terms; R > 1: the rows of a chunk, which mostly
+// select the same pages. Q8_0 pages: one row, a set for every four heads.
 //
 // Infinities and NaNs: the two terms of a query or weight may differ in sign, or
 // one be 0, so that an infinite key or value turns a score or sum to NaN which
@@ -744,7 +744,8 @@ __device__ __forceinline__ void attend_plain(const SparseAttnArgs& a, int r, int
 template <int DH, bool Q8, int GQ, int R, int GP>
 __global__ __launch_bounds__(256) void attn_sparse_kernel(SparseAttnArgs a, int per, int nsplit) {
     constexpr int KB = DH / 32, VH = DH / 128;  // 32-channel blocks, 128-channel halves
-    constexpr int SLOTS = Q8 ? 4 * GQ : 8 * GQ, RS = 8 / GP, QPR = GP / 4;
+    static_assert(Q8 ? R == 1 && GP == 4 * GQ : GQ == 1 && R * GP <= 8);
+    constexpr int SLOTS = Q8 ? 4 * GQ : 8;
     const PagedRows& c = a.c;
     const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6, g4 = lane >> 4, c16 = lane & 15;
     // K/V head fastest: with eight of them each XCD's L2 holds one head's pages
@@ -760,13 +761,13 @@ __global__ __launch_bounds__(256) void attn_sparse_kernel(SparseAttnArgs a, int 
         some |= pos[k] >= 0;
     }
     if (!some) return;
-    // the row and head of a column of set x, and its slot
-    auto row_of = [&](int x) { return R == 1 ? 0 : Q8 ? x / (QPR ? QPR : 1) : min(RS * x + (c16 & 7) / GP, R - 1); };
-    auto head_of = [&](int x) { return Q8 ? 4 * (x % (QPR ? QPR : 1)) + (c16 & 3) : c16 & (GP - 1); };
+    // the row and head of a column of set x
+    const int col_row = R == 1 ? 0 : min((c16 & 7) / GP, R - 1);
+    auto head_of = [&](int x) { return Q8 ? 4 * x + (c16 & 3) : c16 & (GP - 1); };
     auto used = [&](int x) {  // columns that stand for a row and head
-        bool live = head_of(x) < group && (Q8 || RS * x + (c16 & 7) / GP < R);
+        bool live = head_of(x) < group && (Q8 || (c16 & 7) / GP < R);
 #pragma unroll
-        for (int k = 0; k < R; ++k) live = live && (row_of(x) != k || pos[k] >= 0);
+        for (int k = 0; k < R; ++k) live = live && (col_row != k || pos[k] >= 0);
         return live;
     };
     extern __shared__ __align__(16) char list_mem[];
@@ -796,7 +797,7 @@ __global__ __launch_bounds__(256) void attn_sparse_kernel(SparseAttnArgs a, int 
     float qv[GQ][PER][8];  // on the way while the list is built
 #pragma unroll
     for (int x = 0; x < GQ; ++x) {
-        const float* q_row = a.q_rot + (int64_t(min(r0 + row_of(x), c.rows - 1)) * a.Hq + g * group + min(head_of(x), group - 1)) * DH;
+        const float* q_row = a.q_rot + (int64_t(min(r0 + col_row, c.rows - 1)) * a.Hq + g * group + min(head_of(x), group - 1)) * DH;
 #pragma unroll
         for (int y = 0; y < PER; ++y) {
             const float4* p = reinterpret_cast<const float4*>(q_row + 32 * (PER * w + y) + 8 * g4);
@@ -897,7 +898,7 @@ __global__ __launch_bounds__(256) void attn_sparse_kernel(SparseAttnArgs a, int 
 #pragma unroll
                 for (int x = 0; x < GQ; ++x) {
                     next_mine[x][s] = next_nv[s];
-                    if constexpr (R > 1) next_mine[x][s] = min(next_nv[s], max(0, int(le.keys[row_of(x)]) - next_off[s]));
+                    if constexpr (R > 1) next_mine[x][s] = min(next_nv[s], max(0, int(le.keys[col_row]) - next_off[s]));
                 }
                 entry[s] += step_e;
                 block[s] += step_b;
@@ -913,8 +914,8 @@ __global__ __launch_bounds__(256) void attn_sparse_kernel(SparseAttnArgs a, int 
     };
     // the keys through the wave's tile: read as whole rows, lane by lane on (16
     // lanes on 16 rows, as the product wants them, are 64 requests a load: 118 us
-    // of 146 for 500 rows' loads alone), 16 bytes each; of heads of 128 channels
-    // a unit ahead, for 256 there are not the registers
+    // of 146 for 500 rows' loads alone), 16 bytes each; of one row's fp16 heads of
+    // 128 channels a unit ahead, else there are not the registers
     constexpr int LOADS = 2 * CH / 4;  // of 1024 bytes, half of them a half
     constexpr bool AHEAD = DH == 128 && R == 1 && !Q8;
     v4i_t staged[LOADS];
@@ -1071,11 +1072,6 @@ __global__ __launch_bounds__(256) void attn_sparse_kernel(SparseAttnArgs a, int 
             for (int k = 0; k < LOADS; ++k) *reinterpret_cast<v4i_t*>(tile + put_at(k)) = staged[k];
             wave_exchange();
             __builtin_amdgcn_sched_barrier(0);
-            if (AHEAD) {
-                more = next();
-                if (more) stage(next_page, next_off);
-            }
-            __builtin_amdgcn_sched_barrier(0);
             // scores: a block's product, then the key's step of that block
             f4_t s[GQ][2];
 #pragma unroll
@@ -1173,7 +1169,7 @@ __global__ __launch_bounds__(256) void attn_sparse_kernel(SparseAttnArgs a, int 
     for (int x = 0; x < GQ; ++x) {
         const bool marked = (Q8 && low[x] == -INFINITY) || (saw[x] && m[x] == -INFINITY);
         const float sum = kPOne * sum_over_rows(marked ? NAN : l[x]);
-        const int slot = Q8 ? 4 * x + (c16 & 3) : 8 * x + (c16 & 7);
+        const int slot = Q8 ? 4 * x + (c16 & 3) : c16 & 7;
 #pragma unroll
         for (int n = 0; n < 8 * VH; ++n)
 #pragma unroll
@@ -1220,7 +1216,7 @@ __global__ __launch_bounds__(256) void attn_sparse_kernel(SparseAttnArgs a, int 
         }
         return mx;
     };
-    auto slot_of = [&](int k, int h) { return R == 1 ? h : Q8 ? k * GP + h : 8 * (k / RS) + k % RS * GP + h; };
+    auto slot_of = [&](int k, int h) { return k * GP + h; };
     float gate[NI];
     if (nsplit == 1) {
 #pragma unroll
