@@ -35,7 +35,9 @@ def attend_ieee(q, gate, k, v, scale):
 def check_ieee(c, hq, q, proj, seq, pos, sel, got):
     """every result, kind by kind; returns how many of each there were: finite ones,
     infinities, NaNs"""
-    values, dh, grp = c.values().astype(np.float64), c.dh, hq // c.hkv
+    with np.errstate(invalid="ignore"):
+        values = c.values().astype(np.float64)
+    dh, grp = c.dh, hq // c.hkv
     scale, count = float(np.float32(1 / np.sqrt(dh))), np.zeros(3, int)
     for r in range(len(pos)):
         for g in range(c.hkv):
@@ -245,3 +247,128 @@ def test_weights_close_to_the_largest_are_kept_to_fp32(lib, q8, dh, hq, hkv, row
     want = np.tanh(scale * q[..., 3].astype(np.float64) / 2)
     d = np.abs(got.reshape(rows, hq, dh) - want[..., None])
     assert d.max() <= U + 2.0 ** -38, f"{d.max() / U:.3g} of half an fp32 step"
+
+
+# ---- forms of single tokens, wide heads, workspaces -----------------------------------------
+@pytest.mark.parametrize("q8,dh,ps,hq,hkv", [(False, 128, 64, 32, 8), (True, 128, 64, 32, 8), (False, 256, 64, 16, 4), (True, 128, 16, 7, 1), (False, 128, 256, 8, 2), (False, 256, 16, 3, 3),
+                                             (True, 128, 256, 16, 2)])
+@pytest.mark.parametrize("b", [1, 17])
+def test_append_of_single_tokens_equals_oracle(lib, q8, dh, ps, hq, hkv, b):
+    """A row of each sequence: first and last slots of pages, padding and positions past
+    the table, the stored bytes, the rotated queries and the summaries."""
+    rng = np.random.default_rng(ps + dh + b)
+    c = Cache(rng, b, 5, hkv, dh, ps, q8)
+    pos = [int(p) for p in rng.integers(0, 5 * ps, b)]
+    if b > 1:
+        pos[1], pos[2], pos[3], pos[4], pos[5] = 0, ps - 1, -1, 5 * ps, 3 * ps
+    table = c.table.copy()
+    if b > 1:
+        table[6, pos[6] // ps], table[7, pos[7] // ps] = -1, c.n
+    before = copy_of(c)
+    ran = run_append(lib, rng, c, hq, list(range(b)), pos, table=table, row_seq=False, stride_more=1)
+    check_append(before, c, hq, list(range(b)), pos, table, ran)
+
+
+@pytest.mark.parametrize("q8,dh", [(False, 128), (True, 128), (False, 256)])
+def test_append_over_a_cache_of_nans(lib, q8, dh):
+    """What lies in and behind a page's other slots is overwritten or left, and does not
+    reach the rows that are stored: a prompt from position 0 on, then tokens."""
+    rng = np.random.default_rng(3)
+    c = Cache(rng, 2, 6, 2, dh, 16, q8, poison=True)
+    with np.errstate(invalid="ignore"):
+        for seq, pos, row_seq in (([0] * 37 + [1] * 5, list(range(37)) + list(range(5)), True), ([0, 1], [37, 5], False)):
+            before = copy_of(c)
+            ran = run_append(lib, rng, c, 4, seq, pos, row_seq=row_seq)
+            check_append(before, c, 4, seq, pos, c.table, ran)
+
+
+@pytest.mark.parametrize("hq,hkv,dh", [(2, 2, 128), (4, 2, 128), (3, 1, 128), (8, 2, 128), (16, 2, 128), (5, 1, 128), (2, 2, 256), (4, 2, 256), (8, 2, 256), (16, 2, 256), (7, 1, 256)])
+@pytest.mark.parametrize("pages", [33, 512, 513, 2100, 4097])
+def test_select_of_single_tokens_of_every_group(lib, hq, hkv, dh, pages):
+    """Each count of query heads per K/V head at both widths, in one launch (up to 512
+    pages) and in two, rows that see some or all of their pages, a page in twenty gone."""
+    rng = np.random.default_rng(hq * dh + pages)
+    codes, steps, q = select_inputs(rng, 900, hkv, hq, dh, 3)
+    table = rng.integers(0, 900, (3, pages)).astype(np.int32)
+    table[rng.random(table.shape) < 0.05] = -1
+    pos = [pages * 16 - 1, pages * 16 // 2, (pages - 1) * 16]
+    got = run_select(lib, q, codes, steps, table, range(3), pos, 16, 900, 10, 1, 2, row_seq=False)
+    assert np.array_equal(got, select_reference(q, codes, steps, table, range(3), pos, 16, 900, 10, 1, 2))
+
+
+@pytest.mark.parametrize("hq,hkv", [(2, 2), (4, 2), (8, 2), (16, 2), (6, 1)])
+@pytest.mark.parametrize("pages", [300, 500, 767, 1024, 1025])
+def test_select_of_chunks_of_wide_heads(lib, hq, hkv, pages):
+    """256-wide heads up to the most pages whose scores stay in shared memory (over 64 KB
+    of it), and one more; rows of two sequences in one tile."""
+    rng = np.random.default_rng(hq + pages)
+    codes, steps, q = select_inputs(rng, 900, hkv, hq, 256, 11)
+    table = rng.integers(0, 900, (2, pages)).astype(np.int32)
+    seq, pos = [0] * 7 + [1] * 4, [pages * 16 - 7 + i for i in range(7)] + [pages * 8 + i for i in range(4)]
+    got = run_select(lib, q, codes, steps, table, seq, pos, 16, 900, 30, 2, 1)
+    assert np.array_equal(got, select_reference(q, codes, steps, table, seq, pos, 16, 900, 30, 2, 1))
+
+
+GUARD = 4096
+
+
+@pytest.mark.parametrize("hq,hkv,dh,ps,rows,pages,top,row_seq", [(8, 2, 128, 64, 1, 700, 20, False), (16, 2, 256, 16, 5, 513, 9, False), (8, 1, 128, 16, 9, 1025, 40, True),
+                                                                 (8, 2, 128, 16, 3, 5000, 64, False), (8, 8, 128, 16, 2, 17000, 30, False)])
+def test_select_stays_inside_its_workspace(lib, hq, hkv, dh, ps, rows, pages, top, row_seq):
+    rng = np.random.default_rng(pages)
+    codes, steps, q = select_inputs(rng, 300, hkv, hq, dh, rows)
+    table = rng.integers(0, 300, (rows, pages)).astype(np.int32)
+    c = Cache(rng, rows, 1, hkv, dh, ps)
+    c.max_pages, c.n = pages, 300
+    sums = np.zeros((300, c.sum_bytes), np.uint8)
+    sums[:, : hkv * 2 * dh] = codes.reshape(300, -1).view(np.uint8)
+    sums[:, hkv * 2 * dh: hkv * 2 * dh + 4 * hkv] = steps.view(np.uint8).reshape(300, -1)
+    pos = [pages * ps - 1 - r for r in range(rows)]
+    wb, d = lib.hero_attn_select_work_bytes(rows, hkv, pages), [dev(x) for x in (q, sums, table, np.array(pos, np.int32), np.arange(rows, dtype=np.int32))]
+    work, sel = dev(np.full(wb + GUARD, 0xA5, np.uint8)), empty(rows * hkv * top * 4)
+    args = sparse_args(c, hq, rows, ptr(d[3]), dev_seq=ptr(d[4]) if row_seq else None, q_rot=ptr(d[0]), table=ptr(d[2]), work=ptr(work), work_bytes=wb, summaries=ptr(d[1]),
+                       selected=ptr(sel), top=top, sink=1, recent=2)
+    check(lib.hero_attn_select_pages(args, stream()))
+    assert np.all(host(work, np.uint8)[wb:] == 0xA5)
+
+
+@pytest.mark.parametrize("q8,hq,hkv,dh,ps,rows,top,row_seq", [(False, 32, 8, 128, 64, 1, 32, False), (True, 32, 8, 128, 64, 16, 32, False), (False, 16, 4, 256, 64, 8, 48, False),
+                                                              (True, 8, 1, 128, 16, 3, 4096, False), (False, 16, 8, 128, 16, 70, 2100, True), (False, 7, 1, 128, 48, 100, 7, True)])
+def test_attend_stays_inside_its_workspace(lib, q8, hq, hkv, dh, ps, rows, top, row_seq):
+    rng = np.random.default_rng(top)
+    c = Cache(rng, 1 if row_seq else rows, 60, hkv, dh, ps, q8)
+    pos = [60 * ps - 1 - r for r in range(rows)]
+    sel = random_lists(rng, rows, hkv, top, [min(60, top)] * rows)
+    wb = lib.hero_attn_sparse_work_bytes(rows, hq, hkv, dh, ps, top)
+    assert wb > 0
+    d = [dev(x) for x in (rng.standard_normal((rows, hq, dh)).astype(np.float32), rng.standard_normal((rows, 2 * hq * dh)).astype(np.float32), c.bytes(), c.table,
+                          np.array(pos, np.int32), np.zeros(rows, np.int32), sel)]
+    work, out = dev(np.full(wb + GUARD, 0xA5, np.uint8)), empty(rows * hq * dh * 4 + GUARD)
+    args = sparse_args(c, hq, rows, ptr(d[4]), dev_seq=ptr(d[5]) if row_seq else None, q_rot=ptr(d[0]), proj=ptr(d[1]), stride=2 * hq * dh, scale=0.1, pages=ptr(d[2]), table=ptr(d[3]),
+                       work=ptr(work), work_bytes=wb, selected=ptr(d[6]), top=top, out=ptr(out))
+    check(lib.hero_attn_sparse_paged(args, stream()))
+    assert np.all(host(work, np.uint8)[wb:] == 0xA5) and np.all(host(out, np.uint8)[rows * hq * dh * 4:] == 0)
+
+
+@pytest.mark.parametrize("q8", [False, True])
+def test_decoded_rows_with_row_seq_equal_those_without(lib, q8):
+    """Tokens of many sequences, their sequences named: the same stored bytes and lists,
+    and the attention of rows that share nothing in the kernels for chunks."""
+    rng = np.random.default_rng(15)
+    b, hq, hkv, ps, top = 130, 32, 8, 16, 4
+    c = Cache(rng, b, 9, hkv, 128, ps, q8)
+    pos = [int(p) for p in rng.integers(0, 9 * ps, b)]
+    pools, sums = [], []
+    for row_seq in (False, True):
+        one = copy_of(c)
+        ran = run_append(lib, np.random.default_rng(1), one, hq, list(range(b)), pos, row_seq=row_seq)
+        pools.append(one.bytes())
+        sums.append((ran[5], ran[7]))
+    assert np.array_equal(*pools) and all(np.array_equal(x, y) for x, y in zip(*sums))
+    codes, steps, q = select_inputs(rng, c.n, hkv, hq, 128, b)
+    lists = [run_select(lib, q, codes, steps, c.table, range(b), pos, ps, c.n, top, 1, 2, row_seq=r) for r in (False, True)]
+    assert np.array_equal(*lists)
+    proj = rng.standard_normal((b, 2 * hq * 128)).astype(np.float32)
+    for r in (False, True):
+        got, act = run_attend(lib, c, hq, q, proj, range(b), pos, lists[0], row_seq=r)
+        check_attend(c, hq, q, proj, range(b), pos, lists[0], got, act, rows=[0, 1, 2, 3, 64, 65, 128, 129])

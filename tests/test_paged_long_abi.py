@@ -92,3 +92,18 @@ def test_workspaces_grow_with_the_rows(hq, hkv, dh, ps, top):
     assert sizes == sorted(sizes) and sizes[0] >= 0
     sizes = [lib.hero_attn_select_work_bytes(r, hkv, 700) for r in range(1, 300)]
     assert sizes == sorted(sizes)
+
+
+@pytest.mark.parametrize("change", [dict(b=3), dict(b=1, top=40), dict(b=70, seqs=70, hq=16, hkv=8, proj_stride=1 << 15, top=2049), dict(dh=256, hq=4, proj_stride=1 << 15)])
+def test_attention_refuses_a_workspace_that_is_missing_or_small(change):
+    a = sparse_args(**change)
+    need = lib.hero_attn_sparse_work_bytes(a.p.a.b, a.p.a.hq, a.p.a.hkv, a.p.a.dh, a.p.page_size, a.top)
+    assert need > 0
+    for work in (dict(work=None), dict(work=P + 8), dict(work_bytes=need - 1), dict(work_bytes=0), dict(work_bytes=-1)):
+        assert lib.hero_attn_sparse_paged(ctypes.byref(sparse_args(**change, **work)), None) == _lib.HERO_EINVAL
+        assert b"work" in lib.hero_last_error()
+
+
+def test_selection_refuses_a_misaligned_workspace():
+    assert lib.hero_attn_select_pages(ctypes.byref(sparse_args(work=P + 8)), None) == _lib.HERO_EINVAL
+    assert b"work" in lib.hero_last_error()
