@@ -18,10 +18,11 @@
 // channels each, so that a row is read and written in whole words.
 //
 // Bound: for single tokens the dependent reads (position, page id, row), the chain
-// (0.4 us) and the exchange of the bounds: 5.1 us for one row of 32 + 8 heads of
-// 128, 6.7 us for sixteen rows into Q8_0 pages that hold 32 keys on average. For
-// chunks the same latencies and HBM: 1000 rows (41 MB) 15 to 16 us, 8.6 us at a
-// large copy's 4.76 TB/s. Reading back 8192 Q8_0 rows as fp32 (85 MB): 18.3 us,
+// (0.4 us for 128 channels, twice that for 256) and the exchange of the bounds: 4.6
+// us for one row of 32 + 8 heads of 128, 5.6 us for 16 + 4 heads of 256, 6.4 us for
+// sixteen rows into Q8_0 pages that hold 32 keys on average. For chunks the same
+// latencies and HBM: 1000 rows (41 MB) 15.5 us into Q8_0 pages, 14.6 into fp16 ones
+// (256-wide heads 15.5), 8.6 us at a large copy's 4.76 TB/s. Reading back 8192 Q8_0 rows as fp32 (85 MB): 18.3 us,
 // 4.6 TB/s, as a copy.
 #include "hero/device.hpp"
 #include "hero/kernels.hpp"
@@ -31,7 +32,10 @@ namespace hero {
 
 namespace {
 
-constexpr int kApSpread = 61;  // chunks: workgroups per K/V head
+// chunks: workgroups per K/V head, set for eight of them (two workgroups per CU).
+// Fewer heads make fewer workgroups: 1000 rows of one K/V head take 8.0 us (pages
+// of 16: 8.7), of two 8.9, of four 10.3, of eight 14.6
+constexpr int kApSpread = 61;
 
 // x rounded to fp32 by whatever formed it, then to fp16 (the compiler may not
 // round a product to fp16 at once)

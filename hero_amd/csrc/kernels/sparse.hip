@@ -39,7 +39,8 @@ namespace {
 // order (sixty-four tokens: 3.7 TB/s), and 8 us for the choice; 14.4 us at a
 // copy's rate. 500 rows of a chunk over 251 to 258 pages: 18 us, vector
 // instructions (the exact scores take 64-bit products and maxima, about 45
-// instructions for four pages and rows).
+// instructions for four pages and rows). Heads of 256 channels, 16 over 4: 10.7, 28
+// and 16.5 us for the three.
 typedef int v4i_t __attribute__((ext_vector_type(4)));
 
 __device__ __forceinline__ float max_over_rows(float x) {  // over the four g of a column
@@ -356,7 +357,10 @@ __device__ __forceinline__ int row_sees(const PagedRows& c, int r) {
 // into shared memory, then a wave per row chooses: its counts need no barrier.
 // Longer lists of a lone row are faster over many workgroups in two launches:
 // 1000 pages 11 to 12 against 15 us, 4000 pages 15 against 40 us (one sequence;
-// the same times for sixteen).
+// the same times for sixteen). The table's width decides, as the host does not know
+// the positions: the 501 pages that take 8.4 us in a table of their own take 11.7 in
+// one of 4096. Tiles whose rows belong to several sequences score them one after
+// another: sixteen tokens over 501 pages take 41.8 us with row_seq, 12.1 without.
 template <int RT>
 constexpr int kSelThreads = RT == 1 ? 512 : 256;
 template <int DH, int GP, int RT>
@@ -494,7 +498,9 @@ __global__ __launch_bounds__(1024) void choose_pages_long_kernel(SelectArgs a) {
 // over 32 fp16 pages (134 MB) 30 us, 3.7 to 4.6 TB/s of a copy's 4.76, and the
 // merge 4 us. Chunks, what L2 gives and the vector instructions around the
 // products: 500 rows over 16 pages each read 1.5 GB through L2 for 92 MB of
-// distinct bytes, 89 us (Q8_0 pages 140 us, vector instructions).
+// distinct bytes, 88 to 89 us a call among others (98 alone under the profiler; eight
+// heads per K/V head 109, 256-wide heads 85). Q8_0 pages, vector instructions: 140
+// us, eight heads per K/V head 228.
 typedef _Float16 h8_t __attribute__((ext_vector_type(8)));
 typedef _Float16 h2_t __attribute__((ext_vector_type(2)));
 typedef float f4_t __attribute__((ext_vector_type(4)));

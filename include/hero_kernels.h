@@ -357,7 +357,8 @@ int hero_attn_decode_paged(const hero_attn_paged_args* args, void* stream);
  * here equal the ones appended there bit for bit.
  *
  * Rows: row r (of p.a.b) is the token at p.a.positions[r] of sequence
- * row_seq[r] (row_seq NULL: of sequence r). Sequence s owns row s of
+ * row_seq[r] (row_seq NULL: of sequence r; batches of tokens of many sequences are
+ * faster that way). Sequence s owns row s of
  * p.page_table [seqs][max_pages]; entries outside [0, pool_pages) hold nothing:
  * no key is stored to or read from them. A row whose position is negative or
  * past the table, or whose sequence is not in [0, seqs), is left out: its
@@ -390,7 +391,8 @@ int64_t hero_kv_summary_bytes(int64_t pool_pages, int32_t hkv, int32_t head_dim)
  * (nm/src/components.hpp:176-181, nm/src/attention.hpp:76-91; q to p.a.q_rot),
  * k and v to their page slots as fp16 (round to nearest even) or Q8_0
  * (nm/src/quant_i8.hpp:70-80), and the summary of every page a row fell into,
- * over the page's slots up to the row's. Uses p.a.proj, proj_stride, k_off,
+ * over the page's slots up to the row's (hero_attn_decode_paged writes none: a page
+ * it filled has no summary until a row is appended to it here). Uses p.a.proj, proj_stride, k_off,
  * v_off, q_gamma, k_gamma, eps, rope_cs, positions, q_rot, b, hq, hkv, dh, the
  * page fields and everything above but selected, top, sink and recent. The rows
  * of one sequence stand together, positions ascending by one and no left-out
