@@ -116,9 +116,9 @@ struct HeadLane {
 };
 template <int DH>
 __device__ __forceinline__ void load_cs(const float* rope_cs, int pos, int l, float4 (&cs)[2]) {
-    const float4* c4 = reinterpret_cast<const float4*>(rope_cs + int64_t(pos) * DH + 2 * (4 * l % (DH / 2)));
-    cs[0] = c4[0];
-    cs[1] = c4[1];
+    const float* p = rope_cs + int64_t(pos) * DH + 2 * (4 * l % (DH / 2));
+    cs[0] = load4(p);
+    cs[1] = load4(p + 4);
 }
 
 // One K/V head of the run that starts in row r0, by the whole workgroup.

@@ -372,3 +372,86 @@ def test_decoded_rows_with_row_seq_equal_those_without(lib, q8):
     for r in (False, True):
         got, act = run_attend(lib, c, hq, q, proj, range(b), pos, lists[0], row_seq=r)
         check_attend(c, hq, q, proj, range(b), pos, lists[0], got, act, rows=[0, 1, 2, 3, 64, 65, 128, 129])
+
+
+@pytest.mark.parametrize("q8,dh,row_seq", [(False, 128, True), (True, 128, False), (False, 256, True), (False, 256, False)])
+def test_append_and_attend_at_the_alignments_the_header_allows(lib, q8, dh, row_seq):
+    """A projection and norm weights at 4 bytes past an even address, a rotation table at 8,
+    pools, queries and outputs at 16: the results of the aligned calls."""
+    rng = np.random.default_rng(19)
+    hq, hkv, ps, rows, top = 4, 2, 16, 5, 3
+    c = Cache(rng, 1 if row_seq else rows, 4, hkv, dh, ps, q8)
+    kw, rope = hkv * dh, 4 * ps
+    stride = 2 * hq * dh + 2 * kw + 1
+    proj, g = rng.standard_normal(rows * stride).astype(np.float32), (1 + 0.1 * rng.standard_normal((2, dh))).astype(np.float32)
+    cs, seq = oracle.rope_table(dh, 1e6, 32, rope), np.array([0] * rows if row_seq else range(rows), np.int32)
+    pos = np.array([14 + r if row_seq else 13 * r for r in range(rows)], np.int32)
+    sel = np.full((rows, hkv, top), -1, np.int32)
+    for r in range(rows):
+        sel[r, :, : pos[r] // ps + 1] = np.arange(pos[r] // ps + 1)[:top]
+    got = []
+    for off in (0, 1):
+        def put(x, at):
+            raw = np.ascontiguousarray(x).view(np.uint8).reshape(-1)
+            t = dev(np.concatenate([np.zeros(at, np.uint8), raw]))
+            return t, ptr(t) + at
+
+        d = {"proj": put(proj, 4 * off), "gq": put(g[0], 4 * off), "gk": put(g[1], 4 * off), "cs": put(cs, 8 * off), "pages": put(c.bytes(), 16 * off), "table": put(c.table, 4 * off),
+             "pos": put(pos, 4 * off), "seq": put(seq, 4 * off), "sums": put(np.zeros((c.n, c.sum_bytes), np.uint8), 16 * off), "q": put(np.zeros((rows, hq, dh), np.float32), 16 * off),
+             "sel": put(sel, 4 * off), "out": put(np.zeros((rows, hq * dh), np.float32), 16 * off)}
+        p = {k: v[1] for k, v in d.items()}
+        work = empty(max(16, lib.hero_attn_sparse_work_bytes(rows, hq, hkv, dh, ps, top)))
+        args = sparse_args(c, hq, rows, p["pos"], dev_seq=p["seq"] if row_seq else None, proj=p["proj"], stride=stride, gq=p["gq"], gk=p["gk"], cs=p["cs"], q_rot=p["q"], scale=0.1,
+                           pages=p["pages"], table=p["table"], rope=rope, summaries=p["sums"], selected=p["sel"], top=top, out=p["out"], work=ptr(work), work_bytes=work.numel())
+        check(lib.hero_kv_append_paged(args, stream()))
+        check(lib.hero_attn_sparse_paged(args, stream()))
+        got.append([host(d[k][0], np.uint8)[{"pages": 16, "sums": 16, "q": 16, "out": 16}[k] * off:] for k in ("pages", "sums", "q", "out")])
+    for a, b in zip(*got):
+        assert np.array_equal(a, b) and a.any()
+
+
+@pytest.mark.parametrize("q8,dh,hq,hkv,rows", [(False, 128, 8, 2, 2), (True, 128, 8, 2, 2), (True, 128, 8, 1, 2), (False, 256, 8, 2, 2), (False, 128, 32, 8, 130), (False, 256, 16, 8, 130)])
+def test_a_query_that_is_not_finite_stays_in_its_head(lib, q8, dh, hq, hkv, rows):
+    """NaN, infinity and both signs of it in some heads: those are NaN (an infinite channel meets
+    keys of both signs or of zero), the others as without them."""
+    rng = np.random.default_rng(23)
+    c = Cache(rng, 1, 20, hkv, dh, 16, q8)
+    pos = [200 + r % 100 for r in range(rows)]
+    q, proj = rng.standard_normal((rows, hq, dh)).astype(np.float32), rng.standard_normal((rows, 2 * hq * dh)).astype(np.float32)
+    sel = random_lists(rng, rows, hkv, 4, [12] * rows)
+    sel[:, :, 0] = 0
+    bad = np.zeros((rows, hq), bool)
+    for i, (r, h) in enumerate([(0, 1), (1, 0), (1, hq - 1), (rows - 1, 2)]):
+        q[r, h, 3 * i] = (np.nan, np.inf, -np.inf, np.inf)[i]
+        bad[r, h] = True
+    clean = np.where(np.isfinite(q), q, 0).astype(np.float32)
+    got, _ = run_attend(lib, c, hq, q, proj, [0] * rows, pos, sel, row_seq=True)
+    want, _ = run_attend(lib, c, hq, clean, proj, [0] * rows, pos, sel, row_seq=True)
+    x, y = got.reshape(rows, hq, dh), want.reshape(rows, hq, dh)
+    assert np.all(np.isnan(x[bad])) and np.array_equal(bits(x[~bad]), bits(y[~bad]))
+
+
+def test_captured_attention_over_infinities_replays_like_eager_calls(lib):
+    """The rows that are formed again in plain fp32, in a captured graph, with eager calls in between."""
+    import torch
+
+    rng = np.random.default_rng(29)
+    hq, hkv, dh, ps, top, rows = 8, 2, 128, 64, 12, 2
+    c, seq, pos, q, proj, sel = chunk_of(rng, False, dh, ps, hq, hkv, rows, top, False)
+    c.kv[c.table[0, 1], 1, :, 3, 5], c.kv[c.table[1, 2], 0, :, 4, 9] = np.inf, -np.inf
+    want, _ = run_attend(lib, c, hq, q, proj, seq, pos, sel, row_seq=False)
+    wb = lib.hero_attn_sparse_work_bytes(rows, hq, hkv, dh, ps, top)
+    d = [dev(x) for x in (q, proj, c.bytes(), c.table, np.array(pos, np.int32), sel)]
+    work, out = empty(wb), empty(rows * hq * dh * 4)
+    args = sparse_args(c, hq, rows, ptr(d[4]), q_rot=ptr(d[0]), proj=ptr(d[1]), stride=2 * hq * dh, scale=float(np.float32(1 / np.sqrt(dh))), pages=ptr(d[2]), table=ptr(d[3]),
+                       work=ptr(work), work_bytes=wb, selected=ptr(d[5]), top=top, out=ptr(out))
+    graph, side = torch.cuda.CUDAGraph(), torch.cuda.Stream()
+    with torch.cuda.graph(graph, stream=side):
+        check(lib.hero_attn_sparse_paged(args, side.cuda_stream))
+    for _ in range(3):
+        out.zero_()
+        graph.replay()
+        assert np.array_equal(bits(host(out, np.float32)), bits(want.reshape(-1)))
+        again, _ = run_attend(lib, c, hq, q, proj, seq, pos, sel, row_seq=False)
+        assert np.array_equal(bits(again), bits(want))
+    assert np.isinf(want).any() or np.isnan(want).any()
