@@ -9,7 +9,7 @@ from __future__ import annotations
 
 import ctypes
 import os
-from ctypes import POINTER, c_char_p, c_double, c_float, c_int, c_int32, c_int64, c_size_t, c_uint64, c_void_p
+from ctypes import POINTER, c_char_p, c_double, c_float, c_int, c_int32, c_int64, c_size_t, c_uint64, c_uint8, c_void_p
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(HERE, "libhero_amd.so")
@@ -72,6 +72,14 @@ class KvReadArgs(ctypes.Structure):
         ("pool_pages", c_int64), ("summaries", c_void_p), ("positions", c_void_p), ("row_seq", c_void_p),
         ("rows", c_int32), ("seqs", c_int32), ("hkv", c_int32), ("dh", c_int32), ("f16", c_int32),
         ("k_out", c_void_p), ("v_out", c_void_p), ("k_max", c_void_p), ("k_min", c_void_p),
+    ]
+
+
+class AttnQ4Args(ctypes.Structure):
+    _fields_ = [
+        ("a", AttnDecodeArgs), ("pages", c_void_p), ("pool_pages", c_int64), ("page_table", c_void_p), ("page_size", c_int32), ("max_pages", c_int32),
+        ("row_seq", c_void_p), ("seqs", c_int32), ("sinks", c_int32), ("rope_positions", c_int64), ("rope_pos", c_void_p), ("rope_axes", c_int32),
+        ("plane_axis", c_uint8 * 128), ("work", c_void_p), ("work_bytes", c_int64),
     ]
 
 
@@ -167,6 +175,13 @@ SIGNATURES = {
     "hero_attn_select_pages": (c_int, [POINTER(AttnSparseArgs), c_void_p]),
     "hero_attn_sparse_work_bytes": (c_int64, [c_int64, c_int32, c_int32, c_int32, c_int32, c_int32]),
     "hero_attn_sparse_paged": (c_int, [POINTER(AttnSparseArgs), c_void_p]),
+    "hero_attn_q4_page_bytes": (c_int64, [c_int32, c_int32, c_int32]),
+    "hero_kv_append_q4": (c_int, [POINTER(AttnQ4Args), c_void_p]),
+    "hero_kv_read_q4": (c_int, [POINTER(KvReadArgs), c_void_p]),
+    "hero_attn_q4_work_bytes": (c_int64, [c_int64, c_int32, c_int32, c_int32, c_int64, c_int32, c_int32]),
+    "hero_attn_q4": (c_int, [POINTER(AttnQ4Args), c_void_p]),
+    "hero_logprobs_work_bytes": (c_int64, [c_int64, c_int64, c_int32]),
+    "hero_logprobs": (c_int, [c_void_p, c_int64, c_int64, c_int64, c_void_p, c_float, c_int32, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int64, c_void_p]),
     "hero_model_open": (c_int, [c_char_p, POINTER(c_void_p)]),
     "hero_model_open_image": (c_int, [c_void_p, c_size_t, POINTER(c_void_p)]),
     "hero_model_close": (None, [c_void_p]),

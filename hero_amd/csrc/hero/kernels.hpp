@@ -306,6 +306,58 @@ struct SparseAttnArgs {
 int64_t attn_sparse_work_bytes(int64_t rows, int64_t Hq, int64_t Hkv, int64_t Dh, int64_t page_size, int64_t top);
 void launch_attn_sparse(const SparseAttnArgs& a, hipStream_t s);
 
+// ---- the 4-bit paged cache (PagedRows without q8 and summaries; hero/q4.hpp has the layout)
+inline int64_t attn_q4_page_bytes(int64_t Hkv, int64_t Dh, int64_t page_size) { return 2 * Hkv * page_size * Dh * 9 / 16; }
+constexpr int kRopeAxes = 4;
+struct Kv4AppendArgs {
+    PagedRows c;
+    const float* proj;        // as in AttnDecodeArgs
+    int64_t proj_stride, k_off, v_off;
+    const float* q_gamma;
+    const float* k_gamma;
+    float eps;
+    const float* rope_cs;     // [rope_positions][Dh/2][2]
+    int64_t rope_positions;
+    const int32_t* rope_pos;  // [axes][rows]; null: positions (one axis)
+    int axes;
+    uint32_t axis_bits[8];    // the axis of plane i: bits 2 (i % 16) .. of word i / 16
+    float* q_rot;             // [rows][Hq][Dh]
+    int Hq;
+};
+void launch_kv4_append(const Kv4AppendArgs& a, hipStream_t s);
+void launch_kv4_read(const KvReadArgs& a, hipStream_t s);  // out[0], out[1]
+struct Attn4Args {
+    PagedRows c;
+    const float* q_rot;
+    const float* proj;        // the gates: [q | gate] pairs at 0
+    int64_t proj_stride;
+    float score_scale;
+    int Hq;
+    int window, sinks;        // window 0: every key up to the row's position
+    float* out_f32;           // [rows][Hq*Dh]; may be null
+    void* act_out;            // Q8_0 activations [rows][Hq*Dh]; may be null
+    float* work;
+};
+int64_t attn4_work_bytes(int64_t rows, int64_t Hq, int64_t Hkv, int64_t Dh, int64_t span, int64_t window, int64_t sinks);
+void launch_attn4(const Attn4Args& a, hipStream_t s);
+
+// ---- log probabilities of given tokens
+constexpr int kLogprobsTop = 64;  // alternatives at most
+struct LogprobsArgs {
+    const float* logits;      // [m] rows of v at a stride
+    int64_t stride, m, v;
+    const int32_t* targets;   // [m]; outside [0, v): the row is left out
+    float temp;
+    int top;
+    float* logprob;           // [m]; may be null
+    float* entropy;           // [m]; may be null
+    int32_t* top_ids;         // [m][top]
+    float* top_logprobs;      // [m][top]
+    void* work;
+};
+int64_t logprobs_work_bytes(int64_t m, int64_t v, int top);
+void launch_logprobs(const LogprobsArgs& a, hipStream_t s);
+
 // gemma.hip: the Gemma 4 text model's own kernels (one row: a decode step)
 // x[D] = the embedding row of *id times embed_scale, act = its Q8_0 row, and
 // tok[PL] = the per-layer table's row of *id times token_scale

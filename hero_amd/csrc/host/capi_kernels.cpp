@@ -742,4 +742,162 @@ int hero_attn_sparse_paged(const hero_attn_sparse_args* p, void* stream) {
     });
 }
 
+// ---- the 4-bit paged cache
+namespace {
+bool q4_shape(int64_t hkv, int64_t dh, int64_t ps) { return hkv > 0 && hkv <= 1024 && (dh == 128 || dh == 256) && ps >= 16 && ps <= 256 && ps % 16 == 0; }
+
+PagedRows q4_rows(const hero_attn_q4_args* p) {
+    require(p != nullptr, "null args");
+    const hero_attn_decode_args& a = p->a;
+    PagedRows c{};
+    c.pages = static_cast<uint16_t*>(p->pages);
+    c.page_table = p->page_table;
+    c.pool_pages = p->pool_pages;
+    c.page_size = p->page_size;
+    c.max_pages = p->max_pages;
+    c.positions = a.positions;
+    c.row_seq = p->row_seq;
+    c.rows = a.b;
+    c.seqs = p->seqs;
+    c.Hkv = a.hkv;
+    c.Dh = a.dh;
+    check_paged_rows(c, p->row_seq);
+    require(a.hq > 0 && a.hq % a.hkv == 0 && a.hq / a.hkv <= kAttnMaxGroup, "1 to 8 query heads per KV head");
+    require(a.b <= kMaxRowHeads / a.hq, "too many rows");
+    require(c.pages && aligned(c.pages, 16), "pages: 16-byte aligned device memory");
+    require(a.proj && aligned(a.proj, 4), "proj: device memory, 4-byte aligned");
+    require(a.q_rot && aligned(a.q_rot, 16), "q_rot: 16-byte aligned device memory");
+    return c;
+}
+}  // namespace
+
+int64_t hero_attn_q4_page_bytes(int32_t hkv, int32_t head_dim, int32_t page_size) {
+    return q4_shape(hkv, head_dim, page_size) ? attn_q4_page_bytes(hkv, head_dim, page_size) : -1;
+}
+
+int hero_kv_append_q4(const hero_attn_q4_args* p, void* stream) {
+    return guard([&] {
+        Kv4AppendArgs g{};
+        g.c = q4_rows(p);
+        const hero_attn_decode_args& a = p->a;
+        require(a.q_gamma && a.k_gamma && a.rope_cs, "null pointer");
+        require(aligned(a.q_gamma, 4) && aligned(a.k_gamma, 4) && aligned(a.rope_cs, 8) && aligned(p->rope_pos, 4), "misaligned pointer");
+        require(p->rope_positions > 0, "rope_positions must be positive");
+        require(p->rope_axes >= 1 && p->rope_axes <= kRopeAxes, "rope_axes must be in 1 .. 4");
+        require(p->rope_pos || p->rope_axes == 1, "several axes need rope_pos");
+        const int64_t qw = 2 * int64_t(a.hq) * a.dh, kw = int64_t(a.hkv) * a.dh;
+        require(a.k_off >= 0 && a.v_off >= 0 && a.proj_stride >= qw && a.k_off <= a.proj_stride - kw && a.v_off <= a.proj_stride - kw,
+                "q, k or v slices outside the projection row");
+        for (int i = 0; i < a.dh / 2; ++i) {
+            require(p->plane_axis[i] < p->rope_axes, "plane_axis: an axis that there is not");
+            g.axis_bits[i / 16] |= uint32_t(p->plane_axis[i]) << (2 * (i % 16));
+        }
+        g.proj = a.proj;
+        g.proj_stride = a.proj_stride;
+        g.k_off = a.k_off;
+        g.v_off = a.v_off;
+        g.q_gamma = a.q_gamma;
+        g.k_gamma = a.k_gamma;
+        g.eps = a.eps;
+        g.rope_cs = a.rope_cs;
+        g.rope_positions = p->rope_positions;
+        g.rope_pos = p->rope_pos;
+        g.axes = p->rope_axes;
+        g.q_rot = a.q_rot;
+        g.Hq = a.hq;
+        launch_kv4_append(g, as_stream(stream));
+        check_launch("hero_kv_append_q4");
+    });
+}
+
+int hero_kv_read_q4(const hero_kv_read_args* p, void* stream) {
+    return guard([&] {
+        require(p != nullptr, "null args");
+        KvReadArgs g{};
+        g.c.pages = const_cast<uint16_t*>(p->pages);
+        g.c.page_table = p->page_table;
+        g.c.pool_pages = p->pool_pages;
+        g.c.page_size = p->page_size;
+        g.c.max_pages = p->max_pages;
+        g.c.positions = p->positions;
+        g.c.row_seq = p->row_seq;
+        g.c.rows = p->rows;
+        g.c.seqs = p->seqs;
+        g.c.Hkv = p->hkv;
+        g.c.Dh = p->dh;
+        check_paged_rows(g.c, p->row_seq);
+        require(p->f16 == 0 || p->f16 == 1, "f16 must be 0 or 1");
+        require(!p->k_max && !p->k_min, "4-bit pages have no bounds: k_max and k_min must be NULL");
+        require(p->k_out || p->v_out, "no output");
+        require(p->pages && aligned(p->pages, 16), "pages: 16-byte aligned device memory");
+        require(aligned(p->k_out, 16) && aligned(p->v_out, 16), "outputs must be 16-byte aligned");
+        g.f16 = p->f16;
+        g.out[0] = p->k_out;
+        g.out[1] = p->v_out;
+        launch_kv4_read(g, as_stream(stream));
+        check_launch("hero_kv_read_q4");
+    });
+}
+
+int64_t hero_attn_q4_work_bytes(int64_t rows, int32_t hq, int32_t hkv, int32_t head_dim, int64_t max_ctx, int32_t window, int32_t sinks) {
+    if (rows <= 0 || hkv <= 0 || hkv > 1024 || hq <= 0 || hq % hkv || hq / hkv > kAttnMaxGroup || rows > kMaxRowHeads / hq || (head_dim != 128 && head_dim != 256) || max_ctx <= 0 ||
+        max_ctx > (int64_t(1) << 24) || window < 0 || sinks < 0)
+        return -1;
+    return attn4_work_bytes(rows, hq, hkv, head_dim, max_ctx, window, sinks);
+}
+
+int hero_attn_q4(const hero_attn_q4_args* p, void* stream) {
+    return guard([&] {
+        Attn4Args g{};
+        g.c = q4_rows(p);
+        const hero_attn_decode_args& a = p->a;
+        require(a.proj_stride >= 2 * int64_t(a.hq) * a.dh, "gates outside the projection row");
+        require(a.window >= 0, "window must be 0 (every key) or positive");
+        require(p->sinks >= 0 && (p->sinks == 0 || a.window > 0), "sinks: 0, or with a window the first positions that stay visible");
+        require(a.out_f32 || a.act_out, "no output");
+        require(aligned(a.out_f32, 16) && aligned(a.act_out, 16), "outputs must be 16-byte aligned");
+        const int64_t need = attn4_work_bytes(g.c.rows, a.hq, a.hkv, a.dh, int64_t(g.c.max_pages) * g.c.page_size, a.window, p->sinks);
+        require(need == 0 || (p->work && aligned(p->work, 16) && p->work_bytes >= need), "work: 16-byte aligned, hero_attn_q4_work_bytes");
+        g.q_rot = a.q_rot;
+        g.proj = a.proj;
+        g.proj_stride = a.proj_stride;
+        g.score_scale = a.score_scale;
+        g.Hq = a.hq;
+        g.window = a.window;
+        g.sinks = p->sinks;
+        g.out_f32 = a.out_f32;
+        g.act_out = a.act_out;
+        g.work = static_cast<float*>(p->work);
+        launch_attn4(g, as_stream(stream));
+        check_launch("hero_attn_q4");
+    });
+}
+
+// ---- log probabilities
+namespace {
+bool logprobs_shape(int64_t m, int64_t v, int32_t top_n) {
+    return m > 0 && m <= (int64_t(1) << 24) && v > 0 && v <= (int64_t(1) << 24) && top_n >= 0 && top_n <= kLogprobsTop && top_n <= v;
+}
+}  // namespace
+
+int64_t hero_logprobs_work_bytes(int64_t m, int64_t v, int32_t top_n) { return logprobs_shape(m, v, top_n) ? logprobs_work_bytes(m, v, top_n) : -1; }
+
+int hero_logprobs(const float* logits, int64_t stride, int64_t m, int64_t v, const int32_t* targets, float temp, int32_t top_n, float* logprob, float* entropy, int32_t* top_ids, float* top_logprobs,
+                  void* work, int64_t work_bytes, void* stream) {
+    return guard([&] {
+        require(logprobs_shape(m, v, top_n), "m and v in 1 .. 2^24, top_n in 0 .. 64 and at most v");
+        require(logits && aligned(logits, 4), "logits: device memory, 4-byte aligned");
+        require(stride >= v && stride <= (int64_t(1) << 40) / m, "stride must be at least v");
+        require(temp > 0.f && temp <= 3.402823466e38f, "temp must be positive and finite");
+        require((top_n > 0) == (top_ids != nullptr) && (top_n > 0) == (top_logprobs != nullptr), "top_ids and top_logprobs go with top_n > 0");
+        require(logprob || entropy || top_n > 0, "no output");
+        require(targets || !logprob, "logprob needs targets");
+        require(aligned(targets, 4) && aligned(logprob, 4) && aligned(entropy, 4) && aligned(top_ids, 4) && aligned(top_logprobs, 4), "misaligned pointer");
+        const int64_t need = logprobs_work_bytes(m, v, top_n);
+        require(need == 0 || (work && aligned(work, 16) && work_bytes >= need), "work: 16-byte aligned, hero_logprobs_work_bytes");
+        launch_logprobs({logits, stride, m, v, targets, temp, top_n, logprob, entropy, top_ids, top_logprobs, work}, as_stream(stream));
+        check_launch("hero_logprobs");
+    });
+}
+
 }  // extern "C"

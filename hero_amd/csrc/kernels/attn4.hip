@@ -1,0 +1,375 @@
+// attn4.hip -- gated attention over the 4-bit pages of the paged K/V cache: single
+// tokens of many sequences and chunks of prompts, with or without a sliding window
+// behind which the first tokens stay visible.
+#include "hero/device.hpp"
+#include "hero/kernels.hpp"
+#include "hero/paged.hpp"
+#include "hero/q4.hpp"
+
+namespace hero {
+
+namespace {
+
+typedef float f4_t __attribute__((ext_vector_type(4)));
+
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kPOne = 8192.f;  // a weight's terms are of 2^13 2^(s - m); its part in the total is 2^(s - m)
+constexpr float kPSlack = 2.f;   // m may lag the maximum by this: weights stay below 2^15
+constexpr float kLowest = -3.402823466e38f;
+
+__device__ __forceinline__ float column_other(float x) {  // the value of column c ^ 8
+    return __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(x), 0x128, 0xF, 0xF, false));  // row_ror:8
+}
+__device__ __forceinline__ float max_over_p(float x) {
+    x = fmaxf(x, __shfl_xor(x, 16));
+    return fmaxf(x, __shfl_xor(x, 32));
+}
+__device__ __forceinline__ float sum_over_p(float x) {
+    x += __shfl_xor(x, 16);
+    return x + __shfl_xor(x, 32);
+}
+__device__ __forceinline__ float exp2_hw(float x) { return __builtin_amdgcn_exp2f(x); }  // 1 ulp; 0 below its range
+
+// x as two fp16 terms; pinned first, so that both are formed from one rounding of it
+__device__ __forceinline__ void split_f16(float x, _Float16& hi, _Float16& lo) {
+    asm("" : "+v"(x));
+    hi = _Float16(x);
+    lo = _Float16(x - float(hi));
+}
+
+// two neighbouring codes in the low (F = 0) or second (F = 1) fields of a word's halves, as fp16
+template <int F>
+__device__ __forceinline__ q4_h2 codes_of(uint32_t w) {
+    if constexpr (F == 0)  // 0x6400 | c is 1024 + c
+        return __builtin_bit_cast(q4_h2, (w & 0x000F000Fu) | 0x64006400u) - _Float16(1032.f);
+    else                   // 0x6400 | c << 4 is 1024 + 16 c
+        return __builtin_elementwise_fma(__builtin_bit_cast(q4_h2, (w & 0x00F000F0u) | 0x64006400u), q4_h2{_Float16(0.0625f), _Float16(0.0625f)},
+                                         q4_h2{_Float16(-72.f), _Float16(-72.f)});
+}
+
+__device__ __forceinline__ q4_h8 join(q4_h2 a, q4_h2 b, q4_h2 c, q4_h2 d) { return q4_h8{a[0], a[1], b[0], b[1], c[0], c[1], d[0], d[1]}; }
+
+// a lane's share of a record of keys and the one of values
+template <int DH>
+struct TileRegs {
+    uint4 k[DH / 128], v[DH / 128];
+    _Float16 kd[DH / 32];
+    q4_h2 vd[DH / 16];
+    __device__ __forceinline__ void load(const uint8_t* krec, const uint8_t* vrec, int lane) {
+        const int p = lane >> 4, b = lane & 15;
+#pragma unroll
+        for (int h = 0; h < DH / 128; ++h) {
+            k[h] = *reinterpret_cast<const uint4*>(krec + 1024 * h + b * 64 + p * 16);
+            v[h] = *reinterpret_cast<const uint4*>(vrec + 1024 * h + lane * 16);
+        }
+        __builtin_memcpy(kd, __builtin_assume_aligned(krec + 8 * DH + b * (DH / 16), 8), sizeof(kd));
+        __builtin_memcpy(vd, __builtin_assume_aligned(vrec + 8 * DH + p * (DH / 4), 16), sizeof(vd));
+    }
+};
+
+// R rows of up to COLS (row, query head) pairs: pair i is row i / group, head i % group
+template <int DH, int COLS>
+struct Merge {
+    float o[4][COLS][DH], m[4][COLS], l[4][COLS];
+};
+
+template <int DH>
+__device__ __forceinline__ void store_out(const Attn4Args& a, int r, int h, int ch, float o, float l) {
+    const int64_t width = int64_t(a.Hq) * DH, idx = int64_t(r) * width + int64_t(h) * DH + ch;
+    const float gate = a.proj[int64_t(r) * a.proj_stride + int64_t(h) * 2 * DH + DH + ch];
+    const float out = l == 0.f ? 0.f : (o / l) * sigmoid_f32(gate);
+    if (a.out_f32) a.out_f32[idx] = out;
+    if (a.act_out) {
+        float amax = fabsf(out);
+        for (int off = 16; off > 0; off >>= 1) amax = fmaxf(amax, __shfl_xor(amax, off));
+        const float d = amax / 127.f, id = d != 0.f ? 1.f / d : 0.f;
+        int8_t* qs = static_cast<int8_t*>(a.act_out);
+        qs[idx] = int8_t(int(roundf(out * id)));
+        if ((ch & 31) == 0) reinterpret_cast<float*>(qs + int64_t(a.c.rows) * width)[idx >> 5] = half_bits_to_f32(fp32_to_fp16_ref(d));
+    }
+}
+
+// a row's keys: those below `stay`, and from `first` (>= stay) to `pos`
+struct Seen {
+    int stay, first, pos;
+};
+__device__ __forceinline__ Seen row_sees(const Attn4Args& a, int pos) {
+    const int first = a.window > 0 ? max(0, pos - a.window + 1) : 0;
+    return {a.window > 0 ? min(a.sinks, first) : 0, first, pos};
+}
+
+// A workgroup of four waves: R = rows * group pairs of rows r0 .. of one K/V head, one of
+// nsplit equal ranges of their records, two records (32 keys) a wave at a time.
+template <int DH, bool PAIR>
+__global__ __launch_bounds__(256, 2) void attn4_kernel(Attn4Args a, int R, int nsplit) {
+    constexpr int COLS = PAIR ? 8 : 16, H = DH / 128, NS = DH / 32, NV = DH / 16;
+    const PagedRows& c = a.c;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, p = lane >> 4, b = lane & 15;
+    const int split = blockIdx.x % nsplit, g = blockIdx.x / nsplit % c.Hkv, tile0 = blockIdx.x / nsplit / c.Hkv, r0 = tile0 * R;
+    const int group = a.Hq / c.Hkv, tpp = c.page_size / kQ4Tile;
+    __shared__ Merge<DH, COLS> sh;
+
+    const int col = PAIR ? b & 7 : b, mine = min(col / group, R - 1), r = r0 + mine;
+    const bool used = col < R * group && r < c.rows;
+    int seq = 0;
+    const int pos = used ? row_position(c, r, &seq) : -1;
+    const Seen sees = row_sees(a, pos);
+
+    // queries: a power of two brings the head's largest channel below 1
+    q4_h8 qh[NS], ql[PAIR ? 1 : NS];
+    float scale = 0.f;
+    {
+        const float* q = a.q_rot + (int64_t(min(r, c.rows - 1)) * a.Hq + g * group + col % group) * DH + 8 * p;
+        float x[NS][8], amax = 0.f;
+#pragma unroll
+        for (int s = 0; s < NS; ++s) {
+            __builtin_memcpy(x[s], __builtin_assume_aligned(q + 32 * s, 16), 32);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) amax = fmaxf(amax, fabsf(x[s][j]));
+        }
+        amax = max_over_p(amax);
+        const int e = amax > 0.f && amax < INFINITY ? ilogbf(amax) + 1 : 0;
+#pragma unroll
+        for (int s = 0; s < NS; ++s)
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                _Float16 hi, lo;
+                split_f16(ldexpf(x[s][j], -e), hi, lo);
+                if constexpr (PAIR)
+                    qh[s][j] = b < 8 ? hi : lo;
+                else
+                    qh[s][j] = hi, ql[s][j] = lo;
+            }
+        scale = ldexpf(a.score_scale * kLog2e, e);
+    }
+
+    f4_t o[NV];
+#pragma unroll
+    for (int n = 0; n < NV; ++n) o[n] = f4_t{0.f, 0.f, 0.f, 0.f};
+    float m = kLowest, l = 0.f;
+
+    // rows of one sequence at a time (mostly there is one)
+    for (int k0 = 0; k0 < R;) {
+        int s0, k1 = k0 + 1;
+        const int p0 = r0 + k0 < c.rows ? row_position(c, r0 + k0, &s0) : -1;
+        if (p0 < 0) {
+            ++k0;
+            continue;
+        }
+        int lo = p0, hi = p0;
+        for (; k1 < R && r0 + k1 < c.rows; ++k1) {
+            int s1;
+            const int p1 = row_position(c, r0 + k1, &s1);
+            if (p1 < 0 || s1 != s0) break;
+            lo = min(lo, p1), hi = max(hi, p1);
+        }
+        const bool here = used && pos >= 0 && mine >= k0 && mine < k1;
+        k0 = k1;
+        // records: those of the first keys that stay, then from the earliest window to the last row
+        const Seen most = row_sees(a, hi), least = row_sees(a, lo);
+        const int first = least.first / kQ4Tile, stay = min((most.stay + kQ4Tile - 1) / kQ4Tile, first);
+        const int tiles = stay + hi / kQ4Tile - first + 1, units = (tiles + 1) / 2;
+        const int u0 = int(int64_t(units) * split / nsplit), u1 = int(int64_t(units) * (split + 1) / nsplit);
+        const int32_t* table = c.page_table + int64_t(s0) * c.max_pages;
+
+        auto locate = [&](int k, int& t, int64_t& page) {
+            t = k < stay ? k : first + k - stay;
+            const int lp = min(t, hi / kQ4Tile) / tpp;
+            page = __builtin_amdgcn_readfirstlane(table[lp]);
+            page = k < tiles && page >= 0 && page < c.pool_pages ? page : -1;
+        };
+        for (int u = u0 + wave; u < u1; u += 4) {
+            TileRegs<DH> regs[2];
+            int t[2];
+            bool ok[2];
+#pragma unroll
+            for (int x = 0; x < 2; ++x) {
+                int64_t page;
+                locate(2 * u + x, t[x], page);
+                ok[x] = page >= 0;
+                const int64_t pg = page >= 0 ? page : 0;
+                regs[x].load(q4_record<DH>(c, pg, 0, g, t[x] % tpp), q4_record<DH>(c, pg, 1, g, t[x] % tpp), lane);
+            }
+            // scores of keys 16 t + 4 p + i for the lane's column
+            float s[8];
+#pragma unroll
+            for (int x = 0; x < 2; ++x) {
+                f4_t acc = f4_t{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                for (int k = 0; k < NS; ++k) {
+                    const uint4 w4 = regs[x].k[k / 4];
+                    const uint32_t w = k % 4 == 0 ? w4.x : k % 4 == 1 ? w4.y : k % 4 == 2 ? w4.z : w4.w;
+                    const q4_h2 d = {regs[x].kd[k], regs[x].kd[k]};
+                    const q4_h8 f = join(codes_of<0>(w) * d, codes_of<1>(w) * d, codes_of<0>(w >> 8) * d, codes_of<1>(w >> 8) * d);
+                    acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(f, qh[k], acc, 0, 0, 0);
+                    if constexpr (!PAIR) acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(f, ql[k], acc, 0, 0, 0);
+                }
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const float v = PAIR ? acc[i] + column_other(acc[i]) : acc[i];
+                    const int key = kQ4Tile * t[x] + 4 * p + i;
+                    const bool sees_it = here && ok[x] && key <= sees.pos && (key >= sees.first || key < sees.stay);
+                    s[4 * x + i] = sees_it ? v * scale : -INFINITY;
+                }
+            }
+            float best = s[0];
+#pragma unroll
+            for (int i = 1; i < 8; ++i) best = fmaxf(best, s[i]);
+            if (__ballot(best > m + kPSlack)) {
+                const float to = fmaxf(m, max_over_p(best)), f = exp2_hw(m - to);
+                m = to;
+                l *= f;
+#pragma unroll
+                for (int n = 0; n < NV; ++n) o[n] *= f;
+            }
+            q4_h8 w8, w8l;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const float w = exp2_hw(s[i] - m);
+                l += w;
+                _Float16 hi, lo;
+                split_f16(w * kPOne, hi, lo);
+                if constexpr (PAIR)
+                    w8[i] = b < 8 ? hi : lo;
+                else
+                    w8[i] = hi, w8l[i] = lo;
+            }
+            // a slot past the last row, or of a page that holds nothing, may hold anything: its steps count as 0
+#pragma unroll
+            for (int x = 0; x < 2; ++x) {
+                if (!ok[x] || kQ4Tile * t[x] + 15 > hi) {
+#pragma unroll
+                    for (int n = 0; n < NV; ++n)
+#pragma unroll
+                        for (int i = 0; i < 2; ++i)
+                            if (!ok[x] || kQ4Tile * t[x] + 4 * p + 2 * (n & 1) + i > hi) regs[x].vd[n][i] = _Float16(0.f);
+                }
+            }
+#pragma unroll
+            for (int h = 0; h < H; ++h)
+#pragma unroll
+                for (int y = 0; y < 4; ++y) {  // byte y of the words: channels 128 h + 32 y + b and + 16
+                    // 16-bit halves: that byte of two neighbouring keys
+                    const uint32_t pick = 0x0C040C00u + 0x00010001u * y;
+                    const uint4 va = regs[0].v[h], vb = regs[1].v[h];
+                    const uint32_t w0 = __builtin_amdgcn_perm(va.y, va.x, pick), w1 = __builtin_amdgcn_perm(va.w, va.z, pick);
+                    const uint32_t w2 = __builtin_amdgcn_perm(vb.y, vb.x, pick), w3 = __builtin_amdgcn_perm(vb.w, vb.z, pick);
+                    const q4_h2 d0 = regs[0].vd[2 * (4 * h + y)], d1 = regs[0].vd[2 * (4 * h + y) + 1];
+                    const q4_h2 d2 = regs[1].vd[2 * (4 * h + y)], d3 = regs[1].vd[2 * (4 * h + y) + 1];
+                    const q4_h8 fa = join(codes_of<0>(w0) * d0, codes_of<0>(w1) * d1, codes_of<0>(w2) * d2, codes_of<0>(w3) * d3);
+                    const q4_h8 fb = join(codes_of<1>(w0) * d0, codes_of<1>(w1) * d1, codes_of<1>(w2) * d2, codes_of<1>(w3) * d3);
+                    f4_t& oa = o[8 * h + 2 * y];
+                    f4_t& ob = o[8 * h + 2 * y + 1];
+                    oa = __builtin_amdgcn_mfma_f32_16x16x32_f16(fa, w8, oa, 0, 0, 0);
+                    ob = __builtin_amdgcn_mfma_f32_16x16x32_f16(fb, w8, ob, 0, 0, 0);
+                    if constexpr (!PAIR) {
+                        oa = __builtin_amdgcn_mfma_f32_16x16x32_f16(fa, w8l, oa, 0, 0, 0);
+                        ob = __builtin_amdgcn_mfma_f32_16x16x32_f16(fb, w8l, ob, 0, 0, 0);
+                    }
+                }
+        }
+    }
+
+    // the four waves' results
+    l = sum_over_p(l);
+#pragma unroll
+    for (int n = 0; n < NV; ++n) {
+        f4_t v = o[n];
+        if constexpr (PAIR) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) v[i] += column_other(v[i]);
+        }
+        if (b < COLS) *reinterpret_cast<f4_t*>(&sh.o[wave][col][16 * n + 4 * p]) = v;
+    }
+    if (p == 0 && b < COLS) sh.m[wave][col] = m, sh.l[wave][col] = l;
+    __syncthreads();
+    for (int idx = threadIdx.x; idx < R * group * DH; idx += 256) {
+        const int k = idx / DH, ch = idx % DH, row = r0 + k / group;
+        if (row >= c.rows) break;
+        float mx = sh.m[0][k];
+#pragma unroll
+        for (int w = 1; w < 4; ++w) mx = fmaxf(mx, sh.m[w][k]);
+        float lt = 0.f, ot = 0.f;
+#pragma unroll
+        for (int w = 0; w < 4; ++w) {
+            const float f = exp2_hw(sh.m[w][k] - mx);
+            lt += f * sh.l[w][k];
+            ot += f * sh.o[w][k][ch];
+        }
+        ot *= 1.f / kPOne;
+        if (nsplit == 1) {
+            int s;
+            if (row_position(c, row, &s) >= 0) store_out<DH>(a, row, g * group + k % group, ch, ot, lt);
+        } else {
+            float* rec = a.work + ((int64_t(row) * a.Hq + g * group + k % group) * nsplit + split) * (DH + 4);
+            if (ch == 0) rec[0] = mx, rec[1] = lt;
+            rec[4 + ch] = ot;
+        }
+    }
+}
+
+// a workgroup per (row, query head), a lane per channel
+template <int DH>
+__global__ __launch_bounds__(DH) void attn4_combine_kernel(Attn4Args a, int nsplit) {
+    const int r = blockIdx.x / a.Hq, h = blockIdx.x % a.Hq, t = threadIdx.x;
+    int seq;
+    if (row_position(a.c, r, &seq) < 0) return;
+    const float* rec = a.work + int64_t(blockIdx.x) * nsplit * (DH + 4);
+    float mx = kLowest;
+    for (int s = 0; s < nsplit; ++s) mx = fmaxf(mx, rec[int64_t(s) * (DH + 4)]);
+    float l = 0.f, o = 0.f;
+    for (int s = 0; s < nsplit; ++s) {
+        const float f = exp2_hw(rec[int64_t(s) * (DH + 4)] - mx);
+        l += f * rec[int64_t(s) * (DH + 4) + 1];
+        o += f * rec[int64_t(s) * (DH + 4) + 4 + t];
+    }
+    store_out<DH>(a, r, h, t, o, l);
+}
+
+// Rows a workgroup takes, and into how many ranges their keys are split: about four
+// workgroups per CU over all rows and heads, at least eight units of 32 keys each.
+constexpr int64_t kGroups = 1024;
+struct Plan {
+    int R, nsplit;
+    int64_t tiles, most;  // groups of rows; ranges that the keys allow
+};
+Plan attn4_plan(int64_t rows, int64_t group, int64_t Hkv, bool chunk, int64_t span, int64_t window, int64_t sinks) {
+    Plan p;
+    p.R = chunk && rows > 1 ? int(16 / group) : 1;
+    const int64_t keys = window > 0 ? std::min(span, window + sinks + p.R + 2 * kQ4Tile) : span;
+    p.tiles = (rows + p.R - 1) / p.R;
+    p.most = std::max<int64_t>(1, (keys + 31) / 32 / 8);
+    p.nsplit = int(std::max<int64_t>(1, std::min(kGroups / (p.tiles * Hkv), p.most)));
+    return p;
+}
+
+}  // namespace
+
+// Room for any call of up to `rows` rows: where there are several ranges, the workgroups
+// are at most kGroups, of R * group results each.
+int64_t attn4_work_bytes(int64_t rows, int64_t Hq, int64_t Hkv, int64_t Dh, int64_t span, int64_t window, int64_t sinks) {
+    int64_t slots = 0;
+    for (const bool chunk : {false, true}) {
+        const Plan p = attn4_plan(rows, Hq / Hkv, Hkv, chunk, span, window, sinks);
+        if (p.most > 1) slots = std::max(slots, std::min(kGroups, p.tiles * Hkv * p.most) * p.R * (Hq / Hkv));
+    }
+    return slots * (Dh + 4) * 4;
+}
+
+namespace {
+template <int DH, bool PAIR>
+void attn4_sized(const Attn4Args& a, const Plan& p, hipStream_t s) {
+    hipLaunchKernelGGL((attn4_kernel<DH, PAIR>), dim3(unsigned(p.tiles * a.c.Hkv * p.nsplit)), dim3(256), 0, s, a, p.R, p.nsplit);
+    if (p.nsplit > 1) hipLaunchKernelGGL(attn4_combine_kernel<DH>, dim3(unsigned(a.c.rows * a.Hq)), dim3(DH), 0, s, a, p.nsplit);
+}
+}  // namespace
+
+void launch_attn4(const Attn4Args& a, hipStream_t s) {
+    const Plan p = attn4_plan(a.c.rows, a.Hq / a.c.Hkv, a.c.Hkv, a.c.row_seq != nullptr, int64_t(a.c.max_pages) * a.c.page_size, a.window, a.sinks);
+    if (a.c.Dh == 256)
+        p.R == 1 ? attn4_sized<256, true>(a, p, s) : attn4_sized<256, false>(a, p, s);
+    else
+        p.R == 1 ? attn4_sized<128, true>(a, p, s) : attn4_sized<128, false>(a, p, s);
+}
+
+}  // namespace hero

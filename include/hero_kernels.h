@@ -453,6 +453,98 @@ int hero_attn_select_pages(const hero_attn_sparse_args* args, void* stream);
 int64_t hero_attn_sparse_work_bytes(int64_t rows, int32_t hq, int32_t hkv, int32_t head_dim, int32_t page_size, int32_t top);
 int hero_attn_sparse_paged(const hero_attn_sparse_args* args, void* stream);
 
+/* ---- a 4-bit paged cache -----------------------------------------------------
+ * No counterpart in the reference. The paged K/V pool with 4.5 bits a value: 32
+ * neighbouring channels of a row share a step of 8 significant bits (fp16), each
+ * is a code -8 .. 7 times it, which fp16 holds exactly. Rows enter by
+ * hero_kv_append_q4, are attended to by hero_attn_q4 (one token of each of many
+ * sequences, chunks of prompts, or both in one call) and come back by
+ * hero_kv_read_q4. A pool is [pool_pages] pages of hero_attn_q4_page_bytes bytes,
+ * 16-byte aligned; what a page holds where is hero_amd/csrc/hero/q4.hpp's.
+ *
+ * Rows, sequences, page table, page sizes, left-out rows and pages that hold
+ * nothing are as for the long-context calls above (hero_attn_sparse_args): row r
+ * is the token at a.positions[r] of sequence row_seq[r] (NULL: of sequence r).
+ * Heads of 128 or 256 channels, 1 to 8 query heads per K/V head, at most 2^21
+ * (row, query head) pairs a call. */
+typedef struct hero_attn_q4_args {
+    hero_attn_decode_args a;     /* k_cache, v_cache, scores, max_ctx unused */
+    void* pages;
+    int64_t pool_pages;
+    const int32_t* page_table;   /* [seqs][max_pages] */
+    int32_t page_size, max_pages;
+    const int32_t* row_seq;      /* [a.b] or NULL */
+    int32_t seqs;
+    int32_t sinks;               /* with a.window > 0: the first positions, which stay visible behind the window */
+    int64_t rope_positions;      /* rows of a.rope_cs; append leaves out rows past them */
+    const int32_t* rope_pos;     /* [rope_axes][a.b] rotary positions, or NULL: a.positions (rope_axes 1) */
+    int32_t rope_axes;           /* 1 .. 4 */
+    uint8_t plane_axis[128];     /* the axis that turns plane i (channels i and i + dh/2); of dh/2 planes */
+    void* work;
+    int64_t work_bytes;
+} hero_attn_q4_args;
+
+/* Bytes of one page; -1 for shapes that the calls refuse. */
+int64_t hero_attn_q4_page_bytes(int32_t hkv, int32_t head_dim, int32_t page_size);
+
+/* q and k RMSNorm (nm/src/components.hpp:176-181) and rotation (nm/src/attention.hpp:76-91)
+ * formed in 64 bits and rounded to fp32 once (q to a.q_rot), then k and v as 4-bit
+ * blocks to their page slots. Plane i of row r is turned by
+ * rope_cs[rope_pos[plane_axis[i]][r]][i]: with several axes (time, height and
+ * width of an image's tokens) a row has a rotary position on each, apart from
+ * its place in the cache; a row with one outside [0, rope_positions) is left out.
+ * Block: m its value of largest magnitude (of two such the positive one), step d =
+ * fp16(-m / 8) rounded to 8 significant bits (halves up; multiples of 2^-21 below
+ * 2^-14), codes clamp(round(x / d), -8, 7) with halves to even. NaN counts as 0,
+ * what lies past +-65280 as that. Rows may come in any order, but no two rows of
+ * a call for one place. Uses a.proj, proj_stride, k_off, v_off, q_gamma, k_gamma,
+ * eps, rope_cs, positions, q_rot (16-byte aligned), b, hq, hkv, dh, the page, row
+ * and rope fields. */
+int hero_kv_append_q4(const hero_attn_q4_args* args, void* stream);
+
+/* Rows of the 4-bit cache back as fp32 or fp16 (both exact) to k_out and v_out
+ * [rows][hkv*dh], 16-byte aligned, either may be NULL; q8 and summaries are
+ * unused, k_max and k_min must be NULL. Left-out rows stay as they were. */
+int hero_kv_read_q4(const hero_kv_read_args* args, void* stream);
+
+/* Gated GQA attention (nm/src/qwen35.hpp:387-393) of each row over the stored
+ * positions j <= its own, with a.window > 0 (nm/src/attention.hpp:159-176) those of
+ * them past position - window or below `sinks`: softmax(score_scale * q . k), the
+ * weighted sum of the values, sigmoid(gate). The rows' own keys are in the cache
+ * already. A position in a page that holds nothing is not there; a row that sees
+ * none gets zeros. Positions past a sequence's last row of the call have no
+ * influence, whatever the pool holds there; the others hold what
+ * hero_kv_append_q4 stored. Outputs: a.out_f32 and / or a.act_out (Q8_0
+ * activations), at least one, 16-byte aligned. Rows of one sequence should stand
+ * together: neighbouring rows share the reads of their keys. Results agree with
+ * the formula over the stored values to fp32 rounding, save that a query's channels are
+ * kept to 2^-23 of the head's largest and weights to 2^-23 of themselves or
+ * 2^-38 of the row's largest. Uses a.q_rot, proj (the gates), proj_stride, positions,
+ * score_scale, window, b, hq, hkv, dh, the page and row fields, sinks and work
+ * (hero_attn_q4_work_bytes, 16-byte aligned; NULL where that is 0; the sizes
+ * grow with the rows; calls that may overlap need one each). max_ctx of the size
+ * function: max_pages * page_size. */
+int64_t hero_attn_q4_work_bytes(int64_t rows, int32_t hq, int32_t hkv, int32_t head_dim, int64_t max_ctx, int32_t window, int32_t sinks);
+int hero_attn_q4(const hero_attn_q4_args* args, void* stream);
+
+/* ---- log probabilities -------------------------------------------------------
+ * Of m rows of v logits (row r at logits + r * stride), z = logits / temp: the
+ * log probability of token targets[r], logprob[r] = z[targets[r]] - log sum
+ * exp(z); the entropy -sum p log p; and the top_n (0 .. 64, at most v) most likely
+ * tokens, top_ids [m][top_n] by logit descending (ties to the lowest id; NaN last) with
+ * top_logprobs [m][top_n]. The device form of the log probabilities that the
+ * reference's tools print (nm/tools/qwen35_check.cpp:45-67). logprob, entropy, and
+ * the top pair may each be NULL (top_n 0 where the pair is), not all. A row whose target
+ * is outside [0, v) is left out: its outputs stay as they were; targets NULL: every
+ * row counts, and logprob must be NULL. A logit of -inf has probability 0; a row with a
+ * NaN or +inf, or of nothing but -inf, has NaN log probabilities and entropy. Log
+ * probabilities near 0 keep their relative precision (the sum over the other
+ * tokens is formed without the largest). work: hero_logprobs_work_bytes(m, v, top_n)
+ * bytes of device memory, 16-byte aligned (NULL where that is 0; the sizes grow
+ * with the rows). */
+int64_t hero_logprobs_work_bytes(int64_t m, int64_t v, int32_t top_n);
+int hero_logprobs(const float* logits, int64_t stride, int64_t m, int64_t v, const int32_t* targets, float temp, int32_t top_n, float* logprob, float* entropy, int32_t* top_ids, float* top_logprobs, void* work, int64_t work_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
