@@ -18,7 +18,7 @@ constexpr float kPSlack = 2.f;   // m may lag the maximum by this: weights stay 
 constexpr float kLowest = -3.402823466e38f;
 
 __device__ __forceinline__ float column_other(float x) {  // the value of column c ^ 8
-    return __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(x), 0x128, 0xF, 0xF, false));  // row_ror:8
+    return __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(x), 0x128, 0xF, 0xF, true));  // row_ror:8
 }
 __device__ __forceinline__ float max_over_p(float x) {
     x = fmaxf(x, __shfl_xor(x, 16));
@@ -37,15 +37,21 @@ __device__ __forceinline__ void split_f16(float x, _Float16& hi, _Float16& lo) {
     lo = _Float16(x - float(hi));
 }
 
-// two neighbouring codes in the low (F = 0) or second (F = 1) fields of a word's halves, as fp16
-template <int F>
-__device__ __forceinline__ q4_h2 codes_of(uint32_t w) {
-    if constexpr (F == 0)  // 0x6400 | c is 1024 + c
-        return __builtin_bit_cast(q4_h2, (w & 0x000F000Fu) | 0x64006400u) - _Float16(1032.f);
-    else                   // 0x6400 | c << 4 is 1024 + 16 c
-        return __builtin_elementwise_fma(__builtin_bit_cast(q4_h2, (w & 0x00F000F0u) | 0x64006400u), q4_h2{_Float16(0.0625f), _Float16(0.0625f)},
-                                         q4_h2{_Float16(-72.f), _Float16(-72.f)});
-}
+// Two neighbouring codes in the low (F = 0) or second (F = 1) fields of a word's halves, as fp16.
+// The masks are kept in registers that the compiler does not see through: it then joins mask and
+// or into one instruction, which takes no literals.
+struct FieldMasks {
+    uint32_t low = 0x000F000Fu, second = 0x00F000F0u, one = 0x64006400u;
+    __device__ __forceinline__ FieldMasks() { asm("" : "+s"(low), "+s"(second), "+v"(one)); }
+    template <int F>
+    __device__ __forceinline__ q4_h2 codes(uint32_t w) const {
+        if constexpr (F == 0)  // 0x6400 | c is 1024 + c
+            return __builtin_bit_cast(q4_h2, (w & low) | one) - _Float16(1032.f);
+        else                   // 0x6400 | c << 4 is 1024 + 16 c
+            return __builtin_elementwise_fma(__builtin_bit_cast(q4_h2, (w & second) | one), q4_h2{_Float16(0.0625f), _Float16(0.0625f)},
+                                             q4_h2{_Float16(-72.f), _Float16(-72.f)});
+    }
+};
 
 __device__ __forceinline__ q4_h8 join(q4_h2 a, q4_h2 b, q4_h2 c, q4_h2 d) { return q4_h8{a[0], a[1], b[0], b[1], c[0], c[1], d[0], d[1]}; }
 
@@ -66,6 +72,39 @@ struct TileRegs {
         __builtin_memcpy(vd, __builtin_assume_aligned(vrec + 8 * DH + p * (DH / 4), 16), sizeof(vd));
     }
 };
+
+// A wave's ring of units (two records of keys and of values) in shared memory, filled by
+// loads that go there directly: what is in flight takes no registers. Records arrive as
+// they lie, 1 KB a load, but for the keys' 16-byte pieces: piece p of key b goes to place
+// p ^ (b / 4) of the key's 64 bytes, so that the lanes that read one piece of sixteen keys
+// meet every bank once.
+template <int DH, int D>
+struct Ring {
+    static constexpr int H = DH / 128, kLoads = 2 * 3 * H;  // load instructions of a unit
+    struct Slot {
+        uint4 k[2][H][64], v[2][H][64];
+        struct {
+            uint8_t k[DH], v[DH];  // next to each other: one load where they are 128 bytes
+        } steps[2];
+    };
+    Slot slot[D];
+};
+template <int DH, int D>
+__device__ __forceinline__ void ring_fetch(typename Ring<DH, D>::Slot& s, int x, const uint8_t* krec, const uint8_t* vrec, int lane) {
+    constexpr int H = DH / 128;
+#pragma unroll
+    for (int h = 0; h < H; ++h) {
+        lds_dma_b128(krec + 1024 * h + (lane & ~3) * 16 + ((lane ^ lane >> 4) & 3) * 16, lds_offset(&s.k[x][h][0]));
+        lds_dma_b128(vrec + 1024 * h + lane * 16, lds_offset(&s.v[x][h][0]));
+    }
+    if constexpr (H == 1) {
+        const uint8_t* rec = lane < 32 ? krec : vrec - 128;
+        lds_dma_b32(rec + 8 * DH + lane * 4, lds_offset(&s.steps[x].k[0]));
+    } else {
+        lds_dma_b32(krec + 8 * DH + lane * 4, lds_offset(&s.steps[x].k[0]));
+        lds_dma_b32(vrec + 8 * DH + lane * 4, lds_offset(&s.steps[x].v[0]));
+    }
+}
 
 // R rows of up to COLS (row, query head) pairs: pair i is row i / group, head i % group
 template <int DH, int COLS>
@@ -98,25 +137,263 @@ __device__ __forceinline__ Seen row_sees(const Attn4Args& a, int pos) {
     return {a.window > 0 ? min(a.sinks, first) : 0, first, pos};
 }
 
+// The four waves' results of `pairs` = rows x group pairs joined, and stored: as the row's where
+// the keys were not split, else as this range's.
+template <int DH, int COLS>
+__device__ __forceinline__ void merge_waves(const Attn4Args& a, const Merge<DH, COLS>& sh, int r0, int rows, int g, int nsplit, int split) {
+    const int group = a.Hq / a.c.Hkv;
+    for (int idx = threadIdx.x; idx < rows * group * DH; idx += 256) {
+        const int k = idx / DH, ch = idx % DH, row = r0 + k / group;
+        if (row >= a.c.rows) break;
+        float mx = sh.m[0][k];
+#pragma unroll
+        for (int w = 1; w < 4; ++w) mx = fmaxf(mx, sh.m[w][k]);
+        float lt = 0.f, ot = 0.f;
+#pragma unroll
+        for (int w = 0; w < 4; ++w) {
+            const float f = exp2_hw(sh.m[w][k] - mx);
+            lt += f * sh.l[w][k];
+            ot += f * sh.o[w][k][ch];
+        }
+        ot *= 1.f / kPOne;
+        if (nsplit == 1) {
+            int s;
+            if (row_position(a.c, row, &s) >= 0) store_out<DH>(a, row, g * group + k % group, ch, ot, lt);
+        } else {
+            float* rec = a.work + ((int64_t(row) * a.Hq + g * group + k % group) * nsplit + split) * (DH + 4);
+            if (ch == 0) rec[0] = mx, rec[1] = lt;
+            rec[4 + ch] = ot;
+        }
+    }
+}
+
+// One row's query heads of a K/V head: a workgroup of four waves takes one of nsplit equal
+// ranges of the row's records, a wave two records (32 keys) at a time.
+template <int DH, int D>
+__global__ __launch_bounds__(256, DH == 128 ? 3 : 2) void attn4_token_kernel(Attn4Args a, int nsplit) {
+    constexpr int COLS = 8, H = DH / 128, NS = DH / 32, NV = DH / 16;
+    const PagedRows& c = a.c;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), p = lane >> 4, b = lane & 15;
+    const int split = blockIdx.x % nsplit, g = blockIdx.x / nsplit % c.Hkv, r = blockIdx.x / nsplit / c.Hkv;
+    const int group = a.Hq / c.Hkv, tpp = c.page_size / kQ4Tile, col = b & 7;
+    __shared__ union {
+        Ring<DH, D> ring[4];
+        Merge<DH, COLS> merge;
+    } sh;
+    const FieldMasks masks;
+
+    int seq;
+    const int pos = row_position(c, r, &seq);
+    if (pos < 0) return;
+    const Seen sees = row_sees(a, pos);
+    // records: those of the first keys that stay, then from the window's first key on
+    const int first = sees.first / kQ4Tile, stay = min((sees.stay + kQ4Tile - 1) / kQ4Tile, first), last = pos / kQ4Tile;
+    const int tiles = stay + last - first + 1, units = (tiles + 1) / 2;
+    const int u0 = int(int64_t(units) * split / nsplit), u1 = int(int64_t(units) * (split + 1) / nsplit);
+    // read as constant memory: through the scalar cache, apart from the counted vector loads
+    const auto* table = (const __attribute__((address_space(4))) int32_t*)(c.page_table) + int64_t(seq) * c.max_pages;
+    const uint32_t magic = (0x80000000u + tpp - 1) / tpp;  // x / tpp = x magic >> 31 for x < 2^23
+
+    struct Place {
+        int t;          // record of the sequence
+        bool there;
+        uint64_t krec;  // offset of the keys' record in the pool
+    };
+    const uint32_t rec_bytes = 9 * DH, head_bytes = uint32_t(tpp) * rec_bytes, half = head_bytes * c.Hkv;
+    auto locate = [&](int k) {
+        Place w;
+        const int kk = min(k, tiles - 1);
+        w.t = kk < stay ? kk : first + kk - stay;
+        const int lp = int(uint64_t(w.t) * magic >> 31), id = __builtin_amdgcn_readfirstlane(table[lp]);
+        w.there = k < tiles && id >= 0 && id < c.pool_pages;
+        w.krec = uint64_t(w.there ? uint32_t(id) : 0u) * (2 * half) + uint32_t(g * head_bytes + (w.t - lp * tpp) * rec_bytes);
+        return w;
+    };
+    Ring<DH, D>& ring = sh.ring[wave];
+    auto fetch = [&](int at, const Place (&w)[2]) {
+#pragma unroll
+        for (int x = 0; x < 2; ++x) {
+            const uint8_t* krec = reinterpret_cast<const uint8_t*>(c.pages) + w[x].krec;
+            ring_fetch<DH, D>(ring.slot[at], x, krec, krec + half, lane);
+        }
+    };
+
+    // the query in units of log2, a power of two brings the head's largest channel below 2^14
+    q4_h8 q[NS];
+    float unit;
+    {
+        const float* src = a.q_rot + (int64_t(r) * a.Hq + g * group + min(col, group - 1)) * DH + 8 * p;
+        float x[NS][8], amax = 0.f;
+        const float k = a.score_scale * kLog2e;
+#pragma unroll
+        for (int s = 0; s < NS; ++s) {
+            __builtin_memcpy(x[s], __builtin_assume_aligned(src + 32 * s, 16), 32);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) amax = fmaxf(amax, fabsf(x[s][j] *= k));
+        }
+        amax = max_over_p(amax);
+        const int e = amax > 0.f && amax < INFINITY ? min(max(ilogbf(amax) + 1, -100), 117) : 0;
+#pragma unroll
+        for (int s = 0; s < NS; ++s)
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                _Float16 hi, lo;
+                split_f16(ldexpf(x[s][j], 14 - e), hi, lo);
+                q[s][j] = b < 8 ? hi : lo;
+            }
+        unit = ldexpf(1.f, e - 14);
+    }
+    const float slack = kPSlack / unit;
+
+    f4_t o[NV];
+#pragma unroll
+    for (int y = 0; y < NV; ++y) o[y] = f4_t{0.f, 0.f, 0.f, 0.f};
+    float m = kLowest, m2 = kLowest, l = 0.f;  // m in units of the products, m2 = m unit
+
+    const int n = max(0, (u1 - u0 - wave + 3) / 4);  // the wave's units u0 + wave, + 4, ...
+    Place ahead[D][2];
+#pragma unroll
+    for (int d = 0; d < D; ++d) {
+#pragma unroll
+        for (int x = 0; x < 2; ++x) ahead[d][x] = locate(2 * (u0 + wave + 4 * d) + x);
+        if (d < n) fetch(d, ahead[d]);
+    }
+    for (int i0 = 0; i0 < n; i0 += D) {
+#pragma unroll
+        for (int d = 0; d < D; ++d) {
+            const int i = i0 + d;
+            if (i >= n) break;
+            Place(&w)[2] = ahead[d];
+            const typename Ring<DH, D>::Slot& in = ring.slot[d];
+            // the unit's loads are in when at most the ones behind it are outstanding
+            if (i + D - 1 < n)
+                wait_vmcnt<(D - 1) * Ring<DH, D>::kLoads>();
+            else
+                wait_vmcnt<0>();
+            asm volatile("" ::: "memory");
+
+            float s[8];
+#pragma unroll
+            for (int x = 0; x < 2; ++x) {
+                _Float16 kd[NS];
+                __builtin_memcpy(kd, __builtin_assume_aligned(in.steps[x].k + b * 2 * NS, 8), sizeof(kd));
+                f4_t sum = f4_t{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                for (int k = 0; k < NS; ++k) {
+                    const uint4 w4 = in.k[x][k / 4][4 * b + (p ^ b >> 2)];
+                    const uint32_t word = k % 4 == 0 ? w4.x : k % 4 == 1 ? w4.y : k % 4 == 2 ? w4.z : w4.w;
+                    const q4_h2 d = {kd[k], kd[k]};
+                    sum = __builtin_amdgcn_mfma_f32_16x16x32_f16(
+                        join(masks.codes<0>(word) * d, masks.codes<1>(word) * d, masks.codes<0>(word >> 8) * d, masks.codes<1>(word >> 8) * d), q[k], sum, 0, 0, 0);
+                }
+#pragma unroll
+                for (int j = 0; j < 4; ++j) s[4 * x + j] = sum[j] + column_other(sum[j]);
+            }
+            uint4 v[2][H];
+            q4_h2 vd[2][NV];
+#pragma unroll
+            for (int x = 0; x < 2; ++x) {
+#pragma unroll
+                for (int h = 0; h < H; ++h) v[x][h] = in.v[x][h][lane];
+                __builtin_memcpy(vd[x], __builtin_assume_aligned(in.steps[x].v + p * 4 * NV, 16), sizeof(vd[x]));
+            }
+#pragma unroll
+            for (int x = 0; x < 2; ++x) {
+                const int k0 = kQ4Tile * w[x].t;
+                if (!w[x].there || k0 + 15 > pos || (k0 < sees.first && k0 + 15 >= sees.stay)) {  // not all of its keys are seen
+                    bool see[4];
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        const int key = k0 + 4 * p + j;
+                        see[j] = w[x].there && key <= pos && (key >= sees.first || key < sees.stay);
+                        if (!see[j]) s[4 * x + j] = -INFINITY;
+                    }
+                    // slots past the row may hold anything: their steps count as 0
+#pragma unroll
+                    for (int y = 0; y < NV; ++y)
+#pragma unroll
+                        for (int j = 0; j < 2; ++j)
+                            if (!see[2 * (y & 1) + j]) vd[x][y][j] = _Float16(0.f);
+                }
+            }
+            // what the slot held is in registers: the next unit's loads may land there
+            asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+            if (i + D < n) {
+#pragma unroll
+                for (int x = 0; x < 2; ++x) w[x] = locate(2 * (u0 + wave + 4 * (i + D)) + x);
+                fetch(d, w);
+            }
+            float best = s[0];
+#pragma unroll
+            for (int j = 1; j < 8; ++j) best = fmaxf(best, s[j]);
+            if (__ballot(best > m + slack)) {
+                const float to = fmaxf(m, max_over_p(best)), to2 = to == kLowest ? kLowest : to * unit, f = exp2_hw(m2 - to2);
+                m = to, m2 = to2;
+                l *= f;
+#pragma unroll
+                for (int y = 0; y < NV; ++y) o[y] *= f;
+            }
+            q4_h8 w8;
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                const float e = exp2_hw(__builtin_fmaf(s[j], unit, -m2));
+                l += e;
+                const _Float16 hi = _Float16(e * kPOne);  // the scaling is exact, so both terms are of one value
+                w8[j] = b < 8 ? hi : _Float16(__builtin_fmaf(e, kPOne, -float(hi)));
+            }
+#pragma unroll
+            for (int h = 0; h < H; ++h)
+#pragma unroll
+                for (int y = 0; y < 4; ++y) {  // byte y of the words: channels 128 h + 32 y + b and + 16
+                    // 16-bit halves: that byte of two neighbouring keys
+                    const uint32_t pick = 0x0C040C00u + 0x00010001u * y;
+                    const uint32_t w0 = __builtin_amdgcn_perm(v[0][h].y, v[0][h].x, pick), w1 = __builtin_amdgcn_perm(v[0][h].w, v[0][h].z, pick);
+                    const uint32_t w2 = __builtin_amdgcn_perm(v[1][h].y, v[1][h].x, pick), w3 = __builtin_amdgcn_perm(v[1][h].w, v[1][h].z, pick);
+                    const q4_h2 d0 = vd[0][2 * (4 * h + y)], d1 = vd[0][2 * (4 * h + y) + 1];
+                    const q4_h2 d2 = vd[1][2 * (4 * h + y)], d3 = vd[1][2 * (4 * h + y) + 1];
+                    f4_t& oa = o[8 * h + 2 * y];
+                    f4_t& ob = o[8 * h + 2 * y + 1];
+                    oa = __builtin_amdgcn_mfma_f32_16x16x32_f16(join(masks.codes<0>(w0) * d0, masks.codes<0>(w1) * d1, masks.codes<0>(w2) * d2, masks.codes<0>(w3) * d3), w8, oa, 0, 0, 0);
+                    ob = __builtin_amdgcn_mfma_f32_16x16x32_f16(join(masks.codes<1>(w0) * d0, masks.codes<1>(w1) * d1, masks.codes<1>(w2) * d2, masks.codes<1>(w3) * d3), w8, ob, 0, 0, 0);
+                }
+        }
+    }
+    __syncthreads();
+
+    // the four waves' results
+    l = sum_over_p(l);
+#pragma unroll
+    for (int y = 0; y < NV; ++y) {
+        f4_t v = o[y];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) v[i] += column_other(v[i]);
+        if (b < COLS) *reinterpret_cast<f4_t*>(&sh.merge.o[wave][col][16 * y + 4 * p]) = v;
+    }
+    if (p == 0 && b < COLS) sh.merge.m[wave][col] = m2, sh.merge.l[wave][col] = l;
+    __syncthreads();
+    merge_waves<DH, COLS>(a, sh.merge, r, 1, g, nsplit, split);
+}
+
 // A workgroup of four waves: R = rows * group pairs of rows r0 .. of one K/V head, one of
 // nsplit equal ranges of their records, two records (32 keys) a wave at a time.
-template <int DH, bool PAIR>
+template <int DH>
 __global__ __launch_bounds__(256, 2) void attn4_kernel(Attn4Args a, int R, int nsplit) {
-    constexpr int COLS = PAIR ? 8 : 16, H = DH / 128, NS = DH / 32, NV = DH / 16;
+    constexpr int COLS = 16, H = DH / 128, NS = DH / 32, NV = DH / 16;
     const PagedRows& c = a.c;
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, p = lane >> 4, b = lane & 15;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), p = lane >> 4, b = lane & 15;
     const int split = blockIdx.x % nsplit, g = blockIdx.x / nsplit % c.Hkv, tile0 = blockIdx.x / nsplit / c.Hkv, r0 = tile0 * R;
     const int group = a.Hq / c.Hkv, tpp = c.page_size / kQ4Tile;
     __shared__ Merge<DH, COLS> sh;
+    const FieldMasks masks;
 
-    const int col = PAIR ? b & 7 : b, mine = min(col / group, R - 1), r = r0 + mine;
+    const int col = b, mine = min(col / group, R - 1), r = r0 + mine;
     const bool used = col < R * group && r < c.rows;
     int seq = 0;
     const int pos = used ? row_position(c, r, &seq) : -1;
     const Seen sees = row_sees(a, pos);
 
-    // queries: a power of two brings the head's largest channel below 1
-    q4_h8 qh[NS], ql[PAIR ? 1 : NS];
+    // queries: a power of two brings the head's largest channel below 2^14
+    q4_h8 qh[NS], ql[NS];
     float scale = 0.f;
     {
         const float* q = a.q_rot + (int64_t(min(r, c.rows - 1)) * a.Hq + g * group + col % group) * DH + 8 * p;
@@ -134,13 +411,10 @@ __global__ __launch_bounds__(256, 2) void attn4_kernel(Attn4Args a, int R, int n
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
                 _Float16 hi, lo;
-                split_f16(ldexpf(x[s][j], -e), hi, lo);
-                if constexpr (PAIR)
-                    qh[s][j] = b < 8 ? hi : lo;
-                else
-                    qh[s][j] = hi, ql[s][j] = lo;
+                split_f16(ldexpf(x[s][j], 14 - e), hi, lo);
+                qh[s][j] = hi, ql[s][j] = lo;
             }
-        scale = ldexpf(a.score_scale * kLog2e, e);
+        scale = ldexpf(a.score_scale * kLog2e, e - 14);
     }
 
     f4_t o[NV];
@@ -200,16 +474,15 @@ __global__ __launch_bounds__(256, 2) void attn4_kernel(Attn4Args a, int R, int n
                     const uint4 w4 = regs[x].k[k / 4];
                     const uint32_t w = k % 4 == 0 ? w4.x : k % 4 == 1 ? w4.y : k % 4 == 2 ? w4.z : w4.w;
                     const q4_h2 d = {regs[x].kd[k], regs[x].kd[k]};
-                    const q4_h8 f = join(codes_of<0>(w) * d, codes_of<1>(w) * d, codes_of<0>(w >> 8) * d, codes_of<1>(w >> 8) * d);
+                    const q4_h8 f = join(masks.codes<0>(w) * d, masks.codes<1>(w) * d, masks.codes<0>(w >> 8) * d, masks.codes<1>(w >> 8) * d);
                     acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(f, qh[k], acc, 0, 0, 0);
-                    if constexpr (!PAIR) acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(f, ql[k], acc, 0, 0, 0);
+                    acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(f, ql[k], acc, 0, 0, 0);
                 }
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
-                    const float v = PAIR ? acc[i] + column_other(acc[i]) : acc[i];
                     const int key = kQ4Tile * t[x] + 4 * p + i;
                     const bool sees_it = here && ok[x] && key <= sees.pos && (key >= sees.first || key < sees.stay);
-                    s[4 * x + i] = sees_it ? v * scale : -INFINITY;
+                    s[4 * x + i] = sees_it ? acc[i] * scale : -INFINITY;
                 }
             }
             float best = s[0];
@@ -229,10 +502,7 @@ __global__ __launch_bounds__(256, 2) void attn4_kernel(Attn4Args a, int R, int n
                 l += w;
                 _Float16 hi, lo;
                 split_f16(w * kPOne, hi, lo);
-                if constexpr (PAIR)
-                    w8[i] = b < 8 ? hi : lo;
-                else
-                    w8[i] = hi, w8l[i] = lo;
+                w8[i] = hi, w8l[i] = lo;
             }
             // a slot past the last row, or of a page that holds nothing, may hold anything: its steps count as 0
 #pragma unroll
@@ -256,16 +526,14 @@ __global__ __launch_bounds__(256, 2) void attn4_kernel(Attn4Args a, int R, int n
                     const uint32_t w2 = __builtin_amdgcn_perm(vb.y, vb.x, pick), w3 = __builtin_amdgcn_perm(vb.w, vb.z, pick);
                     const q4_h2 d0 = regs[0].vd[2 * (4 * h + y)], d1 = regs[0].vd[2 * (4 * h + y) + 1];
                     const q4_h2 d2 = regs[1].vd[2 * (4 * h + y)], d3 = regs[1].vd[2 * (4 * h + y) + 1];
-                    const q4_h8 fa = join(codes_of<0>(w0) * d0, codes_of<0>(w1) * d1, codes_of<0>(w2) * d2, codes_of<0>(w3) * d3);
-                    const q4_h8 fb = join(codes_of<1>(w0) * d0, codes_of<1>(w1) * d1, codes_of<1>(w2) * d2, codes_of<1>(w3) * d3);
+                    const q4_h8 fa = join(masks.codes<0>(w0) * d0, masks.codes<0>(w1) * d1, masks.codes<0>(w2) * d2, masks.codes<0>(w3) * d3);
+                    const q4_h8 fb = join(masks.codes<1>(w0) * d0, masks.codes<1>(w1) * d1, masks.codes<1>(w2) * d2, masks.codes<1>(w3) * d3);
                     f4_t& oa = o[8 * h + 2 * y];
                     f4_t& ob = o[8 * h + 2 * y + 1];
                     oa = __builtin_amdgcn_mfma_f32_16x16x32_f16(fa, w8, oa, 0, 0, 0);
                     ob = __builtin_amdgcn_mfma_f32_16x16x32_f16(fb, w8, ob, 0, 0, 0);
-                    if constexpr (!PAIR) {
-                        oa = __builtin_amdgcn_mfma_f32_16x16x32_f16(fa, w8l, oa, 0, 0, 0);
-                        ob = __builtin_amdgcn_mfma_f32_16x16x32_f16(fb, w8l, ob, 0, 0, 0);
-                    }
+                    oa = __builtin_amdgcn_mfma_f32_16x16x32_f16(fa, w8l, oa, 0, 0, 0);
+                    ob = __builtin_amdgcn_mfma_f32_16x16x32_f16(fb, w8l, ob, 0, 0, 0);
                 }
         }
     }
@@ -273,62 +541,62 @@ __global__ __launch_bounds__(256, 2) void attn4_kernel(Attn4Args a, int R, int n
     // the four waves' results
     l = sum_over_p(l);
 #pragma unroll
-    for (int n = 0; n < NV; ++n) {
-        f4_t v = o[n];
-        if constexpr (PAIR) {
-#pragma unroll
-            for (int i = 0; i < 4; ++i) v[i] += column_other(v[i]);
-        }
-        if (b < COLS) *reinterpret_cast<f4_t*>(&sh.o[wave][col][16 * n + 4 * p]) = v;
-    }
-    if (p == 0 && b < COLS) sh.m[wave][col] = m, sh.l[wave][col] = l;
+    for (int n = 0; n < NV; ++n) *reinterpret_cast<f4_t*>(&sh.o[wave][col][16 * n + 4 * p]) = o[n];
+    if (p == 0) sh.m[wave][col] = m, sh.l[wave][col] = l;
     __syncthreads();
-    for (int idx = threadIdx.x; idx < R * group * DH; idx += 256) {
-        const int k = idx / DH, ch = idx % DH, row = r0 + k / group;
-        if (row >= c.rows) break;
-        float mx = sh.m[0][k];
-#pragma unroll
-        for (int w = 1; w < 4; ++w) mx = fmaxf(mx, sh.m[w][k]);
-        float lt = 0.f, ot = 0.f;
-#pragma unroll
-        for (int w = 0; w < 4; ++w) {
-            const float f = exp2_hw(sh.m[w][k] - mx);
-            lt += f * sh.l[w][k];
-            ot += f * sh.o[w][k][ch];
-        }
-        ot *= 1.f / kPOne;
-        if (nsplit == 1) {
-            int s;
-            if (row_position(c, row, &s) >= 0) store_out<DH>(a, row, g * group + k % group, ch, ot, lt);
-        } else {
-            float* rec = a.work + ((int64_t(row) * a.Hq + g * group + k % group) * nsplit + split) * (DH + 4);
-            if (ch == 0) rec[0] = mx, rec[1] = lt;
-            rec[4 + ch] = ot;
-        }
-    }
+    merge_waves<DH, COLS>(a, sh, r0, R, g, nsplit, split);
 }
 
-// a workgroup per (row, query head), a lane per channel
+// A workgroup per (row, query head): DH / 4 lanes for four channels each read a range's result, and
+// 1024 / DH such groups take the ranges in turn.
 template <int DH>
-__global__ __launch_bounds__(DH) void attn4_combine_kernel(Attn4Args a, int nsplit) {
-    const int r = blockIdx.x / a.Hq, h = blockIdx.x % a.Hq, t = threadIdx.x;
+__global__ __launch_bounds__(256) void attn4_combine_kernel(Attn4Args a, int nsplit) {
+    constexpr int LN = DH / 4, GR = 256 / LN, kRec = DH + 4, kPass = 4;
+    const int r = blockIdx.x / a.Hq, h = blockIdx.x % a.Hq, t = threadIdx.x, grp = t / LN, ln = t % LN;
     int seq;
     if (row_position(a.c, r, &seq) < 0) return;
-    const float* rec = a.work + int64_t(blockIdx.x) * nsplit * (DH + 4);
+    __shared__ float part[GR][DH], total[4], most[4];
+    extern __shared__ float share[];  // a range's factor
+    const float* rec = a.work + int64_t(blockIdx.x) * nsplit * kRec;
     float mx = kLowest;
-    for (int s = 0; s < nsplit; ++s) mx = fmaxf(mx, rec[int64_t(s) * (DH + 4)]);
-    float l = 0.f, o = 0.f;
-    for (int s = 0; s < nsplit; ++s) {
-        const float f = exp2_hw(rec[int64_t(s) * (DH + 4)] - mx);
-        l += f * rec[int64_t(s) * (DH + 4) + 1];
-        o += f * rec[int64_t(s) * (DH + 4) + 4 + t];
+    for (int s = t; s < nsplit; s += 256) mx = fmaxf(mx, rec[int64_t(s) * kRec]);
+    for (int off = 32; off > 0; off >>= 1) mx = fmaxf(mx, __shfl_xor(mx, off));
+    if ((t & 63) == 0) most[t >> 6] = mx;
+    __syncthreads();
+    mx = fmaxf(fmaxf(most[0], most[1]), fmaxf(most[2], most[3]));
+    float l = 0.f;
+    for (int s = t; s < (nsplit + GR * kPass - 1) / (GR * kPass) * (GR * kPass); s += 256) {
+        float f = 0.f;
+        if (s < nsplit) {
+            f = exp2_hw(rec[int64_t(s) * kRec] - mx);
+            l += f * rec[int64_t(s) * kRec + 1];
+        }
+        share[s] = f;
     }
-    store_out<DH>(a, r, h, t, o, l);
+    for (int off = 32; off > 0; off >>= 1) l += __shfl_xor(l, off);
+    if ((t & 63) == 0) total[t >> 6] = l;
+    __syncthreads();
+    f4_t o = f4_t{0.f, 0.f, 0.f, 0.f};
+    for (int s = grp; s < nsplit; s += GR * kPass) {
+        f4_t v[kPass];
+#pragma unroll
+        for (int k = 0; k < kPass; ++k) v[k] = *reinterpret_cast<const f4_t*>(rec + int64_t(min(s + GR * k, nsplit - 1)) * kRec + 4 + 4 * ln);
+#pragma unroll
+        for (int k = 0; k < kPass; ++k) o += share[s + GR * k] * v[k];
+    }
+    *reinterpret_cast<f4_t*>(&part[grp][4 * ln]) = o;
+    __syncthreads();
+    if (t < DH) {
+        float v = 0.f;
+#pragma unroll
+        for (int k = 0; k < GR; ++k) v += part[k][t];
+        store_out<DH>(a, r, h, t, v, (total[0] + total[1]) + (total[2] + total[3]));
+    }
 }
 
-// Rows a workgroup takes, and into how many ranges their keys are split: about four
+// Rows a workgroup takes, and into how many ranges their keys are split: about three
 // workgroups per CU over all rows and heads, at least eight units of 32 keys each.
-constexpr int64_t kGroups = 1024;
+constexpr int64_t kGroups = 768;
 struct Plan {
     int R, nsplit;
     int64_t tiles, most;  // groups of rows; ranges that the keys allow
@@ -357,19 +625,20 @@ int64_t attn4_work_bytes(int64_t rows, int64_t Hq, int64_t Hkv, int64_t Dh, int6
 }
 
 namespace {
-template <int DH, bool PAIR>
+template <int DH>
 void attn4_sized(const Attn4Args& a, const Plan& p, hipStream_t s) {
-    hipLaunchKernelGGL((attn4_kernel<DH, PAIR>), dim3(unsigned(p.tiles * a.c.Hkv * p.nsplit)), dim3(256), 0, s, a, p.R, p.nsplit);
-    if (p.nsplit > 1) hipLaunchKernelGGL(attn4_combine_kernel<DH>, dim3(unsigned(a.c.rows * a.Hq)), dim3(DH), 0, s, a, p.nsplit);
+    const dim3 grid(unsigned(p.tiles * a.c.Hkv * p.nsplit));
+    if (p.R == 1)
+        hipLaunchKernelGGL((attn4_token_kernel<DH, 2>), grid, dim3(256), 0, s, a, p.nsplit);
+    else
+        hipLaunchKernelGGL(attn4_kernel<DH>, grid, dim3(256), 0, s, a, p.R, p.nsplit);
+    if (p.nsplit > 1) hipLaunchKernelGGL(attn4_combine_kernel<DH>, dim3(unsigned(a.c.rows * a.Hq)), dim3(256), size_t(p.nsplit + 31) / 32 * 128, s, a, p.nsplit);
 }
 }  // namespace
 
 void launch_attn4(const Attn4Args& a, hipStream_t s) {
     const Plan p = attn4_plan(a.c.rows, a.Hq / a.c.Hkv, a.c.Hkv, a.c.row_seq != nullptr, int64_t(a.c.max_pages) * a.c.page_size, a.window, a.sinks);
-    if (a.c.Dh == 256)
-        p.R == 1 ? attn4_sized<256, true>(a, p, s) : attn4_sized<256, false>(a, p, s);
-    else
-        p.R == 1 ? attn4_sized<128, true>(a, p, s) : attn4_sized<128, false>(a, p, s);
+    a.c.Dh == 256 ? attn4_sized<256>(a, p, s) : attn4_sized<128>(a, p, s);
 }
 
 }  // namespace hero

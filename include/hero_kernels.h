@@ -518,8 +518,8 @@ int hero_kv_read_q4(const hero_kv_read_args* args, void* stream);
  * activations), at least one, 16-byte aligned. Rows of one sequence should stand
  * together: neighbouring rows share the reads of their keys. Results agree with
  * the formula over the stored values to fp32 rounding, save that a query's channels are
- * kept to 2^-23 of the head's largest and weights to 2^-23 of themselves or
- * 2^-38 of the row's largest. Uses a.q_rot, proj (the gates), proj_stride, positions,
+ * kept to 2^-22 of themselves or 2^-38 of the head's largest and weights to 2^-22 of
+ * themselves or 2^-38 of the row's largest. Uses a.q_rot, proj (the gates), proj_stride, positions,
  * score_scale, window, b, hq, hkv, dh, the page and row fields, sinks and work
  * (hero_attn_q4_work_bytes, 16-byte aligned; NULL where that is 0; the sizes
  * grow with the rows; calls that may overlap need one each). max_ctx of the size
