@@ -11,6 +11,7 @@ namespace hero {
 namespace {
 
 typedef float f4_t __attribute__((ext_vector_type(4)));
+typedef float f2_t __attribute__((ext_vector_type(2)));
 
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kPOne = 8192.f;  // a weight's terms are of 2^13 2^(s - m); its part in the total is 2^(s - m)
@@ -28,6 +29,8 @@ __device__ __forceinline__ float sum_over_p(float x) {
     x += __shfl_xor(x, 16);
     return x + __shfl_xor(x, 32);
 }
+// (the cache's values are 4-bit: nothing here has to replay a reference's rounding, as exp_f32 does)
+__device__ __forceinline__ float gate_of(float x) { return 1.f / (1.f + expf(-x)); }
 __device__ __forceinline__ float exp2_hw(float x) { return __builtin_amdgcn_exp2f(x); }  // 1 ulp; 0 below its range
 
 // x as two fp16 terms; pinned first, so that both are formed from one rounding of it
@@ -116,7 +119,7 @@ template <int DH>
 __device__ __forceinline__ void store_out(const Attn4Args& a, int r, int h, int ch, float o, float l) {
     const int64_t width = int64_t(a.Hq) * DH, idx = int64_t(r) * width + int64_t(h) * DH + ch;
     const float gate = a.proj[int64_t(r) * a.proj_stride + int64_t(h) * 2 * DH + DH + ch];
-    const float out = l == 0.f ? 0.f : (o / l) * sigmoid_f32(gate);
+    const float out = l == 0.f ? 0.f : (o / l) * gate_of(gate);
     if (a.out_f32) a.out_f32[idx] = out;
     if (a.act_out) {
         float amax = fabsf(out);
@@ -338,7 +341,7 @@ __global__ __launch_bounds__(256, DH == 128 ? 3 : 2) void attn4_token_kernel(Att
             for (int j = 0; j < 8; ++j) {
                 const float e = exp2_hw(__builtin_fmaf(s[j], unit, -m2));
                 l += e;
-                const _Float16 hi = _Float16(e * kPOne);  // the scaling is exact, so both terms are of one value
+                const _Float16 hi = _Float16(__builtin_fmaf(e, kPOne, 0.f));  // the scaling is exact, so both terms are of one value
                 w8[j] = b < 8 ? hi : _Float16(__builtin_fmaf(e, kPOne, -float(hi)));
             }
 #pragma unroll
@@ -547,6 +550,462 @@ __global__ __launch_bounds__(256, 2) void attn4_kernel(Attn4Args a, int R, int n
     merge_waves<DH, COLS>(a, sh, r0, R, g, nsplit, split);
 }
 
+// Many rows: a workgroup takes 128 columns, (row, query head) pairs of consecutive rows and one K/V head, 32
+// for each of its four waves, and one of nsplit ranges of their keys. The products are of
+// 32 x 32 x 16 (lane = 32 f + x below):
+//   scores   S^T[key][column]: lane (f, x) brings channels 16 s + 8 f .. + 7 of key x for step s, and gets keys 8 y +
+//            4 f + i (register 4 y + i) of column x.
+//   values   O^T[channel][column] over the 16 keys of a record: a lane's scores of the record, in order of
+//            their registers, are its operand, so lane (f, x) brings keys 4 f + i and 8 + 4 f + i of channel x.
+// The waves share the work of turning a unit's records (32 keys) into fp16 operands in shared memory. A unit
+// passes in steps: its loads, its operands, its scores, its weights and values, a barrier apart, and
+// an iteration holds one step of each of several units: the matrix cores multiply
+// the next unit's scores while the vector units form this one's weights, and this
+// one's values while they form operands.
+constexpr int kListed = 256, kRing = 5;
+struct Listed {
+    uint64_t krec;   // offset of the keys' record in the pool
+    int key, edge;   // its first position (-1: not there); whether some row does not see all of it
+};
+
+template <int DH>
+__global__ __launch_bounds__(256, DH == 128 ? 2 : 1) void attn4_chunk_kernel(Attn4Args a, int R, int nsplit) {
+    constexpr int H = DH / 128, NS = DH / 16, NB = DH / 32;
+    constexpr int WK = NB / 2, WV = 2 * H;  // words of keys, and bytes of words of values, that a lane turns into operands
+    typedef float f16_t __attribute__((ext_vector_type(16)));
+    const PagedRows& c = a.c;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), f = lane >> 5, p = lane >> 4, b = lane & 15;
+    // neighbouring workgroups, which go to different XCDs, take different heads: each L2 holds the records of its own
+    const int g = blockIdx.x % c.Hkv, split = blockIdx.x / c.Hkv % nsplit, r0 = blockIdx.x / c.Hkv / nsplit * R;
+    const int group = a.Hq / c.Hkv, tpp = c.page_size / kQ4Tile;
+    const uint32_t magic = (0x80000000u + tpp - 1) / tpp;  // x / tpp = x magic >> 31 for x < 2^23
+    const uint32_t rec_bytes = 9 * DH, head_bytes = uint32_t(tpp) * rec_bytes, half = head_bytes * c.Hkv;
+    const FieldMasks masks;
+    const uint8_t* const pool = reinterpret_cast<const uint8_t*>(c.pages);
+    __shared__ uint4 ops_k[2][NS][64];     // operands, a lane's 16 bytes each
+    __shared__ uint2 ops_v[2][NB][2][64][2];
+    __shared__ struct {
+        uint4 codes[2][2][H][64];    // keys, values; record; as they lie
+        uint8_t steps[2][2][DH];
+    } raw[kRing];
+    __shared__ Listed list[kListed];
+
+    // the workgroup's rows, two a lane
+    int row_pos[2], row_of[2];
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+        const int i = lane + 64 * k;
+        row_pos[k] = i < R && r0 + i < c.rows ? row_position(c, r0 + i, &row_of[k]) : -1;
+    }
+    // the lane's column, and its query in units of log2, two terms; a power of two brings the head's largest channel below 2^14
+    const int col = wave * 32 + (lane & 31), i_row = min(min(col / group, R - 1), c.rows - 1 - r0);
+    const int row = col < R * group && r0 + col / group < c.rows ? i_row : -1, head = g * group + col % group;
+    q4_h8 qh[NS], ql[NS];
+    float unit;
+    {
+        const float* src = a.q_rot + (int64_t(r0 + i_row) * a.Hq + head) * DH + 8 * f;
+        const float k = a.score_scale * kLog2e;
+        f4_t x[NS][2];
+        float amax = 0.f;
+#pragma unroll
+        for (int s = 0; s < NS; ++s)
+#pragma unroll
+            for (int j = 0; j < 2; ++j) x[s][j] = *reinterpret_cast<const f4_t*>(src + 16 * s + 4 * j) * k;
+#pragma unroll
+        for (int s = 0; s < NS; ++s)
+#pragma unroll
+            for (int j = 0; j < 8; ++j) amax = fmaxf(amax, fabsf(x[s][j / 4][j % 4]));
+        amax = fmaxf(amax, __shfl_xor(amax, 32));
+        const int e = amax > 0.f && amax < INFINITY ? min(max(ilogbf(amax) + 1, -100), 117) : 0;
+#pragma unroll
+        for (int s = 0; s < NS; ++s)
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                _Float16 hi, lo;
+                split_f16(ldexpf(x[s][j / 4][j % 4], 14 - e), hi, lo);
+                qh[s][j] = hi, ql[s][j] = lo;
+            }
+        unit = ldexpf(1.f, e - 14);
+    }
+    const float slack = kPSlack / unit;
+    uint64_t valid[2] = {__ballot(row_pos[0] >= 0), __ballot(row_pos[1] >= 0)};
+    if (!(valid[0] | valid[1])) return;
+    const uint64_t all[2] = {valid[0], valid[1]};
+    auto of_row = [&](const int (&v)[2], int i) {
+        const int x = __shfl(v[0], i & 63), y = __shfl(v[1], i & 63);  // by all lanes
+        return i < 64 ? x : y;
+    };
+    const int pos = of_row(row_pos, i_row);
+    const Seen sees = row_sees(a, pos);
+    float m = kLowest, m2 = kLowest, l = 0.f;  // m in units of the products, m2 = m unit
+    const f16_t zero = {};
+    f16_t o[NB];
+#pragma unroll
+    for (int n = 0; n < NB; ++n) o[n] = zero;
+
+    // the rows of one sequence at a time (mostly there is one)
+    while (valid[0] | valid[1]) {
+        const int lead = valid[0] ? __ffsll((unsigned long long)valid[0]) - 1 : 63 + __ffsll((unsigned long long)valid[1]);
+        const int seq = __builtin_amdgcn_readfirstlane(of_row(row_of, lead));
+        uint64_t mine[2];
+        int lo = 0x7FFFFFFF, hi = -1;
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+            const bool in = row_of[k] == seq && (valid[k] >> lane & 1);
+            mine[k] = __ballot(in);
+            valid[k] &= ~mine[k];
+            if (in) lo = min(lo, row_pos[k]), hi = max(hi, row_pos[k]);
+        }
+        for (int off = 32; off > 0; off >>= 1) lo = min(lo, __shfl_xor(lo, off)), hi = max(hi, __shfl_xor(hi, off));
+        lo = __builtin_amdgcn_readfirstlane(lo), hi = __builtin_amdgcn_readfirstlane(hi);
+        const bool whole = mine[0] == all[0] && mine[1] == all[1];
+        const bool here = row >= 0 && ((row < 64 ? mine[0] : mine[1]) >> (row & 63) & 1);
+
+        // records: those of the first keys that stay, then from the earliest window to the last row
+        const Seen most = row_sees(a, hi), least = row_sees(a, lo);
+        const int first = least.first / kQ4Tile, stay = min((most.stay + kQ4Tile - 1) / kQ4Tile, first);
+        const int tiles = stay + hi / kQ4Tile - first + 1, units = (tiles + 1) / 2;
+        const int u0 = int(int64_t(units) * split / nsplit), u1 = int(int64_t(units) * (split + 1) / nsplit);
+        if (u0 >= u1) continue;
+
+        // The range's records are looked up by all lanes, kListed at a time: where each is, and whether some row
+        // does not see all of it. In the loop that is a read of shared memory and one branch.
+        auto look_up = [&](int from) {
+            const int k = 2 * from + int(threadIdx.x), at_t = k < stay ? k : first + min(k, tiles - 1) - stay, lp = int(uint64_t(at_t) * magic >> 31), in = at_t - lp * tpp;
+            const int id = c.page_table[int64_t(seq) * c.max_pages + lp], k0 = kQ4Tile * at_t;
+            const bool there = k < tiles && id >= 0 && id < c.pool_pages;
+            Listed e;
+            e.krec = uint64_t(there ? uint32_t(id) : 0u) * (2 * half) + uint32_t(g) * head_bytes + uint32_t(in) * rec_bytes;
+            e.key = there ? k0 : -1;
+            e.edge = !whole || !there || k0 + 15 > lo || (k0 < most.first && k0 + 15 >= least.stay);
+            list[threadIdx.x] = e;
+        };
+        struct Two {
+            uint64_t krec0, krec1;
+            int at;  // in the list
+            bool edge;
+        };
+        int listed = u0;  // the list's first unit
+        auto locate = [&](int u) __attribute__((always_inline)) {
+            Two w;
+            w.at = 2 * (u - listed);
+            const Listed e0 = list[w.at], e1 = list[w.at + 1];
+            auto uniform = [](uint64_t v) {
+                return uint64_t(uint32_t(__builtin_amdgcn_readfirstlane(int(v >> 32)))) << 32 | uint32_t(__builtin_amdgcn_readfirstlane(int(v)));
+            };
+            w.krec0 = uniform(e0.krec), w.krec1 = uniform(e1.krec);
+            w.edge = __builtin_amdgcn_readfirstlane(e0.edge | e1.edge);
+            return w;
+        };
+
+        // A unit's records go to shared memory as they lie, five units ahead: each wave moves one record.
+        constexpr int kLoads = H + 1;  // instructions of a wave
+        auto fetch = [&](uint64_t krec0, uint64_t krec1, int slot) __attribute__((always_inline)) {
+            const int kv = wave >> 1, x = wave & 1;
+            const uint8_t* rec = pool + (x ? krec1 : krec0) + (kv ? half : 0u);
+#pragma unroll
+            for (int h = 0; h < H; ++h) lds_dma_b128(rec + 1024 * h + uint32_t(lane * 16), lds_offset(&raw[slot].codes[kv][x][h][0]));
+            if (lane < DH / 4) lds_dma_b32(rec + 8 * DH + uint32_t(lane * 4), lds_offset(&raw[slot].steps[kv][x][0]));
+        };
+        // a wave's share of a unit: half of the words of one record of keys, one byte of every word of both records of values
+        uint32_t raw_k[WK];
+        _Float16 raw_kd[WK];
+        uint4 raw_v[WV];
+        q4_h2 raw_vd[WV][2];
+        const int k_first = wave / 2 * WK;
+        auto take = [&](int slot_k, int slot_v) __attribute__((always_inline)) {
+            const uint8_t* codes = reinterpret_cast<const uint8_t*>(&raw[slot_k].codes[0][wave & 1][k_first / 4][0]) + b * 64 + p * 16 + k_first % 4 * 4;
+            __builtin_memcpy(raw_k, __builtin_assume_aligned(codes, 4 * WK), sizeof(raw_k));
+            __builtin_memcpy(raw_kd, __builtin_assume_aligned(&raw[slot_k].steps[0][wave & 1][(b * NB + k_first) * 2], 2 * WK), sizeof(raw_kd));
+#pragma unroll
+            for (int j = 0; j < WV; ++j) {
+                const int x = j / H, h = j % H;
+                raw_v[j] = raw[slot_v].codes[1][x][h][lane];
+                __builtin_memcpy(raw_vd[j], __builtin_assume_aligned(&raw[slot_v].steps[1][x][(p * NB + 4 * h + wave) * 8], 8), 8);
+            }
+        };
+        // slots past the last row may hold anything: their steps count as 0
+        auto clean_v = [&](int at) __attribute__((always_inline)) {
+#pragma unroll
+            for (int j = 0; j < WV; ++j) {
+                const int k0 = list[at + j / H].key;
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                    if (k0 < 0 || k0 + 4 * p + i > hi) raw_vd[j][i / 2][i % 2] = _Float16(0.f);
+            }
+        };
+        auto form_k = [&](int at, int s) __attribute__((always_inline)) {
+            const uint32_t word = raw_k[s];
+            const q4_h2 d = {raw_kd[s], raw_kd[s]};
+            ops_k[at][2 * (k_first + s) + p / 2][32 * (p & 1) + 16 * (wave & 1) + b] =
+                __builtin_bit_cast(uint4, join(masks.codes<0>(word) * d, masks.codes<1>(word) * d, masks.codes<0>(word >> 8) * d, masks.codes<1>(word >> 8) * d));
+        };
+        const uint32_t pick = 0x0C040C00u + 0x00010001u * wave;  // a byte of two neighbouring keys, in 16-bit halves
+        auto form_v = [&](int at, int j) __attribute__((always_inline)) {
+            const int x = j / H, h = j % H;
+            const uint32_t w0 = __builtin_amdgcn_perm(raw_v[j].y, raw_v[j].x, pick), w1 = __builtin_amdgcn_perm(raw_v[j].w, raw_v[j].z, pick);
+            const q4_h2 d0 = raw_vd[j][0], d1 = raw_vd[j][1];
+            uint2(*to)[2] = &ops_v[at][4 * h + wave][x][32 * (p & 1) + b];
+            to[0][p / 2] = make_uint2(__builtin_bit_cast(uint32_t, masks.codes<0>(w0) * d0), __builtin_bit_cast(uint32_t, masks.codes<0>(w1) * d1));
+            to[16][p / 2] = make_uint2(__builtin_bit_cast(uint32_t, masks.codes<1>(w0) * d0), __builtin_bit_cast(uint32_t, masks.codes<1>(w1) * d1));
+        };
+        // piece i of WK + WV: the unit's next but one keys, the next values
+        auto form = [&](int k_at, int v_at, int i) __attribute__((always_inline)) {
+            if (i < WK)
+                form_k(k_at, i);
+            else
+                form_v(v_at, i - WK);
+        };
+        auto operand_k = [&](int at, int k) __attribute__((always_inline)) { return __builtin_bit_cast(q4_h8, ops_k[at][k][lane]); };
+        auto operand_v = [&](int at, int n, int x) __attribute__((always_inline)) { return *reinterpret_cast<const q4_h8*>(&ops_v[at][n][x][lane][0]); };
+        // shared memory alone: loads stay in flight across it
+        auto barrier = [] {
+            asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+            __builtin_amdgcn_s_barrier();
+            asm volatile("" ::: "memory");
+        };
+
+        barrier();  // the last run's list and operands are done with
+        look_up(u0);
+        barrier();
+        // (units behind the range's last one are read and not used; records behind the last one are page 0's)
+        Two w1 = locate(u0 + 1);
+        bool edge = false;
+        int slot = 0;  // of the unit that comes next
+        {
+            const Two w0 = locate(u0);
+            edge = w0.edge;
+            const Two w2 = locate(u0 + 2), w3 = locate(u0 + 3), w4 = locate(u0 + 4);
+            fetch(w0.krec0, w0.krec1, 0);
+            fetch(w1.krec0, w1.krec1, 1);
+            fetch(w2.krec0, w2.krec1, 2);
+            fetch(w3.krec0, w3.krec1, 3);
+            fetch(w4.krec0, w4.krec1, 4);
+        }
+        wait_vmcnt<2 * kLoads>();
+        barrier();
+        take(0, 0);
+        if (edge) clean_v(0);
+#pragma unroll
+        for (int i = 0; i < WK + WV; ++i) form(0, 0, i);
+        take(1, 0);
+#pragma unroll
+        for (int i = 0; i < WK; ++i) form_k(1, i);
+        barrier();
+        f16_t s = zero;
+#pragma unroll
+        for (int k = 0; k < NS; ++k) {
+            s = __builtin_amdgcn_mfma_f32_32x32x16_f16(operand_k(0, k), qh[k], s, 0, 0, 0);
+            s = __builtin_amdgcn_mfma_f32_32x32x16_f16(operand_k(0, k), ql[k], s, 0, 0, 0);
+        }
+        barrier();
+        auto hide = [&](f16_t& s, int at) __attribute__((always_inline)) {
+#pragma unroll
+            for (int x = 0; x < 2; ++x) {
+                const int k0 = list[at + x].key;
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    const int key = k0 + 8 * (i / 4) + 4 * f + i % 4;
+                    if (!(here && k0 >= 0 && key <= pos && (key >= sees.first || key < sees.stay))) s[8 * x + i] = -INFINITY;
+                }
+            }
+        };
+        auto rescale = [&](float best) __attribute__((always_inline)) {
+            if (__builtin_expect(__ballot(best > m + slack) != 0, 0)) {
+                const float to = fmaxf(m, fmaxf(best, __shfl_xor(best, 32))), to2 = to == kLowest ? kLowest : to * unit, x = exp2_hw(m2 - to2);
+                m = to, m2 = to2;
+                l *= x;
+#pragma unroll
+                for (int n = 0; n < NB; ++n) o[n] *= x;
+            }
+        };
+        if (edge) hide(s, 0);
+        {
+            float best = s[0];
+#pragma unroll
+            for (int i = 1; i < 16; ++i) best = fmaxf(best, s[i]);
+            rescale(best);
+        }
+        // here: the scores of unit u and their maxima, the keys of u + 1 and the values of u as operands, units u + 1 and
+        // u + 2 in shared memory, u + 3 and u + 4 on the way
+        auto iterate = [&](const int u, const int now) __attribute__((always_inline)) {
+            // The next unit's scores, and between their products this one's weights, ... (The order is kept: the
+            // compiler's own has the vector instructions first and the products behind them.)
+            f16_t ahead = zero;
+            uint32_t terms_h[8], terms_l[8];
+            q4_h8 x_now = operand_k(now ^ 1, 0), x_next = operand_k(now ^ 1, 1);
+            __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+            for (int k = 0; k < NS; ++k) {
+                const q4_h8 x_then = operand_k(now ^ 1, k + 2 < NS ? k + 2 : k);
+                __builtin_amdgcn_sched_barrier(0);
+                ahead = __builtin_amdgcn_mfma_f32_32x32x16_f16(x_now, qh[k], ahead, 0, 0, 0);
+                if (k % (NS / 8) == 0) {  // two weights, as two terms; pinned to their place in the order
+                    const int i = k / (NS / 8);
+                    const float e0 = exp2_hw(__builtin_fmaf(s[2 * i], unit, -m2)), e1 = exp2_hw(__builtin_fmaf(s[2 * i + 1], unit, -m2));
+                    l += e0;
+                    l += e1;
+                    // Conversions in pairs and remainders in fp32: instructions that round to one half of a
+                    // register (fma_mixlo) take twice as long. Pinned, or the compiler makes those of them.
+                    const q4_h2 hi = __builtin_convertvector((f2_t{e0 * kPOne, e1 * kPOne}), q4_h2);
+                    float d0 = __builtin_fmaf(e0, kPOne, -float(hi[0])), d1 = __builtin_fmaf(e1, kPOne, -float(hi[1]));
+                    asm volatile("" : "+v"(d0), "+v"(d1));
+                    const q4_h2 lo = __builtin_convertvector((f2_t{d0, d1}), q4_h2);
+                    terms_h[i] = __builtin_bit_cast(uint32_t, hi), terms_l[i] = __builtin_bit_cast(uint32_t, lo);
+                    asm volatile("" : "+v"(terms_h[i]), "+v"(terms_l[i]));
+                }
+                ahead = __builtin_amdgcn_mfma_f32_32x32x16_f16(x_now, ql[k], ahead, 0, 0, 0);
+                x_now = x_next, x_next = x_then;
+                __builtin_amdgcn_sched_barrier(0);
+            }
+            q4_h8 wh[2], wl[2];
+            __builtin_memcpy(wh, terms_h, 32);
+            __builtin_memcpy(wl, terms_l, 32);
+            // ... this unit's values, and between their products operands of the units to come and the next unit's maxima
+            const int slot1 = slot == kRing - 1 ? 0 : slot + 1, slot2 = slot1 == kRing - 1 ? 0 : slot1 + 1;
+            take(slot2, slot1);
+            q4_h8 v_now[2] = {operand_v(now, 0, 0), operand_v(now, 0, 1)};
+            if (__builtin_expect(w1.edge, 0)) {
+                clean_v(w1.at);
+                hide(ahead, w1.at);
+            }
+            float best = -INFINITY;
+            __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+            for (int i = 0; i < NB; ++i) {
+                const int j = min(i + 1, NB - 1);
+                const q4_h8 v_next[2] = {operand_v(now, j, 0), operand_v(now, j, 1)};
+                __builtin_amdgcn_sched_barrier(0);
+                // (products of one accumulator behind each other: it is passed on, not read again)
+                o[i] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v_now[0], wh[0], o[i], 0, 0, 0);
+                o[i] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v_now[0], wl[0], o[i], 0, 0, 0);
+                form(now, now ^ 1, i);
+#pragma unroll
+                for (int y = 0; y < 16 / NB; ++y) best = fmaxf(best, ahead[i * (16 / NB) + y]);
+                o[i] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v_now[1], wh[1], o[i], 0, 0, 0);
+                o[i] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v_now[1], wl[1], o[i], 0, 0, 0);
+                v_now[0] = v_next[0], v_now[1] = v_next[1];
+                __builtin_amdgcn_sched_barrier(0);
+            }
+            const Two w5 = locate(u + 5);
+            fetch(w5.krec0, w5.krec1, slot);
+            w1 = locate(u + 2);
+            slot = slot1;
+            rescale(best);
+            wait_vmcnt<2 * kLoads>();
+            barrier();
+            s = ahead;
+        };
+        for (int u = u0; u < u1; u += 2) {
+            if (u + 6 >= listed + kListed / 2) {  // the two units' locate would leave the list
+                barrier();
+                look_up(u);
+                w1.at -= 2 * (u - listed);
+                listed = u;
+                barrier();
+            }
+            iterate(u, 0);
+            if (u + 1 < u1) iterate(u + 1, 1);
+        }
+    }
+
+    // register 4 y + i of block n: channel 32 n + 8 y + 4 f + i of the column
+    const float total = l + __shfl_xor(l, 32);
+    if (row < 0 || pos < 0) return;  // (both lanes of a column)
+    const int r = r0 + row;
+    if (nsplit > 1) {
+        float* rec = a.work + ((int64_t(r) * a.Hq + head) * nsplit + split) * (DH + 4);
+        if (f == 0) rec[0] = m2, rec[1] = total;
+#pragma unroll
+        for (int n = 0; n < NB; ++n)
+#pragma unroll
+            for (int y = 0; y < 4; ++y)
+                *reinterpret_cast<f4_t*>(rec + 4 + 32 * n + 8 * y + 4 * f) = f4_t{o[n][4 * y], o[n][4 * y + 1], o[n][4 * y + 2], o[n][4 * y + 3]} * (1.f / kPOne);
+        return;
+    }
+    const int64_t width = int64_t(a.Hq) * DH, at = int64_t(r) * width + int64_t(head) * DH + 4 * f;
+    const float* gates = a.proj + int64_t(r) * a.proj_stride + int64_t(head) * 2 * DH + DH + 4 * f;
+    const float share = total == 0.f ? 0.f : 1.f / (total * kPOne);
+#pragma unroll
+    for (int n = 0; n < NB; ++n) {
+        float v[16], amax = 0.f;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+            v[i] = total == 0.f ? 0.f : o[n][i] * share * gate_of(gates[32 * n + 8 * (i / 4) + i % 4]);
+            amax = fmaxf(amax, fabsf(v[i]));
+        }
+        if (a.out_f32)
+#pragma unroll
+            for (int y = 0; y < 4; ++y) *reinterpret_cast<f4_t*>(a.out_f32 + at + 32 * n + 8 * y) = f4_t{v[4 * y], v[4 * y + 1], v[4 * y + 2], v[4 * y + 3]};
+        if (a.act_out) {
+            amax = fmaxf(amax, __shfl_xor(amax, 32));
+            const float d = amax / 127.f, id = d != 0.f ? 1.f / d : 0.f;
+            int8_t* qs = static_cast<int8_t*>(a.act_out);
+#pragma unroll
+            for (int y = 0; y < 4; ++y) {
+                uint32_t codes = 0;
+#pragma unroll
+                for (int i = 0; i < 4; ++i) codes |= uint32_t(int(roundf(v[4 * y + i] * id)) & 0xFF) << (8 * i);
+                *reinterpret_cast<uint32_t*>(qs + at + 32 * n + 8 * y) = codes;
+            }
+            if (f == 0) reinterpret_cast<float*>(qs + int64_t(c.rows) * width)[(at >> 5) + n] = half_bits_to_f32(fp32_to_fp16_ref(d));
+        }
+    }
+}
+
+// Few ranges: DH / 4 lanes for a (row, query head), four channels each
+constexpr int kFewRanges = 8;
+template <int DH>
+__global__ __launch_bounds__(256) void attn4_combine_few_kernel(Attn4Args a, int nsplit) {
+    constexpr int LN = DH / 4, kRec = DH + 4;
+    const int64_t item = int64_t(blockIdx.x) * (256 / LN) + threadIdx.x / LN;
+    const int ch = threadIdx.x % LN * 4;
+    if (item >= int64_t(a.c.rows) * a.Hq) return;
+    const int r = int(item / a.Hq), h = int(item % a.Hq);
+    int seq;
+    if (row_position(a.c, r, &seq) < 0) return;
+    const float* rec = a.work + item * nsplit * kRec;
+    f4_t v[kFewRanges];
+    float m[kFewRanges], l[kFewRanges], mx = kLowest;
+#pragma unroll
+    for (int s = 0; s < kFewRanges; ++s) {
+        const float* at = rec + min(s, nsplit - 1) * kRec;
+        m[s] = at[0], l[s] = at[1];
+        v[s] = *reinterpret_cast<const f4_t*>(at + 4 + ch);
+    }
+    const float* gates = a.proj + int64_t(r) * a.proj_stride + int64_t(h) * 2 * DH + DH + ch;
+    float gate[4];
+    __builtin_memcpy(gate, gates, 16);
+#pragma unroll
+    for (int s = 0; s < kFewRanges; ++s) mx = fmaxf(mx, m[s]);
+    float total = 0.f;
+    f4_t o = f4_t{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int s = 0; s < kFewRanges; ++s) {
+        const float f = s < nsplit ? exp2_hw(m[s] - mx) : 0.f;
+        total += f * l[s];
+        o += s < nsplit ? f * v[s] : f4_t{0.f, 0.f, 0.f, 0.f};
+    }
+    const int64_t width = int64_t(a.Hq) * DH, at = int64_t(r) * width + int64_t(h) * DH + ch;
+    float amax = 0.f;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        o[i] = total == 0.f ? 0.f : o[i] / total * gate_of(gate[i]);
+        amax = fmaxf(amax, fabsf(o[i]));
+    }
+    if (a.out_f32) *reinterpret_cast<f4_t*>(a.out_f32 + at) = o;
+    if (a.act_out) {
+        for (int off = 1; off < 8; off <<= 1) amax = fmaxf(amax, __shfl_xor(amax, off));
+        const float d = amax / 127.f, id = d != 0.f ? 1.f / d : 0.f;
+        int8_t* qs = static_cast<int8_t*>(a.act_out);
+        uint32_t codes = 0;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) codes |= uint32_t(int(roundf(o[i] * id)) & 0xFF) << (8 * i);
+        *reinterpret_cast<uint32_t*>(qs + at) = codes;
+        if (ch % 32 == 0) reinterpret_cast<float*>(qs + int64_t(a.c.rows) * width)[at >> 5] = half_bits_to_f32(fp32_to_fp16_ref(d));
+    }
+}
+
 // A workgroup per (row, query head): DH / 4 lanes for four channels each read a range's result, and
 // 1024 / DH such groups take the ranges in turn.
 template <int DH>
@@ -594,32 +1053,41 @@ __global__ __launch_bounds__(256) void attn4_combine_kernel(Attn4Args a, int nsp
     }
 }
 
-// Rows a workgroup takes, and into how many ranges their keys are split: about three
-// workgroups per CU over all rows and heads, at least eight units of 32 keys each.
-constexpr int64_t kGroups = 768;
+// Rows a workgroup takes, and into how many ranges their keys are split. Tokens: three workgroups per CU, eight
+// units of 32 keys each at least. Chunks: one workgroup per CU with at least eight units, and (128-wide
+// heads, of which two fit) two with at least 64: 512 rows over 16000 keys take 534 us in one range, 307 in two, 275 in
+// four; 1000 rows over 1024 each 63 us in one, 62 in two, 78 in four.
+enum class Form { token, few, chunk };
 struct Plan {
+    Form form;
     int R, nsplit;
-    int64_t tiles, most;  // groups of rows; ranges that the keys allow
+    int64_t tiles, groups, most;  // groups of rows; workgroups at most where keys are split; ranges that the keys allow
 };
-Plan attn4_plan(int64_t rows, int64_t group, int64_t Hkv, bool chunk, int64_t span, int64_t window, int64_t sinks) {
+Plan attn4_plan(Form form, int64_t rows, int64_t group, int64_t Hkv, int64_t Dh, int64_t span, int64_t window, int64_t sinks) {
     Plan p;
-    p.R = chunk && rows > 1 ? int(16 / group) : 1;
-    const int64_t keys = window > 0 ? std::min(span, window + sinks + p.R + 2 * kQ4Tile) : span;
+    p.form = form;
+    p.R = form == Form::token ? 1 : int((form == Form::few ? 16 : 128) / group);
+    p.groups = form == Form::chunk ? 512 : 768;
+    const int64_t keys = window > 0 ? std::min(span, window + sinks + p.R + 2 * kQ4Tile) : span, units = (keys + 31) / 32;
     p.tiles = (rows + p.R - 1) / p.R;
-    p.most = std::max<int64_t>(1, (keys + 31) / 32 / 8);
-    p.nsplit = int(std::max<int64_t>(1, std::min(kGroups / (p.tiles * Hkv), p.most)));
+    p.most = std::max<int64_t>(1, units / 8);
+    const int64_t each = p.tiles * Hkv;
+    p.nsplit = int(std::max<int64_t>(1, form != Form::chunk ? std::min(p.groups / each, p.most)
+                                                            : std::max(std::min(256 / each, p.most), Dh == 128 ? std::min(p.groups / each, units / 64) : 0)));
     return p;
 }
+// rows that belong to sequences of their own have no keys in common
+Form attn4_form(bool row_seq, int64_t rows, int64_t group) { return !row_seq || rows == 1 ? Form::token : rows * group <= 16 ? Form::few : Form::chunk; }
 
 }  // namespace
 
-// Room for any call of up to `rows` rows: where there are several ranges, the workgroups
-// are at most kGroups, of R * group results each.
+// Room for any call of up to `rows` rows, of any form: where there are several ranges, the workgroups are
+// at most p.groups, of R * group results each.
 int64_t attn4_work_bytes(int64_t rows, int64_t Hq, int64_t Hkv, int64_t Dh, int64_t span, int64_t window, int64_t sinks) {
     int64_t slots = 0;
-    for (const bool chunk : {false, true}) {
-        const Plan p = attn4_plan(rows, Hq / Hkv, Hkv, chunk, span, window, sinks);
-        if (p.most > 1) slots = std::max(slots, std::min(kGroups, p.tiles * Hkv * p.most) * p.R * (Hq / Hkv));
+    for (const Form form : {Form::token, Form::few, Form::chunk}) {
+        const Plan p = attn4_plan(form, rows, Hq / Hkv, Hkv, Dh, span, window, sinks);
+        if (p.most > 1) slots = std::max(slots, std::min(p.groups, p.tiles * Hkv * p.most) * p.R * (Hq / Hkv));
     }
     return slots * (Dh + 4) * 4;
 }
@@ -628,16 +1096,24 @@ namespace {
 template <int DH>
 void attn4_sized(const Attn4Args& a, const Plan& p, hipStream_t s) {
     const dim3 grid(unsigned(p.tiles * a.c.Hkv * p.nsplit));
-    if (p.R == 1)
+    if (p.form == Form::chunk)
+        hipLaunchKernelGGL(attn4_chunk_kernel<DH>, grid, dim3(256), 0, s, a, p.R, p.nsplit);
+    else if (p.form == Form::token)
         hipLaunchKernelGGL((attn4_token_kernel<DH, 2>), grid, dim3(256), 0, s, a, p.nsplit);
     else
         hipLaunchKernelGGL(attn4_kernel<DH>, grid, dim3(256), 0, s, a, p.R, p.nsplit);
-    if (p.nsplit > 1) hipLaunchKernelGGL(attn4_combine_kernel<DH>, dim3(unsigned(a.c.rows * a.Hq)), dim3(256), size_t(p.nsplit + 31) / 32 * 128, s, a, p.nsplit);
+    if (p.nsplit == 1) return;
+    const int64_t heads = int64_t(a.c.rows) * a.Hq;
+    if (p.nsplit <= kFewRanges)
+        hipLaunchKernelGGL(attn4_combine_few_kernel<DH>, dim3(unsigned((heads * (DH / 4) + 255) / 256)), dim3(256), 0, s, a, p.nsplit);
+    else
+        hipLaunchKernelGGL(attn4_combine_kernel<DH>, dim3(unsigned(heads)), dim3(256), size_t(p.nsplit + 31) / 32 * 128, s, a, p.nsplit);
 }
 }  // namespace
 
 void launch_attn4(const Attn4Args& a, hipStream_t s) {
-    const Plan p = attn4_plan(a.c.rows, a.Hq / a.c.Hkv, a.c.Hkv, a.c.row_seq != nullptr, int64_t(a.c.max_pages) * a.c.page_size, a.window, a.sinks);
+    const int64_t group = a.Hq / a.c.Hkv;
+    const Plan p = attn4_plan(attn4_form(a.c.row_seq, a.c.rows, group), a.c.rows, group, a.c.Hkv, a.c.Dh, int64_t(a.c.max_pages) * a.c.page_size, a.window, a.sinks);
     a.c.Dh == 256 ? attn4_sized<256>(a, p, s) : attn4_sized<128>(a, p, s);
 }
 
