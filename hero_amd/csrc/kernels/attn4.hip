@@ -58,24 +58,6 @@ struct FieldMasks {
 
 __device__ __forceinline__ q4_h8 join(q4_h2 a, q4_h2 b, q4_h2 c, q4_h2 d) { return q4_h8{a[0], a[1], b[0], b[1], c[0], c[1], d[0], d[1]}; }
 
-// a lane's share of a record of keys and the one of values
-template <int DH>
-struct TileRegs {
-    uint4 k[DH / 128], v[DH / 128];
-    _Float16 kd[DH / 32];
-    q4_h2 vd[DH / 16];
-    __device__ __forceinline__ void load(const uint8_t* krec, const uint8_t* vrec, int lane) {
-        const int p = lane >> 4, b = lane & 15;
-#pragma unroll
-        for (int h = 0; h < DH / 128; ++h) {
-            k[h] = *reinterpret_cast<const uint4*>(krec + 1024 * h + b * 64 + p * 16);
-            v[h] = *reinterpret_cast<const uint4*>(vrec + 1024 * h + lane * 16);
-        }
-        __builtin_memcpy(kd, __builtin_assume_aligned(krec + 8 * DH + b * (DH / 16), 8), sizeof(kd));
-        __builtin_memcpy(vd, __builtin_assume_aligned(vrec + 8 * DH + p * (DH / 4), 16), sizeof(vd));
-    }
-};
-
 // A wave's ring of units (two records of keys and of values) in shared memory, filled by
 // loads that go there directly: what is in flight takes no registers. Records arrive as
 // they lie, 1 KB a load, but for the keys' 16-byte pieces: piece p of key b goes to place
@@ -170,27 +152,56 @@ __device__ __forceinline__ void merge_waves(const Attn4Args& a, const Merge<DH, 
     }
 }
 
-// One row's query heads of a K/V head: a workgroup of four waves takes one of nsplit equal
-// ranges of the row's records, a wave two records (32 keys) at a time.
-template <int DH, int D>
-__global__ __launch_bounds__(256, DH == 128 ? 3 : 2) void attn4_token_kernel(Attn4Args a, int nsplit) {
-    constexpr int COLS = 8, H = DH / 128, NS = DH / 32, NV = DH / 16;
+// The rows of a run: neighbours, of one sequence. A run is short where its (row, query head) pairs fit the 16
+// columns of a product. The length of the one that starts in row r, 0 if none does or it is longer than `most`.
+__device__ __forceinline__ int short_run(const PagedRows& c, int64_t r, int most) {
+    int seq, other;
+    if (r >= c.rows || row_position(c, int(r), &seq) < 0 || (r > 0 && row_position(c, int(r) - 1, &other) >= 0 && other == seq)) return 0;
+    int n = 1;
+    bool on = true;
+#pragma unroll 4
+    for (int d = 1; d <= most; ++d) {
+        const int64_t i = min(r + d, int64_t(c.rows) - 1);
+        on = on && row_position(c, int(i), &other) >= 0 && other == seq && r + d < c.rows;
+        n += on;
+    }
+    return n <= most ? n : 0;
+}
+
+// One row (PAIR), or the short runs of rows b, b + stride, ...: a workgroup of four waves takes one K/V head and
+// one of nsplit equal ranges of the run's records, a wave two records (32 keys) at a time. PAIR:
+// the two terms of up to 8 query heads are the 16 columns, those of head h columns h and h + 8, added where both are
+// done. Else the columns are the run's pairs, and each term has a product of its own.
+template <int DH, int D, bool PAIR>
+__global__ __launch_bounds__(256, DH == 128 && PAIR ? 3 : 2) void attn4_short_kernel(Attn4Args a, int nsplit, int stride) {
+    constexpr int COLS = PAIR ? 8 : 16, H = DH / 128, NS = DH / 32, NV = DH / 16;
     const PagedRows& c = a.c;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), p = lane >> 4, b = lane & 15;
-    const int split = blockIdx.x % nsplit, g = blockIdx.x / nsplit % c.Hkv, r = blockIdx.x / nsplit / c.Hkv;
-    const int group = a.Hq / c.Hkv, tpp = c.page_size / kQ4Tile, col = b & 7;
+    const int split = blockIdx.x % nsplit, g = blockIdx.x / nsplit % c.Hkv, first_row = blockIdx.x / nsplit / c.Hkv;
+    const int group = a.Hq / c.Hkv, tpp = c.page_size / kQ4Tile, col = PAIR ? b & 7 : b;
     __shared__ union {
         Ring<DH, D> ring[4];
         Merge<DH, COLS> merge;
     } sh;
     const FieldMasks masks;
 
+    auto attend = [&](const int r, const int rows) __attribute__((always_inline)) {
     int seq;
-    const int pos = row_position(c, r, &seq);
-    if (pos < 0) return;
-    const Seen sees = row_sees(a, pos);
-    // records: those of the first keys that stay, then from the window's first key on
-    const int first = sees.first / kQ4Tile, stay = min((sees.stay + kQ4Tile - 1) / kQ4Tile, first), last = pos / kQ4Tile;
+    const int pos0 = row_position(c, r, &seq);
+    if (pos0 < 0) return;
+    // the column's row; the run's first and last position
+    const int mine = PAIR ? 0 : min(col / group, rows - 1);
+    int pos = pos0, lo = pos0, hi = pos0;
+    if constexpr (!PAIR) {
+        int s;
+        pos = row_position(c, r + mine, &s);
+        lo = hi = pos;
+        for (int off = 1; off < 16; off <<= 1) lo = min(lo, __shfl_xor(lo, off)), hi = max(hi, __shfl_xor(hi, off));
+        lo = __builtin_amdgcn_readfirstlane(lo), hi = __builtin_amdgcn_readfirstlane(hi);
+    }
+    const Seen sees = row_sees(a, pos), most = row_sees(a, hi), least = row_sees(a, lo);
+    // records: those of the first keys that stay, then from the earliest window's first key on
+    const int first = least.first / kQ4Tile, stay = min((most.stay + kQ4Tile - 1) / kQ4Tile, first), last = hi / kQ4Tile;
     const int tiles = stay + last - first + 1, units = (tiles + 1) / 2;
     const int u0 = int(int64_t(units) * split / nsplit), u1 = int(int64_t(units) * (split + 1) / nsplit);
     // read as constant memory: through the scalar cache, apart from the counted vector loads
@@ -221,11 +232,11 @@ __global__ __launch_bounds__(256, DH == 128 ? 3 : 2) void attn4_token_kernel(Att
         }
     };
 
-    // the query in units of log2, a power of two brings the head's largest channel below 2^14
-    q4_h8 q[NS];
+    // the queries in units of log2, a power of two brings the head's largest channel below 2^14
+    q4_h8 q[NS], q2[PAIR ? 1 : NS];
     float unit;
     {
-        const float* src = a.q_rot + (int64_t(r) * a.Hq + g * group + min(col, group - 1)) * DH + 8 * p;
+        const float* src = a.q_rot + (int64_t(r + mine) * a.Hq + g * group + (PAIR ? min(col, group - 1) : col % group)) * DH + 8 * p;
         float x[NS][8], amax = 0.f;
         const float k = a.score_scale * kLog2e;
 #pragma unroll
@@ -242,7 +253,8 @@ __global__ __launch_bounds__(256, DH == 128 ? 3 : 2) void attn4_token_kernel(Att
             for (int j = 0; j < 8; ++j) {
                 _Float16 hi, lo;
                 split_f16(ldexpf(x[s][j], 14 - e), hi, lo);
-                q[s][j] = b < 8 ? hi : lo;
+                q[s][j] = PAIR && b >= 8 ? lo : hi;
+                if constexpr (!PAIR) q2[s][j] = lo;
             }
         unit = ldexpf(1.f, e - 14);
     }
@@ -286,11 +298,12 @@ __global__ __launch_bounds__(256, DH == 128 ? 3 : 2) void attn4_token_kernel(Att
                     const uint4 w4 = in.k[x][k / 4][4 * b + (p ^ b >> 2)];
                     const uint32_t word = k % 4 == 0 ? w4.x : k % 4 == 1 ? w4.y : k % 4 == 2 ? w4.z : w4.w;
                     const q4_h2 d = {kd[k], kd[k]};
-                    sum = __builtin_amdgcn_mfma_f32_16x16x32_f16(
-                        join(masks.codes<0>(word) * d, masks.codes<1>(word) * d, masks.codes<0>(word >> 8) * d, masks.codes<1>(word >> 8) * d), q[k], sum, 0, 0, 0);
+                    const q4_h8 f = join(masks.codes<0>(word) * d, masks.codes<1>(word) * d, masks.codes<0>(word >> 8) * d, masks.codes<1>(word >> 8) * d);
+                    sum = __builtin_amdgcn_mfma_f32_16x16x32_f16(f, q[k], sum, 0, 0, 0);
+                    if constexpr (!PAIR) sum = __builtin_amdgcn_mfma_f32_16x16x32_f16(f, q2[k], sum, 0, 0, 0);
                 }
 #pragma unroll
-                for (int j = 0; j < 4; ++j) s[4 * x + j] = sum[j] + column_other(sum[j]);
+                for (int j = 0; j < 4; ++j) s[4 * x + j] = PAIR ? sum[j] + column_other(sum[j]) : sum[j];
             }
             uint4 v[2][H];
             q4_h2 vd[2][NV];
@@ -303,20 +316,20 @@ __global__ __launch_bounds__(256, DH == 128 ? 3 : 2) void attn4_token_kernel(Att
 #pragma unroll
             for (int x = 0; x < 2; ++x) {
                 const int k0 = kQ4Tile * w[x].t;
-                if (!w[x].there || k0 + 15 > pos || (k0 < sees.first && k0 + 15 >= sees.stay)) {  // not all of its keys are seen
-                    bool see[4];
+                if (!w[x].there || k0 + 15 > lo || (k0 < most.first && k0 + 15 >= least.stay)) {  // some row does not see all of it
+                    bool none[4];
 #pragma unroll
                     for (int j = 0; j < 4; ++j) {
                         const int key = k0 + 4 * p + j;
-                        see[j] = w[x].there && key <= pos && (key >= sees.first || key < sees.stay);
-                        if (!see[j]) s[4 * x + j] = -INFINITY;
+                        none[j] = !w[x].there || key > hi;
+                        if (none[j] || key > pos || (key < sees.first && key >= sees.stay)) s[4 * x + j] = -INFINITY;
                     }
-                    // slots past the row may hold anything: their steps count as 0
+                    // slots past the last row may hold anything: their steps count as 0
 #pragma unroll
                     for (int y = 0; y < NV; ++y)
 #pragma unroll
                         for (int j = 0; j < 2; ++j)
-                            if (!see[2 * (y & 1) + j]) vd[x][y][j] = _Float16(0.f);
+                            if (none[2 * (y & 1) + j]) vd[x][y][j] = _Float16(0.f);
                 }
             }
             // what the slot held is in registers: the next unit's loads may land there
@@ -336,13 +349,25 @@ __global__ __launch_bounds__(256, DH == 128 ? 3 : 2) void attn4_token_kernel(Att
 #pragma unroll
                 for (int y = 0; y < NV; ++y) o[y] *= f;
             }
-            q4_h8 w8;
+            // Two weights at a time, as two terms of one value (the scaling is exact). Conversions in pairs and
+            // remainders in fp32: instructions that round to one half of a register (fma_mixlo) take twice as
+            // long. Pinned, or the compiler makes those of them.
+            q4_h8 w8, w8l;
 #pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                const float e = exp2_hw(__builtin_fmaf(s[j], unit, -m2));
-                l += e;
-                const _Float16 hi = _Float16(__builtin_fmaf(e, kPOne, 0.f));  // the scaling is exact, so both terms are of one value
-                w8[j] = b < 8 ? hi : _Float16(__builtin_fmaf(e, kPOne, -float(hi)));
+            for (int j = 0; j < 8; j += 2) {
+                const float e0 = exp2_hw(__builtin_fmaf(s[j], unit, -m2)), e1 = exp2_hw(__builtin_fmaf(s[j + 1], unit, -m2));
+                l += e0;
+                l += e1;
+                const q4_h2 h2 = __builtin_convertvector((f2_t{e0 * kPOne, e1 * kPOne}), q4_h2);
+                float d0 = __builtin_fmaf(e0, kPOne, -float(h2[0])), d1 = __builtin_fmaf(e1, kPOne, -float(h2[1]));
+                asm volatile("" : "+v"(d0), "+v"(d1));
+                const q4_h2 l2 = __builtin_convertvector((f2_t{d0, d1}), q4_h2);
+                if constexpr (PAIR) {
+                    const q4_h2 t = b < 8 ? h2 : l2;
+                    w8[j] = t[0], w8[j + 1] = t[1];
+                } else {
+                    w8[j] = h2[0], w8[j + 1] = h2[1], w8l[j] = l2[0], w8l[j + 1] = l2[1];
+                }
             }
 #pragma unroll
             for (int h = 0; h < H; ++h)
@@ -356,8 +381,12 @@ __global__ __launch_bounds__(256, DH == 128 ? 3 : 2) void attn4_token_kernel(Att
                     const q4_h2 d2 = vd[1][2 * (4 * h + y)], d3 = vd[1][2 * (4 * h + y) + 1];
                     f4_t& oa = o[8 * h + 2 * y];
                     f4_t& ob = o[8 * h + 2 * y + 1];
-                    oa = __builtin_amdgcn_mfma_f32_16x16x32_f16(join(masks.codes<0>(w0) * d0, masks.codes<0>(w1) * d1, masks.codes<0>(w2) * d2, masks.codes<0>(w3) * d3), w8, oa, 0, 0, 0);
-                    ob = __builtin_amdgcn_mfma_f32_16x16x32_f16(join(masks.codes<1>(w0) * d0, masks.codes<1>(w1) * d1, masks.codes<1>(w2) * d2, masks.codes<1>(w3) * d3), w8, ob, 0, 0, 0);
+                    const q4_h8 fa = join(masks.codes<0>(w0) * d0, masks.codes<0>(w1) * d1, masks.codes<0>(w2) * d2, masks.codes<0>(w3) * d3);
+                    const q4_h8 fb = join(masks.codes<1>(w0) * d0, masks.codes<1>(w1) * d1, masks.codes<1>(w2) * d2, masks.codes<1>(w3) * d3);
+                    oa = __builtin_amdgcn_mfma_f32_16x16x32_f16(fa, w8, oa, 0, 0, 0);
+                    if constexpr (!PAIR) oa = __builtin_amdgcn_mfma_f32_16x16x32_f16(fa, w8l, oa, 0, 0, 0);
+                    ob = __builtin_amdgcn_mfma_f32_16x16x32_f16(fb, w8, ob, 0, 0, 0);
+                    if constexpr (!PAIR) ob = __builtin_amdgcn_mfma_f32_16x16x32_f16(fb, w8l, ob, 0, 0, 0);
                 }
         }
     }
@@ -368,186 +397,29 @@ __global__ __launch_bounds__(256, DH == 128 ? 3 : 2) void attn4_token_kernel(Att
 #pragma unroll
     for (int y = 0; y < NV; ++y) {
         f4_t v = o[y];
+        if constexpr (PAIR) {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) v[i] += column_other(v[i]);
+            for (int i = 0; i < 4; ++i) v[i] += column_other(v[i]);
+        }
         if (b < COLS) *reinterpret_cast<f4_t*>(&sh.merge.o[wave][col][16 * y + 4 * p]) = v;
     }
     if (p == 0 && b < COLS) sh.merge.m[wave][col] = m2, sh.merge.l[wave][col] = l;
     __syncthreads();
-    merge_waves<DH, COLS>(a, sh.merge, r, 1, g, nsplit, split);
-}
+    merge_waves<DH, COLS>(a, sh.merge, r, rows, g, nsplit, split);
+    };
 
-// A workgroup of four waves: R = rows * group pairs of rows r0 .. of one K/V head, one of
-// nsplit equal ranges of their records, two records (32 keys) a wave at a time.
-template <int DH>
-__global__ __launch_bounds__(256, 2) void attn4_kernel(Attn4Args a, int R, int nsplit) {
-    constexpr int COLS = 16, H = DH / 128, NS = DH / 32, NV = DH / 16;
-    const PagedRows& c = a.c;
-    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), p = lane >> 4, b = lane & 15;
-    const int split = blockIdx.x % nsplit, g = blockIdx.x / nsplit % c.Hkv, tile0 = blockIdx.x / nsplit / c.Hkv, r0 = tile0 * R;
-    const int group = a.Hq / c.Hkv, tpp = c.page_size / kQ4Tile;
-    __shared__ Merge<DH, COLS> sh;
-    const FieldMasks masks;
-
-    const int col = b, mine = min(col / group, R - 1), r = r0 + mine;
-    const bool used = col < R * group && r < c.rows;
-    int seq = 0;
-    const int pos = used ? row_position(c, r, &seq) : -1;
-    const Seen sees = row_sees(a, pos);
-
-    // queries: a power of two brings the head's largest channel below 2^14
-    q4_h8 qh[NS], ql[NS];
-    float scale = 0.f;
-    {
-        const float* q = a.q_rot + (int64_t(min(r, c.rows - 1)) * a.Hq + g * group + col % group) * DH + 8 * p;
-        float x[NS][8], amax = 0.f;
-#pragma unroll
-        for (int s = 0; s < NS; ++s) {
-            __builtin_memcpy(x[s], __builtin_assume_aligned(q + 32 * s, 16), 32);
-#pragma unroll
-            for (int j = 0; j < 8; ++j) amax = fmaxf(amax, fabsf(x[s][j]));
-        }
-        amax = max_over_p(amax);
-        const int e = amax > 0.f && amax < INFINITY ? ilogbf(amax) + 1 : 0;
-#pragma unroll
-        for (int s = 0; s < NS; ++s)
-#pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                _Float16 hi, lo;
-                split_f16(ldexpf(x[s][j], 14 - e), hi, lo);
-                qh[s][j] = hi, ql[s][j] = lo;
+    if constexpr (PAIR) {
+        attend(first_row, 1);
+    } else {
+        for (int64_t base = first_row; base < c.rows; base += 64 * int64_t(stride)) {
+            const int found = short_run(c, base + int64_t(lane) * stride, 16 / group);  // by a lane each
+            for (uint64_t left = __ballot(found > 0); left; left &= left - 1) {
+                const int at = __ffsll((unsigned long long)left) - 1;
+                __syncthreads();  // the last run's results are read
+                attend(int(base + int64_t(at) * stride), __builtin_amdgcn_readlane(found, at));
             }
-        scale = ldexpf(a.score_scale * kLog2e, e - 14);
-    }
-
-    f4_t o[NV];
-#pragma unroll
-    for (int n = 0; n < NV; ++n) o[n] = f4_t{0.f, 0.f, 0.f, 0.f};
-    float m = kLowest, l = 0.f;
-
-    // rows of one sequence at a time (mostly there is one)
-    for (int k0 = 0; k0 < R;) {
-        int s0, k1 = k0 + 1;
-        const int p0 = r0 + k0 < c.rows ? row_position(c, r0 + k0, &s0) : -1;
-        if (p0 < 0) {
-            ++k0;
-            continue;
-        }
-        int lo = p0, hi = p0;
-        for (; k1 < R && r0 + k1 < c.rows; ++k1) {
-            int s1;
-            const int p1 = row_position(c, r0 + k1, &s1);
-            if (p1 < 0 || s1 != s0) break;
-            lo = min(lo, p1), hi = max(hi, p1);
-        }
-        const bool here = used && pos >= 0 && mine >= k0 && mine < k1;
-        k0 = k1;
-        // records: those of the first keys that stay, then from the earliest window to the last row
-        const Seen most = row_sees(a, hi), least = row_sees(a, lo);
-        const int first = least.first / kQ4Tile, stay = min((most.stay + kQ4Tile - 1) / kQ4Tile, first);
-        const int tiles = stay + hi / kQ4Tile - first + 1, units = (tiles + 1) / 2;
-        const int u0 = int(int64_t(units) * split / nsplit), u1 = int(int64_t(units) * (split + 1) / nsplit);
-        const int32_t* table = c.page_table + int64_t(s0) * c.max_pages;
-
-        auto locate = [&](int k, int& t, int64_t& page) {
-            t = k < stay ? k : first + k - stay;
-            const int lp = min(t, hi / kQ4Tile) / tpp;
-            page = __builtin_amdgcn_readfirstlane(table[lp]);
-            page = k < tiles && page >= 0 && page < c.pool_pages ? page : -1;
-        };
-        for (int u = u0 + wave; u < u1; u += 4) {
-            TileRegs<DH> regs[2];
-            int t[2];
-            bool ok[2];
-#pragma unroll
-            for (int x = 0; x < 2; ++x) {
-                int64_t page;
-                locate(2 * u + x, t[x], page);
-                ok[x] = page >= 0;
-                const int64_t pg = page >= 0 ? page : 0;
-                regs[x].load(q4_record<DH>(c, pg, 0, g, t[x] % tpp), q4_record<DH>(c, pg, 1, g, t[x] % tpp), lane);
-            }
-            // scores of keys 16 t + 4 p + i for the lane's column
-            float s[8];
-#pragma unroll
-            for (int x = 0; x < 2; ++x) {
-                f4_t acc = f4_t{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-                for (int k = 0; k < NS; ++k) {
-                    const uint4 w4 = regs[x].k[k / 4];
-                    const uint32_t w = k % 4 == 0 ? w4.x : k % 4 == 1 ? w4.y : k % 4 == 2 ? w4.z : w4.w;
-                    const q4_h2 d = {regs[x].kd[k], regs[x].kd[k]};
-                    const q4_h8 f = join(masks.codes<0>(w) * d, masks.codes<1>(w) * d, masks.codes<0>(w >> 8) * d, masks.codes<1>(w >> 8) * d);
-                    acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(f, qh[k], acc, 0, 0, 0);
-                    acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(f, ql[k], acc, 0, 0, 0);
-                }
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const int key = kQ4Tile * t[x] + 4 * p + i;
-                    const bool sees_it = here && ok[x] && key <= sees.pos && (key >= sees.first || key < sees.stay);
-                    s[4 * x + i] = sees_it ? acc[i] * scale : -INFINITY;
-                }
-            }
-            float best = s[0];
-#pragma unroll
-            for (int i = 1; i < 8; ++i) best = fmaxf(best, s[i]);
-            if (__ballot(best > m + kPSlack)) {
-                const float to = fmaxf(m, max_over_p(best)), f = exp2_hw(m - to);
-                m = to;
-                l *= f;
-#pragma unroll
-                for (int n = 0; n < NV; ++n) o[n] *= f;
-            }
-            q4_h8 w8, w8l;
-#pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                const float w = exp2_hw(s[i] - m);
-                l += w;
-                _Float16 hi, lo;
-                split_f16(w * kPOne, hi, lo);
-                w8[i] = hi, w8l[i] = lo;
-            }
-            // a slot past the last row, or of a page that holds nothing, may hold anything: its steps count as 0
-#pragma unroll
-            for (int x = 0; x < 2; ++x) {
-                if (!ok[x] || kQ4Tile * t[x] + 15 > hi) {
-#pragma unroll
-                    for (int n = 0; n < NV; ++n)
-#pragma unroll
-                        for (int i = 0; i < 2; ++i)
-                            if (!ok[x] || kQ4Tile * t[x] + 4 * p + 2 * (n & 1) + i > hi) regs[x].vd[n][i] = _Float16(0.f);
-                }
-            }
-#pragma unroll
-            for (int h = 0; h < H; ++h)
-#pragma unroll
-                for (int y = 0; y < 4; ++y) {  // byte y of the words: channels 128 h + 32 y + b and + 16
-                    // 16-bit halves: that byte of two neighbouring keys
-                    const uint32_t pick = 0x0C040C00u + 0x00010001u * y;
-                    const uint4 va = regs[0].v[h], vb = regs[1].v[h];
-                    const uint32_t w0 = __builtin_amdgcn_perm(va.y, va.x, pick), w1 = __builtin_amdgcn_perm(va.w, va.z, pick);
-                    const uint32_t w2 = __builtin_amdgcn_perm(vb.y, vb.x, pick), w3 = __builtin_amdgcn_perm(vb.w, vb.z, pick);
-                    const q4_h2 d0 = regs[0].vd[2 * (4 * h + y)], d1 = regs[0].vd[2 * (4 * h + y) + 1];
-                    const q4_h2 d2 = regs[1].vd[2 * (4 * h + y)], d3 = regs[1].vd[2 * (4 * h + y) + 1];
-                    const q4_h8 fa = join(masks.codes<0>(w0) * d0, masks.codes<0>(w1) * d1, masks.codes<0>(w2) * d2, masks.codes<0>(w3) * d3);
-                    const q4_h8 fb = join(masks.codes<1>(w0) * d0, masks.codes<1>(w1) * d1, masks.codes<1>(w2) * d2, masks.codes<1>(w3) * d3);
-                    f4_t& oa = o[8 * h + 2 * y];
-                    f4_t& ob = o[8 * h + 2 * y + 1];
-                    oa = __builtin_amdgcn_mfma_f32_16x16x32_f16(fa, w8, oa, 0, 0, 0);
-                    ob = __builtin_amdgcn_mfma_f32_16x16x32_f16(fb, w8, ob, 0, 0, 0);
-                    oa = __builtin_amdgcn_mfma_f32_16x16x32_f16(fa, w8l, oa, 0, 0, 0);
-                    ob = __builtin_amdgcn_mfma_f32_16x16x32_f16(fb, w8l, ob, 0, 0, 0);
-                }
         }
     }
-
-    // the four waves' results
-    l = sum_over_p(l);
-#pragma unroll
-    for (int n = 0; n < NV; ++n) *reinterpret_cast<f4_t*>(&sh.o[wave][col][16 * n + 4 * p]) = o[n];
-    if (p == 0) sh.m[wave][col] = m, sh.l[wave][col] = l;
-    __syncthreads();
-    merge_waves<DH, COLS>(a, sh, r0, R, g, nsplit, split);
 }
 
 // Many rows: a workgroup takes 128 columns, (row, query head) pairs of consecutive rows and one K/V head, 32
@@ -569,14 +441,15 @@ struct Listed {
 };
 
 template <int DH>
-__global__ __launch_bounds__(256, DH == 128 ? 2 : 1) void attn4_chunk_kernel(Attn4Args a, int R, int nsplit) {
+__global__ __launch_bounds__(256, DH == 128 ? 2 : 1) void attn4_chunk_kernel(Attn4Args a, int R, int nsplit, int parts) {
     constexpr int H = DH / 128, NS = DH / 16, NB = DH / 32;
     constexpr int WK = NB / 2, WV = 2 * H;  // words of keys, and bytes of words of values, that a lane turns into operands
     typedef float f16_t __attribute__((ext_vector_type(16)));
     const PagedRows& c = a.c;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), f = lane >> 5, p = lane >> 4, b = lane & 15;
     // neighbouring workgroups, which go to different XCDs, take different heads: each L2 holds the records of its own
-    const int g = blockIdx.x % c.Hkv, split = blockIdx.x / c.Hkv % nsplit, r0 = blockIdx.x / c.Hkv / nsplit * R;
+    const int g = blockIdx.x % c.Hkv, split = blockIdx.x / c.Hkv % nsplit;
+    const int tiles_r = (c.rows + R - 1) / R, part = blockIdx.x / c.Hkv / nsplit / tiles_r, r0 = blockIdx.x / c.Hkv / nsplit % tiles_r * R;
     const int group = a.Hq / c.Hkv, tpp = c.page_size / kQ4Tile;
     const uint32_t magic = (0x80000000u + tpp - 1) / tpp;  // x / tpp = x magic >> 31 for x < 2^23
     const uint32_t rec_bytes = 9 * DH, head_bytes = uint32_t(tpp) * rec_bytes, half = head_bytes * c.Hkv;
@@ -629,8 +502,44 @@ __global__ __launch_bounds__(256, DH == 128 ? 2 : 1) void attn4_chunk_kernel(Att
     }
     const float slack = kPSlack / unit;
     uint64_t valid[2] = {__ballot(row_pos[0] >= 0), __ballot(row_pos[1] >= 0)};
+    if (parts > 1) {
+        // Rows of short runs are not this kernel's. Bit i of `on`: row r0 - 16 + i goes on the run of the row before
+        // it; `most` such bits in a row are a run of more rows than that, and it holds all of them.
+        const int most = 16 / group;
+        uint64_t on[3], all_on[3], bits[3], in[3];
+#pragma unroll
+        for (int k = 0; k < 3; ++k) {
+            const int64_t r = int64_t(r0) - 16 + lane + 64 * k;
+            int s0 = 0, s1 = 0;
+            const bool ok = r >= 1 && r < c.rows;
+            const int at = ok ? int(r) : min(1, c.rows - 1);
+            const int p0 = row_position(c, max(at - 1, 0), &s0), p1 = row_position(c, at, &s1);
+            on[k] = all_on[k] = bits[k] = __ballot(ok && p0 >= 0 && p1 >= 0 && s0 == s1);
+        }
+        auto down = [](uint64_t (&v)[3]) { v[0] = v[0] >> 1 | v[1] << 63, v[1] = v[1] >> 1 | v[2] << 63, v[2] >>= 1; };
+        auto up = [](uint64_t (&v)[3]) { v[2] = v[2] << 1 | v[1] >> 63, v[1] = v[1] << 1 | v[0] >> 63, v[0] <<= 1; };
+        for (int d = 1; d < most; ++d) {
+            down(bits);
+#pragma unroll
+            for (int k = 0; k < 3; ++k) all_on[k] &= bits[k];
+        }
+#pragma unroll
+        for (int k = 0; k < 3; ++k) in[k] = bits[k] = all_on[k];
+        for (int d = 1; d < most; ++d) {
+            up(bits);
+#pragma unroll
+            for (int k = 0; k < 3; ++k) in[k] |= bits[k];
+        }
+        down(all_on);
+        valid[0] &= (in[0] | all_on[0]) >> 16 | (in[1] | all_on[1]) << 48;
+        valid[1] &= (in[1] | all_on[1]) >> 16 | (in[2] | all_on[2]) << 48;
+#pragma unroll
+        for (int k = 0; k < 2; ++k)
+            if (!(valid[k] >> lane & 1)) row_pos[k] = -1;
+    }
     if (!(valid[0] | valid[1])) return;
     const uint64_t all[2] = {valid[0], valid[1]};
+    uint64_t done[2] = {0, 0};  // rows of the runs that this workgroup takes
     auto of_row = [&](const int (&v)[2], int i) {
         const int x = __shfl(v[0], i & 63), y = __shfl(v[1], i & 63);  // by all lanes
         return i < 64 ? x : y;
@@ -643,8 +552,9 @@ __global__ __launch_bounds__(256, DH == 128 ? 2 : 1) void attn4_chunk_kernel(Att
 #pragma unroll
     for (int n = 0; n < NB; ++n) o[n] = zero;
 
-    // the rows of one sequence at a time (mostly there is one)
-    while (valid[0] | valid[1]) {
+    // The rows of one sequence at a time: mostly there is one. Where a second sequence begins among a workgroup's rows
+    // another workgroup (part 1) takes what is not the first's.
+    for (int run = 0; (valid[0] | valid[1]) && (parts == 1 || part == 1 || run == 0); ++run) {
         const int lead = valid[0] ? __ffsll((unsigned long long)valid[0]) - 1 : 63 + __ffsll((unsigned long long)valid[1]);
         const int seq = __builtin_amdgcn_readfirstlane(of_row(row_of, lead));
         uint64_t mine[2];
@@ -654,11 +564,14 @@ __global__ __launch_bounds__(256, DH == 128 ? 2 : 1) void attn4_chunk_kernel(Att
             const bool in = row_of[k] == seq && (valid[k] >> lane & 1);
             mine[k] = __ballot(in);
             valid[k] &= ~mine[k];
+            if (part == 0 || run > 0) done[k] |= mine[k];
             if (in) lo = min(lo, row_pos[k]), hi = max(hi, row_pos[k]);
         }
+        if (part == 1 && run == 0) continue;
         for (int off = 32; off > 0; off >>= 1) lo = min(lo, __shfl_xor(lo, off)), hi = max(hi, __shfl_xor(hi, off));
         lo = __builtin_amdgcn_readfirstlane(lo), hi = __builtin_amdgcn_readfirstlane(hi);
-        const bool whole = mine[0] == all[0] && mine[1] == all[1];
+        // (columns of rows that this workgroup does not store may hold anything: none of them touches another)
+        const bool whole = (mine[0] == all[0] && mine[1] == all[1]) || (parts > 1 && (part == 0 || (run == 1 && !(valid[0] | valid[1]))));
         const bool here = row >= 0 && ((row < 64 ? mine[0] : mine[1]) >> (row & 63) & 1);
 
         // records: those of the first keys that stay, then from the earliest window to the last row
@@ -911,7 +824,7 @@ __global__ __launch_bounds__(256, DH == 128 ? 2 : 1) void attn4_chunk_kernel(Att
 
     // register 4 y + i of block n: channel 32 n + 8 y + 4 f + i of the column
     const float total = l + __shfl_xor(l, 32);
-    if (row < 0 || pos < 0) return;  // (both lanes of a column)
+    if (row < 0 || !((row < 64 ? done[0] : done[1]) >> (row & 63) & 1)) return;  // (both lanes of a column)
     const int r = r0 + row;
     if (nsplit > 1) {
         float* rec = a.work + ((int64_t(r) * a.Hq + head) * nsplit + split) * (DH + 4);
@@ -1059,24 +972,22 @@ __global__ __launch_bounds__(256) void attn4_combine_kernel(Attn4Args a, int nsp
 // four; 1000 rows over 1024 each 63 us in one, 62 in two, 78 in four.
 enum class Form { token, few, chunk };
 struct Plan {
-    Form form;
     int R, nsplit;
     int64_t tiles, groups, most;  // groups of rows; workgroups at most where keys are split; ranges that the keys allow
 };
-Plan attn4_plan(Form form, int64_t rows, int64_t group, int64_t Hkv, int64_t Dh, int64_t span, int64_t window, int64_t sinks) {
+Plan attn4_plan(Form form, int64_t rows, int64_t seqs, int64_t group, int64_t Hkv, int64_t Dh, int64_t span, int64_t window, int64_t sinks) {
     Plan p;
-    p.form = form;
     p.R = form == Form::token ? 1 : int((form == Form::few ? 16 : 128) / group);
     p.groups = form == Form::chunk ? 512 : 768;
     const int64_t keys = window > 0 ? std::min(span, window + sinks + p.R + 2 * kQ4Tile) : span, units = (keys + 31) / 32;
-    p.tiles = (rows + p.R - 1) / p.R;
+    p.tiles = form == Form::few && seqs > 1 ? rows : (rows + p.R - 1) / p.R;  // (rows of several sequences are mostly alone)
     p.most = std::max<int64_t>(1, units / 8);
     const int64_t each = p.tiles * Hkv;
     p.nsplit = int(std::max<int64_t>(1, form != Form::chunk ? std::min(p.groups / each, p.most)
                                                             : std::max(std::min(256 / each, p.most), Dh == 128 ? std::min(p.groups / each, units / 64) : 0)));
     return p;
 }
-// rows that belong to sequences of their own have no keys in common
+// rows that belong to sequences of their own have no keys in common; few rows are short runs, however they stand
 Form attn4_form(bool row_seq, int64_t rows, int64_t group) { return !row_seq || rows == 1 ? Form::token : rows * group <= 16 ? Form::few : Form::chunk; }
 
 }  // namespace
@@ -1086,7 +997,7 @@ Form attn4_form(bool row_seq, int64_t rows, int64_t group) { return !row_seq || 
 int64_t attn4_work_bytes(int64_t rows, int64_t Hq, int64_t Hkv, int64_t Dh, int64_t span, int64_t window, int64_t sinks) {
     int64_t slots = 0;
     for (const Form form : {Form::token, Form::few, Form::chunk}) {
-        const Plan p = attn4_plan(form, rows, Hq / Hkv, Hkv, Dh, span, window, sinks);
+        const Plan p = attn4_plan(form, rows, 1, Hq / Hkv, Hkv, Dh, span, window, sinks);
         if (p.most > 1) slots = std::max(slots, std::min(p.groups, p.tiles * Hkv * p.most) * p.R * (Hq / Hkv));
     }
     return slots * (Dh + 4) * 4;
@@ -1094,16 +1005,23 @@ int64_t attn4_work_bytes(int64_t rows, int64_t Hq, int64_t Hkv, int64_t Dh, int6
 
 namespace {
 template <int DH>
-void attn4_sized(const Attn4Args& a, const Plan& p, hipStream_t s) {
-    const dim3 grid(unsigned(p.tiles * a.c.Hkv * p.nsplit));
-    if (p.form == Form::chunk)
-        hipLaunchKernelGGL(attn4_chunk_kernel<DH>, grid, dim3(256), 0, s, a, p.R, p.nsplit);
-    else if (p.form == Form::token)
-        hipLaunchKernelGGL((attn4_token_kernel<DH, 2>), grid, dim3(256), 0, s, a, p.nsplit);
-    else
-        hipLaunchKernelGGL(attn4_kernel<DH>, grid, dim3(256), 0, s, a, p.R, p.nsplit);
+void attn4_sized(const Attn4Args& a, hipStream_t s) {
+    const int64_t rows = a.c.rows, Hkv = a.c.Hkv, group = a.Hq / Hkv;
+    const Form form = attn4_form(a.c.row_seq, rows, group);
+    const Plan p = attn4_plan(form, rows, a.c.seqs, group, Hkv, DH, int64_t(a.c.max_pages) * a.c.page_size, a.window, a.sinks);
+    const bool runs = form == Form::few || (form == Form::chunk && a.c.seqs > 1);  // short ones, to be found
+    if (form == Form::token)
+        hipLaunchKernelGGL((attn4_short_kernel<DH, 2, true>), dim3(unsigned(rows * Hkv * p.nsplit)), dim3(256), 0, s, a, p.nsplit, 1);
+    if (runs) {
+        const int64_t stride = std::min(rows, std::max<int64_t>(1, 768 / (Hkv * p.nsplit)));
+        hipLaunchKernelGGL((attn4_short_kernel<DH, 2, false>), dim3(unsigned(stride * Hkv * p.nsplit)), dim3(256), 0, s, a, p.nsplit, int(stride));
+    }
+    if (form == Form::chunk) {
+        const int parts = runs ? 2 : 1;
+        hipLaunchKernelGGL(attn4_chunk_kernel<DH>, dim3(unsigned(p.tiles * Hkv * p.nsplit * parts)), dim3(256), 0, s, a, p.R, p.nsplit, parts);
+    }
     if (p.nsplit == 1) return;
-    const int64_t heads = int64_t(a.c.rows) * a.Hq;
+    const int64_t heads = rows * a.Hq;
     if (p.nsplit <= kFewRanges)
         hipLaunchKernelGGL(attn4_combine_few_kernel<DH>, dim3(unsigned((heads * (DH / 4) + 255) / 256)), dim3(256), 0, s, a, p.nsplit);
     else
@@ -1112,9 +1030,7 @@ void attn4_sized(const Attn4Args& a, const Plan& p, hipStream_t s) {
 }  // namespace
 
 void launch_attn4(const Attn4Args& a, hipStream_t s) {
-    const int64_t group = a.Hq / a.c.Hkv;
-    const Plan p = attn4_plan(attn4_form(a.c.row_seq, a.c.rows, group), a.c.rows, group, a.c.Hkv, a.c.Dh, int64_t(a.c.max_pages) * a.c.page_size, a.window, a.sinks);
-    a.c.Dh == 256 ? attn4_sized<256>(a, p, s) : attn4_sized<128>(a, p, s);
+    a.c.Dh == 256 ? attn4_sized<256>(a, s) : attn4_sized<128>(a, s);
 }
 
 }  // namespace hero

@@ -384,6 +384,42 @@ def test_long_rows_split_over_workgroups(lib, hq, hkv, dh, rows, first, window, 
     compare(*run_attend(lib, rng, c, hq, [0] * rows if row_seq else range(rows), pos, window, sinks, row_seq, work_more=64))
 
 
+@pytest.mark.parametrize("window,sinks", [(0, 0), (70, 5)])
+@pytest.mark.parametrize("hq,hkv,dh", [(32, 8, 128), (8, 1, 128), (4, 4, 128), (6, 2, 128), (16, 4, 256)])
+def test_runs_of_every_length_in_one_call(lib, hq, hkv, dh, window, sinks):
+    """Single tokens and runs of a few rows (drafts) of many sequences in any order, chunks that begin and end at any row
+    of a group of columns, padding between some of them, the same sequence twice."""
+    rng = np.random.default_rng(hq + window)
+    few = 16 // (hq // hkv)
+    c = Pool(rng, 30, 5, hkv, dh)
+    seq, pos = [], []
+    lengths = [1, 1, few, few + 1, 2, 40, 1, 37, few - 1, 1, 64, few + 2, 1, 1, 3, 61, few, few, 1]
+    for i, n in enumerate(lengths):
+        n = max(1, n)
+        s = int(rng.permutation(30)[0]) if i in (4, 9) else i
+        first = int(rng.integers(0, 320 - n))
+        seq += [s] * n
+        pos += list(range(first, first + n))
+        if i in (2, 7, 8):
+            seq, pos = seq + [s], pos + [-1]
+    compare(*run_attend(lib, rng, c, hq, seq, pos, window, sinks, work_more=64))
+    order = rng.permutation(30)[: 23]
+    compare(*run_attend(lib, rng, c, hq, order.tolist(), rng.integers(0, 320, 23).tolist(), window, sinks))
+    compare(*run_attend(lib, rng, c, hq, order[: few].tolist(), rng.integers(0, 320, few).tolist(), window, sinks))
+    compare(*run_attend(lib, rng, c, hq, [order[0]] * few, (np.arange(few) + 250).tolist(), window, sinks))
+
+
+@pytest.mark.parametrize("hq,hkv,dh,rows", [(8, 2, 128, 20), (4, 1, 256, 9), (8, 1, 128, 2), (4, 4, 128, 100)])
+def test_long_runs_and_single_tokens_split_over_workgroups(lib, hq, hkv, dh, rows):
+    """rows of several sequences with contexts of thousands: the ranges of both kinds of run are joined alike"""
+    rng = np.random.default_rng(rows)
+    c = Pool(rng, 3, 40, hkv, dh)
+    half = rows // 2
+    seq = [0] + [1] * (rows - half - 1) + [2] * half
+    pos = [2500] + list(range(1800, 1800 + rows - half - 1)) + list(range(2000, 2000 + half))
+    compare(*run_attend(lib, rng, c, hq, seq, pos, work_more=64))
+
+
 @pytest.mark.parametrize("row_seq", [False, True])
 def test_what_no_row_sees_has_no_influence(lib, row_seq):
     """Slots past the rows, whole pages behind them, pages before a window: NaN steps there change nothing.
