@@ -8,13 +8,19 @@
 // Keeping the largest out of R leaves the small differences that a nearly certain
 // token's log probability and entropy consist of; in a sum 1 + R they would drown.
 //
-// A row is cut into ranges, one for each wave: the running M, c, R and the
-// entropy's sum T lane by lane, and the range's best keys as a sorted list, one a lane. A
-// key is the logit in an order-preserving form, then the id's complement, so
-// that equal logits rank by ascending id and no two keys are equal. A second launch, a wave
-// per row, joins the ranges.
+// A row is cut into ranges, one for each wave: the running M, c, R and the entropy's sum T, and
+// for the alternatives nothing but the largest of every 64 logits. A second launch, a workgroup per row, joins the
+// ranges, takes the n-th largest of 256 groups of these maxima for a bar that n logits reach at least, and
+// reads the few blocks again whose largest reaches it. (Sorted lists that each wave keeps along the
+// way: one row of 151936 with twenty alternatives 16.2 us instead of 11.3, 1000 rows 219 instead of 116.)
+//
+// What bounds it: many rows, the memory: 1000 rows of 151936 at 5.7 TB/s in 106 us, and 9 us for the joins. Few rows, the
+// two launches: of one row's 11.3 us the first takes 4.1 (3.6 with one logit per lane), the second 6, each round
+// to memory and back about 1 us of it.
 #include "hero/device.hpp"
 #include "hero/kernels.hpp"
+
+#include <type_traits>
 
 namespace hero {
 
@@ -23,7 +29,7 @@ namespace {
 constexpr float kLog2eF = 1.4426950408889634f, kLn2F = 0.6931471805599453f, kLowestF = -3.402823466e38f;
 constexpr int kBatch = 16;  // logits a lane takes at a time
 
-struct RangeSum {  // what a range leaves behind, before its keys
+struct RangeSum {  // what a range leaves behind
     float m, c, r, t;
 };
 
@@ -35,49 +41,6 @@ __device__ __forceinline__ uint32_t order_of(float x) {
 __device__ __forceinline__ float logit_of(uint32_t order) {
     return order == 0u ? __uint_as_float(0x7FC00000u) : __uint_as_float(order & 0x80000000u ? order & 0x7FFFFFFFu : ~order);
 }
-__device__ __forceinline__ uint64_t key_of(float x, uint32_t id) { return uint64_t(order_of(x)) << 32 | (0xFFFFFFFFu - id); }
-
-__device__ __forceinline__ uint64_t lane_key(uint64_t v, int lane) {
-    return uint64_t(uint32_t(__builtin_amdgcn_readlane(int(v >> 32), lane))) << 32 | uint32_t(__builtin_amdgcn_readlane(int(v), lane));
-}
-__device__ __forceinline__ uint64_t lane_before(uint64_t v) {  // the value of lane - 1 (wave_shr:1)
-    return uint64_t(uint32_t(__builtin_amdgcn_update_dpp(0, int(v >> 32), 0x138, 0xF, 0xF, false))) << 32 |
-           uint32_t(__builtin_amdgcn_update_dpp(0, int(v), 0x138, 0xF, 0xF, false));
-}
-
-// The best keys so far, descending, one a lane; `least` the top-th of them (0: not that many yet)
-struct TopList {
-    uint64_t mine = 0, least = 0;
-    // up to kBatch keys a lane (0: none)
-    __device__ __forceinline__ void add(const uint64_t (&key)[kBatch], int top, int lane) {
-        uint64_t best = key[0];
-#pragma unroll
-        for (int j = 1; j < kBatch; ++j) best = key[j] > best ? key[j] : best;
-        uint64_t bar = least;
-        if (__popcll(__ballot(best > bar)) > top) {
-            // more lanes with a better key than there are places: the top-th largest of the
-            // lanes' best, to 24 bits, is a bar that the keys to take all reach
-            uint32_t at = 0;
-            const uint32_t hi = uint32_t(best >> 32);
-#pragma unroll
-            for (int bit = 31; bit >= 8; --bit)
-                if (__popcll(__ballot(hi >= (at | 1u << bit))) >= top) at |= 1u << bit;
-            const uint64_t from = uint64_t(at) << 32;
-            if (from > bar) bar = from - 1;
-        }
-#pragma unroll
-        for (int j = 0; j < kBatch; ++j) {
-            for (uint64_t hits = __ballot(key[j] > bar); hits; hits &= hits - 1) {
-                const uint64_t k = lane_key(key[j], __ffsll((unsigned long long)hits) - 1);
-                if (k <= least) continue;
-                const int place = __popcll(__ballot(mine > k));
-                const uint64_t before = lane_before(mine);
-                mine = lane < place ? mine : lane == place ? k : before;
-                least = lane_key(mine, top - 1);
-            }
-        }
-    }
-};
 
 // the larger of two running maxima takes the other's sums over
 __device__ __forceinline__ void join(RangeSum& a, const RangeSum& b, float k2) {
@@ -93,43 +56,102 @@ __device__ __forceinline__ void join(RangeSum& a, const RangeSum& b, float k2) {
     a.t = ta + tb;
 }
 
+// over the wave's lanes, in every lane
+template <class F>
+__device__ __forceinline__ float over_lanes(float v, F f) {
+    auto with = [](float x, auto ctrl) { return __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(x), decltype(ctrl)::value, 0xF, 0xF, true)); };
+    v = f(v, with(v, std::integral_constant<int, 0xB1>{}));   // quad_perm [1,0,3,2]
+    v = f(v, with(v, std::integral_constant<int, 0x4E>{}));   // quad_perm [2,3,0,1]
+    v = f(v, with(v, std::integral_constant<int, 0x141>{}));  // row_half_mirror
+    v = f(v, with(v, std::integral_constant<int, 0x140>{}));  // row_mirror
+    auto at = [&](int lane) { return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(v), lane)); };
+    return f(f(at(0), at(16)), f(at(32), at(48)));
+}
+__device__ __forceinline__ void join_lanes(RangeSum& s, float k2) {
+    const RangeSum all{over_lanes(s.m, [](float x, float y) { return fmaxf(x, y); }), 0.f, 0.f, 0.f};
+    join(s, all, k2);
+    auto sum = [](float x, float y) { return x + y; };
+    s = {all.m, over_lanes(s.c, sum), over_lanes(s.r, sum), over_lanes(s.t, sum)};
+}
+
+// Of every 64 kBatch logits sixteen blocks, one of each four lanes: sixteen neighbours of every 256.
+constexpr int kBlocks = 16, kKept = 64;  // blocks of a batch; batches whose blocks' maxima a wave keeps before it stores them
+__device__ __forceinline__ int block_id(int block, int k, int i) { return block / kBlocks * 64 * kBatch + 256 * k + 16 * (block % kBlocks) + i; }
 struct LogprobsWork {
-    RangeSum* sums;   // [m][ranges]
-    uint64_t* keys;   // [m][ranges][top]
+    RangeSum* sums;      // [m][ranges]
+    uint32_t* maxima;    // [m][blocks], as order_of
 };
 
-// a wave per range: whole batches of 64 kBatch logits
+// A wave per range: whole batches of 64 kBatch logits, one ahead. Lane l brings logits 4 l .. 4 l + 3 of each
+// 256; the row's last four stand in for ones past its end, and count once.
 template <bool TOP>
-__global__ __launch_bounds__(256) void logprobs_range_kernel(LogprobsArgs a, LogprobsWork w, int ranges, int per) {
+__global__ __launch_bounds__(256) void logprobs_range_kernel(LogprobsArgs a, LogprobsWork w, int ranges, int per, int blocks) {
+    constexpr int kStep = 64 * kBatch;
     const int lane = threadIdx.x & 63;
-    const int64_t item = int64_t(blockIdx.x) * 4 + (threadIdx.x >> 6);
+    const int64_t item = int64_t(blockIdx.x) * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     if (item >= a.m * ranges) return;
     const int64_t row = item / ranges;
-    if (a.targets && (a.targets[row] < 0 || a.targets[row] >= a.v)) return;
-    const int64_t first = (item % ranges) * per * int64_t(64 * kBatch), last = min(a.v, first + int64_t(per) * 64 * kBatch);
+    const int first = int(item % ranges) * per * kStep, last = int(min(a.v, int64_t(first) + int64_t(per) * kStep)), v_end = int(a.v);
     const float* x = a.logits + row * a.stride;
     const float k2 = kLog2eF / a.temp;
     RangeSum s{kLowestF, 0.f, 0.f, 0.f};
-    TopList list;
-    for (int64_t at = first; at < last; at += 64 * kBatch) {
+    float ahead[kBatch];
+    // Stores would hold up the wait for the loads behind them: 1000 rows of 151936 take 103 us without the maxima, 118 with a store for each
+    // batch or each four.
+    __shared__ uint32_t kept[TOP ? 4 : 1][TOP ? kKept * kBlocks : 4];
+    uint32_t* maxima = kept[TOP ? threadIdx.x >> 6 : 0];
+    auto store = [&](int batch, int n) {  // n batches, from the range's batch on
+        uint32_t* to = w.maxima + row * blocks + (first / kStep + batch) * kBlocks;
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        for (int i = 4 * lane; i < n * kBlocks; i += 256) __builtin_memcpy(to + i, maxima + i, 16);
+    };
+#pragma unroll 1
+    for (int at = first - kStep; at < last; at += kStep) {
         float v[kBatch];
-        const int64_t mine = at + 4 * lane;
-        if (at + 64 * kBatch <= last) {
 #pragma unroll
-            for (int k = 0; k < kBatch / 4; ++k) __builtin_memcpy(v + 4 * k, x + mine + 256 * k, 16);
-        } else {
+        for (int j = 0; j < kBatch; ++j) v[j] = ahead[j];
+        if (const int next = at + kStep; next < last) {
+            if (v_end >= 4) {
+#pragma unroll
+                for (int k = 0; k < kBatch / 4; ++k) __builtin_memcpy(ahead + 4 * k, x + min(next + 4 * lane + 256 * k, v_end - 4), 16);
+            } else {
+#pragma unroll
+                for (int j = 0; j < 4; ++j) ahead[j] = x[min(j, v_end - 1)];
+            }
+        }
+        if (at < first) {  // the first batch is on its way
+            if (a.targets && (a.targets[row] < 0 || a.targets[row] >= a.v)) return;
+            continue;
+        }
+        const float missing = TOP ? __uint_as_float(0x7FC00000u) : -INFINITY;  // (NaN: below -inf among the maxima)
+        bool partial = false;
+        if (at + kStep > last) {
+            partial = true;
 #pragma unroll
             for (int j = 0; j < kBatch; ++j) {
-                const int64_t i = mine + 256 * (j / 4) + j % 4;
-                v[j] = x[min(i, a.v - 1)];
-                if (i >= last) v[j] = -INFINITY;
+                const int from = at + 4 * lane + 256 * (j / 4), i = v_end >= 4 ? min(from, v_end - 4) + j % 4 : j < 4 ? from + j : last;
+                if (i < from || i >= last) v[j] = missing;
             }
         }
         float best = v[0];
 #pragma unroll
         for (int j = 1; j < kBatch; ++j) best = fmaxf(best, v[j]);
-        if (best > s.m) {
-            RangeSum next{best, 0.f, 0.f, 0.f};
+        if constexpr (TOP) {
+            auto with = [](float x, auto ctrl) { return fmaxf(x, __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(x), decltype(ctrl)::value, 0xF, 0xF, true))); };
+            const float four = with(with(best, std::integral_constant<int, 0xB1>{}), std::integral_constant<int, 0x4E>{});
+            const int batch = (at - first) / kStep;
+            maxima[batch % kKept * kBlocks + lane / 4] = order_of(four);
+            if (batch % kKept == kKept - 1) store(batch - (kKept - 1), kKept);
+            if (partial) {
+#pragma unroll
+                for (int j = 0; j < kBatch; ++j) {
+                    const int from = at + 4 * lane + 256 * (j / 4), i = v_end >= 4 ? min(from, v_end - 4) + j % 4 : j < 4 ? from + j : last;
+                    if (i < from || i >= last) v[j] = -INFINITY;
+                }
+            }
+        }
+        if (__ballot(best > s.m)) {  // one maximum for the wave: one of 64 would change in most batches
+            const RangeSum next{over_lanes(best, [](float x, float y) { return fmaxf(x, y); }), 0.f, 0.f, 0.f};
             join(s, next, k2);
         }
 #pragma unroll
@@ -141,91 +163,197 @@ __global__ __launch_bounds__(256) void logprobs_range_kernel(LogprobsArgs a, Log
             s.r += e;
             s.t += e * fmaxf(d, -200.f);
         }
-        if constexpr (TOP) {
-            if (list.least == 0 || __ballot(best >= logit_of(uint32_t(list.least >> 32)))) {
-                uint64_t key[kBatch];
-#pragma unroll
-                for (int j = 0; j < kBatch; ++j) {
-                    const int64_t i = mine + 256 * (j / 4) + j % 4;
-                    key[j] = i < last ? key_of(v[j], uint32_t(i)) : 0;
-                }
-                list.add(key, a.top, lane);
-            }
-        }
     }
-    for (int off = 32; off > 0; off >>= 1) {
-        const RangeSum o{__shfl_xor(s.m, off), __shfl_xor(s.c, off), __shfl_xor(s.r, off), __shfl_xor(s.t, off)};
-        join(s, o, k2);
+    if constexpr (TOP) {
+        const int batches = (last - first + kStep - 1) / kStep;
+        store(batches - batches % kKept, batches % kKept);
     }
+    join_lanes(s, k2);
     if (lane == 0) w.sums[item] = s;
-    if (TOP && lane < a.top) w.keys[item * a.top + lane] = list.mine;
 }
 
-// a wave per row
-__global__ __launch_bounds__(64) void logprobs_join_kernel(LogprobsArgs a, LogprobsWork w, int ranges) {
+// A workgroup per row. The last wave joins the sums; the others look for the alternatives.
+constexpr int kJoinThreads = 512, kGathered = 4096, kListed = 256;
+__global__ __launch_bounds__(kJoinThreads) void logprobs_join_kernel(LogprobsArgs a, LogprobsWork w, int ranges, int blocks) {
     const int64_t row = blockIdx.x;
-    const int lane = threadIdx.x;
+    const int t = threadIdx.x, lane = t & 63, wave = t >> 6, v_end = int(a.v);
     const int target = a.targets ? a.targets[row] : 0;
     if (target < 0 || target >= a.v) return;
+    __shared__ uint64_t gathered[kGathered];
+    __shared__ uint32_t groups[kJoinThreads], listed[kListed], bar, count, keys;
+    __shared__ float of_row[2];  // the largest logit and the logarithm of the sum
     const float* x = a.logits + row * a.stride;
     const float own = a.logprob ? x[target] : 0.f, k2 = kLog2eF / a.temp;
-    RangeSum s{kLowestF, 0.f, 0.f, 0.f};
-    for (int i = lane; i < ranges; i += 64) join(s, w.sums[row * ranges + i], k2);
-    for (int off = 32; off > 0; off >>= 1) {
-        const RangeSum o{__shfl_xor(s.m, off), __shfl_xor(s.c, off), __shfl_xor(s.r, off), __shfl_xor(s.t, off)};
-        join(s, o, k2);
+    const uint32_t* maxima = w.maxima + row * blocks;
+    const bool last = wave == kJoinThreads / 64 - 1;
+    auto maximum = [&](int i) { return i < blocks ? maxima[i] : 0u; };
+    uint32_t held[8];
+    if (a.top) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) held[j] = maximum(t + j * kJoinThreads);
+        uint32_t most = 0;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) most = max(most, held[j]);
+        for (int i = t + 8 * kJoinThreads; i < blocks; i += kJoinThreads) most = max(most, maxima[i]);
+        groups[t] = most;
     }
-    if (s.m == INFINITY) s.r = __uint_as_float(0x7FC00000u);
-    const float log_sum = logf(s.c) + log1pf(s.r / s.c);
-    if (lane == 0) {
-        if (a.logprob) a.logprob[row] = (own - s.m) / a.temp - log_sum;
-        if (a.entropy) a.entropy[row] = log_sum - kLn2F * s.t / (s.c + s.r);
+    if (t == 0) count = 0, keys = 0;
+    __syncthreads();
+    if (last) {
+        RangeSum s{kLowestF, 0.f, 0.f, 0.f};
+        for (int i = lane; i < ranges; i += 64) join(s, w.sums[row * ranges + i], k2);
+        join_lanes(s, k2);
+        if (s.m == INFINITY) s.r = __uint_as_float(0x7FC00000u);
+        const float log_sum = logf(s.c) + log1pf(s.r / s.c);
+        if (lane == 0) {
+            of_row[0] = s.m, of_row[1] = log_sum;
+            if (a.logprob) a.logprob[row] = (own - s.m) / a.temp - log_sum;
+            if (a.entropy) a.entropy[row] = log_sum - kLn2F * s.t / (s.c + s.r);
+        }
     }
     if (a.top == 0) return;
-    TopList list;
-    const int n = ranges * a.top;
-    for (int at = 0; at < n; at += 64 * kBatch) {
-        uint64_t key[kBatch];
+    // The smallest of the largest of 256 groups' maxima, top of them and those that share 20 bits with the last
+    // (0 where fewer hold anything).
+    if (wave == 0) {
+        uint32_t of[4], found = 0;
 #pragma unroll
-        for (int j = 0; j < kBatch; ++j) {
-            const int i = at + 64 * j + lane;
-            key[j] = i < n ? w.keys[row * n + i] : 0;
+        for (int j = 0; j < 4; ++j) of[j] = max(groups[lane + 64 * j], groups[lane + 64 * j + 256]);
+#pragma unroll
+        for (int bit = 31; bit >= 12; --bit) {
+            int n = 0;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) n += __popcll(__ballot(of[j] >= (found | 1u << bit)));
+            if (n >= a.top) found |= 1u << bit;
         }
-        list.add(key, a.top, lane);
+        uint32_t least = ~0u;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) least = min(least, of[j] >= found ? of[j] : ~0u);
+        for (int off = 32; off > 0; off >>= 1) least = min(least, uint32_t(__shfl_xor(int(least), off)));
+        if (lane == 0) bar = least;
     }
-    if (lane < a.top) {
-        a.top_ids[row * a.top + lane] = int32_t(0xFFFFFFFFu - uint32_t(list.mine));
-        a.top_logprobs[row * a.top + lane] = (logit_of(uint32_t(list.mine >> 32)) - s.m) / a.temp - log_sum;
+    __syncthreads();
+    auto list = [&](uint32_t m, int i) {
+        if (i < blocks && m >= bar)
+            if (const uint32_t at = atomicAdd(&count, 1u); at < kListed) listed[at] = i;
+    };
+#pragma unroll
+    for (int j = 0; j < 8; ++j) list(held[j], t + j * kJoinThreads);
+    for (int i = t + 8 * kJoinThreads; i < blocks; i += kJoinThreads) list(maxima[i], i);
+    __syncthreads();
+    // Blocks that reach the bar, each by sixteen lanes: their logits that do. (The order of the keys differs from run to
+    // run, their places do not: no two are equal.) Where too many tie at the bar, only those above it; where
+    // these are too many, those above the exact bar, which are fewer than top.
+    const bool few = count <= kListed;
+    const int candidates = few ? int(count) : blocks;
+    auto each = [&](auto f) {
+        for (int i = t / 16; i < candidates; i += kJoinThreads / 16) {
+            const int block = few ? int(listed[i]) : i;
+            if (maxima[block] < bar) continue;
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+                if (const int id = block_id(block, j, t & 15); id < v_end) f(order_of(x[id]), id);
+        }
+    };
+    bool above = !few;
+#pragma unroll 1
+    for (bool exact = false;;) {
+        each([&](uint32_t order, int id) {
+            if (order >= bar && !(above && order == bar))
+                if (const uint32_t at = atomicAdd(&keys, 1u); at < kGathered) gathered[at] = uint64_t(order) << 32 | (0xFFFFFFFFu - uint32_t(id));
+        });
+        __syncthreads();
+        if (keys <= kGathered || exact) break;
+        uint32_t known = 0, left = a.top;  // the bar's upper bytes; how many of the logits that share them it is
+        if (above) {
+            exact = true;
+#pragma unroll 1
+            for (int shift = 24; shift >= 0; shift -= 8) {
+                __syncthreads();
+                if (t < 256) groups[t] = 0;
+                __syncthreads();
+                each([&](uint32_t order, int) {
+                    if (order >= bar && uint64_t(order) >> (shift + 8) == uint64_t(known) >> (shift + 8)) atomicAdd(&groups[order >> shift & 255], 1u);
+                });
+                __syncthreads();
+                int byte = 255;
+                for (; byte > 0 && groups[byte] < left; --byte) left -= groups[byte];
+                known |= uint32_t(byte) << shift;
+            }
+        }
+        above = true;
+        __syncthreads();
+        if (t == 0) {
+            keys = 0;
+            if (exact) bar = known;
+        }
+        __syncthreads();
+    }
+    if (above && keys < uint32_t(a.top)) {
+        // the lowest ids among the equal ones
+        __syncthreads();
+        if (wave == 0) {
+            uint32_t have = keys;
+            for (int i = 0; i < blocks && have < uint32_t(a.top); i += 64) {
+                const uint64_t reach = __ballot(i + lane < blocks && maxima[min(i + lane, blocks - 1)] >= bar);
+                for (int j = 0; j < 64; ++j) {  // 64 ids of a batch, in their order
+                    const int id = (i / kBlocks * kBatch + j) * 64 + lane;
+                    if ((reach >> (j / kBatch * kBlocks) & ((1u << kBlocks) - 1)) == 0 || have >= uint32_t(a.top)) continue;
+                    const uint64_t equal = __ballot(id < v_end && order_of(x[min(id, v_end - 1)]) == bar);
+                    const uint32_t at = have + __builtin_amdgcn_mbcnt_hi(uint32_t(equal >> 32), __builtin_amdgcn_mbcnt_lo(uint32_t(equal), 0));
+                    if ((equal >> lane & 1) && at < uint32_t(a.top)) gathered[at] = uint64_t(bar) << 32 | (0xFFFFFFFFu - uint32_t(id));
+                    have += __popcll(equal);
+                }
+            }
+            if (lane == 0) keys = min(have, uint32_t(a.top));
+        }
+        __syncthreads();
+    }
+    const int found = int(keys);
+    for (int i = t; i < found; i += kJoinThreads) {
+        const uint64_t k = gathered[i];
+        int place = 0;
+#pragma unroll 4
+        for (int j = 0; j < found; ++j) place += gathered[j] > k;
+        if (place >= a.top) continue;
+        a.top_ids[row * a.top + place] = int32_t(0xFFFFFFFFu - uint32_t(k));
+        a.top_logprobs[row * a.top + place] = (logit_of(uint32_t(k >> 32)) - of_row[0]) / a.temp - of_row[1];
     }
 }
 
-// Ranges of a row: about 2048 waves over all rows, at least one batch each.
+// Ranges of a row: about 2048 waves over all rows, at least one batch each (4096 and 8192 waves: 16 rows of 262144 and 1000
+// rows of 151936 take 2 to 6 % longer).
+constexpr int64_t kWaves = 2048;
 void logprobs_plan(int64_t m, int64_t v, int* ranges, int* per) {
-    const int64_t batches = (v + 64 * kBatch - 1) / (64 * kBatch), want = std::max<int64_t>(1, std::min(batches, 4096 / m));
+    const int64_t batches = (v + 64 * kBatch - 1) / (64 * kBatch), want = std::max<int64_t>(1, std::min(batches, kWaves / m));
     *per = int((batches + want - 1) / want);
     *ranges = int((batches + *per - 1) / *per);
 }
 
 }  // namespace
 
+namespace {
+int64_t blocks_of(int64_t v) { return (v + 64 * kBatch - 1) / (64 * kBatch) * kBlocks; }
+}  // namespace
+
 int64_t logprobs_work_bytes(int64_t m, int64_t v, int top) {
-    // m ranges(m) is at most 4096 or m
-    const int64_t batches = (v + 64 * kBatch - 1) / (64 * kBatch), parts = std::max(m, std::min<int64_t>(4096, m * batches));
-    return parts * int64_t(sizeof(RangeSum) + 8 * top);
+    // m ranges(m) is at most kWaves or m
+    const int64_t batches = (v + 64 * kBatch - 1) / (64 * kBatch), parts = std::max(m, std::min(kWaves, m * batches));
+    return parts * int64_t(sizeof(RangeSum)) + (top ? m * blocks_of(v) * 4 : 0);
 }
 
 void launch_logprobs(const LogprobsArgs& a, hipStream_t s) {
     int ranges, per;
     logprobs_plan(a.m, a.v, &ranges, &per);
+    const int blocks = int(blocks_of(a.v));
     LogprobsWork w;
     w.sums = static_cast<RangeSum*>(a.work);
-    w.keys = reinterpret_cast<uint64_t*>(w.sums + a.m * ranges);
+    w.maxima = reinterpret_cast<uint32_t*>(w.sums + a.m * ranges);
     const dim3 grid(unsigned((a.m * ranges + 3) / 4));
     if (a.top)
-        hipLaunchKernelGGL(logprobs_range_kernel<true>, grid, dim3(256), 0, s, a, w, ranges, per);
+        hipLaunchKernelGGL(logprobs_range_kernel<true>, grid, dim3(256), 0, s, a, w, ranges, per, blocks);
     else
-        hipLaunchKernelGGL(logprobs_range_kernel<false>, grid, dim3(256), 0, s, a, w, ranges, per);
-    hipLaunchKernelGGL(logprobs_join_kernel, dim3(unsigned(a.m)), dim3(64), 0, s, a, w, ranges);
+        hipLaunchKernelGGL(logprobs_range_kernel<false>, grid, dim3(256), 0, s, a, w, ranges, per, blocks);
+    hipLaunchKernelGGL(logprobs_join_kernel, dim3(unsigned(a.m)), dim3(kJoinThreads), 0, s, a, w, ranges, blocks);
 }
 
 }  // namespace hero

@@ -103,6 +103,39 @@ def test_orders_that_fill_the_lists_again_and_again(lib, order):
     compare(run(lib, x, t, 1.0, 64), x, t, 1.0, 64)
 
 
+@pytest.mark.parametrize("case", ["equal", "two values", "together", "together, ties", "every 16384", "NaN but ten"])
+@pytest.mark.parametrize("v", [8192, 60000])
+def test_many_logits_among_the_largest(lib, case, v):
+    rng = np.random.default_rng(v)
+    x = (rng.standard_normal((3, v)) * 2).astype(np.float32)
+    if case == "equal":
+        x[:] = 1.25
+    elif case == "two values":
+        x[:] = np.where(rng.random((3, v)) < 0.5, 3, -1)
+    elif case.startswith("together"):  # a few thousand neighbours far above all others
+        x[:, 1000:6500] += 100
+        if case.endswith("ties"):
+            x[:, 1000:6500] = np.round(x[:, 1000:6500] / 4) * 4
+    elif case == "every 16384":
+        x[:, np.arange(v) % 16384 < 2000] += 40
+    else:
+        x[:] = np.nan
+        x[:, 7:7 + 64 * 90:64 * 9] = np.arange(10, dtype=np.float32)
+    t = [5, 1001, 7]
+    got = run(lib, x, t, 1.0, 64)
+    if case == "NaN but ten":
+        for r in range(3):
+            assert got["top_ids"][r].tolist() == [7 + 576 * i for i in range(9, -1, -1)] + [i for i in range(55) if i != 7][:54]
+    else:
+        compare(got, x, t, 1.0, 64)
+
+
+def test_ranges_of_many_batches(lib):
+    rng = np.random.default_rng(1)
+    x = (rng.standard_normal((2, 3000017)) * 3).astype(np.float32)
+    compare(run(lib, x, [0, 3000016], 1.0, 20), x, [0, 3000016], 1.0, 20)
+
+
 def test_zeros_of_both_signs_tie(lib):
     x = np.full((1, 5000), -1, np.float32)
     x[0, [4000, 17, 900, 3]] = [0.0, -0.0, 0.0, -0.0]
