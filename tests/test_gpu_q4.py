@@ -201,6 +201,22 @@ def test_append_of_thousands_of_rows(lib):
     run_append(lib, rng, c, 1, [0] * 1200 + [1] * 900, list(range(63, 1263)) + list(range(900)), rope=1300)
 
 
+@pytest.mark.parametrize("hq,hkv,dh", [(9, 3, 128), (5, 5, 256), (48, 6, 128)])
+def test_append_of_many_heads(lib, hq, hkv, dh):
+    rng = np.random.default_rng(hq)
+    rows = 25000 // (hq + 2 * hkv) + 5
+    c = Pool(rng, 3, -(-rows // 64) + 1, hkv, dh)
+    c.table[1, 0] = -1
+    rows -= rows % 3  # (every row a place of its own)
+    seq, pos = np.arange(rows) * 3 // rows, np.arange(rows) % (rows // 3) + 10
+    pos[rng.integers(0, rows, 20)] = -1
+    kw, stride = hkv * dh, 2 * hq * dh + 2 * hkv * dh + 5
+    proj = rng.standard_normal((rows, stride)).astype(np.float32)
+    proj[::7, -2 * kw:] = np.round(proj[::7, -2 * kw:] * 4)  # ties and blocks of equal magnitudes
+    proj[3, -kw - 5 + 9], proj[5, -kw - 5 + 3], proj[6, 2 * hq * dh + 1] = np.nan, np.inf, 1e30
+    run_append(lib, rng, c, hq, seq, pos, proj=proj, stride_more=5, rope_pos=rng.integers(0, 200, (2, rows)), plane_axis=rng.integers(0, 2, dh // 2).tolist())
+
+
 def test_append_blocks_at_borders(lib):
     """Values: blocks of zeros, subnormal steps, exact ties, equal magnitudes of both signs, the
     largest that the format holds, infinities and NaN. Keys: a weight of 0, a row of zeros, non-finite rows."""
