@@ -13,13 +13,20 @@ namespace {
 typedef float f4_t __attribute__((ext_vector_type(4)));
 typedef float f2_t __attribute__((ext_vector_type(2)));
 
-constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kLog2e = 1.4426950408889634f, kLog2eLow = 1.92596303e-8f, kLn2 = 0.6931471805599453f;  // (log2(e) - float(log2(e)))
 constexpr float kPOne = 8192.f;  // a weight's terms are of 2^13 2^(s - m); its part in the total is 2^(s - m)
 constexpr float kPSlack = 2.f;   // m may lag the maximum by this: weights stay below 2^15
 constexpr float kLowest = -3.402823466e38f;
 
 __device__ __forceinline__ float column_other(float x) {  // the value of column c ^ 8
     return __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(x), 0x128, 0xF, 0xF, true));  // row_ror:8
+}
+__device__ __forceinline__ int max_of_wave(int x) {
+    x = max(x, __builtin_amdgcn_update_dpp(0, x, 0xB1, 0xF, 0xF, true));   // quad_perm [1,0,3,2]
+    x = max(x, __builtin_amdgcn_update_dpp(0, x, 0x4E, 0xF, 0xF, true));   // quad_perm [2,3,0,1]
+    x = max(x, __builtin_amdgcn_update_dpp(0, x, 0x141, 0xF, 0xF, true));  // row_half_mirror
+    x = max(x, __builtin_amdgcn_update_dpp(0, x, 0x140, 0xF, 0xF, true));  // row_mirror
+    return max(max(__builtin_amdgcn_readlane(x, 0), __builtin_amdgcn_readlane(x, 16)), max(__builtin_amdgcn_readlane(x, 32), __builtin_amdgcn_readlane(x, 48)));
 }
 __device__ __forceinline__ float max_over_p(float x) {
     x = fmaxf(x, __shfl_xor(x, 16));
@@ -29,9 +36,20 @@ __device__ __forceinline__ float sum_over_p(float x) {
     x += __shfl_xor(x, 16);
     return x + __shfl_xor(x, 32);
 }
-// (the cache's values are 4-bit: nothing here has to replay a reference's rounding, as exp_f32 does)
-__device__ __forceinline__ float gate_of(float x) { return 1.f / (1.f + expf(-x)); }
+__device__ __forceinline__ float max_of_8(float x) {  // neighbouring lanes
+    x = fmaxf(x, __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(x), 0xB1, 0xF, 0xF, true)));          // quad_perm [1,0,3,2]
+    x = fmaxf(x, __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(x), 0x4E, 0xF, 0xF, true)));          // quad_perm [2,3,0,1]
+    return fmaxf(x, __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(x), 0x141, 0xF, 0xF, true)));      // row_half_mirror
+}
 __device__ __forceinline__ float exp2_hw(float x) { return __builtin_amdgcn_exp2f(x); }  // 1 ulp; 0 below its range
+// 1 / (1 + exp(-x)), 4 ulp: x log2(e) as the product's rounding and what it left; beyond +-200 as there, 1 or 0. (The
+// cache's values are 4-bit: nothing here has to replay a reference's rounding, as exp_f32 does.)
+__device__ __forceinline__ float gate_of(float x) {
+    const float at = -__builtin_amdgcn_fmed3f(x, -200.f, 200.f), t = at * kLog2e;
+    const float rest = __builtin_fmaf(at, kLog2eLow, __builtin_fmaf(at, kLog2e, -t));
+    const float gate = __builtin_amdgcn_rcpf(1.f + exp2_hw(t) * __builtin_fmaf(rest, kLn2, 1.f));
+    return x == x ? gate : x;
+}
 
 // x as two fp16 terms; pinned first, so that both are formed from one rounding of it
 __device__ __forceinline__ void split_f16(float x, _Float16& hi, _Float16& lo) {
@@ -108,9 +126,23 @@ __device__ __forceinline__ void store_out(const Attn4Args& a, int r, int h, int 
         for (int off = 16; off > 0; off >>= 1) amax = fmaxf(amax, __shfl_xor(amax, off));
         const float d = amax / 127.f, id = d != 0.f ? 1.f / d : 0.f;
         int8_t* qs = static_cast<int8_t*>(a.act_out);
-        qs[idx] = int8_t(int(roundf(out * id)));
+        qs[idx] = int8_t(round_code(out * id));
         if ((ch & 31) == 0) reinterpret_cast<float*>(qs + int64_t(a.c.rows) * width)[idx >> 5] = half_bits_to_f32(fp32_to_fp16_ref(d));
     }
+}
+
+// Four neighbouring channels, by neighbouring lanes: channel `at` of the outputs and the next.
+__device__ __forceinline__ void store_four(const Attn4Args& a, int64_t at, f4_t v) {
+    if (a.out_f32) *reinterpret_cast<f4_t*>(a.out_f32 + at) = v;
+    if (!a.act_out) return;
+    const float amax = max_of_8(fmaxf(fmaxf(fabsf(v[0]), fabsf(v[1])), fmaxf(fabsf(v[2]), fabsf(v[3]))));
+    const float d = amax / 127.f, id = d != 0.f ? 1.f / d : 0.f;
+    uint32_t codes = 0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) codes |= uint32_t(round_code(v[i] * id) & 0xFF) << (8 * i);
+    int8_t* qs = static_cast<int8_t*>(a.act_out);
+    *reinterpret_cast<uint32_t*>(qs + at) = codes;
+    if (at % 32 == 0) reinterpret_cast<float*>(qs + int64_t(a.c.rows) * a.Hq * a.c.Dh)[at >> 5] = half_bits_to_f32(fp32_to_fp16_ref(d));
 }
 
 // a row's keys: those below `stay`, and from `first` (>= stay) to `pos`
@@ -455,13 +487,23 @@ __global__ __launch_bounds__(256, DH == 128 ? 2 : 1) void attn4_chunk_kernel(Att
     const uint32_t rec_bytes = 9 * DH, head_bytes = uint32_t(tpp) * rec_bytes, half = head_bytes * c.Hkv;
     const FieldMasks masks;
     const uint8_t* const pool = reinterpret_cast<const uint8_t*>(c.pages);
-    __shared__ uint4 ops_k[2][NS][64];     // operands, a lane's 16 bytes each
-    __shared__ uint2 ops_v[2][NB][2][64][2];
-    __shared__ struct {
-        uint4 codes[2][2][H][64];    // keys, values; record; as they lie
-        uint8_t steps[2][2][DH];
-    } raw[kRing];
-    __shared__ Listed list[kListed];
+    struct Units {
+        uint4 ops_k[2][NS][64];      // operands, a lane's 16 bytes each
+        uint2 ops_v[2][NB][2][64][2];
+        struct {
+            uint4 codes[2][2][H][64];  // keys, values; record; as they lie
+            uint8_t steps[2][2][DH];
+        } raw[kRing];
+        Listed list[kListed];
+    };
+    __shared__ union {
+        Units units;
+        float out[4][32][DH + 4];    // a wave's columns
+    } sh;
+    auto& ops_k = sh.units.ops_k;
+    auto& ops_v = sh.units.ops_v;
+    auto& raw = sh.units.raw;
+    auto& list = sh.units.list;
 
     // the workgroup's rows, two a lane
     int row_pos[2], row_of[2];
@@ -470,6 +512,14 @@ __global__ __launch_bounds__(256, DH == 128 ? 2 : 1) void attn4_chunk_kernel(Att
         const int i = lane + 64 * k;
         row_pos[k] = i < R && r0 + i < c.rows ? row_position(c, r0 + i, &row_of[k]) : -1;
     }
+    int near_pos[3] = {}, near_seq[3] = {};  // of rows r0 - 16 + lane + 64 k
+    if (parts > 1)
+#pragma unroll
+        for (int k = 0; k < 3; ++k) {
+            const int r = r0 - 16 + lane + 64 * k, at = min(max(r, 0), c.rows - 1);
+            const int at_pos = row_position(c, at, &near_seq[k]);
+            near_pos[k] = r == at ? at_pos : -1;
+        }
     // the lane's column, and its query in units of log2, two terms; a power of two brings the head's largest channel below 2^14
     const int col = wave * 32 + (lane & 31), i_row = min(min(col / group, R - 1), c.rows - 1 - r0);
     const int row = col < R * group && r0 + col / group < c.rows ? i_row : -1, head = g * group + col % group;
@@ -507,14 +557,12 @@ __global__ __launch_bounds__(256, DH == 128 ? 2 : 1) void attn4_chunk_kernel(Att
         // it; `most` such bits in a row are a run of more rows than that, and it holds all of them.
         const int most = 16 / group;
         uint64_t on[3], all_on[3], bits[3], in[3];
+        int s_last = -1;  // (of row r0 - 17: no window reaches back to it)
 #pragma unroll
         for (int k = 0; k < 3; ++k) {
-            const int64_t r = int64_t(r0) - 16 + lane + 64 * k;
-            int s0 = 0, s1 = 0;
-            const bool ok = r >= 1 && r < c.rows;
-            const int at = ok ? int(r) : min(1, c.rows - 1);
-            const int p0 = row_position(c, max(at - 1, 0), &s0), p1 = row_position(c, at, &s1);
-            on[k] = all_on[k] = bits[k] = __ballot(ok && p0 >= 0 && p1 >= 0 && s0 == s1);
+            const int s = near_pos[k] >= 0 ? near_seq[k] : -1, before = __builtin_amdgcn_update_dpp(s_last, s, 0x138, 0xF, 0xF, false);  // wave_shr:1
+            on[k] = all_on[k] = bits[k] = __ballot(s >= 0 && s == before);
+            s_last = __builtin_amdgcn_readlane(s, 63);
         }
         auto down = [](uint64_t (&v)[3]) { v[0] = v[0] >> 1 | v[1] << 63, v[1] = v[1] >> 1 | v[2] << 63, v[2] >>= 1; };
         auto up = [](uint64_t (&v)[3]) { v[2] = v[2] << 1 | v[1] >> 63, v[1] = v[1] << 1 | v[0] >> 63, v[0] <<= 1; };
@@ -552,6 +600,13 @@ __global__ __launch_bounds__(256, DH == 128 ? 2 : 1) void attn4_chunk_kernel(Att
 #pragma unroll
     for (int n = 0; n < NB; ++n) o[n] = zero;
 
+    // shared memory alone: loads stay in flight across it
+    auto barrier = [] {
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+        __builtin_amdgcn_s_barrier();
+        asm volatile("" ::: "memory");
+    };
+
     // The rows of one sequence at a time: mostly there is one. Where a second sequence begins among a workgroup's rows
     // another workgroup (part 1) takes what is not the first's.
     for (int run = 0; (valid[0] | valid[1]) && (parts == 1 || part == 1 || run == 0); ++run) {
@@ -568,8 +623,7 @@ __global__ __launch_bounds__(256, DH == 128 ? 2 : 1) void attn4_chunk_kernel(Att
             if (in) lo = min(lo, row_pos[k]), hi = max(hi, row_pos[k]);
         }
         if (part == 1 && run == 0) continue;
-        for (int off = 32; off > 0; off >>= 1) lo = min(lo, __shfl_xor(lo, off)), hi = max(hi, __shfl_xor(hi, off));
-        lo = __builtin_amdgcn_readfirstlane(lo), hi = __builtin_amdgcn_readfirstlane(hi);
+        lo = -max_of_wave(-lo), hi = max_of_wave(hi);
         // (columns of rows that this workgroup does not store may hold anything: none of them touches another)
         const bool whole = (mine[0] == all[0] && mine[1] == all[1]) || (parts > 1 && (part == 0 || (run == 1 && !(valid[0] | valid[1]))));
         const bool here = row >= 0 && ((row < 64 ? mine[0] : mine[1]) >> (row & 63) & 1);
@@ -671,13 +725,6 @@ __global__ __launch_bounds__(256, DH == 128 ? 2 : 1) void attn4_chunk_kernel(Att
         };
         auto operand_k = [&](int at, int k) __attribute__((always_inline)) { return __builtin_bit_cast(q4_h8, ops_k[at][k][lane]); };
         auto operand_v = [&](int at, int n, int x) __attribute__((always_inline)) { return *reinterpret_cast<const q4_h8*>(&ops_v[at][n][x][lane][0]); };
-        // shared memory alone: loads stay in flight across it
-        auto barrier = [] {
-            asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-            __builtin_amdgcn_s_barrier();
-            asm volatile("" ::: "memory");
-        };
-
         barrier();  // the last run's list and operands are done with
         look_up(u0);
         barrier();
@@ -822,53 +869,55 @@ __global__ __launch_bounds__(256, DH == 128 ? 2 : 1) void attn4_chunk_kernel(Att
         }
     }
 
-    // register 4 y + i of block n: channel 32 n + 8 y + 4 f + i of the column
+    // Results by way of shared memory: register 4 y + i of block n is channel 32 n + 8 y + 4 f + i of the column, and then
+    // a lane takes four neighbouring channels of one column (or, of 128, of every other) after another. Stores of whole
+    // rows, and a short loop where the columns' own order unrolls to 24 KB of instructions that every call fetches anew.
     const float total = l + __shfl_xor(l, 32);
-    if (row < 0 || !((row < 64 ? done[0] : done[1]) >> (row & 63) & 1)) return;  // (both lanes of a column)
-    const int r = r0 + row;
-    if (nsplit > 1) {
-        float* rec = a.work + ((int64_t(r) * a.Hq + head) * nsplit + split) * (DH + 4);
-        if (f == 0) rec[0] = m2, rec[1] = total;
+    const int mine = row >= 0 && ((row < 64 ? done[0] : done[1]) >> (row & 63) & 1) ? r0 + row : -1;
+    wait_vmcnt<0>();
+    barrier();
 #pragma unroll
-        for (int n = 0; n < NB; ++n)
+    for (int n = 0; n < NB; ++n)
 #pragma unroll
-            for (int y = 0; y < 4; ++y)
-                *reinterpret_cast<f4_t*>(rec + 4 + 32 * n + 8 * y + 4 * f) = f4_t{o[n][4 * y], o[n][4 * y + 1], o[n][4 * y + 2], o[n][4 * y + 3]} * (1.f / kPOne);
-        return;
-    }
-    const int64_t width = int64_t(a.Hq) * DH, at = int64_t(r) * width + int64_t(head) * DH + 4 * f;
-    const float* gates = a.proj + int64_t(r) * a.proj_stride + int64_t(head) * 2 * DH + DH + 4 * f;
-    const float share = total == 0.f ? 0.f : 1.f / (total * kPOne);
+        for (int y = 0; y < 4; ++y)
+            *reinterpret_cast<f4_t*>(&sh.out[wave][lane & 31][32 * n + 8 * y + 4 * f]) = f4_t{o[n][4 * y], o[n][4 * y + 1], o[n][4 * y + 2], o[n][4 * y + 3]};
+    wave_exchange();
+    const float share = nsplit > 1 ? 1.f / kPOne : total == 0.f ? 0.f : 1.f / (total * kPOne);
+    const int ch = 4 * lane % DH;
+    constexpr int kAtOnce = 8, kColumns = 256 / DH;
+#pragma unroll 1
+    for (int k = 0; k < 32; k += kAtOnce * kColumns) {
+        f4_t gate[kAtOnce];
+        if (nsplit == 1)  // a round's loads together: one by one they were half of the time of a short call
 #pragma unroll
-    for (int n = 0; n < NB; ++n) {
-        float v[16], amax = 0.f;
-#pragma unroll
-        for (int i = 0; i < 16; ++i) {
-            v[i] = total == 0.f ? 0.f : o[n][i] * share * gate_of(gates[32 * n + 8 * (i / 4) + i % 4]);
-            amax = fmaxf(amax, fabsf(v[i]));
-        }
-        if (a.out_f32)
-#pragma unroll
-            for (int y = 0; y < 4; ++y) *reinterpret_cast<f4_t*>(a.out_f32 + at + 32 * n + 8 * y) = f4_t{v[4 * y], v[4 * y + 1], v[4 * y + 2], v[4 * y + 3]};
-        if (a.act_out) {
-            amax = fmaxf(amax, __shfl_xor(amax, 32));
-            const float d = amax / 127.f, id = d != 0.f ? 1.f / d : 0.f;
-            int8_t* qs = static_cast<int8_t*>(a.act_out);
-#pragma unroll
-            for (int y = 0; y < 4; ++y) {
-                uint32_t codes = 0;
-#pragma unroll
-                for (int i = 0; i < 4; ++i) codes |= uint32_t(int(roundf(v[4 * y + i] * id)) & 0xFF) << (8 * i);
-                *reinterpret_cast<uint32_t*>(qs + at + 32 * n + 8 * y) = codes;
+            for (int j = 0; j < kAtOnce; ++j) {
+                const int at_col = k + j * kColumns + 4 * lane / DH, to = max(__shfl(mine, at_col), r0), h = g * group + (wave * 32 + at_col) % group;
+                __builtin_memcpy(&gate[j], a.proj + int64_t(to) * a.proj_stride + int64_t(h) * 2 * DH + DH + ch, 16);
             }
-            if (f == 0) reinterpret_cast<float*>(qs + int64_t(c.rows) * width)[(at >> 5) + n] = half_bits_to_f32(fp32_to_fp16_ref(d));
+#pragma unroll
+        for (int j = 0; j < kAtOnce; ++j) {
+            const int at_col = k + j * kColumns + 4 * lane / DH, to = __shfl(mine, at_col), h = g * group + (wave * 32 + at_col) % group;
+            const float of = __shfl(share, at_col);
+            f4_t v = *reinterpret_cast<const f4_t*>(&sh.out[wave][at_col][ch]) * of;
+            if (nsplit > 1) {
+                const float at_m = __shfl(m2, at_col), at_total = __shfl(total, at_col);
+                if (to >= 0) {
+                    float* rec = a.work + ((int64_t(to) * a.Hq + h) * nsplit + split) * (DH + 4);
+                    if (ch == 0) rec[0] = at_m, rec[1] = at_total;
+                    *reinterpret_cast<f4_t*>(rec + 4 + ch) = v;
+                }
+                continue;
+            }
+#pragma unroll
+            for (int i = 0; i < 4; ++i) v[i] = of == 0.f ? 0.f : v[i] * gate_of(gate[j][i]);
+            if (to >= 0) store_four(a, (int64_t(to) * a.Hq + h) * DH + ch, v);
         }
     }
 }
 
 // Few ranges: DH / 4 lanes for a (row, query head), four channels each
 constexpr int kFewRanges = 8;
-template <int DH>
+template <int DH, int N>
 __global__ __launch_bounds__(256) void attn4_combine_few_kernel(Attn4Args a, int nsplit) {
     constexpr int LN = DH / 4, kRec = DH + 4;
     const int64_t item = int64_t(blockIdx.x) * (256 / LN) + threadIdx.x / LN;
@@ -878,10 +927,10 @@ __global__ __launch_bounds__(256) void attn4_combine_few_kernel(Attn4Args a, int
     int seq;
     if (row_position(a.c, r, &seq) < 0) return;
     const float* rec = a.work + item * nsplit * kRec;
-    f4_t v[kFewRanges];
-    float m[kFewRanges], l[kFewRanges], mx = kLowest;
+    f4_t v[N];
+    float m[N], l[N], mx = kLowest;
 #pragma unroll
-    for (int s = 0; s < kFewRanges; ++s) {
+    for (int s = 0; s < N; ++s) {
         const float* at = rec + min(s, nsplit - 1) * kRec;
         m[s] = at[0], l[s] = at[1];
         v[s] = *reinterpret_cast<const f4_t*>(at + 4 + ch);
@@ -890,33 +939,18 @@ __global__ __launch_bounds__(256) void attn4_combine_few_kernel(Attn4Args a, int
     float gate[4];
     __builtin_memcpy(gate, gates, 16);
 #pragma unroll
-    for (int s = 0; s < kFewRanges; ++s) mx = fmaxf(mx, m[s]);
+    for (int s = 0; s < N; ++s) mx = fmaxf(mx, m[s]);
     float total = 0.f;
     f4_t o = f4_t{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-    for (int s = 0; s < kFewRanges; ++s) {
+    for (int s = 0; s < N; ++s) {
         const float f = s < nsplit ? exp2_hw(m[s] - mx) : 0.f;
         total += f * l[s];
         o += s < nsplit ? f * v[s] : f4_t{0.f, 0.f, 0.f, 0.f};
     }
-    const int64_t width = int64_t(a.Hq) * DH, at = int64_t(r) * width + int64_t(h) * DH + ch;
-    float amax = 0.f;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        o[i] = total == 0.f ? 0.f : o[i] / total * gate_of(gate[i]);
-        amax = fmaxf(amax, fabsf(o[i]));
-    }
-    if (a.out_f32) *reinterpret_cast<f4_t*>(a.out_f32 + at) = o;
-    if (a.act_out) {
-        for (int off = 1; off < 8; off <<= 1) amax = fmaxf(amax, __shfl_xor(amax, off));
-        const float d = amax / 127.f, id = d != 0.f ? 1.f / d : 0.f;
-        int8_t* qs = static_cast<int8_t*>(a.act_out);
-        uint32_t codes = 0;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) codes |= uint32_t(int(roundf(o[i] * id)) & 0xFF) << (8 * i);
-        *reinterpret_cast<uint32_t*>(qs + at) = codes;
-        if (ch % 32 == 0) reinterpret_cast<float*>(qs + int64_t(a.c.rows) * width)[at >> 5] = half_bits_to_f32(fp32_to_fp16_ref(d));
-    }
+    for (int i = 0; i < 4; ++i) o[i] = total == 0.f ? 0.f : o[i] / total * gate_of(gate[i]);
+    store_four(a, (int64_t(r) * a.Hq + h) * DH + ch, o);
 }
 
 // A workgroup per (row, query head): DH / 4 lanes for four channels each read a range's result, and
@@ -1022,8 +1056,11 @@ void attn4_sized(const Attn4Args& a, hipStream_t s) {
     }
     if (p.nsplit == 1) return;
     const int64_t heads = rows * a.Hq;
-    if (p.nsplit <= kFewRanges)
-        hipLaunchKernelGGL(attn4_combine_few_kernel<DH>, dim3(unsigned((heads * (DH / 4) + 255) / 256)), dim3(256), 0, s, a, p.nsplit);
+    const dim3 few(unsigned((heads * (DH / 4) + 255) / 256));
+    if (p.nsplit <= kFewRanges / 2)
+        hipLaunchKernelGGL((attn4_combine_few_kernel<DH, kFewRanges / 2>), few, dim3(256), 0, s, a, p.nsplit);
+    else if (p.nsplit <= kFewRanges)
+        hipLaunchKernelGGL((attn4_combine_few_kernel<DH, kFewRanges>), few, dim3(256), 0, s, a, p.nsplit);
     else
         hipLaunchKernelGGL(attn4_combine_kernel<DH>, dim3(unsigned(heads)), dim3(256), size_t(p.nsplit + 31) / 32 * 128, s, a, p.nsplit);
 }
