@@ -1,6 +1,28 @@
 // attn4.hip -- gated attention over the 4-bit pages of the paged K/V cache: single
 // tokens of many sequences and chunks of prompts, with or without a sliding window
 // behind which the first tokens stay visible.
+//
+// For a (row, query head) pair over the keys j that the row sees, in one pass with a running maximum m:
+//   s_j = scale log2(e) q . k_j,   o = sum 2^(s_j - m) v_j,   l = sum 2^(s_j - m),   out = o / l * sigmoid(gate).
+// A cached value is an fp16 number (a code times its block's step, exact), so both sums are products for the matrix
+// instructions. What they multiply it with is split into two fp16 terms of 22 bits together, queries as well
+// as weights, and each product is taken once for each term: results are those of fp32, at twice the products.
+// Scores and sums are held in fp32; m lags the true maximum by up to kPSlack, which saves most rescalings.
+//
+// Three forms. One row of a sequence: the two terms fill the 16 columns of one product with up to 8
+// query heads; what counts is the read of the cache (attn4_short_kernel<PAIR>). Chunks: 128 columns of a
+// workgroup, 128 / group rows, share the work of turning records into operands, and the products bound it
+// (attn4_chunk_kernel). Few rows, and runs of a few rows among chunks: a short kernel without PAIR, as the columns'
+// other halves would be idle in a chunk's workgroup. Keys are split into ranges where there are few
+// workgroups, and combined by a second launch.
+//
+// Measured, 32 query and 8 K/V heads of 128, in pages of 64: sixteen tokens of 32000 keys each 123 us, 4.9 TB/s of cache in
+// the first launch (a copy of gigabytes: 5.1); the same over windows of 4096 26 us; one token of 32000 keys 19.8 us, of which
+// about 3 are spent before the first records arrive, 2 after the last ones and 4 on the second launch, and 6 keep the vector units
+// busy with turning codes into operands; one token of 300 keys 8.8 us, latencies and instruction fetches. 500 rows
+// over 16000 keys 260 us, 1.05 PFLOP/s of products (fp16 matrix products of 8192^3 reach 1.17); 1000 rows of three
+// sequences over windows of 1024 80 us: 250 workgroups of 34 units each, 44 us for these, and about 20 from start to first and from
+// last product to end.
 #include "hero/device.hpp"
 #include "hero/kernels.hpp"
 #include "hero/paged.hpp"
@@ -218,238 +240,238 @@ __global__ __launch_bounds__(256, DH == 128 && PAIR ? 3 : 2) void attn4_short_ke
     const FieldMasks masks;
 
     auto attend = [&](const int r, const int rows) __attribute__((always_inline)) {
-    const int mine = PAIR ? 0 : min(col / group, rows - 1);  // the column's row
-    float x[NS][8];
-    {
-        const float* src = a.q_rot + (int64_t(r + mine) * a.Hq + g * group + (PAIR ? min(col, group - 1) : col % group)) * DH + 8 * p;
+        const int mine = PAIR ? 0 : min(col / group, rows - 1);  // the column's row
+        float x[NS][8];
+        {
+            const float* src = a.q_rot + (int64_t(r + mine) * a.Hq + g * group + (PAIR ? min(col, group - 1) : col % group)) * DH + 8 * p;
 #pragma unroll
-        for (int s = 0; s < NS; ++s) __builtin_memcpy(x[s], __builtin_assume_aligned(src + 32 * s, 16), 32);
-    }
-    int seq;
-    const int pos0 = row_position(c, r, &seq);
-    if (pos0 < 0) return;
-    // the run's first and last position
-    int pos = pos0, lo = pos0, hi = pos0;
-    if constexpr (!PAIR) {
-        int s;
-        pos = row_position(c, r + mine, &s);
-        lo = hi = pos;
-        for (int off = 1; off < 16; off <<= 1) lo = min(lo, __shfl_xor(lo, off)), hi = max(hi, __shfl_xor(hi, off));
-        lo = __builtin_amdgcn_readfirstlane(lo), hi = __builtin_amdgcn_readfirstlane(hi);
-    }
-    const Seen sees = row_sees(a, pos), most = row_sees(a, hi), least = row_sees(a, lo);
-    // records: those of the first keys that stay, then from the earliest window's first key on
-    const int first = least.first / kQ4Tile, stay = min((most.stay + kQ4Tile - 1) / kQ4Tile, first), last = hi / kQ4Tile;
-    const int tiles = stay + last - first + 1, units = (tiles + 1) / 2;
-    const int u0 = int(uint32_t(units) * uint32_t(split) / uint32_t(nsplit)), u1 = int(uint32_t(units) * uint32_t(split + 1) / uint32_t(nsplit));  // (units at most 2^19, ranges 768)
-    // read as constant memory: through the scalar cache, apart from the counted vector loads
-    const auto* table = (const __attribute__((address_space(4))) int32_t*)(c.page_table) + int64_t(seq) * c.max_pages;
-    const uint32_t magic = (0x80000000u + tpp - 1) / tpp;  // x / tpp = x magic >> 31 for x < 2^23
-
-    struct Place {
-        int t;          // record of the sequence
-        bool there;
-        uint64_t krec;  // offset of the keys' record in the pool
-    };
-    const uint32_t rec_bytes = 9 * DH, head_bytes = uint32_t(tpp) * rec_bytes, half = head_bytes * c.Hkv;
-    auto locate = [&](int k) {
-        Place w;
-        const int kk = min(k, tiles - 1);
-        w.t = kk < stay ? kk : first + kk - stay;
-        const int lp = int(uint64_t(w.t) * magic >> 31), id = __builtin_amdgcn_readfirstlane(table[lp]);
-        w.there = k < tiles && id >= 0 && id < c.pool_pages;
-        w.krec = uint64_t(w.there ? uint32_t(id) : 0u) * (2 * half) + uint32_t(g * head_bytes + (w.t - lp * tpp) * rec_bytes);
-        return w;
-    };
-    Ring<DH, D>& ring = sh.ring[wave];
-    auto fetch = [&](int at, const Place (&w)[2]) {
-#pragma unroll
-        for (int x = 0; x < 2; ++x) {
-            const uint8_t* krec = reinterpret_cast<const uint8_t*>(c.pages) + w[x].krec;
-            ring_fetch<DH, D>(ring.slot[at], x, krec, krec + half, lane);
+            for (int s = 0; s < NS; ++s) __builtin_memcpy(x[s], __builtin_assume_aligned(src + 32 * s, 16), 32);
         }
-    };
+        int seq;
+        const int pos0 = row_position(c, r, &seq);
+        if (pos0 < 0) return;
+        // the run's first and last position
+        int pos = pos0, lo = pos0, hi = pos0;
+        if constexpr (!PAIR) {
+            int s;
+            pos = row_position(c, r + mine, &s);
+            lo = hi = pos;
+            for (int off = 1; off < 16; off <<= 1) lo = min(lo, __shfl_xor(lo, off)), hi = max(hi, __shfl_xor(hi, off));
+            lo = __builtin_amdgcn_readfirstlane(lo), hi = __builtin_amdgcn_readfirstlane(hi);
+        }
+        const Seen sees = row_sees(a, pos), most = row_sees(a, hi), least = row_sees(a, lo);
+        // records: those of the first keys that stay, then from the earliest window's first key on
+        const int first = least.first / kQ4Tile, stay = min((most.stay + kQ4Tile - 1) / kQ4Tile, first), last = hi / kQ4Tile;
+        const int tiles = stay + last - first + 1, units = (tiles + 1) / 2;
+        const int u0 = int(uint32_t(units) * uint32_t(split) / uint32_t(nsplit)), u1 = int(uint32_t(units) * uint32_t(split + 1) / uint32_t(nsplit));  // (units at most 2^19, ranges 768)
+        // read as constant memory: through the scalar cache, apart from the counted vector loads
+        const auto* table = (const __attribute__((address_space(4))) int32_t*)(c.page_table) + int64_t(seq) * c.max_pages;
+        const uint32_t magic = (0x80000000u + tpp - 1) / tpp;  // x / tpp = x magic >> 31 for x < 2^23
 
-    const int n = max(0, (u1 - u0 - wave + 3) / 4);  // the wave's units u0 + wave, + 4, ...
-    Place ahead[D][2];
+        struct Place {
+            int t;          // record of the sequence
+            bool there;
+            uint64_t krec;  // offset of the keys' record in the pool
+        };
+        const uint32_t rec_bytes = 9 * DH, head_bytes = uint32_t(tpp) * rec_bytes, half = head_bytes * c.Hkv;
+        auto locate = [&](int k) {
+            Place w;
+            const int kk = min(k, tiles - 1);
+            w.t = kk < stay ? kk : first + kk - stay;
+            const int lp = int(uint64_t(w.t) * magic >> 31), id = __builtin_amdgcn_readfirstlane(table[lp]);
+            w.there = k < tiles && id >= 0 && id < c.pool_pages;
+            w.krec = uint64_t(w.there ? uint32_t(id) : 0u) * (2 * half) + uint32_t(g * head_bytes + (w.t - lp * tpp) * rec_bytes);
+            return w;
+        };
+        Ring<DH, D>& ring = sh.ring[wave];
+        auto fetch = [&](int at, const Place (&w)[2]) {
 #pragma unroll
-    for (int d = 0; d < D; ++d) {
+            for (int x = 0; x < 2; ++x) {
+                const uint8_t* krec = reinterpret_cast<const uint8_t*>(c.pages) + w[x].krec;
+                ring_fetch<DH, D>(ring.slot[at], x, krec, krec + half, lane);
+            }
+        };
+
+        const int n = max(0, (u1 - u0 - wave + 3) / 4);  // the wave's units u0 + wave, + 4, ...
+        Place ahead[D][2];
 #pragma unroll
-        for (int x = 0; x < 2; ++x) ahead[d][x] = locate(2 * (u0 + wave + 4 * d) + x);
-    }
-    // The queries are in by now, for they wait for nothing; from here on the compiler, which does not see the records' loads, has
-    // none of its own to wait for, and the queries turn into operands while the records are on their way.
+        for (int d = 0; d < D; ++d) {
 #pragma unroll
-    for (int s = 0; s < NS; ++s)
-#pragma unroll
-        for (int j = 0; j < 8; ++j) asm volatile("" : "+v"(x[s][j]));
-#pragma unroll
-    for (int d = 0; d < D; ++d)
-        if (d < n) fetch(d, ahead[d]);
-    // the queries in units of log2, a power of two brings the head's largest channel below 2^14
-    q4_h8 q[NS], q2[PAIR ? 1 : NS];
-    float unit;
-    {
-        float amax = 0.f;
-        const float k = a.score_scale * kLog2e;
+            for (int x = 0; x < 2; ++x) ahead[d][x] = locate(2 * (u0 + wave + 4 * d) + x);
+        }
+        // The queries are in by now, for they wait for nothing; from here on the compiler, which does not see the records' loads, has
+        // none of its own to wait for, and the queries turn into operands while the records are on their way.
 #pragma unroll
         for (int s = 0; s < NS; ++s)
 #pragma unroll
-            for (int j = 0; j < 8; ++j) amax = fmaxf(amax, fabsf(x[s][j] *= k));
-        amax = max_over_p(amax);
-        const int e = amax > 0.f && amax < INFINITY ? min(max(ilogbf(amax) + 1, -100), 117) : 0;
+            for (int j = 0; j < 8; ++j) asm volatile("" : "+v"(x[s][j]));
 #pragma unroll
-        for (int s = 0; s < NS; ++s)
+        for (int d = 0; d < D; ++d)
+            if (d < n) fetch(d, ahead[d]);
+        // the queries in units of log2, a power of two brings the head's largest channel below 2^14
+        q4_h8 q[NS], q2[PAIR ? 1 : NS];
+        float unit;
+        {
+            float amax = 0.f;
+            const float k = a.score_scale * kLog2e;
 #pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                _Float16 hi, lo;
-                split_f16(ldexpf(x[s][j], 14 - e), hi, lo);
-                q[s][j] = PAIR && b >= 8 ? lo : hi;
-                if constexpr (!PAIR) q2[s][j] = lo;
-            }
-        unit = ldexpf(1.f, e - 14);
-    }
-    const float slack = kPSlack / unit;
-
-    f4_t o[NV];
+            for (int s = 0; s < NS; ++s)
 #pragma unroll
-    for (int y = 0; y < NV; ++y) o[y] = f4_t{0.f, 0.f, 0.f, 0.f};
-    float m = kLowest, m2 = kLowest, l = 0.f;  // m in units of the products, m2 = m unit
-
-    // (One copy of the body: a wave has few units, and those of a call's first ones are spent on fetching instructions.)
-    int at = 0;  // unit i's slot
-#pragma unroll 1
-    for (int i = 0; i < n; ++i) {
-        const Place w[2] = {ahead[0][0], ahead[0][1]};
-        const typename Ring<DH, D>::Slot& in = ring.slot[at];
-        // the unit's loads are in when at most the ones behind it are outstanding
-        if (i + D - 1 < n)
-            wait_vmcnt<(D - 1) * Ring<DH, D>::kLoads>();
-        else
-            wait_vmcnt<0>();
-        asm volatile("" ::: "memory");
-
-        float s[8];
+                for (int j = 0; j < 8; ++j) amax = fmaxf(amax, fabsf(x[s][j] *= k));
+            amax = max_over_p(amax);
+            const int e = amax > 0.f && amax < INFINITY ? min(max(ilogbf(amax) + 1, -100), 117) : 0;
 #pragma unroll
-        for (int x = 0; x < 2; ++x) {
-            _Float16 kd[NS];
-            __builtin_memcpy(kd, __builtin_assume_aligned(in.steps[x].k + b * 2 * NS, 8), sizeof(kd));
-            f4_t sum = f4_t{0.f, 0.f, 0.f, 0.f};
+            for (int s = 0; s < NS; ++s)
 #pragma unroll
-            for (int k = 0; k < NS; ++k) {
-                const uint4 w4 = in.k[x][k / 4][4 * b + (p ^ b >> 2)];
-                const uint32_t word = k % 4 == 0 ? w4.x : k % 4 == 1 ? w4.y : k % 4 == 2 ? w4.z : w4.w;
-                const q4_h2 d = {kd[k], kd[k]};
-                const q4_h8 f = join(masks.codes<0>(word) * d, masks.codes<1>(word) * d, masks.codes<0>(word >> 8) * d, masks.codes<1>(word >> 8) * d);
-                sum = __builtin_amdgcn_mfma_f32_16x16x32_f16(f, q[k], sum, 0, 0, 0);
-                if constexpr (!PAIR) sum = __builtin_amdgcn_mfma_f32_16x16x32_f16(f, q2[k], sum, 0, 0, 0);
-            }
-#pragma unroll
-            for (int j = 0; j < 4; ++j) s[4 * x + j] = PAIR ? sum[j] + column_other(sum[j]) : sum[j];
-        }
-        uint4 v[2][H];
-        q4_h2 vd[2][NV];
-#pragma unroll
-        for (int x = 0; x < 2; ++x) {
-#pragma unroll
-            for (int h = 0; h < H; ++h) v[x][h] = in.v[x][h][lane];
-            __builtin_memcpy(vd[x], __builtin_assume_aligned(in.steps[x].v + p * 4 * NV, 16), sizeof(vd[x]));
-        }
-#pragma unroll
-        for (int x = 0; x < 2; ++x) {
-            const int k0 = kQ4Tile * w[x].t;
-            if (!w[x].there || k0 + 15 > lo || (k0 < most.first && k0 + 15 >= least.stay)) {  // some row does not see all of it
-                bool none[4];
-#pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    const int key = k0 + 4 * p + j;
-                    none[j] = !w[x].there || key > hi;
-                    if (none[j] || key > pos || (key < sees.first && key >= sees.stay)) s[4 * x + j] = -INFINITY;
+                for (int j = 0; j < 8; ++j) {
+                    _Float16 hi, lo;
+                    split_f16(ldexpf(x[s][j], 14 - e), hi, lo);
+                    q[s][j] = PAIR && b >= 8 ? lo : hi;
+                    if constexpr (!PAIR) q2[s][j] = lo;
                 }
-                // slots past the last row may hold anything: their steps count as 0
-#pragma unroll
-                for (int y = 0; y < NV; ++y)
-#pragma unroll
-                    for (int j = 0; j < 2; ++j)
-                        if (none[2 * (y & 1) + j]) vd[x][y][j] = _Float16(0.f);
-            }
+            unit = ldexpf(1.f, e - 14);
         }
-        // what the slot held is in registers: the next unit's loads may land there
-        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-#pragma unroll
-        for (int d = 0; d + 1 < D; ++d) ahead[d][0] = ahead[d + 1][0], ahead[d][1] = ahead[d + 1][1];
-        if (i + D < n) {
-#pragma unroll
-            for (int x = 0; x < 2; ++x) ahead[D - 1][x] = locate(2 * (u0 + wave + 4 * (i + D)) + x);
-            fetch(at, ahead[D - 1]);
-        }
-        at = at + 1 == D ? 0 : at + 1;
-        float best = s[0];
-#pragma unroll
-        for (int j = 1; j < 8; ++j) best = fmaxf(best, s[j]);
-        if (__ballot(best > m + slack)) {
-            const float to = fmaxf(m, max_over_p(best)), to2 = to == kLowest ? kLowest : to * unit, f = exp2_hw(m2 - to2);
-            m = to, m2 = to2;
-            l *= f;
-#pragma unroll
-            for (int y = 0; y < NV; ++y) o[y] *= f;
-        }
-        // Two weights at a time, as two terms of one value (the scaling is exact). Conversions in pairs and
-        // remainders in fp32: instructions that round to one half of a register (fma_mixlo) take twice as
-        // long. Pinned, or the compiler makes those of them.
-        q4_h8 w8, w8l;
-#pragma unroll
-        for (int j = 0; j < 8; j += 2) {
-            const float e0 = exp2_hw(__builtin_fmaf(s[j], unit, -m2)), e1 = exp2_hw(__builtin_fmaf(s[j + 1], unit, -m2));
-            l += e0;
-            l += e1;
-            const q4_h2 h2 = __builtin_convertvector((f2_t{e0 * kPOne, e1 * kPOne}), q4_h2);
-            float d0 = __builtin_fmaf(e0, kPOne, -float(h2[0])), d1 = __builtin_fmaf(e1, kPOne, -float(h2[1]));
-            asm volatile("" : "+v"(d0), "+v"(d1));
-            const q4_h2 l2 = __builtin_convertvector((f2_t{d0, d1}), q4_h2);
-            if constexpr (PAIR) {
-                const q4_h2 t = b < 8 ? h2 : l2;
-                w8[j] = t[0], w8[j + 1] = t[1];
-            } else {
-                w8[j] = h2[0], w8[j + 1] = h2[1], w8l[j] = l2[0], w8l[j + 1] = l2[1];
-            }
-        }
-#pragma unroll
-        for (int h = 0; h < H; ++h)
-#pragma unroll
-            for (int y = 0; y < 4; ++y) {  // byte y of the words: channels 128 h + 32 y + b and + 16
-                // 16-bit halves: that byte of two neighbouring keys
-                const uint32_t pick = 0x0C040C00u + 0x00010001u * y;
-                const uint32_t w0 = __builtin_amdgcn_perm(v[0][h].y, v[0][h].x, pick), w1 = __builtin_amdgcn_perm(v[0][h].w, v[0][h].z, pick);
-                const uint32_t w2 = __builtin_amdgcn_perm(v[1][h].y, v[1][h].x, pick), w3 = __builtin_amdgcn_perm(v[1][h].w, v[1][h].z, pick);
-                const q4_h2 d0 = vd[0][2 * (4 * h + y)], d1 = vd[0][2 * (4 * h + y) + 1];
-                const q4_h2 d2 = vd[1][2 * (4 * h + y)], d3 = vd[1][2 * (4 * h + y) + 1];
-                f4_t& oa = o[8 * h + 2 * y];
-                f4_t& ob = o[8 * h + 2 * y + 1];
-                const q4_h8 fa = join(masks.codes<0>(w0) * d0, masks.codes<0>(w1) * d1, masks.codes<0>(w2) * d2, masks.codes<0>(w3) * d3);
-                const q4_h8 fb = join(masks.codes<1>(w0) * d0, masks.codes<1>(w1) * d1, masks.codes<1>(w2) * d2, masks.codes<1>(w3) * d3);
-                oa = __builtin_amdgcn_mfma_f32_16x16x32_f16(fa, w8, oa, 0, 0, 0);
-                if constexpr (!PAIR) oa = __builtin_amdgcn_mfma_f32_16x16x32_f16(fa, w8l, oa, 0, 0, 0);
-                ob = __builtin_amdgcn_mfma_f32_16x16x32_f16(fb, w8, ob, 0, 0, 0);
-                if constexpr (!PAIR) ob = __builtin_amdgcn_mfma_f32_16x16x32_f16(fb, w8l, ob, 0, 0, 0);
-            }
-    }
-    __syncthreads();
+        const float slack = kPSlack / unit;
 
-    // the four waves' results
-    l = sum_over_p(l);
+        f4_t o[NV];
 #pragma unroll
-    for (int y = 0; y < NV; ++y) {
-        f4_t v = o[y];
-        if constexpr (PAIR) {
+        for (int y = 0; y < NV; ++y) o[y] = f4_t{0.f, 0.f, 0.f, 0.f};
+        float m = kLowest, m2 = kLowest, l = 0.f;  // m in units of the products, m2 = m unit
+
+        // (One copy of the body: a wave has few units, and those of a call's first ones are spent on fetching instructions.)
+        int at = 0;  // unit i's slot
+#pragma unroll 1
+        for (int i = 0; i < n; ++i) {
+            const Place w[2] = {ahead[0][0], ahead[0][1]};
+            const typename Ring<DH, D>::Slot& in = ring.slot[at];
+            // the unit's loads are in when at most the ones behind it are outstanding
+            if (i + D - 1 < n)
+                wait_vmcnt<(D - 1) * Ring<DH, D>::kLoads>();
+            else
+                wait_vmcnt<0>();
+            asm volatile("" ::: "memory");
+
+            float s[8];
 #pragma unroll
-            for (int i = 0; i < 4; ++i) v[i] += column_other(v[i]);
+            for (int x = 0; x < 2; ++x) {
+                _Float16 kd[NS];
+                __builtin_memcpy(kd, __builtin_assume_aligned(in.steps[x].k + b * 2 * NS, 8), sizeof(kd));
+                f4_t sum = f4_t{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                for (int k = 0; k < NS; ++k) {
+                    const uint4 w4 = in.k[x][k / 4][4 * b + (p ^ b >> 2)];
+                    const uint32_t word = k % 4 == 0 ? w4.x : k % 4 == 1 ? w4.y : k % 4 == 2 ? w4.z : w4.w;
+                    const q4_h2 d = {kd[k], kd[k]};
+                    const q4_h8 f = join(masks.codes<0>(word) * d, masks.codes<1>(word) * d, masks.codes<0>(word >> 8) * d, masks.codes<1>(word >> 8) * d);
+                    sum = __builtin_amdgcn_mfma_f32_16x16x32_f16(f, q[k], sum, 0, 0, 0);
+                    if constexpr (!PAIR) sum = __builtin_amdgcn_mfma_f32_16x16x32_f16(f, q2[k], sum, 0, 0, 0);
+                }
+#pragma unroll
+                for (int j = 0; j < 4; ++j) s[4 * x + j] = PAIR ? sum[j] + column_other(sum[j]) : sum[j];
+            }
+            uint4 v[2][H];
+            q4_h2 vd[2][NV];
+#pragma unroll
+            for (int x = 0; x < 2; ++x) {
+#pragma unroll
+                for (int h = 0; h < H; ++h) v[x][h] = in.v[x][h][lane];
+                __builtin_memcpy(vd[x], __builtin_assume_aligned(in.steps[x].v + p * 4 * NV, 16), sizeof(vd[x]));
+            }
+#pragma unroll
+            for (int x = 0; x < 2; ++x) {
+                const int k0 = kQ4Tile * w[x].t;
+                if (!w[x].there || k0 + 15 > lo || (k0 < most.first && k0 + 15 >= least.stay)) {  // some row does not see all of it
+                    bool none[4];
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        const int key = k0 + 4 * p + j;
+                        none[j] = !w[x].there || key > hi;
+                        if (none[j] || key > pos || (key < sees.first && key >= sees.stay)) s[4 * x + j] = -INFINITY;
+                    }
+                    // slots past the last row may hold anything: their steps count as 0
+#pragma unroll
+                    for (int y = 0; y < NV; ++y)
+#pragma unroll
+                        for (int j = 0; j < 2; ++j)
+                            if (none[2 * (y & 1) + j]) vd[x][y][j] = _Float16(0.f);
+                }
+            }
+            // what the slot held is in registers: the next unit's loads may land there
+            asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+#pragma unroll
+            for (int d = 0; d + 1 < D; ++d) ahead[d][0] = ahead[d + 1][0], ahead[d][1] = ahead[d + 1][1];
+            if (i + D < n) {
+#pragma unroll
+                for (int x = 0; x < 2; ++x) ahead[D - 1][x] = locate(2 * (u0 + wave + 4 * (i + D)) + x);
+                fetch(at, ahead[D - 1]);
+            }
+            at = at + 1 == D ? 0 : at + 1;
+            float best = s[0];
+#pragma unroll
+            for (int j = 1; j < 8; ++j) best = fmaxf(best, s[j]);
+            if (__ballot(best > m + slack)) {
+                const float to = fmaxf(m, max_over_p(best)), to2 = to == kLowest ? kLowest : to * unit, f = exp2_hw(m2 - to2);
+                m = to, m2 = to2;
+                l *= f;
+#pragma unroll
+                for (int y = 0; y < NV; ++y) o[y] *= f;
+            }
+            // Two weights at a time, as two terms of one value (the scaling is exact). Conversions in pairs and
+            // remainders in fp32: instructions that round to one half of a register (fma_mixlo) take twice as
+            // long. Pinned, or the compiler makes those of them.
+            q4_h8 w8, w8l;
+#pragma unroll
+            for (int j = 0; j < 8; j += 2) {
+                const float e0 = exp2_hw(__builtin_fmaf(s[j], unit, -m2)), e1 = exp2_hw(__builtin_fmaf(s[j + 1], unit, -m2));
+                l += e0;
+                l += e1;
+                const q4_h2 h2 = __builtin_convertvector((f2_t{e0 * kPOne, e1 * kPOne}), q4_h2);
+                float d0 = __builtin_fmaf(e0, kPOne, -float(h2[0])), d1 = __builtin_fmaf(e1, kPOne, -float(h2[1]));
+                asm volatile("" : "+v"(d0), "+v"(d1));
+                const q4_h2 l2 = __builtin_convertvector((f2_t{d0, d1}), q4_h2);
+                if constexpr (PAIR) {
+                    const q4_h2 t = b < 8 ? h2 : l2;
+                    w8[j] = t[0], w8[j + 1] = t[1];
+                } else {
+                    w8[j] = h2[0], w8[j + 1] = h2[1], w8l[j] = l2[0], w8l[j + 1] = l2[1];
+                }
+            }
+#pragma unroll
+            for (int h = 0; h < H; ++h)
+#pragma unroll
+                for (int y = 0; y < 4; ++y) {  // byte y of the words: channels 128 h + 32 y + b and + 16
+                    // 16-bit halves: that byte of two neighbouring keys
+                    const uint32_t pick = 0x0C040C00u + 0x00010001u * y;
+                    const uint32_t w0 = __builtin_amdgcn_perm(v[0][h].y, v[0][h].x, pick), w1 = __builtin_amdgcn_perm(v[0][h].w, v[0][h].z, pick);
+                    const uint32_t w2 = __builtin_amdgcn_perm(v[1][h].y, v[1][h].x, pick), w3 = __builtin_amdgcn_perm(v[1][h].w, v[1][h].z, pick);
+                    const q4_h2 d0 = vd[0][2 * (4 * h + y)], d1 = vd[0][2 * (4 * h + y) + 1];
+                    const q4_h2 d2 = vd[1][2 * (4 * h + y)], d3 = vd[1][2 * (4 * h + y) + 1];
+                    f4_t& oa = o[8 * h + 2 * y];
+                    f4_t& ob = o[8 * h + 2 * y + 1];
+                    const q4_h8 fa = join(masks.codes<0>(w0) * d0, masks.codes<0>(w1) * d1, masks.codes<0>(w2) * d2, masks.codes<0>(w3) * d3);
+                    const q4_h8 fb = join(masks.codes<1>(w0) * d0, masks.codes<1>(w1) * d1, masks.codes<1>(w2) * d2, masks.codes<1>(w3) * d3);
+                    oa = __builtin_amdgcn_mfma_f32_16x16x32_f16(fa, w8, oa, 0, 0, 0);
+                    if constexpr (!PAIR) oa = __builtin_amdgcn_mfma_f32_16x16x32_f16(fa, w8l, oa, 0, 0, 0);
+                    ob = __builtin_amdgcn_mfma_f32_16x16x32_f16(fb, w8, ob, 0, 0, 0);
+                    if constexpr (!PAIR) ob = __builtin_amdgcn_mfma_f32_16x16x32_f16(fb, w8l, ob, 0, 0, 0);
+                }
         }
-        if (b < COLS) *reinterpret_cast<f4_t*>(&sh.merge.o[wave][col][16 * y + 4 * p]) = v;
-    }
-    if (p == 0 && b < COLS) sh.merge.m[wave][col] = m2, sh.merge.l[wave][col] = l;
-    __syncthreads();
-    merge_waves<DH, COLS>(a, sh.merge, r, rows, g, nsplit, split);
+        __syncthreads();
+
+        // the four waves' results
+        l = sum_over_p(l);
+#pragma unroll
+        for (int y = 0; y < NV; ++y) {
+            f4_t v = o[y];
+            if constexpr (PAIR) {
+#pragma unroll
+                for (int i = 0; i < 4; ++i) v[i] += column_other(v[i]);
+            }
+            if (b < COLS) *reinterpret_cast<f4_t*>(&sh.merge.o[wave][col][16 * y + 4 * p]) = v;
+        }
+        if (p == 0 && b < COLS) sh.merge.m[wave][col] = m2, sh.merge.l[wave][col] = l;
+        __syncthreads();
+        merge_waves<DH, COLS>(a, sh.merge, r, rows, g, nsplit, split);
     };
 
     if constexpr (PAIR) {
@@ -1033,7 +1055,8 @@ Plan attn4_plan(Form form, int64_t rows, int64_t seqs, int64_t group, int64_t Hk
                                                             : std::max(std::min(256 / each, p.most), Dh == 128 ? std::min(p.groups / each, units / 64) : 0)));
     return p;
 }
-// rows that belong to sequences of their own have no keys in common; few rows are short runs, however they stand
+// rows that belong to sequences of their own have no keys in common; few rows are short runs, however they stand (four rows of one
+// sequence over 16000 keys 24.7 us, as a chunk 36.7; over 1000 keys 17.7 and 24.8)
 Form attn4_form(bool row_seq, int64_t rows, int64_t group) { return !row_seq || rows == 1 ? Form::token : rows * group <= 16 ? Form::few : Form::chunk; }
 
 }  // namespace

@@ -253,6 +253,28 @@ def test_captured_and_replayed(lib, m, v, top):
         assert bool(res[0]["lp"].all())
 
 
+def test_calls_at_once(lib):
+    """on two streams, a workspace each"""
+    import torch
+
+    rng = np.random.default_rng(6)
+    m, v, top = 3, 50000, 20
+    want, sides, xs = [], [torch.cuda.Stream(), torch.cuda.Stream()], []
+    for _ in sides:
+        x = (rng.standard_normal((m, v)) * 3).astype(np.float32)
+        t = rng.integers(0, v, m)
+        want.append(run(lib, x, t, 1.0, top))
+        xs.append((dev(x), dev(t.astype(np.int32)), empty(4 * m), empty(4 * m), empty(4 * m * top), empty(4 * m * top), empty(lib.hero_logprobs_work_bytes(m, v, top))))
+    torch.cuda.synchronize()
+    for _ in range(3):
+        for s, (x, t, lp, ent, ids, tlp, work) in zip(sides, xs):
+            check(lib.hero_logprobs(ptr(x), v, m, v, ptr(t), 1.0, top, ptr(lp), ptr(ent), ptr(ids), ptr(tlp), ptr(work), lib.hero_logprobs_work_bytes(m, v, top), s.cuda_stream))
+    torch.cuda.synchronize()
+    for w, (_, _, lp, ent, ids, tlp, _) in zip(want, xs):
+        for k, got in (("logprob", lp), ("entropy", ent), ("top_ids", ids), ("top_logprobs", tlp)):
+            assert np.array_equal(host(got, w[k].dtype, w[k].shape), w[k]), k
+
+
 def test_a_serving_step(lib):
     """Tokens enter a 4-bit cache, attend to it, pass an output projection of Q8_0 weights into logits, and the
     next tokens' log probabilities come out: four steps of three sequences against the formulas in 64 bits on

@@ -436,6 +436,81 @@ def test_long_runs_and_single_tokens_split_over_workgroups(lib, hq, hkv, dh, row
     compare(*run_attend(lib, rng, c, hq, seq, pos, work_more=64))
 
 
+@pytest.mark.parametrize("hkv,dh,rows,first,row_seq", [(256, 128, 17, 9000, True), (128, 256, 17, 9000, True), (768, 128, 1, 5000, False), (160, 128, 17, 2100, True)])
+def test_long_ranges(lib, hkv, dh, rows, first, row_seq):
+    """So many heads that thousands of keys are left to a workgroup: compared for some of the heads. Pages that a
+    sequence has more than once."""
+    rng = np.random.default_rng(hkv + dh)
+    c = Pool(rng, 1, 20, hkv, dh)
+    c.max_pages = -(-(first + rows) // 64)
+    c.table = rng.integers(0, c.n, (1, c.max_pages)).astype(np.int32)
+    pos, seq = np.arange(first, first + rows, dtype=np.int32), np.zeros(rows, np.int32)
+    q = rng.standard_normal((rows, hkv, dh)).astype(np.float32)
+    stride = 2 * hkv * dh
+    proj = rng.standard_normal((rows, stride)).astype(np.float32)
+    d = {k: dev(v) for k, v in dict(q=q, proj=proj, pages=c.rec, table=c.table, pos=pos, seq=seq).items()}
+    wb = lib.hero_attn_q4_work_bytes(rows, hkv, hkv, dh, c.max_pages * 64, 0, 0)
+    out, work = empty(rows * hkv * dh * 4), dev(np.full(max(wb, 16), 0xFF, np.uint8))
+    args = q4_args(c, hkv, rows, ptr(d["pos"]), ptr(d["seq"]) if row_seq else None, proj=ptr(d["proj"]), stride=stride, q_rot=ptr(d["q"]), scale=dh ** -0.5, out=ptr(out),
+                   pages=ptr(d["pages"]), table=ptr(d["table"]), work=ptr(work), work_bytes=wb)
+    check(lib.hero_attn_q4(args, stream()))
+    heads = [0, hkv // 3, hkv - 1]
+    few = Pool(rng, 1, 1, len(heads), dh)
+    few.rec, few.n, few.table, few.max_pages = c.rec[:, :, heads], c.n, c.table, c.max_pages
+    gate = proj.reshape(rows, hkv, 2, dh)[:, heads, 1]
+    compare(host(out, np.float32, (rows, hkv, dh))[:, heads], *attend64(few, len(heads), q[:, heads], gate, seq, pos, dh ** -0.5, 0, 0))
+
+
+def test_calls_at_once_and_one_workspace_after_another(lib):
+    """Calls of every form: on two streams at once with a workspace each, and on one stream with one for all, give what they
+    give alone."""
+    import torch
+
+    rng = np.random.default_rng(5)
+    hq, hkv, dh, seqs = 8, 2, 128, 3
+    c = Pool(rng, seqs, 40, hkv, dh)
+    calls = []
+    for seq, pos, row_seq in [([0, 1, 2], [2500, 1700, 9], False), ([1] * 3, [2000, 2001, 2002], True), ([0] * 50 + [2] + [1] * 49, [*range(2000, 2050), 77, *range(1800, 1849)], True)]:
+        rows = len(pos)
+        d = {k: dev(v) for k, v in dict(q=rng.standard_normal((rows, hq, dh)).astype(np.float32), proj=rng.standard_normal((rows, 2 * hq * dh)).astype(np.float32), pages=c.rec,
+                                        table=c.table, pos=np.array(pos, np.int32), seq=np.array(seq, np.int32)).items()}
+        wb = lib.hero_attn_q4_work_bytes(rows, hq, hkv, dh, c.max_pages * 64, 0, 0)
+        calls.append((rows, row_seq, d, wb))
+
+    def run(call, work, on):
+        rows, row_seq, d, wb = call
+        out = torch.zeros(rows * hq * dh * 4, dtype=torch.uint8, device="cuda")
+        torch.cuda.synchronize()
+        args = q4_args(c, hq, rows, ptr(d["pos"]), ptr(d["seq"]) if row_seq else None, proj=ptr(d["proj"]), stride=2 * hq * dh, q_rot=ptr(d["q"]), scale=0.1, out=ptr(out),
+                       pages=ptr(d["pages"]), table=ptr(d["table"]), work=ptr(work), work_bytes=wb)
+        return out, lambda: check(lib.hero_attn_q4(args, on))
+
+    alone = []
+    for call in calls:
+        out, go = run(call, empty(call[3]), stream())
+        go()
+        alone.append(out)
+    torch.cuda.synchronize()
+    shared = empty(max(call[3] for call in calls))
+    sides = [torch.cuda.Stream(), torch.cuda.Stream()]
+    own = [[empty(call[3]) for call in calls] for _ in sides]
+    for on in (None, *sides):
+        again = [run(call, shared, stream() if on is None else on.cuda_stream) for call in calls * 2]
+        for _, go in again:
+            go()
+        torch.cuda.synchronize()
+        for (out, _), want in zip(again, alone * 2):
+            assert torch.equal(out, want)
+    both = [[run(call, w, s.cuda_stream) for call, w in zip(calls, own[k])] for k, s in enumerate(sides)]
+    for one, two in zip(both[0], both[1][::-1]):
+        one[1]()
+        two[1]()
+    torch.cuda.synchronize()
+    for k in (0, 1):
+        for (out, _), want in zip(both[k], alone):
+            assert torch.equal(out, want)
+
+
 @pytest.mark.parametrize("row_seq", [False, True])
 def test_what_no_row_sees_has_no_influence(lib, row_seq):
     """Slots past the rows, whole pages behind them, pages before a window: NaN steps there change nothing.
