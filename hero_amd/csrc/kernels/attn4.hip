@@ -1035,9 +1035,11 @@ __global__ __launch_bounds__(256) void attn4_combine_kernel(Attn4Args a, int nsp
 }
 
 // Rows a workgroup takes, and into how many ranges their keys are split. Tokens: three workgroups per CU, eight
-// units of 32 keys each at least. Chunks: one workgroup per CU with at least eight units, and (128-wide
-// heads, of which two fit) two with at least 64: 512 rows over 16000 keys take 534 us in one range, 307 in two, 275 in
-// four; 1000 rows over 1024 each 63 us in one, 62 in two, 78 in four.
+// units of 32 keys each at least. Chunks: one workgroup per CU with at least eight units; two (of 128-wide heads, of which two
+// fit) where one would have 45 units or more: a unit takes 1.3 us alone and 1.0 us of each of two, and the ranges'
+// combination costs 5 to 13 us. 500 rows over 16000 keys, 258 units: 315 us in two ranges, 275 in four; 300 rows over
+// 4000, 45 units: 82 in four, 72 in six; 1000 rows over 2500, 94 units: 131 in one, 118 in two; over 1000, 34 units: 64 and
+// 68; 500 rows of two sequences over 2250, 35 units: 75 in two, 82 in four.
 enum class Form { token, few, chunk };
 struct Plan {
     int R, nsplit;
@@ -1051,8 +1053,12 @@ Plan attn4_plan(Form form, int64_t rows, int64_t seqs, int64_t group, int64_t Hk
     p.tiles = form == Form::few && seqs > 1 ? rows : (rows + p.R - 1) / p.R;  // (rows of several sequences are mostly alone)
     p.most = std::max<int64_t>(1, units / 8);
     const int64_t each = p.tiles * Hkv;
-    p.nsplit = int(std::max<int64_t>(1, form != Form::chunk ? std::min(p.groups / each, p.most)
-                                                            : std::max(std::min(256 / each, p.most), Dh == 128 ? std::min(p.groups / each, units / 64) : 0)));
+    if (form != Form::chunk) {
+        p.nsplit = int(std::max<int64_t>(1, std::min(p.groups / each, p.most)));
+    } else {
+        const int64_t one = std::max<int64_t>(1, std::min(256 / each, p.most)), two = Dh == 128 ? std::min(p.groups / each, p.most) : 1;
+        p.nsplit = int(units >= 45 * one ? std::max(one, two) : one);
+    }
     return p;
 }
 // rows that belong to sequences of their own have no keys in common; few rows are short runs, however they stand (four rows of one
