@@ -10,9 +10,9 @@
 // Scores and sums are held in fp32; m lags the true maximum by up to kPSlack, which saves most rescalings.
 //
 // Three forms. One row of a sequence: the two terms fill the 16 columns of one product with up to 8
-// query heads; what counts is the read of the cache (attn4_short_kernel<PAIR>). Chunks: 128 columns of a
+// query heads; what counts is the read of the cache (attn4_short_kernel). Chunks: 128 columns of a
 // workgroup, 128 / group rows, share the work of turning records into operands, and the products bound it
-// (attn4_chunk_kernel). Few rows, and runs of a few rows among chunks: a short kernel without PAIR, as the columns'
+// (attn4_chunk_kernel). Few rows, and runs of a few rows among chunks: the short kernel again, as the columns'
 // other halves would be idle in a chunk's workgroup. Keys are split into ranges where there are few
 // workgroups, and combined by a second launch.
 //
@@ -27,6 +27,8 @@
 #include "hero/kernels.hpp"
 #include "hero/paged.hpp"
 #include "hero/q4.hpp"
+
+#include <type_traits>
 
 namespace hero {
 
@@ -222,24 +224,26 @@ __device__ __forceinline__ int short_run(const PagedRows& c, int64_t r, int most
     return n <= most ? n : 0;
 }
 
-// One row (PAIR), or the short runs of rows b, b + stride, ...: a workgroup of four waves takes one K/V head and
-// one of nsplit equal ranges of the run's records, a wave two records (32 keys) at a time. PAIR:
+// One row (ONE), or the short runs of rows b, b + stride, ...: a workgroup of four waves takes one K/V head and
+// one of nsplit equal ranges of the run's records, a wave two records (32 keys) at a time. A row alone (PAIR):
 // the two terms of up to 8 query heads are the 16 columns, those of head h columns h and h + 8, added where both are
 // done. Else the columns are the run's pairs, and each term has a product of its own.
-template <int DH, int D, bool PAIR>
-__global__ __launch_bounds__(256, DH == 128 && PAIR ? 3 : 2) void attn4_short_kernel(Attn4Args a, int nsplit, int stride) {
-    constexpr int COLS = PAIR ? 8 : 16, H = DH / 128, NS = DH / 32, NV = DH / 16;
+template <int DH, int D, bool ONE>
+__global__ __launch_bounds__(256, DH == 128 && ONE ? 3 : 2) void attn4_short_kernel(Attn4Args a, int nsplit, int stride) {
+    constexpr int COLS = ONE ? 8 : 16, H = DH / 128, NS = DH / 32, NV = DH / 16;
     const PagedRows& c = a.c;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), p = lane >> 4, b = lane & 15;
     const int split = blockIdx.x % nsplit, g = blockIdx.x / nsplit % c.Hkv, first_row = blockIdx.x / nsplit / c.Hkv;
-    const int group = a.Hq / c.Hkv, tpp = c.page_size / kQ4Tile, col = PAIR ? b & 7 : b;
+    const int group = a.Hq / c.Hkv, tpp = c.page_size / kQ4Tile;
     __shared__ union {
         Ring<DH, D> ring[4];
         Merge<DH, COLS> merge;
     } sh;
     const FieldMasks masks;
 
-    auto attend = [&](const int r, const int rows) __attribute__((always_inline)) {
+    auto attend = [&](auto pair, const int r, const int rows) __attribute__((always_inline)) {
+        constexpr bool PAIR = decltype(pair)::value;
+        const int col = PAIR ? b & 7 : b;
         const int mine = PAIR ? 0 : min(col / group, rows - 1);  // the column's row
         float x[NS][8];
         {
@@ -467,22 +471,26 @@ __global__ __launch_bounds__(256, DH == 128 && PAIR ? 3 : 2) void attn4_short_ke
 #pragma unroll
                 for (int i = 0; i < 4; ++i) v[i] += column_other(v[i]);
             }
-            if (b < COLS) *reinterpret_cast<f4_t*>(&sh.merge.o[wave][col][16 * y + 4 * p]) = v;
+            if (!PAIR || b < 8) *reinterpret_cast<f4_t*>(&sh.merge.o[wave][col][16 * y + 4 * p]) = v;
         }
-        if (p == 0 && b < COLS) sh.merge.m[wave][col] = m2, sh.merge.l[wave][col] = l;
+        if (p == 0 && (!PAIR || b < 8)) sh.merge.m[wave][col] = m2, sh.merge.l[wave][col] = l;
         __syncthreads();
         merge_waves<DH, COLS>(a, sh.merge, r, rows, g, nsplit, split);
     };
 
-    if constexpr (PAIR) {
-        attend(first_row, 1);
+    if constexpr (ONE) {
+        attend(std::true_type{}, first_row, 1);
     } else {
         for (int64_t base = first_row; base < c.rows; base += 64 * int64_t(stride)) {
             const int found = short_run(c, base + int64_t(lane) * stride, 16 / group);  // by a lane each
             for (uint64_t left = __ballot(found > 0); left; left &= left - 1) {
                 const int at = __ffsll((unsigned long long)left) - 1;
                 __syncthreads();  // the last run's results are read
-                attend(int(base + int64_t(at) * stride), __builtin_amdgcn_readlane(found, at));
+                const int r = int(base + int64_t(at) * stride), rows = __builtin_amdgcn_readlane(found, at);
+                if (rows == 1)
+                    attend(std::true_type{}, r, 1);
+                else
+                    attend(std::false_type{}, r, rows);
             }
         }
     }
@@ -1088,7 +1096,8 @@ void attn4_sized(const Attn4Args& a, hipStream_t s) {
     if (form == Form::token)
         hipLaunchKernelGGL((attn4_short_kernel<DH, 2, true>), dim3(unsigned(rows * Hkv * p.nsplit)), dim3(256), 0, s, a, p.nsplit, 1);
     if (runs) {
-        const int64_t stride = std::min(rows, std::max<int64_t>(1, 768 / (Hkv * p.nsplit)));
+        // two workgroups per CU are there at once: with three, 64 tokens of 8000 keys take 225 us instead of 215
+        const int64_t stride = std::min(rows, std::max<int64_t>(1, 512 / (Hkv * p.nsplit)));
         hipLaunchKernelGGL((attn4_short_kernel<DH, 2, false>), dim3(unsigned(stride * Hkv * p.nsplit)), dim3(256), 0, s, a, p.nsplit, int(stride));
     }
     if (form == Form::chunk) {

@@ -516,7 +516,8 @@ int hero_kv_read_q4(const hero_kv_read_args* args, void* stream);
  * influence, whatever the pool holds there; the others hold what
  * hero_kv_append_q4 stored. Outputs: a.out_f32 and / or a.act_out (Q8_0
  * activations), at least one, 16-byte aligned. Rows of one sequence should stand
- * together: neighbouring rows share the reads of their keys. Results agree with
+ * together: neighbouring rows share the reads of their keys; where row r is
+ * sequence r, row_seq NULL is the faster form. Results agree with
  * the formula over the stored values to fp32 rounding, save that a query's channels are
  * kept to 2^-22 of themselves or 2^-38 of the head's largest and weights to 2^-22 of
  * themselves or 2^-38 of the row's largest. Uses a.q_rot, proj (the gates), proj_stride, positions,
