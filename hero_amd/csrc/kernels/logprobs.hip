@@ -175,7 +175,8 @@ __global__ __launch_bounds__(256) void logprobs_range_kernel(LogprobsArgs a, Log
 // A workgroup per row. The last wave joins the sums; the others look for the alternatives.
 constexpr int kJoinThreads = 512, kGathered = 4096, kListed = 256;
 __global__ __launch_bounds__(kJoinThreads) void logprobs_join_kernel(LogprobsArgs a, LogprobsWork w, int ranges, int blocks) {
-    const int64_t row = blockIdx.x;
+    const int64_t row = int64_t(blockIdx.y) * gridDim.x + blockIdx.x;
+    if (row >= a.m) return;
     const int t = threadIdx.x, lane = t & 63, wave = t >> 6, v_end = int(a.v);
     const int target = a.targets ? a.targets[row] : 0;
     if (target < 0 || target >= a.v) return;
@@ -353,7 +354,8 @@ void launch_logprobs(const LogprobsArgs& a, hipStream_t s) {
         hipLaunchKernelGGL(logprobs_range_kernel<true>, grid, dim3(256), 0, s, a, w, ranges, per, blocks);
     else
         hipLaunchKernelGGL(logprobs_range_kernel<false>, grid, dim3(256), 0, s, a, w, ranges, per, blocks);
-    hipLaunchKernelGGL(logprobs_join_kernel, dim3(unsigned(a.m)), dim3(kJoinThreads), 0, s, a, w, ranges, blocks);
+    const unsigned wide = unsigned(std::min<int64_t>(a.m, 1 << 16));  // (a dimension has less than 2^32 threads)
+    hipLaunchKernelGGL(logprobs_join_kernel, dim3(wide, unsigned((a.m + wide - 1) / wide)), dim3(kJoinThreads), 0, s, a, w, ranges, blocks);
 }
 
 }  // namespace hero

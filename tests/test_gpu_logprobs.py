@@ -253,6 +253,24 @@ def test_captured_and_replayed(lib, m, v, top):
         assert bool(res[0]["lp"].all())
 
 
+def test_millions_of_rows(lib):
+    """more workgroups of the second launch than one dimension of a grid takes"""
+    import torch
+
+    m, v = (1 << 23) + 77, 3
+    x = torch.randn(m, v, device="cuda")
+    t = torch.randint(0, v, (m,), device="cuda", dtype=torch.int32)
+    lp, ids, tlp, wb = empty(4 * m), empty(4 * m), empty(4 * m), lib.hero_logprobs_work_bytes(m, v, 1)
+    work = empty(wb)
+    check(lib.hero_logprobs(ptr(x), v, m, v, ptr(t), 1.0, 1, ptr(lp), None, ptr(ids), ptr(tlp), ptr(work), wb, stream()))
+    torch.cuda.synchronize()
+    want = torch.log_softmax(x.double(), -1)
+    # three terms: a few roundings of values below 2^4
+    assert (lp.view(torch.float32) - want.gather(1, t.long()[:, None])[:, 0]).abs().max().item() <= 2.0 ** -19
+    assert torch.equal(ids.view(torch.int32).long(), x.argmax(-1))
+    assert (tlp.view(torch.float32) - want.max(-1).values).abs().max().item() <= 2.0 ** -19
+
+
 def test_calls_at_once(lib):
     """on two streams, a workspace each"""
     import torch
