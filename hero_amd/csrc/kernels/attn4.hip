@@ -866,6 +866,8 @@ __global__ __launch_bounds__(256, DH == 128 ? 2 : 1) void attn4_chunk_kernel(Att
             // ... this unit's values, and between their products operands of the units to come and the next unit's maxima
             const int slot1 = slot == kRing - 1 ? 0 : slot + 1, slot2 = slot1 == kRing - 1 ? 0 : slot1 + 1;
             take(slot2, slot1);
+            const Two w5 = locate(u + 5), w2 = locate(u + 2);
+            fetch(w5.krec0, w5.krec1, slot);  // (unit u's records have been operands since the last barrier)
             q4_h8 v_now[2] = {operand_v(now, 0, 0), operand_v(now, 0, 1)};
             if (__builtin_expect(w1.edge, 0)) {
                 clean_v(w1.at);
@@ -889,9 +891,7 @@ __global__ __launch_bounds__(256, DH == 128 ? 2 : 1) void attn4_chunk_kernel(Att
                 v_now[0] = v_next[0], v_now[1] = v_next[1];
                 __builtin_amdgcn_sched_barrier(0);
             }
-            const Two w5 = locate(u + 5);
-            fetch(w5.krec0, w5.krec1, slot);
-            w1 = locate(u + 2);
+            w1 = w2;
             slot = slot1;
             rescale(best);
             wait_vmcnt<2 * kLoads>();
