@@ -155,18 +155,21 @@ __device__ __forceinline__ void store_out(const Attn4Args& a, int r, int h, int 
     }
 }
 
-// Four neighbouring channels, by neighbouring lanes: channel `at` of the outputs and the next.
-__device__ __forceinline__ void store_four(const Attn4Args& a, int64_t at, f4_t v) {
-    if (a.out_f32) *reinterpret_cast<f4_t*>(a.out_f32 + at) = v;
-    if (!a.act_out) return;
+// Four neighbouring channels, by neighbouring lanes: channel `at` of the outputs and the next. Returns the step of
+// the lane's block of Q8_0, whose place is store_step's.
+__device__ __forceinline__ float store_four(const Attn4Args& a, int64_t at, f4_t v, bool live) {
+    if (a.out_f32 && live) *reinterpret_cast<f4_t*>(a.out_f32 + at) = v;
+    if (!a.act_out) return 0.f;
     const float amax = max_of_8(fmaxf(fmaxf(fabsf(v[0]), fabsf(v[1])), fmaxf(fabsf(v[2]), fabsf(v[3]))));
     const float d = amax / 127.f, id = d != 0.f ? 1.f / d : 0.f;
     uint32_t codes = 0;
 #pragma unroll
     for (int i = 0; i < 4; ++i) codes |= uint32_t(round_code(v[i] * id) & 0xFF) << (8 * i);
-    int8_t* qs = static_cast<int8_t*>(a.act_out);
-    *reinterpret_cast<uint32_t*>(qs + at) = codes;
-    if (at % 32 == 0) reinterpret_cast<float*>(qs + int64_t(a.c.rows) * a.Hq * a.c.Dh)[at >> 5] = half_bits_to_f32(fp32_to_fp16_ref(d));
+    if (live) *reinterpret_cast<uint32_t*>(static_cast<int8_t*>(a.act_out) + at) = codes;
+    return d;
+}
+__device__ __forceinline__ void store_step(const Attn4Args& a, int64_t block, float d) {
+    reinterpret_cast<float*>(static_cast<int8_t*>(a.act_out) + int64_t(a.c.rows) * a.Hq * a.c.Dh)[block] = half_bits_to_f32(fp32_to_fp16_ref(d));
 }
 
 // a row's keys: those below `stay`, and from `first` (>= stay) to `pos`
@@ -915,7 +918,7 @@ __global__ __launch_bounds__(256, DH == 128 ? 2 : 1) void attn4_chunk_kernel(Att
     // a lane takes four neighbouring channels of one column (or, of 128, of every other) after another. Stores of whole
     // rows, and a short loop where the columns' own order unrolls to 24 KB of instructions that every call fetches anew.
     const float total = l + __shfl_xor(l, 32);
-    const int mine = row >= 0 && ((row < 64 ? done[0] : done[1]) >> (row & 63) & 1) ? r0 + row : -1;
+    const bool live = row >= 0 && ((row < 64 ? done[0] : done[1]) >> (row & 63) & 1);
     wait_vmcnt<0>();
     barrier();
 #pragma unroll
@@ -923,37 +926,43 @@ __global__ __launch_bounds__(256, DH == 128 ? 2 : 1) void attn4_chunk_kernel(Att
 #pragma unroll
         for (int y = 0; y < 4; ++y)
             *reinterpret_cast<f4_t*>(&sh.out[wave][lane & 31][32 * n + 8 * y + 4 * f]) = f4_t{o[n][4 * y], o[n][4 * y + 1], o[n][4 * y + 2], o[n][4 * y + 3]};
+    if (f == 0) {  // behind a column its (row, query head), -1: none, and what else is known of it
+        const int r = live ? r0 + row : r0;
+        const float pair = __int_as_float(live ? r * a.Hq + head : -1), share = total == 0.f ? 0.f : 1.f / (total * kPOne);
+        *reinterpret_cast<f4_t*>(&sh.out[wave][lane][DH]) = nsplit > 1 ? f4_t{pair, m2, total, 0.f} : f4_t{pair, share, __int_as_float(r), __int_as_float(head)};
+    }
     wave_exchange();
-    const float share = nsplit > 1 ? 1.f / kPOne : total == 0.f ? 0.f : 1.f / (total * kPOne);
-    const int ch = 4 * lane % DH;
     constexpr int kAtOnce = 8, kColumns = 256 / DH;
+    const int ch = 4 * lane % DH;
 #pragma unroll 1
-    for (int k = 0; k < 32; k += kAtOnce * kColumns) {
-        f4_t gate[kAtOnce];
+    for (int k = 4 * lane / DH; k < 32; k += kAtOnce * kColumns) {
+        f4_t of[kAtOnce], gate[kAtOnce];
+#pragma unroll
+        for (int j = 0; j < kAtOnce; ++j) of[j] = *reinterpret_cast<const f4_t*>(&sh.out[wave][k + j * kColumns][DH]);
         if (nsplit == 1)  // a round's loads together: one by one they were half of the time of a short call
 #pragma unroll
-            for (int j = 0; j < kAtOnce; ++j) {
-                const int at_col = k + j * kColumns + 4 * lane / DH, to = max(__shfl(mine, at_col), r0), h = g * group + (wave * 32 + at_col) % group;
-                __builtin_memcpy(&gate[j], a.proj + int64_t(to) * a.proj_stride + int64_t(h) * 2 * DH + DH + ch, 16);
-            }
+            for (int j = 0; j < kAtOnce; ++j)
+                __builtin_memcpy(&gate[j], a.proj + int64_t(__float_as_int(of[j][2])) * a.proj_stride + int64_t(__float_as_int(of[j][3])) * 2 * DH + DH + ch, 16);
+        float step = 0.f;  // of every eighth column, by its eight lanes one each
 #pragma unroll
         for (int j = 0; j < kAtOnce; ++j) {
-            const int at_col = k + j * kColumns + 4 * lane / DH, to = __shfl(mine, at_col), h = g * group + (wave * 32 + at_col) % group;
-            const float of = __shfl(share, at_col);
-            f4_t v = *reinterpret_cast<const f4_t*>(&sh.out[wave][at_col][ch]) * of;
+            const int64_t pair = __float_as_int(of[j][0]);
+            f4_t v = *reinterpret_cast<const f4_t*>(&sh.out[wave][k + j * kColumns][ch]);
             if (nsplit > 1) {
-                const float at_m = __shfl(m2, at_col), at_total = __shfl(total, at_col);
-                if (to >= 0) {
-                    float* rec = a.work + ((int64_t(to) * a.Hq + h) * nsplit + split) * (DH + 4);
-                    if (ch == 0) rec[0] = at_m, rec[1] = at_total;
-                    *reinterpret_cast<f4_t*>(rec + 4 + ch) = v;
+                if (pair >= 0) {
+                    float* rec = a.work + (pair * nsplit + split) * (DH + 4);
+                    if (ch == 0) rec[0] = of[j][1], rec[1] = of[j][2];
+                    *reinterpret_cast<f4_t*>(rec + 4 + ch) = v * (1.f / kPOne);
                 }
                 continue;
             }
 #pragma unroll
-            for (int i = 0; i < 4; ++i) v[i] = of == 0.f ? 0.f : v[i] * gate_of(gate[j][i]);
-            if (to >= 0) store_four(a, (int64_t(to) * a.Hq + h) * DH + ch, v);
+            for (int i = 0; i < 4; ++i) v[i] = of[j][1] == 0.f ? 0.f : v[i] * of[j][1] * gate_of(gate[j][i]);
+            const float d = store_four(a, pair * DH + ch, v, pair >= 0);
+            step = (lane & 7) == j ? d : step;
         }
+        if (nsplit == 1 && a.act_out)
+            if (const int64_t pair = __float_as_int(sh.out[wave][k + (lane & 7) * kColumns][DH]); pair >= 0) store_step(a, pair * (DH / 32) + ch / 32, step);
     }
 }
 
@@ -992,7 +1001,9 @@ __global__ __launch_bounds__(256) void attn4_combine_few_kernel(Attn4Args a, int
     }
 #pragma unroll
     for (int i = 0; i < 4; ++i) o[i] = total == 0.f ? 0.f : o[i] / total * gate_of(gate[i]);
-    store_four(a, (int64_t(r) * a.Hq + h) * DH + ch, o);
+    const int64_t at = (int64_t(r) * a.Hq + h) * DH + ch;
+    const float d = store_four(a, at, o, true);
+    if (a.act_out && ch % 32 == 0) store_step(a, at / 32, d);
 }
 
 // A workgroup per (row, query head): DH / 4 lanes for four channels each read a range's result, and
