@@ -1053,8 +1053,9 @@ __global__ __launch_bounds__(256) void attn4_combine_kernel(Attn4Args a, int nsp
     }
 }
 
-// Rows a workgroup takes, and into how many ranges their keys are split. Tokens: three workgroups per CU, eight
-// units of 32 keys each at least. Chunks: one workgroup per CU with at least eight units; two (of 128-wide heads, of which two
+// Rows a workgroup takes, and into how many ranges their keys are split. Tokens and few rows: as many workgroups as are
+// there at once, three per CU of single rows of 128-wide heads and else two (with three, eight rows over 16000 keys of 256-wide
+// heads take 46 us instead of 42, four rows of one sequence over 32000 35 instead of 28), eight units of 32 keys each at least. Chunks: one workgroup per CU with at least eight units; two (of 128-wide heads, of which two
 // fit) where one would have 45 units or more: a unit takes 1.3 us alone and 1.0 us of each of two, and the ranges'
 // combination costs 5 to 13 us. 500 rows over 16000 keys, 258 units: 315 us in two ranges, 275 in four; 300 rows over
 // 4000, 45 units: 82 in four, 72 in six; 1000 rows over 2500, 94 units: 131 in one, 118 in two; over 1000, 34 units: 64 and
@@ -1067,7 +1068,7 @@ struct Plan {
 Plan attn4_plan(Form form, int64_t rows, int64_t seqs, int64_t group, int64_t Hkv, int64_t Dh, int64_t span, int64_t window, int64_t sinks) {
     Plan p;
     p.R = form == Form::token ? 1 : int((form == Form::few ? 16 : 128) / group);
-    p.groups = form == Form::chunk ? 512 : 768;
+    p.groups = form != Form::token || Dh == 256 ? 512 : 768;
     const int64_t keys = window > 0 ? std::min(span, window + sinks + p.R + 2 * kQ4Tile) : span, units = (keys + 31) / 32;
     p.tiles = form == Form::few && seqs > 1 ? rows : (rows + p.R - 1) / p.R;  // (rows of several sequences are mostly alone)
     p.most = std::max<int64_t>(1, units / 8);
