@@ -16,13 +16,13 @@
 // other halves would be idle in a chunk's workgroup. Keys are split into ranges where there are few
 // workgroups, and combined by a second launch.
 //
-// Measured, 32 query and 8 K/V heads of 128, in pages of 64: sixteen tokens of 32000 keys each 123 us, 4.9 TB/s of cache in
-// the first launch (a copy of gigabytes: 5.1); the same over windows of 4096 26 us; one token of 32000 keys 19.8 us, of which
+// Measured, 32 query and 8 K/V heads of 128, in pages of 64: sixteen tokens of 32000 keys each 121 to 127 us, 4.9 TB/s of cache
+// in the first launch (a copy of gigabytes: 5.1); the same over windows of 4096 26 us; one token of 32000 keys 19.8 us, of which
 // about 3 are spent before the first records arrive, 2 after the last ones and 4 on the second launch, and 6 keep the vector units
 // busy with turning codes into operands; one token of 300 keys 8.8 us, latencies and instruction fetches. 500 rows
-// over 16000 keys 260 us, 1.05 PFLOP/s of products (fp16 matrix products of 8192^3 reach 1.17); 1000 rows of three
-// sequences over windows of 1024 80 us: 250 workgroups of 34 units each, 44 us for these, and about 20 from start to first and from
-// last product to end.
+// over 16000 keys 253 to 261 us, 1.07 PFLOP/s of products (fp16 matrix products of 8192^3 reach 1.17); 1000 rows of three
+// sequences over windows of 1024 76 us: 250 workgroups of 34 units each, 44 us for these, about 16 from start to first and from
+// last product to end, 5 for the launch that looks for short runs.
 #include "hero/device.hpp"
 #include "hero/kernels.hpp"
 #include "hero/paged.hpp"
