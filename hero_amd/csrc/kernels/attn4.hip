@@ -326,7 +326,7 @@ __global__ __launch_bounds__(256, DH == 128 && ONE ? 3 : 2) void attn4_short_ker
 #pragma unroll
                 for (int j = 0; j < 8; ++j) amax = fmaxf(amax, fabsf(x[s][j] *= k));
             amax = max_over_p(amax);
-            const int e = amax > 0.f && amax < INFINITY ? min(max(ilogbf(amax) + 1, -100), 117) : 0;
+            const int e = amax > 0.f && amax < INFINITY ? max(ilogbf(amax) + 1, -100) : 0;  // (128 at most: unit and slack are normal)
 #pragma unroll
             for (int s = 0; s < NS; ++s)
 #pragma unroll
@@ -584,7 +584,7 @@ __global__ __launch_bounds__(256, DH == 128 ? 2 : 1) void attn4_chunk_kernel(Att
 #pragma unroll
             for (int j = 0; j < 8; ++j) amax = fmaxf(amax, fabsf(x[s][j / 4][j % 4]));
         amax = fmaxf(amax, __shfl_xor(amax, 32));
-        const int e = amax > 0.f && amax < INFINITY ? min(max(ilogbf(amax) + 1, -100), 117) : 0;
+        const int e = amax > 0.f && amax < INFINITY ? max(ilogbf(amax) + 1, -100) : 0;  // (128 at most: unit and slack are normal)
 #pragma unroll
         for (int s = 0; s < NS; ++s)
 #pragma unroll

@@ -520,8 +520,9 @@ int hero_kv_read_q4(const hero_kv_read_args* args, void* stream);
  * sequence r, row_seq NULL is the faster form. Results agree with
  * the formula over the stored values to fp32 rounding, save that a query's channels are
  * kept to 2^-22 of themselves or 2^-38 of the head's largest and weights to 2^-22 of
- * themselves or 2^-38 of the row's largest. Uses a.q_rot, proj (the gates), proj_stride, positions,
- * score_scale, window, b, hq, hkv, dh, the page and row fields, sinks and work
+ * themselves or 2^-38 of the row's largest. score_scale * q and the scores, each times
+ * log2(e), have to be within fp32's range: past it a row may be NaN. Uses a.q_rot, proj
+ * (the gates), proj_stride, positions, score_scale, window, b, hq, hkv, dh, the page and row fields, sinks and work
  * (hero_attn_q4_work_bytes, 16-byte aligned; NULL where that is 0; the sizes
  * grow with the rows; calls that may overlap need one each). max_ctx of the size
  * function: max_pages * page_size. */

@@ -581,6 +581,26 @@ def test_extreme_rows(lib, what, row_seq):
     compare(got, want, bound, largest)
 
 
+@pytest.mark.parametrize("form", ["token", "few", "chunk"])
+@pytest.mark.parametrize("dh,hkv", [(128, 2), (256, 1)])
+@pytest.mark.parametrize("top", [118, 120, 125, 128])
+def test_queries_up_to_the_largest_that_fp32_holds(lib, top, dh, hkv, form):
+    """Queries just below 2^top in units of log2 over keys of steps about 2^-18. One key has all codes 7 where the others'
+    are random: it takes all of the weight, so a row is its value times the gate, with one rounding for the
+    division, one for the product and the gate's 4 ulp. Then keys of zeros: the mean of the values."""
+    rng = np.random.default_rng(top + dh)
+    hq, n, best = 4 * hkv, 150, 37
+    c = Pool(rng, 1, 3, hkv, dh)
+    c.rec[:, 0, ..., 8 * dh:] = round8(rng.uniform(1, 2, c.rec[:, 0, ..., 8 * dh:].shape[:-1] + (dh // 2,)) * -8 * 2.0 ** -18).view(np.uint8)
+    c.store(c.table[0, 0], 0, best, np.full((hkv, dh), 7), np.full((hkv, dh // 32), 2.0 ** -18, np.float16))
+    rows = {"token": 1, "few": 3, "chunk": 30}[form]
+    q = (rng.uniform(0.5, 0.999, (rows, hq, dh)) * 2.0 ** top / np.log2(np.e)).astype(np.float32)
+    got, want, _, _ = run_attend(lib, rng, c, hq, [0] * rows, list(range(n - rows, n)), row_seq=form != "token", q=q, scale=1.0)
+    assert np.all(np.abs(got - want) <= 2.0 ** -20 * np.abs(want))
+    c.rec[:, 0, ..., : 8 * dh] = 0x88
+    compare(*run_attend(lib, rng, c, hq, [0] * rows, list(range(n - rows, n)), row_seq=form != "token", q=q, scale=1.0))
+
+
 def test_queries_that_are_not_finite_give_rows_that_are_not(lib):
     rng = np.random.default_rng(5)
     c = Pool(rng, 2, 2, 2)
