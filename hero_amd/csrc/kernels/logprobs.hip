@@ -42,11 +42,21 @@ __device__ __forceinline__ float logit_of(uint32_t order) {
     return order == 0u ? __uint_as_float(0x7FC00000u) : __uint_as_float(order & 0x80000000u ? order & 0x7FFFFFFFu : ~order);
 }
 
+// Differences of logits over temp. From temp 1 on those of their halves, and twice the quotient: what a difference loses by
+// that is below 2^-149, and two logits may be further apart than fp32 reaches where the quotient is not. Below, a
+// difference that does not fit has no quotient that does.
+struct Scale {
+    float part, back, temp, k2;  // 1 or 1/2, its reciprocal; 1 / part / temp in units of log2
+    __device__ __forceinline__ explicit Scale(float t) : part(t >= 1.f ? 0.5f : 1.f), back(t >= 1.f ? 2.f : 1.f), temp(t), k2(kLog2eF * back / t) {}
+    __device__ __forceinline__ float log2_of(float x, float m_part) const { return __builtin_fmaf(x, part, -m_part) * k2; }  // (m_part: m times part)
+    __device__ __forceinline__ float of(float x, float m) const { return __builtin_fmaf(x, part, -(m * part)) / temp * back; }
+};
+
 // the larger of two running maxima takes the other's sums over
-__device__ __forceinline__ void join(RangeSum& a, const RangeSum& b, float k2) {
-    const float m = fmaxf(a.m, b.m);
+__device__ __forceinline__ void join(RangeSum& a, const RangeSum& b, const Scale& scale) {
+    const float m = fmaxf(a.m, b.m), m_part = m * scale.part;
     // (m - m: 0, also for equal infinities)
-    const float da = a.m == m ? 0.f : (a.m - m) * k2, db = b.m == m ? 0.f : (b.m - m) * k2;
+    const float da = a.m == m ? 0.f : scale.log2_of(a.m, m_part), db = b.m == m ? 0.f : scale.log2_of(b.m, m_part);
     const float fa = __builtin_amdgcn_exp2f(da), fb = __builtin_amdgcn_exp2f(db);
     const float sa = a.m == m ? a.r : (a.r + a.c) * fa, sb = b.m == m ? b.r : (b.r + b.c) * fb;
     const float ta = a.m == m ? a.t : fa * a.t + fmaxf(da, -200.f) * sa, tb = b.m == m ? b.t : fb * b.t + fmaxf(db, -200.f) * sb;
@@ -67,9 +77,9 @@ __device__ __forceinline__ float over_lanes(float v, F f) {
     auto at = [&](int lane) { return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(v), lane)); };
     return f(f(at(0), at(16)), f(at(32), at(48)));
 }
-__device__ __forceinline__ void join_lanes(RangeSum& s, float k2) {
+__device__ __forceinline__ void join_lanes(RangeSum& s, const Scale& scale) {
     const RangeSum all{over_lanes(s.m, [](float x, float y) { return fmaxf(x, y); }), 0.f, 0.f, 0.f};
-    join(s, all, k2);
+    join(s, all, scale);
     auto sum = [](float x, float y) { return x + y; };
     s = {all.m, over_lanes(s.c, sum), over_lanes(s.r, sum), over_lanes(s.t, sum)};
 }
@@ -93,8 +103,9 @@ __global__ __launch_bounds__(256) void logprobs_range_kernel(LogprobsArgs a, Log
     const int64_t row = item / ranges;
     const int first = int(item % ranges) * per * kStep, last = int(min(a.v, int64_t(first) + int64_t(per) * kStep)), v_end = int(a.v);
     const float* x = a.logits + row * a.stride;
-    const float k2 = kLog2eF / a.temp;
+    const Scale scale(a.temp);
     RangeSum s{kLowestF, 0.f, 0.f, 0.f};
+    float m_part = kLowestF * scale.part;
     float ahead[kBatch];
     // Stores would hold up the wait for the loads behind them: 1000 rows of 151936 take 103 us without the maxima, 118 with a store for each
     // batch or each four.
@@ -152,11 +163,12 @@ __global__ __launch_bounds__(256) void logprobs_range_kernel(LogprobsArgs a, Log
         }
         if (__ballot(best > s.m)) {  // one maximum for the wave: one of 64 would change in most batches
             const RangeSum next{over_lanes(best, [](float x, float y) { return fmaxf(x, y); }), 0.f, 0.f, 0.f};
-            join(s, next, k2);
+            join(s, next, scale);
+            m_part = s.m * scale.part;
         }
 #pragma unroll
         for (int j = 0; j < kBatch; ++j) {
-            const float d = (v[j] - s.m) * k2;
+            const float d = scale.log2_of(v[j], m_part);
             const bool top = v[j] == s.m;
             const float e = top ? 0.f : __builtin_amdgcn_exp2f(d);
             s.c += top ? 1.f : 0.f;
@@ -168,7 +180,7 @@ __global__ __launch_bounds__(256) void logprobs_range_kernel(LogprobsArgs a, Log
         const int batches = (last - first + kStep - 1) / kStep;
         store(batches - batches % kKept, batches % kKept);
     }
-    join_lanes(s, k2);
+    join_lanes(s, scale);
     if (lane == 0) w.sums[item] = s;
 }
 
@@ -184,7 +196,8 @@ __global__ __launch_bounds__(kJoinThreads) void logprobs_join_kernel(LogprobsArg
     __shared__ uint32_t groups[kJoinThreads], listed[kListed], bar, count, keys;
     __shared__ float of_row[2];  // the largest logit and the logarithm of the sum
     const float* x = a.logits + row * a.stride;
-    const float own = a.logprob ? x[target] : 0.f, k2 = kLog2eF / a.temp;
+    const float own = a.logprob ? x[target] : 0.f;
+    const Scale scale(a.temp);
     const uint32_t* maxima = w.maxima + row * blocks;
     const bool last = wave == kJoinThreads / 64 - 1;
     auto maximum = [&](int i) { return i < blocks ? maxima[i] : 0u; };
@@ -202,13 +215,13 @@ __global__ __launch_bounds__(kJoinThreads) void logprobs_join_kernel(LogprobsArg
     __syncthreads();
     if (last) {
         RangeSum s{kLowestF, 0.f, 0.f, 0.f};
-        for (int i = lane; i < ranges; i += 64) join(s, w.sums[row * ranges + i], k2);
-        join_lanes(s, k2);
+        for (int i = lane; i < ranges; i += 64) join(s, w.sums[row * ranges + i], scale);
+        join_lanes(s, scale);
         if (s.m == INFINITY) s.r = __uint_as_float(0x7FC00000u);
         const float log_sum = logf(s.c) + log1pf(s.r / s.c);
         if (lane == 0) {
             of_row[0] = s.m, of_row[1] = log_sum;
-            if (a.logprob) a.logprob[row] = (own - s.m) / a.temp - log_sum;
+            if (a.logprob) a.logprob[row] = scale.of(own, s.m) - log_sum;
             if (a.entropy) a.entropy[row] = log_sum - kLn2F * s.t / (s.c + s.r);
         }
     }
@@ -317,7 +330,7 @@ __global__ __launch_bounds__(kJoinThreads) void logprobs_join_kernel(LogprobsArg
         for (int j = 0; j < found; ++j) place += gathered[j] > k;
         if (place >= a.top) continue;
         a.top_ids[row * a.top + place] = int32_t(0xFFFFFFFFu - uint32_t(k));
-        a.top_logprobs[row * a.top + place] = (logit_of(uint32_t(k >> 32)) - of_row[0]) / a.temp - of_row[1];
+        a.top_logprobs[row * a.top + place] = scale.of(logit_of(uint32_t(k >> 32)), of_row[0]) - of_row[1];
     }
 }
 

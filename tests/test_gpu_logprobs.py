@@ -173,6 +173,25 @@ def test_rows_that_are_not_finite(lib):
     compare(got, x, t, 1.0, 64, rows=np.array([4]))
 
 
+@pytest.mark.parametrize("temp", [1.0, 2.0, 1e38, 3.4e38])
+@pytest.mark.parametrize("m,v", [(1, 200000), (3, 2000), (2100, 600)])
+def test_logits_further_apart_than_fp32_reaches(lib, m, v, temp):
+    """Logits over all of fp32's range, masks of its lowest value among them: differences pass it, quotients by temp do
+    not (but for temp 1, where one that does is -inf)."""
+    rng = np.random.default_rng(v)
+    x = rng.uniform(-3.4e38, 3.4e38, (m, v)).astype(np.float32)
+    x[rng.random((m, v)) < 0.2] = np.finfo(np.float32).min
+    t = rng.integers(0, v, m)
+    t[0] = x[0].argmin()
+    got = run(lib, x, t, temp, 5)
+    if temp > 1:
+        return compare(got, x, t, temp, 5)
+    lp, ent, ids, top_lp, *_ = formulas(x, t, temp, 5)
+    with np.errstate(over="ignore"):  # one logit has it all, the others' log probabilities are differences
+        assert np.allclose(got["logprob"], lp.astype(np.float32), rtol=2.0 ** -22, atol=0) and np.allclose(got["top_logprobs"], top_lp.astype(np.float32), rtol=2.0 ** -22, atol=0)
+    assert np.array_equal(got["top_ids"], ids) and not got["entropy"].any() and not ent.any()
+
+
 def test_nearly_certain_tokens_keep_their_precision(lib):
     """log probabilities and entropies of 1e-3 down to 1e-30, to a relative 2^-23 (v / 64 + 40 + 2 * distance)"""
     v = 2000
