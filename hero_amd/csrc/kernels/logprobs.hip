@@ -166,15 +166,20 @@ __global__ __launch_bounds__(256) void logprobs_range_kernel(LogprobsArgs a, Log
             join(s, next, scale);
             m_part = s.m * scale.part;
         }
+        // a batch's own sums first: a row of 262144 adds 256 of them and not 4096 terms, whose roundings go the same way where the
+        // terms are equal (5e-5 of the sum, so 4e-6)
+        float r = 0.f, t = 0.f;
 #pragma unroll
         for (int j = 0; j < kBatch; ++j) {
             const float d = scale.log2_of(v[j], m_part);
             const bool top = v[j] == s.m;
             const float e = top ? 0.f : __builtin_amdgcn_exp2f(d);
             s.c += top ? 1.f : 0.f;
-            s.r += e;
-            s.t += e * fmaxf(d, -200.f);
+            r += e;
+            t += e * fmaxf(d, -200.f);
         }
+        s.r += r;
+        s.t += t;
     }
     if constexpr (TOP) {
         const int batches = (last - first + kStep - 1) / kStep;

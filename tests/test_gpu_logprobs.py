@@ -192,6 +192,26 @@ def test_logits_further_apart_than_fp32_reaches(lib, m, v, temp):
     assert np.array_equal(got["top_ids"], ids) and not got["entropy"].any() and not ent.any()
 
 
+def test_sums_of_thousands_of_equal_terms(lib):
+    """Rows that one wave each sums alone, all logits but one equal: every addition to a sum errs to the same side then.
+    A lane adds up 16 terms and then v / 1024 such sums, which bounds the sum's error by 2^-24 of it for each of these, for
+    the 12 joins and 4 more; a term's exponent and the logarithms as in compare()."""
+    import torch
+
+    m, v = 1030, 262144
+    gap = np.resize(np.array([2.5, 1.375, 5.875, 3.75, 5.625, 11.0]), m)
+    x = (-torch.from_numpy(gap.astype(np.float32)).cuda())[:, None].expand(m, v).contiguous()
+    x[:, 77] = 0
+    t = dev(np.full(m, 77, np.int32))
+    lp, ent, wb = empty(4 * m), empty(4 * m), lib.hero_logprobs_work_bytes(m, v, 0)
+    work = empty(wb)
+    check(lib.hero_logprobs(x.data_ptr(), v, m, v, ptr(t), 1.0, 0, ptr(lp), ptr(ent), None, None, ptr(work), wb, stream()))
+    r = (v - 1) * np.exp(-gap)
+    rel, dist, want = 2.0 ** -24 * (v / 1024 + 16 + 12 + 4) + 2.0 ** -23 * (gap + 1), gap * r / (1 + r), np.log1p(r)
+    assert np.all(np.abs(host(lp, np.float32) + want) <= rel + 2.0 ** -21 * want)
+    assert np.all(np.abs(host(ent, np.float32) - (want + dist)) <= rel + 2 * rel * dist + 2.0 ** -21 * (want + dist))
+
+
 def test_nearly_certain_tokens_keep_their_precision(lib):
     """log probabilities and entropies of 1e-3 down to 1e-30, to a relative 2^-23 (v / 64 + 40 + 2 * distance)"""
     v = 2000
