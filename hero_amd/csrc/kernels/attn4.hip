@@ -427,11 +427,12 @@ __global__ __launch_bounds__(256, DH == 128 && ONE ? 3 : 2) void attn4_short_ker
             // remainders in fp32: instructions that round to one half of a register (fma_mixlo) take twice as
             // long. Pinned, or the compiler makes those of them.
             q4_h8 w8, w8l;
+            float weights = 0.f;  // (a unit's weights first: roundings of thousands of equal ones would go the same way)
 #pragma unroll
             for (int j = 0; j < 8; j += 2) {
                 const float e0 = exp2_hw(__builtin_fmaf(s[j], unit, -m2)), e1 = exp2_hw(__builtin_fmaf(s[j + 1], unit, -m2));
-                l += e0;
-                l += e1;
+                weights += e0;
+                weights += e1;
                 const q4_h2 h2 = __builtin_convertvector((f2_t{e0 * kPOne, e1 * kPOne}), q4_h2);
                 float d0 = __builtin_fmaf(e0, kPOne, -float(h2[0])), d1 = __builtin_fmaf(e1, kPOne, -float(h2[1]));
                 asm volatile("" : "+v"(d0), "+v"(d1));
@@ -443,6 +444,7 @@ __global__ __launch_bounds__(256, DH == 128 && ONE ? 3 : 2) void attn4_short_ker
                     w8[j] = h2[0], w8[j + 1] = h2[1], w8l[j] = l2[0], w8l[j + 1] = l2[1];
                 }
             }
+            l += weights;
 #pragma unroll
             for (int h = 0; h < H; ++h)
 #pragma unroll
@@ -837,6 +839,7 @@ __global__ __launch_bounds__(256, DH == 128 ? 2 : 1) void attn4_chunk_kernel(Att
             // The next unit's scores, and between their products this one's weights, ... (The order is kept: the
             // compiler's own has the vector instructions first and the products behind them.)
             f16_t ahead = zero;
+            float weights = 0.f;  // (a unit's weights first: roundings of thousands of equal ones would go the same way)
             uint32_t terms_h[8], terms_l[8];
             q4_h8 x_now = operand_k(now ^ 1, 0), x_next = operand_k(now ^ 1, 1);
             __builtin_amdgcn_sched_barrier(0);
@@ -848,8 +851,8 @@ __global__ __launch_bounds__(256, DH == 128 ? 2 : 1) void attn4_chunk_kernel(Att
                 if (k % (NS / 8) == 0) {  // two weights, as two terms; pinned to their place in the order
                     const int i = k / (NS / 8);
                     const float e0 = exp2_hw(__builtin_fmaf(s[2 * i], unit, -m2)), e1 = exp2_hw(__builtin_fmaf(s[2 * i + 1], unit, -m2));
-                    l += e0;
-                    l += e1;
+                    weights += e0;
+                    weights += e1;
                     // Conversions in pairs and remainders in fp32: instructions that round to one half of a
                     // register (fma_mixlo) take twice as long. Pinned, or the compiler makes those of them.
                     const q4_h2 hi = __builtin_convertvector((f2_t{e0 * kPOne, e1 * kPOne}), q4_h2);
@@ -863,6 +866,7 @@ __global__ __launch_bounds__(256, DH == 128 ? 2 : 1) void attn4_chunk_kernel(Att
                 x_now = x_next, x_next = x_then;
                 __builtin_amdgcn_sched_barrier(0);
             }
+            l += weights;
             q4_h8 wh[2], wl[2];
             __builtin_memcpy(wh, terms_h, 32);
             __builtin_memcpy(wl, terms_l, 32);

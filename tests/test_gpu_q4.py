@@ -461,6 +461,38 @@ def test_long_ranges(lib, hkv, dh, rows, first, row_seq):
     compare(host(out, np.float32, (rows, hkv, dh))[:, heads], *attend64(few, len(heads), q[:, heads], gate, seq, pos, dh ** -0.5, 0, 0))
 
 
+@pytest.mark.parametrize("hkv,rows,row_seq,keys_a_sum", [(264, 17, True, 32), (768, 1, False, 128)])
+def test_totals_of_equal_weights(lib, hkv, rows, row_seq, keys_a_sum):
+    """So many heads that the keys are not split, and all weights but the first key's equal: every addition to the
+    total errs to the same side then. Values but the first key's are 0, so that the total alone decides. It is off by 2^-24 of itself for each
+    sum that a lane adds to it (one for so many keys), for the 16 terms of such a sum and 40 joins at most; 2^-22
+    for the weights' exponents and 2^-22 for the end's roundings."""
+    rng = np.random.default_rng(hkv)
+    n, dh = 60000, 128
+    c = Pool(rng, 1, 2, hkv, spare=0)
+    c.max_pages, c.table = -(-n // 64), np.ones((1, -(-n // 64)), np.int32)
+    c.table[0, 0] = 0
+    c.rec[..., : 8 * dh] = 0x88  # codes 0
+    c.rec[..., 8 * dh:] = np.ones(dh // 2, np.float16).view(np.uint8)
+    first, ones = np.zeros((hkv, dh), np.int64), np.ones((hkv, dh // 32), np.float16)
+    first[:, 0] = 7
+    c.store(0, 0, 0, first, ones)
+    c.store(0, 1, 0, first, ones)
+    q = np.zeros((rows, hkv, dh), np.float32)
+    q[..., 0] = np.linspace(0.2, 0.8, hkv)
+    pos = np.arange(n - rows, n, dtype=np.int32)
+    d = {k: dev(v) for k, v in dict(q=q, proj=np.zeros((rows, 2 * hkv * dh), np.float32), pages=c.rec, table=c.table, pos=pos, seq=np.zeros(rows, np.int32)).items()}
+    wb = lib.hero_attn_q4_work_bytes(rows, hkv, hkv, dh, c.max_pages * 64, 0, 0)
+    out, work = empty(rows * hkv * dh * 4), empty(max(wb, 16))
+    args = q4_args(c, hkv, rows, ptr(d["pos"]), ptr(d["seq"]) if row_seq else None, proj=ptr(d["proj"]), stride=2 * hkv * dh, q_rot=ptr(d["q"]), out=ptr(out), pages=ptr(d["pages"]),
+                   table=ptr(d["table"]), work=ptr(work), work_bytes=wb)
+    check(lib.hero_attn_q4(args, stream()))
+    got = host(out, np.float32, (rows, hkv, dh))
+    want = 0.5 * 7 / (1 + pos[:, None] * np.exp(-7 * q[..., 0].astype(np.float64)))
+    assert not got[..., 1:].any()
+    assert np.abs(got[..., 0] / want - 1).max() <= 2.0 ** -24 * (n / keys_a_sum + 16 + 40) + 2.0 ** -21
+
+
 def test_calls_at_once_and_one_workspace_after_another(lib):
     """Calls of every form: on two streams at once with a workspace each, and on one stream with one for all, give what they
     give alone."""
