@@ -192,6 +192,15 @@ def test_logits_further_apart_than_fp32_reaches(lib, m, v, temp):
     assert np.array_equal(got["top_ids"], ids) and not got["entropy"].any() and not ent.any()
 
 
+def test_alternatives_of_rows_that_one_wave_reads_alone(lib):
+    """more batches than maxima are kept before they are stored"""
+    rng = np.random.default_rng(9)
+    m, v = 1100, 70001
+    x = (rng.standard_normal((m, v), dtype=np.float32) * 3).astype(np.float32)
+    t = rng.integers(0, v, m)
+    compare(run(lib, x, t, 1.0, 20), x, t, 1.0, 20, rows=np.array([0, 1, 5, 500, 1098, 1099]))
+
+
 def test_sums_of_thousands_of_equal_terms(lib):
     """Rows that one wave each sums alone, all logits but one equal: every addition to a sum errs to the same side then.
     A lane adds up 16 terms and then v / 1024 such sums, which bounds the sum's error by 2^-24 of it for each of these, for
