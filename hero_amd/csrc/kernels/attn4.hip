@@ -16,12 +16,15 @@
 // other halves would be idle in a chunk's workgroup. Keys are split into ranges where there are few
 // workgroups, and combined by a second launch.
 //
-// Measured, 32 query and 8 K/V heads of 128, in pages of 64: sixteen tokens of 32000 keys each 121 to 127 us, 4.9 TB/s of cache
-// in the first launch (a copy of gigabytes: 5.1); the same over windows of 4096 26 us; one token of 32000 keys 19.8 us, of which
+// Measured, 32 query and 8 K/V heads of 128, in pages of 64 (where two figures stand, on different cards): sixteen tokens of 32000
+// keys each 121 to 129 us, 4.9 TB/s of cache
+// in the first launch (a copy of gigabytes: 5.1); the same over windows of 4096 26 us; one token of 32000 keys 19.9 us, of which
 // about 3 are spent before the first records arrive, 2 after the last ones and 4 on the second launch, and 6 keep the vector units
-// busy with turning codes into operands; one token of 300 keys 8.8 us, latencies and instruction fetches. 500 rows
-// over 16000 keys 253 to 261 us, 1.07 PFLOP/s of products (fp16 matrix products of 8192^3 reach 1.17); 1000 rows of three
-// sequences over windows of 1024 76 us: 250 workgroups of 34 units each, 44 us for these, about 16 from start to first and from
+// busy with turning codes into operands; one token of 300 keys 8.8 us, latencies and instruction fetches (12.1 us with a table of
+// 32768 positions, whose 96 ranges are nearly all empty). 500 rows
+// over 16000 keys 253 to 266 us, 1.05 to 1.00 PFLOP/s of products (fp16 matrix products of 8192^3 reach 1.17), the same of 16 heads of 256
+// 274 us; 1000 rows of three
+// sequences over windows of 1024 77 us: 250 workgroups of 34 units each, 44 us for these, about 16 from start to first and from
 // last product to end, 5 for the launch that looks for short runs.
 #include "hero/device.hpp"
 #include "hero/kernels.hpp"
@@ -1059,11 +1062,12 @@ __global__ __launch_bounds__(256) void attn4_combine_kernel(Attn4Args a, int nsp
 
 // Rows a workgroup takes, and into how many ranges their keys are split. Tokens and few rows: as many workgroups as are
 // there at once, three per CU of single rows of 128-wide heads and else two (with three, eight rows over 16000 keys of 256-wide
-// heads take 46 us instead of 42, four rows of one sequence over 32000 35 instead of 28), eight units of 32 keys each at least. Chunks: one workgroup per CU with at least eight units; two (of 128-wide heads, of which two
-// fit) where one would have 45 units or more: a unit takes 1.3 us alone and 1.0 us of each of two, and the ranges'
-// combination costs 5 to 13 us. 500 rows over 16000 keys, 258 units: 315 us in two ranges, 275 in four; 300 rows over
-// 4000, 45 units: 82 in four, 72 in six; 1000 rows over 2500, 94 units: 131 in one, 118 in two; over 1000, 34 units: 64 and
-// 68; 500 rows of two sequences over 2250, 35 units: 75 in two, 82 in four.
+// heads take 46 us instead of 42, four rows of one sequence over 32000 34 instead of 26), eight units of 32 keys each at least. Chunks: one workgroup per CU with at least eight units; two (of 128-wide heads, of which two
+// fit) where one would have 45 units or more: two that share a CU are ahead of one in the long run, but the ranges'
+// combination costs 5 to 10 us. 500 rows over 16000 keys, 258 units: 284 us in two ranges, 262 in four; 300 rows over
+// 4000, 45 units: 65 in four, 63 in six; 1000 rows over 2500, 94 units: 127 in one, 123 in two; over windows of 1024, 34 units: 52 and
+// 61; 500 rows of two sequences over 2250, 35 units: 82 in two, 89 in four. All of this goes by what the table has room for, which the host knows, and
+// not by the rows' positions, which are the device's.
 enum class Form { token, few, chunk };
 struct Plan {
     int R, nsplit;
@@ -1086,7 +1090,7 @@ Plan attn4_plan(Form form, int64_t rows, int64_t seqs, int64_t group, int64_t Hk
     return p;
 }
 // rows that belong to sequences of their own have no keys in common; few rows are short runs, however they stand (four rows of one
-// sequence over 16000 keys 24.7 us, as a chunk 36.7; over 1000 keys 17.7 and 24.8)
+// sequence over 16000 keys 23.6 us, as a chunk 32.2; over 1000 keys 16.8 and 23.0)
 Form attn4_form(bool row_seq, int64_t rows, int64_t group) { return !row_seq || rows == 1 ? Form::token : rows * group <= 16 ? Form::few : Form::chunk; }
 
 }  // namespace
@@ -1112,7 +1116,7 @@ void attn4_sized(const Attn4Args& a, hipStream_t s) {
     if (form == Form::token)
         hipLaunchKernelGGL((attn4_short_kernel<DH, 2, true>), dim3(unsigned(rows * Hkv * p.nsplit)), dim3(256), 0, s, a, p.nsplit, 1);
     if (runs) {
-        // two workgroups per CU are there at once: with three, 64 tokens of 8000 keys take 225 us instead of 215
+        // two workgroups per CU are there at once: with three, 64 tokens of 8000 keys take 220 us instead of 210
         const int64_t stride = std::min(rows, std::max<int64_t>(1, 512 / (Hkv * p.nsplit)));
         hipLaunchKernelGGL((attn4_short_kernel<DH, 2, false>), dim3(unsigned(stride * Hkv * p.nsplit)), dim3(256), 0, s, a, p.nsplit, int(stride));
     }
